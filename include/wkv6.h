@@ -360,6 +360,96 @@ int wkv6_backward_with_state(void *stream, int dtype, int algo, int64_t B, int64
                              void *gr, void *gk, void *gv, void *gw, void *gu, float *gs0,
                              void *workspace, size_t workspace_bytes);
 
+/* ---- What a training step does behind the model's last layer -----------------------------
+ * No counterpart in the reference, whose losses and optimizers are the framework's above it.
+ *
+ * Losses over logits.  `logits` are B * T rows of V values of `dtype`, row (b, t) at element b * stride_b + t * stride_t of them,
+ * the values of a row next to each other; rows need no alignment beyond the element's, and may overlap.  ids (B,T) name the
+ * token that stands at each place; mask (B,T), one byte each, or NULL.  A token COUNTS if its mask is not zero and its id is not
+ * negative; the row of one that does not is not read, and its gradient is zero.  An id of V or more makes its token's log
+ * probability and gradient NaN.  temperature > 0 divides the logits.  All other arrays are fp32 and contiguous:
+ *   logps (B,T)    log probability of the token that stands there, 0 where none counts
+ *   stats (B,T,2)  what wkv6_logits_backward needs of each row
+ *   coef           dL/dlogp: (B,T), of wkv6_preference_loss (B)
+ * stats, coef and grad may be NULL where no gradient is wanted.  grad (B,T,V), contiguous, of `dtype`: the forward call writes
+ * the gradient of the loss too, for an arriving gradient of 1, in the pass over the logits that it makes anyway.
+ * No address needs more than its element's alignment here; workspace: 16 bytes. */
+enum { WKV6_REDUCE_SUM = 0, WKV6_REDUCE_MEAN = 1, WKV6_REDUCE_MEAN_OF_TEXTS = 2 };
+enum { WKV6_PREFERENCE_SIGMOID = 0, WKV6_PREFERENCE_HINGE = 1, WKV6_PREFERENCE_IPO = 2 };
+
+int wkv6_token_logprobs(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                        const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                        float temperature, float *logps, float *stats);
+
+/* loss (1) = sum or mean over counted tokens of -logp; no counted token: 0. */
+size_t wkv6_loss_workspace_bytes(int64_t B, int64_t T);
+int wkv6_cross_entropy(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                       const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                       int reduction, float *loss, float *stats, float *coef, void *grad,
+                       void *workspace, size_t workspace_bytes);
+
+/* Clipped policy loss: with ratio = exp(logp - old_logps) (1 where old_logps is NULL: the sampling model is this one) and
+ * e = ref_logps - logp (no such term where NULL), the mean over counted tokens of
+ *   kl_weight (exp(e) - e - 1) - min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A),   A = advantages[b adv_stride_b + t adv_stride_t]
+ * WKV6_REDUCE_MEAN: over all tokens; WKV6_REDUCE_MEAN_OF_TEXTS: over each text's tokens, then over the texts that have any.
+ * means (2): the same mean of exp(e) - e - 1, and of whether the clamped term was the smaller one. */
+int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                     const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                     const float *old_logps, const float *advantages, int64_t adv_stride_b, int64_t adv_stride_t, const float *ref_logps,
+                     float clip_low, float clip_high, float kl_weight, float temperature, int reduction,
+                     float *loss, float *logps, float *means, float *stats, float *coef, void *grad,
+                     void *workspace, size_t workspace_bytes);
+
+/* Preference loss of B / 2 pairs of texts, text b chosen and text b + B / 2 rejected.  text_logps (B): sum of a text's logps
+ * (average != 0: over its counted tokens' number); d = (chosen - rejected) - the same of ref_logps ((B), NULL for none); loss =
+ * the mean over pairs of
+ *   SIGMOID  -(1 - label_smoothing) log sigmoid(beta d) - label_smoothing log sigmoid(-beta d)
+ *   HINGE    max(0, 1 - beta d)            IPO  (d - 1 / (2 beta))^2
+ * coef holds dL/dlogp of every token of a text: strides (1, 0) for wkv6_logits_backward. */
+int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                         const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                         const float *ref_logps, int kind, double beta, double label_smoothing, int average,
+                         float *loss, float *text_logps, float *stats, float *coef,
+                         void *workspace, size_t workspace_bytes);
+
+/* grad = upstream * dL/dlogits from stats and coef[b * coef_stride_b + t * coef_stride_t]; upstream: one value on the device, or
+ * NULL for 1.  grad_is_there != 0 (a forward call wrote grad): nothing is done where upstream is 1. */
+int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                         const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                         float temperature, const float *stats, const float *coef, int64_t coef_stride_b, int64_t coef_stride_t,
+                         const float *upstream, int grad_is_there, void *grad);
+
+/* Optimizers.  `tensors` lies in HOST memory and may be freed when the call returns.  Addresses need their element's alignment,
+ * scales 8 bytes, workspace 16.  param and grad are of `dtype`, dense and in the same order of elements. */
+typedef struct wkv6_adamw_tensor {
+    void *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    float *scales, *master;
+    int64_t numel;
+} wkv6_adamw_tensor;
+
+/* norm (1) = the 2-norm of the grads of `count` tensors together (nothing else of them is looked at), added up in 64 bits and
+ * always in the same order. */
+size_t wkv6_grad_norm_workspace_bytes(int64_t count);
+int wkv6_grad_norm(void *stream, int dtype, int64_t count, const wkv6_adamw_tensor *tensors, float *norm,
+                   void *workspace, size_t workspace_bytes);
+
+/* One step of AdamW over `count` tensors, in place.  With g' = g * max_grad_norm / max(*grad_norm, max_grad_norm) (max_grad_norm 0:
+ * g' = g), t = *step + 1 (written back) and lr = *lr_device where that is given:
+ *   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * master (fp32) or NULL: the weights that are updated, of which param then is the rounded copy.
+ * moment_bits 32: exp_avg and exp_avg_sq are m and v in fp32.  8: they are m and sqrt(v) as float8 (e4m3, no infinities)
+ * under scales, fp32 (ceil(numel / 256), 2): m's and sqrt(v)'s for each 256 elements.  They are rounded up or down at random, the
+ * mean kept; the random bits are a function of seed, t, the tensor's place in the list and the element's in the tensor.
+ * skip_nonfinite: where *grad_norm is no finite number nothing is changed.  grad_norm may be NULL where neither needs it. */
+size_t wkv6_adamw_workspace_bytes(int64_t count);
+int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, const wkv6_adamw_tensor *tensors,
+                    int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed,
+                    void *workspace, size_t workspace_bytes);
+
 /* ---- XLA custom-call surface (replaces the pybind module `gpu_ops`,
  * rwkv_kernel/jax_kernel/gpu_ops.cpp:20-43) ---------------------------------------------- */
 

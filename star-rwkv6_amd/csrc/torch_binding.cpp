@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <optional>
 #include <vector>
@@ -333,6 +334,254 @@ struct ShiftMix : torch::autograd::Function<ShiftMix> {
   }
 };
 
+// ---- losses over logits (wkv6_token_logprobs and its kin) ----
+
+// Logits as the kernels read them: (B, T, V), a row's values next to each other.
+struct Logits {
+  Tensor x, ids, mask;
+  int64_t B, T, V;
+  int code;
+  const int64_t *id() const { return static_cast<const int64_t *>(in(ids)); }
+  const uint8_t *counted() const { return static_cast<const uint8_t *>(in(mask)); }
+};
+
+Tensor given(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
+
+Logits logits_of(const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask) {
+  return {x, ids, given(mask), x.size(0), x.size(1), x.size(2), code_of(x.scalar_type())};
+}
+
+Tensor fp32(const Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+
+// What a node keeps of the rows for its backward.
+void keep_rows(AutogradContext *ctx, const Logits &l, const Tensor &stats, const Tensor &coef, double temperature) {
+  ctx->saved_data["temperature"] = temperature;
+  ctx->save_for_backward({l.x, l.ids, l.mask, stats, coef});
+}
+
+// Memory for the gradient that a forward writes beside its loss, or nothing where the backward writes it: in half precision, where
+// a training scales its loss up for the gradient's sake (so what arrives is not 1, and what is too small without it would be
+// lost here), and into a graph, whose replays may run the backward again and again after one forward.
+Tensor gradient_ahead(const Logits &l, bool wanted) {
+  if (!wanted || l.x.scalar_type() == at::kHalf || is_captured()) return Tensor();
+  return at::empty({l.B, l.T, l.V}, l.x.options());
+}
+
+// The gradient by the logits of sum(coef * logps), times `upstream` (undefined for 1).  `ahead`: what a forward wrote, for an upstream of 1.
+Tensor logits_backward(const variable_list &saved, double temperature, const Tensor &coef, int64_t coef_stride_b, int64_t coef_stride_t,
+                       const Tensor &upstream, const Tensor &ahead) {
+  const Logits l = logits_of(saved[0], saved[1], saved[2]);
+  const Tensor grad = ahead.defined() ? ahead : at::empty({l.B, l.T, l.V}, l.x.options());
+  check(wkv6_logits_backward(stream_of(l.x), l.code, l.B, l.T, l.V, in(l.x), l.x.stride(0), l.x.stride(1), l.id(), l.counted(),
+                             static_cast<float>(temperature), in_f(saved[3]), in_f(coef), coef_stride_b, coef_stride_t, in_f(upstream),
+                             ahead.defined(), out(grad)));
+  return grad;
+}
+
+Tensor arriving(const Tensor &g) { return g.to(at::kFloat).contiguous(); }
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, double temperature, bool wanted) {
+    const c10::DeviceGuard guard(x.device());
+    const Logits l = logits_of(x, ids, mask);
+    const Tensor lp = fp32(x, {l.B, l.T}), stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor();
+    check(wkv6_token_logprobs(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(),
+                              static_cast<float>(temperature), out_f(lp), out_f(stats)));
+    keep_rows(ctx, l, stats, Tensor(), temperature);
+    return lp;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const c10::DeviceGuard guard(s[0].device());
+    const Tensor coef = arriving(grads[0]);
+    return {logits_backward(s, ctx->saved_data["temperature"].toDouble(), coef, s[0].size(1), 1, Tensor(), Tensor()), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, int64_t reduction, bool wanted) {
+    const c10::DeviceGuard guard(x.device());
+    const Logits l = logits_of(x, ids, mask);
+    const Tensor loss = fp32(x, {}), stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor(), coef = wanted ? fp32(x, {l.B, l.T}) : Tensor();
+    const Tensor grad = gradient_ahead(l, wanted);
+    const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
+    const Tensor ws = bytes(x, n);
+    check(wkv6_cross_entropy(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(),
+                             static_cast<int>(reduction), out_f(loss), out_f(stats), out_f(coef), out(grad), out(ws), n));
+    keep_rows(ctx, l, stats, coef, 1.0);
+    keep(ctx, grad, "grad");
+    return loss;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const c10::DeviceGuard guard(s[0].device());
+    const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad"), up = arriving(grads[0]);
+    return {logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, const std::optional<Tensor> &old_logps,
+                               const Tensor &advantages, const std::optional<Tensor> &ref_logps, double clip_low, double clip_high, double kl_weight,
+                               double temperature, int64_t reduction, bool wanted) {
+    const c10::DeviceGuard guard(x.device());
+    const Logits l = logits_of(x, ids, mask);
+    const Tensor loss = fp32(x, {}), lp = fp32(x, {l.B, l.T}), means = fp32(x, {2});
+    const Tensor stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor(), coef = wanted ? fp32(x, {l.B, l.T}) : Tensor();
+    const Tensor grad = gradient_ahead(l, wanted);
+    const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
+    const Tensor ws = bytes(x, n);
+    check(wkv6_policy_loss(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(), in_f(given(old_logps)),
+                           in_f(advantages), advantages.stride(0), advantages.stride(1), in_f(given(ref_logps)), static_cast<float>(clip_low),
+                           static_cast<float>(clip_high), static_cast<float>(kl_weight), static_cast<float>(temperature),
+                           static_cast<int>(reduction), out_f(loss), out_f(lp), out_f(means), out_f(stats), out_f(coef), out(grad), out(ws), n));
+    keep_rows(ctx, l, stats, coef, temperature);
+    keep(ctx, grad, "grad");
+    ctx->mark_non_differentiable({lp, means});
+    ctx->set_materialize_grads(false);
+    return {loss, lp, means};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const at::NoGradGuard no_grad;
+    variable_list res(12);
+    if (!grads[0].defined()) return res;
+    const auto s = ctx->get_saved_variables();
+    const c10::DeviceGuard guard(s[0].device());
+    const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad"), up = arriving(grads[0]);
+    res[0] = logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead);
+    return res;
+  }
+};
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, const std::optional<Tensor> &ref_logps,
+                               int64_t kind, double beta, double label_smoothing, bool average, bool wanted) {
+    const c10::DeviceGuard guard(x.device());
+    const Logits l = logits_of(x, ids, mask);
+    const Tensor loss = fp32(x, {}), text = fp32(x, {l.B});
+    const Tensor stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor(), coef = wanted ? fp32(x, {l.B}) : Tensor();
+    const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
+    const Tensor ws = bytes(x, n);
+    check(wkv6_preference_loss(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(), in_f(given(ref_logps)),
+                               static_cast<int>(kind), beta, label_smoothing, average, out_f(loss), out_f(text), out_f(stats), out_f(coef), out(ws), n));
+    keep_rows(ctx, l, stats, coef, 1.0);
+    ctx->mark_non_differentiable({text});
+    ctx->set_materialize_grads(false);
+    return {loss, text};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const at::NoGradGuard no_grad;
+    variable_list res(9);
+    if (!grads[0].defined()) return res;
+    const auto s = ctx->get_saved_variables();
+    const c10::DeviceGuard guard(s[0].device());
+    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor());
+    return res;
+  }
+};
+
+// ---- AdamW ----
+
+bool same_layout(const Tensor &a, const Tensor &b) {
+  return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
+}
+
+using Tensors = std::vector<Tensor>;
+
+void on_one_device(const Tensor &t, const Tensor &like, const char *what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "wkv6: ", what, " must be on the parameters' GPU");
+}
+
+Tensor grad_norm(const Tensors &grads) {
+  TORCH_CHECK(!grads.empty() && grads[0].is_cuda() && code_of(grads[0].scalar_type()) >= 0, "wkv6: gradients are bf16, fp16 or fp32 tensors on the GPU");
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(grads[0].device());
+  Tensors kept;   // (dense copies of what is not, until the kernels are enqueued)
+  std::vector<wkv6_adamw_tensor> rows;
+  for (const Tensor &g : grads) {
+    on_one_device(g, grads[0], "gradients");
+    TORCH_CHECK(g.scalar_type() == grads[0].scalar_type() && g.layout() == at::kStrided, "wkv6: gradients are dense and of one dtype");
+    const Tensor d = g.is_non_overlapping_and_dense() ? g : g.contiguous();
+    kept.push_back(d);
+    rows.push_back({nullptr, in(d), nullptr, nullptr, nullptr, nullptr, d.numel()});
+  }
+  const Tensor norm = fp32(grads[0], {});
+  const size_t n = wkv6_grad_norm_workspace_bytes(rows.size());
+  const Tensor ws = bytes(grads[0], n);
+  check(wkv6_grad_norm(stream_of(grads[0]), code_of(grads[0].scalar_type()), rows.size(), rows.data(), out_f(norm), out(ws), n));
+  return norm;
+}
+
+// The step; returns the gradients' norm, `norm` itself where it is given, nothing where nobody asks for it.
+Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &exp_avgs, const Tensors &exp_avg_sqs, const Tensor &step,
+                  const Tensors &scales, const Tensors &masters, const Tensor &lr_device, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, double max_grad_norm, bool skip_nonfinite, Tensor norm, int64_t seed) {
+  const size_t count = params.size();
+  TORCH_CHECK(count > 0 && grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count,
+              "wkv6: one gradient and two moments for each parameter");
+  const Tensor &first = params[0];
+  const ScalarType type = first.scalar_type(), moment = exp_avgs[0].scalar_type();
+  TORCH_CHECK(first.is_cuda() && code_of(type) >= 0, "wkv6: parameters are bf16, fp16 or fp32 tensors on the GPU");
+  TORCH_CHECK(moment == at::kFloat || moment == at::kFloat8_e4m3fn, "wkv6: moments are float32 or float8_e4m3fn");
+  const bool eight = moment == at::kFloat8_e4m3fn;
+  TORCH_CHECK(eight ? scales.size() == count : scales.empty(), "wkv6: moments in 8 bits, and no others, have scales");
+  TORCH_CHECK(masters.empty() || (masters.size() == count && type != at::kFloat), "wkv6: one master for each parameter of 16 bits");
+  on_one_device(step, first, "step");
+  TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 1, "wkv6: step is one int64");
+  for (const Tensor *t : {&lr_device, const_cast<const Tensor *>(&norm)}) {
+    if (!t->defined()) continue;
+    on_one_device(*t, first, "lr and grad_norm");
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == 1, "wkv6: lr and grad_norm are one float32");
+  }
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(first.device());
+  Tensors kept;
+  std::vector<wkv6_adamw_tensor> rows;
+  std::vector<const void *> seen;
+  for (size_t i = 0; i < count; ++i) {
+    const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
+    for (const Tensor *t : {&p, &grads[i], &m, &v}) {
+      on_one_device(*t, first, "gradients and moments");
+      TORCH_CHECK(t->layout() == at::kStrided && t->sizes() == p.sizes(), "wkv6: a gradient and its moments have the parameter's shape");
+    }
+    TORCH_CHECK(p.scalar_type() == type && grads[i].scalar_type() == type, "wkv6: parameters and gradients of a call have one dtype");
+    TORCH_CHECK(m.scalar_type() == moment && v.scalar_type() == moment, "wkv6: moments of a call have one dtype");
+    TORCH_CHECK(p.is_non_overlapping_and_dense() && same_layout(m, p) && same_layout(v, p), "wkv6: parameters are dense, their moments laid out like them");
+    wkv6_adamw_tensor row{out(p), nullptr, out(m), out(v), nullptr, nullptr, p.numel()};
+    if (eight) {
+      on_one_device(scales[i], first, "scales");
+      TORCH_CHECK(scales[i].scalar_type() == at::kFloat && scales[i].is_contiguous() && scales[i].dim() == 2 && scales[i].size(1) == 2 &&
+                      scales[i].size(0) == (p.numel() + 255) / 256, "wkv6: scales are float32 (ceil(numel / 256), 2)");
+      row.scales = out_f(scales[i]);
+    }
+    if (!masters.empty()) {
+      on_one_device(masters[i], first, "masters");
+      TORCH_CHECK(masters[i].scalar_type() == at::kFloat && same_layout(masters[i], p), "wkv6: masters are float32, laid out like their parameters");
+      row.master = out_f(masters[i]);
+    }
+    Tensor g = grads[i];
+    if (!same_layout(g, p)) g = at::empty_like(p).copy_(g);
+    kept.push_back(g);
+    row.grad = in(g);
+    rows.push_back(row);
+    if (p.numel() > 0) seen.push_back(row.param);
+  }
+  std::sort(seen.begin(), seen.end());
+  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "wkv6: a parameter is given twice");
+  if (!norm.defined() && (max_grad_norm > 0. || skip_nonfinite)) norm = grad_norm(kept);
+  const size_t n = wkv6_adamw_workspace_bytes(count);
+  const Tensor ws = bytes(first, n);
+  check(wkv6_adamw_step(stream_of(first), code_of(type), eight ? 8 : 32, count, rows.data(), static_cast<int64_t *>(out(step)), in_f(lr_device), lr, beta1,
+                        beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, in_f(norm), static_cast<uint32_t>(seed), out(ws), n));
+  for (const Tensors *l : {&params, &exp_avgs, &exp_avg_sqs, &scales, &masters})
+    for (const Tensor &t : *l)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // (what autograd saved of them is no longer what it was)
+  if (!step.is_inference()) step.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 // (B, H, N, N)
 at::DimVector state_shape(const Dims &d) {
   TORCH_CHECK(d.H > 0, "wkv6: tensors without channels have no state");   // (the size per head below divides by it)
@@ -463,8 +712,6 @@ py::object try_gn_gate(int64_t N, const py::object &r_, const py::object &k_, co
   }));
 }
 
-Tensor given(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
-
 }  // namespace
 
 PYBIND11_MODULE(_wkv6_torch, m) {
@@ -489,6 +736,42 @@ PYBIND11_MODULE(_wkv6_torch, m) {
     const ScalarType st = state_code == WKV6_F32 ? at::kFloat : state_code == WKV6_F16 ? at::kHalf : at::kBFloat16;
     return wrap(unlocked([&] { return forward_with_state(H, given(map), r, k, v, w, u, given(s0), algo, st, backward_follows); }));
   }, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg("backward_follows") = false);
+  m.def("token_logprobs", [](const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, double temperature) {
+    const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
+    return unlocked([&] { return TokenLogprobs::apply(x, ids, mask, temperature, wanted); });
+  });
+  m.def("cross_entropy", [](const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, int64_t reduction) {
+    const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
+    return unlocked([&] { return CrossEntropy::apply(x, ids, mask, reduction, wanted); });
+  });
+  m.def("policy_loss", [](const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, const std::optional<Tensor> &old_logps,
+                          const Tensor &advantages, const std::optional<Tensor> &ref_logps, double clip_low, double clip_high, double kl_weight,
+                          double temperature, int64_t reduction) {
+    const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
+    const variable_list o = unlocked([&] {
+      return PolicyLoss::apply(x, ids, mask, old_logps, advantages, ref_logps, clip_low, clip_high, kl_weight, temperature,
+                               reduction, wanted);
+    });
+    return py::make_tuple(wrap(o[0]), wrap(o[1]), wrap(o[2]));
+  });
+  m.def("preference_loss", [](const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, const std::optional<Tensor> &ref_logps,
+                              int64_t kind, double beta, double label_smoothing, bool average) {
+    const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
+    const variable_list o = unlocked([&] {
+      return PreferenceLoss::apply(x, ids, mask, ref_logps, kind, beta, label_smoothing, average, wanted);
+    });
+    return py::make_tuple(wrap(o[0]), wrap(o[1]));
+  });
+  m.def("grad_norm", [](const Tensors &grads) { return unlocked([&] { return grad_norm(grads); }); });
+  m.def("adamw_step", [](const Tensors &params, const Tensors &grads, const Tensors &exp_avgs, const Tensors &exp_avg_sqs, const Tensor &step,
+                         const Tensors &scales, const Tensors &masters, const std::optional<Tensor> &lr_device, double lr, double beta1,
+                         double beta2, double eps, double weight_decay, double max_grad_norm, bool skip_nonfinite,
+                         const std::optional<Tensor> &norm, int64_t seed) {
+    return wrap(unlocked([&] {
+      return adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, scales, masters, given(lr_device), lr, beta1, beta2, eps, weight_decay,
+                        max_grad_norm, skip_nonfinite, given(norm), seed);
+    }));
+  });
   m.def("forward_gn_gate", [](int64_t H, const std::optional<Tensor> &map, const Tensor &r, const Tensor &k, const Tensor &v, const Tensor &w,
                               const Tensor &u, const std::optional<Tensor> &s0, const Tensor &gate, const Tensor &scale,
                               const Tensor &offset, double eps, bool want_state) {

@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <initializer_list>
 
 // Workspace of wkv6_backward_static: device memory the library owns, one copy per GPU.  In host
 // code the name below is only a handle for hipGetSymbolAddress; the address that kernels, copies and
@@ -302,6 +303,165 @@ int wkv6_gn_gate_backward_sums(void *stream, int dtype, int64_t B, int64_t T, in
                                const float *gn_scale, const float *gn_offset,
                                void *gy, void *ggate, float *gscale, float *goffset) {
     return gn_gate_backward(stream, dtype, B, T, C, H, gout, y, stats, gate, gn_scale, gn_offset, gy, ggate, gscale, goffset, true);
+}
+
+// ---- losses over logits, AdamW ----
+
+static bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+static size_t element_size(int dtype) { return dtype == WKV6_F32 ? 4 : 2; }
+
+// Rows of logits: what every call on them asks for.
+static int check_rows(int dtype, int64_t B, int64_t T, int64_t V, const void *logits, int64_t stride_b, int64_t stride_t,
+                      const int64_t *ids, float temperature) {
+    if (dtype != WKV6_BF16 && dtype != WKV6_F16 && dtype != WKV6_F32) return WKV6_ERR_ARG;
+    if (B <= 0 || T <= 0 || V <= 0 || stride_b < 0 || stride_t < 0) return WKV6_ERR_ARG;
+    if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || 1.f / temperature > 3.4e38f) return WKV6_ERR_ARG;
+    if (!logits || !ids || !aligned(logits, element_size(dtype)) || !aligned(ids, 8)) return WKV6_ERR_ARG;
+    // a launch has a workgroup per row; nothing overflows in offsets of V * rows elements
+    if (B > 0x7fffffffLL || T > 0x7fffffffLL || B * T > 0x7fffffffLL || V > 0x7fffffffLL) return WKV6_ERR_UNSUPPORTED;
+    return WKV6_OK;
+}
+static wkv6::LossRows rows_of(int64_t B, int64_t T, int64_t V, const void *logits, int64_t stride_b, int64_t stride_t,
+                              const int64_t *ids, const uint8_t *mask, float temperature, float *logps, float *stats) {
+    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr};
+}
+static bool floats(std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (!aligned(p, 4)) return false;
+    return true;
+}
+
+int wkv6_token_logprobs(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                        const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                        float temperature, float *logps, float *stats) {
+    const int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, temperature);
+    if (rc != WKV6_OK) return rc;
+    if (!logps || !floats({logps, stats})) return WKV6_ERR_ARG;
+    return finish(wkv6::loss_rows((hipStream_t)stream, dtype, rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, temperature, logps, stats),
+                                  wkv6::LossTerms{}, nullptr, nullptr));
+}
+
+size_t wkv6_loss_workspace_bytes(int64_t B, int64_t T) {
+    return B > 0 && T > 0 && B <= 0x7fffffffLL && T <= 0x7fffffffLL && B * T <= 0x7fffffffLL ? wkv6::loss_workspace_bytes(B, T) : 0;
+}
+
+static int check_loss_workspace(int64_t B, int64_t T, const void *workspace, size_t bytes) {
+    return workspace && aligned16(workspace) && bytes >= wkv6::loss_workspace_bytes(B, T) ? WKV6_OK : WKV6_ERR_WORKSPACE;
+}
+
+int wkv6_cross_entropy(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                       const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                       int reduction, float *loss, float *stats, float *coef, void *grad,
+                       void *workspace, size_t workspace_bytes) {
+    int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, 1.f);
+    if (rc != WKV6_OK) return rc;
+    if (!loss || !floats({loss, stats, coef}) || !aligned(grad, element_size(dtype)) || (grad && (!stats || !coef))) return WKV6_ERR_ARG;
+    if (reduction != WKV6_REDUCE_SUM && reduction != WKV6_REDUCE_MEAN) return WKV6_ERR_ARG;
+    rc = check_loss_workspace(B, T, workspace, workspace_bytes);
+    if (rc != WKV6_OK) return rc;
+    wkv6::LossTerms l{};
+    l.kind = wkv6::kLossCrossEntropy, l.reduction = reduction, l.loss = loss, l.coef = coef;
+    return finish(wkv6::loss_rows((hipStream_t)stream, dtype, rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, 1.f, nullptr, stats), l, grad,
+                                  workspace));
+}
+
+int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                     const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                     const float *old_logps, const float *advantages, int64_t adv_stride_b, int64_t adv_stride_t, const float *ref_logps,
+                     float clip_low, float clip_high, float kl_weight, float temperature, int reduction,
+                     float *loss, float *logps, float *means, float *stats, float *coef, void *grad,
+                     void *workspace, size_t workspace_bytes) {
+    int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, temperature);
+    if (rc != WKV6_OK) return rc;
+    if (!advantages || !loss || !logps || !means || adv_stride_b < 0 || adv_stride_t < 0) return WKV6_ERR_ARG;
+    if (!floats({old_logps, advantages, ref_logps, loss, logps, means, stats, coef}) || !aligned(grad, element_size(dtype)) || (grad && (!stats || !coef))) return WKV6_ERR_ARG;
+    if (!(clip_low >= 0.f) || !(clip_high >= 0.f) || kl_weight != kl_weight) return WKV6_ERR_ARG;
+    if (reduction != WKV6_REDUCE_MEAN && reduction != WKV6_REDUCE_MEAN_OF_TEXTS) return WKV6_ERR_ARG;
+    rc = check_loss_workspace(B, T, workspace, workspace_bytes);
+    if (rc != WKV6_OK) return rc;
+    wkv6::LossTerms l{};
+    l.kind = wkv6::kLossPolicy, l.reduction = reduction, l.loss = loss, l.means = means, l.coef = coef;
+    l.old_logps = old_logps, l.ref_logps = ref_logps, l.advantages = advantages, l.adv_stride_b = adv_stride_b, l.adv_stride_t = adv_stride_t;
+    l.clip_low = clip_low, l.clip_high = clip_high, l.kl_weight = kl_weight;
+    return finish(wkv6::loss_rows((hipStream_t)stream, dtype, rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, temperature, logps, stats), l, grad,
+                                  workspace));
+}
+
+int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                         const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                         const float *ref_logps, int kind, double beta, double label_smoothing, int average,
+                         float *loss, float *text_logps, float *stats, float *coef, void *workspace, size_t workspace_bytes) {
+    int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, 1.f);
+    if (rc != WKV6_OK) return rc;
+    if (B % 2 != 0 || !loss || !text_logps || !floats({ref_logps, loss, text_logps, stats, coef})) return WKV6_ERR_ARG;
+    if (kind < WKV6_PREFERENCE_SIGMOID || kind > WKV6_PREFERENCE_IPO || !(beta > 0.) || !(label_smoothing >= 0. && label_smoothing < 0.5)) return WKV6_ERR_ARG;
+    if (kind != WKV6_PREFERENCE_SIGMOID && label_smoothing != 0.) return WKV6_ERR_ARG;
+    rc = check_loss_workspace(B, T, workspace, workspace_bytes);
+    if (rc != WKV6_OK) return rc;
+    wkv6::LossRows a = rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, 1.f, nullptr, stats);
+    a.exact = static_cast<double *>(workspace);
+    const int run = finish(wkv6::loss_rows((hipStream_t)stream, dtype, a, wkv6::LossTerms{}, nullptr, nullptr));
+    if (run != WKV6_OK) return run;
+    return finish(wkv6::loss_preference((hipStream_t)stream, a, wkv6::PreferenceTerms{kind, average, beta, label_smoothing, ref_logps, loss, text_logps, coef}));
+}
+
+int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
+                         const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
+                         float temperature, const float *stats, const float *coef, int64_t coef_stride_b, int64_t coef_stride_t,
+                         const float *upstream, int grad_is_there, void *grad) {
+    const int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, temperature);
+    if (rc != WKV6_OK) return rc;
+    if (!stats || !coef || !grad || coef_stride_b < 0 || coef_stride_t < 0 || (grad_is_there && !upstream)) return WKV6_ERR_ARG;
+    if (!floats({stats, coef, upstream}) || !aligned(grad, element_size(dtype))) return WKV6_ERR_ARG;
+    return finish(wkv6::loss_grad((hipStream_t)stream, dtype,
+                                  rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, temperature, nullptr, const_cast<float *>(stats)),
+                                  wkv6::LossGrad{coef, coef_stride_b, coef_stride_t, upstream, grad_is_there, grad}));
+}
+
+static_assert(sizeof(wkv6_adamw_tensor) == sizeof(wkv6::AdamwTensor), "one layout");
+
+static int check_tensors(int dtype, int64_t count, const wkv6_adamw_tensor *tensors, bool grads_only, int moment_bits) {
+    if (dtype != WKV6_BF16 && dtype != WKV6_F16 && dtype != WKV6_F32) return WKV6_ERR_ARG;
+    if (count <= 0 || count > 0x7fffffffLL || !tensors) return WKV6_ERR_ARG;
+    const size_t es = element_size(dtype), ms = moment_bits == 32 ? 4 : 1;
+    for (int64_t i = 0; i < count; ++i) {
+        const wkv6_adamw_tensor &t = tensors[i];
+        if (t.numel < 0 || t.numel >= (1LL << 40)) return WKV6_ERR_ARG;
+        if (t.numel == 0) continue;
+        if (!t.grad || !aligned(t.grad, es)) return WKV6_ERR_ARG;
+        if (grads_only) continue;
+        if (!t.param || !t.exp_avg || !t.exp_avg_sq || (moment_bits == 8 && !t.scales)) return WKV6_ERR_ARG;
+        if (!aligned(t.param, es) || !aligned(t.exp_avg, ms) || !aligned(t.exp_avg_sq, ms) || !aligned(t.scales, 8) || !aligned(t.master, 4)) return WKV6_ERR_ARG;
+    }
+    return WKV6_OK;
+}
+
+size_t wkv6_grad_norm_workspace_bytes(int64_t count) { return count > 0 && count <= 0x7fffffffLL ? wkv6::grad_norm_workspace_bytes(count) : 0; }
+
+int wkv6_grad_norm(void *stream, int dtype, int64_t count, const wkv6_adamw_tensor *tensors, float *norm, void *workspace, size_t workspace_bytes) {
+    const int rc = check_tensors(dtype, count, tensors, true, 0);
+    if (rc != WKV6_OK) return rc;
+    if (!norm || !aligned(norm, 4)) return WKV6_ERR_ARG;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < wkv6::grad_norm_workspace_bytes(count)) return WKV6_ERR_WORKSPACE;
+    return finish(wkv6::grad_norm((hipStream_t)stream, dtype, count, reinterpret_cast<const wkv6::AdamwTensor *>(tensors), norm, workspace));
+}
+
+size_t wkv6_adamw_workspace_bytes(int64_t count) { return count > 0 && count <= 0x7fffffffLL ? wkv6::adamw_workspace_bytes(count) : 0; }
+
+int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, const wkv6_adamw_tensor *tensors,
+                    int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed,
+                    void *workspace, size_t workspace_bytes) {
+    if (moment_bits != 8 && moment_bits != 32) return WKV6_ERR_ARG;
+    const int rc = check_tensors(dtype, count, tensors, false, moment_bits);
+    if (rc != WKV6_OK) return rc;
+    if (!step || !aligned(step, 8) || !floats({lr_device, grad_norm})) return WKV6_ERR_ARG;
+    if (!(lr >= 0.) || !(beta1 >= 0. && beta1 < 1.) || !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || !(weight_decay >= 0.) || !(max_grad_norm >= 0.)) return WKV6_ERR_ARG;
+    if ((max_grad_norm > 0. || skip_nonfinite) && !grad_norm) return WKV6_ERR_ARG;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < wkv6::adamw_workspace_bytes(count)) return WKV6_ERR_WORKSPACE;
+    return finish(wkv6::adamw_step((hipStream_t)stream, dtype, moment_bits, count, reinterpret_cast<const wkv6::AdamwTensor *>(tensors),
+                                   wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed},
+                                   workspace));
 }
 
 static int check_mix(int dtype, int64_t B, int64_t T, int64_t C, int64_t R) {

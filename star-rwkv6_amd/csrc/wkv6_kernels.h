@@ -334,4 +334,74 @@ hipError_t chunk_backward(hipStream_t st, int64_t B, int64_t T, int64_t H,
 // sum over the batch of (B, C) partials -> (C), both in the output type (for the paths without a fused sum)
 hipError_t sum_over_batch(hipStream_t st, int out_dtype, int64_t B, int64_t C, const void *partials, void *sum);
 
+// --- losses over the logits of a vocabulary (wkv6_loss.hip) ---
+// Rows of V logits at b * stride_b + t * stride_t (elements; any alignment of an element); ids (B,T), mask (B,T) or null.
+struct LossRows {
+    int64_t B, T, V, stride_b, stride_t;
+    const void *logits;
+    const int64_t *ids;
+    const uint8_t *mask;
+    float inv_temperature;
+    float *logps;   // (B,T) or null
+    float *stats;   // (B,T,2) top and sum of a row, or null
+    double *exact;  // (B,T) logps in 64 bits, or null
+};
+struct LossCounts {
+    int *by_text, *tokens, *texts;   // counted tokens of each text; of each counting workgroup's texts: tokens, texts that have any
+    int blocks;
+};
+enum { kLossNone = 0, kLossCrossEntropy = 1, kLossPolicy = 2 };
+enum { kLossSum = 0, kLossMean = 1, kLossMeanOfTexts = 2 };
+struct LossTerms {
+    int kind, reduction;
+    const float *old_logps, *ref_logps;   // (B,T), either may be null
+    const float *advantages;
+    int64_t adv_stride_b, adv_stride_t;
+    float clip_low, clip_high, kl_weight;
+    float *loss, *means;                  // 1 and 2 values
+    float *coef;                          // (B,T): dL/dlp, or null
+    float *terms;                         // set inside: `count` arrays (B,T) in the workspace
+    int count;
+};
+enum { kPreferenceSigmoid = 0, kPreferenceHinge = 1, kPreferenceIpo = 2 };
+struct PreferenceTerms {
+    int kind, average;
+    double beta, label_smoothing;
+    const float *ref_logps;   // (B) or null
+    float *loss, *text_logps; // 1 and (B)
+    float *coef;              // (B) or null
+};
+struct LossGrad {
+    const float *coef;
+    int64_t coef_stride_b, coef_stride_t;
+    const float *upstream;    // one value, or null for 1
+    int is_there;             // grad holds the gradient for an upstream of 1
+    void *grad;               // (B,T,V)
+};
+size_t loss_workspace_bytes(int64_t B, int64_t T);
+hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *grad, void *workspace);   // grad: (B,T,V) or null
+hipError_t loss_preference(hipStream_t st, LossRows a, PreferenceTerms l);   // reads a.exact
+hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g);     // reads a.stats
+
+// --- AdamW over many tensors (wkv6_adamw.hip) ---
+struct AdamwTensor {
+    void *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;   // fp32, or float8 under `scales`
+    float *scales, *master;
+    int64_t numel;
+};
+struct AdamwStep {
+    int64_t *step;                // on the device: steps taken, advanced by one
+    const float *lr_device;       // one value, or null for lr
+    double lr, beta1, beta2, eps, weight_decay, max_grad_norm;   // max_grad_norm 0: gradients as they are
+    int skip_nonfinite;
+    const float *grad_norm;       // one value, or null where neither of the two needs it
+    uint32_t seed;
+};
+size_t grad_norm_workspace_bytes(int64_t count);
+hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor *tensors, float *norm, void *workspace);
+size_t adamw_workspace_bytes(int64_t count);
+hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s, void *workspace);
+
 }  // namespace wkv6

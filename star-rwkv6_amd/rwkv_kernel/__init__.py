@@ -18,6 +18,9 @@ State arguments (reference doc, rwkv_kernel/__init__.py:14-38):
                 values in [0, state_kinds).  Defaults: all zeros if state_kinds == 1, arange(batch) if
                 state_kinds == batch, otherwise it must be given.
 Returns (y, final_state or None).
+
+The torch flavour also has what a training step does behind the model's last layer (torch_training.py): cross_entropy, token_logprobs,
+preference_loss, policy_loss, grad_norm, adamw_step and the optimizer AdamW.
 """
 import os
 
@@ -27,9 +30,12 @@ if os.environ["KERAS_BACKEND"] == "jax":
     from .jax_rwkv_kernel import RWKVKernelOperator
 elif os.environ["KERAS_BACKEND"] == "torch":
     from .torch_rwkv_kernel import RWKVKernelOperator
+    from .torch_training import AdamW, adamw_step, cross_entropy, grad_norm, policy_loss, preference_loss, token_logprobs
 else:
     from .ops_rwkv_kernal import RWKVKernelOperator
 
 from .ops_rwkv_kernal import RWKVKernelOperator as OPSKernelOperator
 
 __all__ = ["RWKVKernelOperator", "OPSKernelOperator"]
+if os.environ["KERAS_BACKEND"] == "torch":
+    __all__ += ["AdamW", "adamw_step", "cross_entropy", "grad_norm", "policy_loss", "preference_loss", "token_logprobs"]

@@ -16,7 +16,7 @@ BF16, F16, F32 = 0, 1, 2
 ALGO_AUTO, ALGO_SCAN, ALGO_CHUNK = 0, 1, 2
 STATIC_SCRATCH_BYTES = 64 << 20   # WKV6_STATIC_SCRATCH_BYTES
 
-_i64, _int, _p, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
+_i64, _int, _p, _sz, _f, _d = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes); one entry per symbol include/wkv6.h declares
 SIGNATURES = {
@@ -59,6 +59,16 @@ SIGNATURES = {
     "wkv6_forward_save": (_int, [_p, _int, _int] + [_i64] * 4 + [_p] * 6 + [_p, _sz]),
     "wkv6_backward_saved": (_int, [_p, _int, _int] + [_i64] * 4 + [_p] * 11 + [_p, _sz]),
     "wkv6_backward_saved_sum": (_int, [_p, _int, _int] + [_i64] * 4 + [_p] * 12 + [_p, _sz]),
+    "wkv6_token_logprobs": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 2 + [_f] + [_p] * 2),
+    "wkv6_loss_workspace_bytes": (_sz, [_i64] * 2),
+    "wkv6_cross_entropy": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 2 + [_int] + [_p] * 4 + [_p, _sz]),
+    "wkv6_policy_loss": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 4 + [_i64] * 2 + [_p] + [_f] * 4 + [_int] + [_p] * 6 + [_p, _sz]),
+    "wkv6_preference_loss": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 3 + [_int, _d, _d, _int] + [_p] * 5 + [_sz]),
+    "wkv6_logits_backward": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 2 + [_f] + [_p] * 2 + [_i64] * 2 + [_p, _int, _p]),
+    "wkv6_adamw_workspace_bytes": (_sz, [_i64]),
+    "wkv6_adamw_step": (_int, [_p, _int, _int, _i64, _p, _p, _p] + [_d] * 6 + [_int, _p, ctypes.c_uint32, _p, _sz]),
+    "wkv6_grad_norm_workspace_bytes": (_sz, [_i64]),
+    "wkv6_grad_norm": (_int, [_p, _int, _i64, _p, _p, _p, _sz]),
     "wkv6_create_descriptor": (_sz, [_int] * 7 + [_p]),
     "wkv_forward": (None, [_p, ctypes.POINTER(_p), ctypes.c_char_p, _sz]),
     "wkv_backward": (None, [_p, ctypes.POINTER(_p), ctypes.c_char_p, _sz]),
@@ -68,6 +78,12 @@ SIGNATURES = {
     "wkv6_last_status": (_int, []),
     "wkv6_last_hip_error": (_int, []),
 }
+
+
+class AdamwTensor(ctypes.Structure):
+    """wkv6_adamw_tensor"""
+    _fields_ = [(name, _p) for name in ("param", "grad", "exp_avg", "exp_avg_sq", "scales", "master")] + [("numel", _i64)]
+
 
 _lib = None
 _torch = None

@@ -1,0 +1,431 @@
+"""The losses over logits (token_logprobs, cross_entropy, preference_loss, policy_loss) against their formulas in float64 on the
+same rounded logits, with torch's autograd for the gradients.
+
+Tolerances, u = 2^-24.  The kernels keep a row's largest logit and the sum of exp((x - top) / temperature) in fp32.  With R the largest
+|x - top| / temperature of the row, an exponent is formed with two roundings (2 R u, as a relative error of its exp), exp itself
+has one unit in the last place (2 u), and a sum of V values of which one thread adds at most V / 256 + 8 has at most as many
+roundings (u each): E = u (2 R + V / 256 + 12), relative, for the sum, and as an absolute error for log(sum).  lp then is one product
+and a difference in 64 bits: |lp| u more where it is stored.  p = exp / sum is off by 2 E p; a gradient c (1[id] - p) by |c| (2 E p + 2 u),
+and by what c is off; then it is rounded once to its own type (half its eps, and half the smallest subnormal number)."""
+import math
+
+import pytest
+import torch
+
+import rwkv_kernel
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+SMALLEST = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
+# vocabularies on either side of what a vector, a wave, a workgroup and the kernels' size classes hold
+VOCABULARIES = [1, 2, 7, 8, 9, 63, 64, 255, 1000, 2047, 2048, 2049, 4100, 8191, 16384, 16392, 32768, 50277, 65536, 65537, 131073, 151936, 170001]
+
+
+def _case(B, T, V, dtype, seed, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, T, V, generator=g) * std
+    ids = torch.randint(0, V, (B, T), generator=g)
+    x.scatter_add_(2, ids[..., None], torch.full((B, T, 1), 4.0))
+    return x.to(dtype).cuda(), ids.cuda(), (torch.rand(B, T, generator=g) < 0.7).cuda(), g
+
+
+def _lp64(x, ids, mask, temperature=1.0):
+    """lp in float64 on the CPU with a graph to the leaf it returns, and E of each row."""
+    leaf = x.detach().cpu().double().requires_grad_(True)
+    counted = torch.ones_like(ids.cpu(), dtype=torch.bool) if mask is None else mask.cpu() != 0
+    counted = counted & (ids.cpu() >= 0)
+    z = torch.where(counted[..., None], leaf, torch.zeros((), dtype=torch.float64)) / temperature
+    lse = torch.logsumexp(z, -1)
+    lp = z.gather(-1, ids.cpu().clamp(min=0)[..., None])[..., 0] - lse
+    lp = torch.where(counted, lp, torch.zeros_like(lp))
+    finite = torch.where(torch.isfinite(z), z, z.amax(-1, keepdim=True)).detach()
+    R = (finite.amax(-1) - finite.amin(-1))
+    E = U * (2 * R + x.shape[-1] / 256 + 12)
+    return leaf, lp, counted, E, torch.exp(z - lse[..., None]).detach()
+
+
+def _within(name, got, want, tol):
+    got, want = got.detach().cpu().double(), want.detach()
+    assert got.shape == want.shape, name
+    off = (got - want).abs() - tol
+    assert bool((off <= 0).all()) and bool(torch.isfinite(got).all()), "%s: %.3e beyond its tolerance" % (name, float(off.max()))
+
+
+def _grad_within(name, got, want, p, c, c_off, E, dtype, temperature=1.0):
+    """c, c_off (B,T): the coefficient of each row and how far it may be off."""
+    c, c_off = c.abs()[..., None] / temperature, c_off[..., None] / temperature
+    tol = c * (2 * E[..., None] * p + 3 * U) + c_off
+    tol = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol) + SMALLEST[dtype]
+    assert got.dtype == dtype, name
+    _within(name, got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", VOCABULARIES)
+def test_token_logprobs(V, dtype):
+    print("token_logprobs", V, dtype, flush=True)
+    B, T, tau = 2, 3, 0.7
+    x, ids, mask, g = _case(B, T, V, dtype, V)
+    mask[0, 0], mask[1, 2] = True, False
+    x[1, 2] = float("nan")                       # a row that does not count is not looked at
+    gout = torch.randn(B, T, generator=g)
+    leaf, lp, counted, E, p = _lp64(x, ids, mask, tau)
+    with torch.no_grad():
+        alone = rwkv_kernel.token_logprobs(x, ids, mask, temperature=tau)
+    xr = x.clone().requires_grad_(True)
+    got = rwkv_kernel.token_logprobs(xr, ids, mask, temperature=tau)
+    assert torch.equal(alone, got.detach()) and got.dtype == torch.float32
+    _within("lp", got, lp, E + 2 * U * lp.abs())
+    lp.backward(gout.double())
+    got.backward(gout.cuda())
+    c = torch.where(counted, gout.double(), torch.zeros(()).double())
+    _grad_within("grad", xr.grad, leaf.grad, p, c, 2 * U * c.abs(), E, dtype, tau)
+    assert bool((xr.grad[1, 2] == 0).all())
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,V", [(1, 1, 5), (3, 5, 1000), (2, 33, 4099), (1, 300, 257), (40, 1, 96), (2, 4, 65536), (1, 2, 151936)])
+def test_cross_entropy(B, T, V, dtype, reduction):
+    print("cross_entropy", B, T, V, dtype, flush=True)
+    x, ids, mask, _ = _case(B, T, V, dtype, B * T + V)
+    mask[0, 0] = True
+    if T > 3:
+        ids[0, 2] = -100
+    scale = 1.0 if dtype == torch.bfloat16 else 512.0
+    for up in (1.0, scale, 0.3):
+        leaf, lp, counted, E, p = _lp64(x, ids, mask)
+        n = int(counted.sum()) if reduction == "mean" else 1
+        loss = -lp.sum() / n
+        xr = x.clone().requires_grad_(True)
+        got = rwkv_kernel.cross_entropy(xr, ids, mask, reduction=reduction)
+        assert got.dtype == torch.float32 and got.shape == ()
+        with torch.no_grad():
+            assert torch.equal(got.detach(), rwkv_kernel.cross_entropy(x, ids, mask, reduction=reduction))
+        _within("loss", got, loss, ((E + 4 * U * lp.abs()) * counted).sum() / n + 2 * U * loss.abs())
+        loss.backward(torch.tensor(up).double())
+        got.backward(torch.tensor(up).cuda())
+        c = torch.where(counted, torch.tensor(float(torch.tensor(up))).double() / n, torch.zeros(()).double())
+        _grad_within("grad", xr.grad, leaf.grad, p, c, 4 * U * c, E, dtype)
+
+
+def test_flat_logits_and_texts_are_one():
+    x, ids, mask, _ = _case(3, 7, 500, torch.bfloat16, 1)
+    flat = rwkv_kernel.cross_entropy(x.view(21, 500), ids.view(21), mask.view(21))
+    assert torch.equal(flat, rwkv_kernel.cross_entropy(x, ids, mask))
+    lp = rwkv_kernel.token_logprobs(x.view(21, 500), ids.view(21))
+    assert lp.shape == (21,) and torch.equal(lp.view(3, 7), rwkv_kernel.token_logprobs(x, ids))
+
+
+def _preference(lp, counted, ref, beta, kind, smoothing, average):
+    P = lp.shape[0] // 2
+    s = lp.sum(1) / (counted.sum(1).clamp(min=1) if average else 1)
+    r = torch.zeros_like(s) if ref is None else ref.cpu().double()
+    d = s[:P] - s[P:] - (r[:P] - r[P:])
+    sig = torch.nn.functional.logsigmoid
+    each = {"sigmoid": lambda: -(1 - smoothing) * sig(beta * d) - smoothing * sig(-beta * d),
+            "hinge": lambda: torch.relu(1 - beta * d), "ipo": lambda: (d - 0.5 / beta) ** 2}[kind]()
+    return each.mean(), s, d
+
+
+@pytest.mark.parametrize("kind,smoothing,average,with_ref", [("sigmoid", 0.0, False, True), ("sigmoid", 0.1, False, False), ("sigmoid", 0.0, True, True),
+                                                             ("hinge", 0.0, False, True), ("ipo", 0.0, True, True)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("P,T,V", [(1, 1, 50), (3, 9, 1000), (20, 70, 130), (1, 3, 65536)])
+def test_preference_loss(P, T, V, dtype, kind, smoothing, average, with_ref):
+    print("preference_loss", P, T, V, dtype, kind, flush=True)
+    x, ids, mask, g = _case(2 * P, T, V, dtype, P + T + V)
+    if P > 1:
+        mask[1] = False                      # a text of which no token counts
+    beta = 0.1
+    leaf, lp, counted, E, p = _lp64(x, ids, mask)
+    # (away from the hinge's corner, where the gradient jumps)
+    ref = (lp.detach().sum(1) + torch.randn(2 * P, generator=g).double() * 3).float().cuda() if with_ref else None
+    loss, s, d = _preference(lp, counted, ref, beta, kind, smoothing, average)
+    assert kind != "hinge" or float((1 - beta * d.detach()).abs().min()) > 1e-4
+    xr = x.clone().requires_grad_(True)
+    got, got_s = rwkv_kernel.preference_loss(xr, ids, mask, ref, beta=beta, kind=kind, label_smoothing=smoothing, average=average)
+    with torch.no_grad():
+        again, _ = rwkv_kernel.preference_loss(x, ids, mask, ref, beta=beta, kind=kind, label_smoothing=smoothing, average=average)
+    assert torch.equal(got.detach(), again) and not got_s.requires_grad
+    s_off = (E * counted).sum(1) / (counted.sum(1).clamp(min=1) if average else 1)
+    _within("s", got_s, s, s_off + 2 * U * s.abs())
+    d_off = s_off[:P] + s_off[P:]
+    # dl/dd is at most beta or 2 |d - 1 / (2 beta)|, and changes by at most beta^2 / 4 or 2 times what d is off by
+    slope = 2 * (d - 0.5 / beta).abs() + 2 * d_off if kind == "ipo" else torch.full_like(d, beta)
+    _within("loss", got, loss, (slope * d_off).mean() + 2 * U * loss.abs())
+    loss.backward()
+    got.backward()
+    length = counted.sum(1).clamp(min=1).double() if average else torch.ones(2 * P).double()
+    c = (slope.detach().repeat(2) / P / length)[:, None].expand(lp.shape) * counted
+    bend = {"sigmoid": beta * beta / 4, "hinge": 0.0, "ipo": 2.0}[kind]
+    c_off = (bend * d_off.repeat(2) / P / length)[:, None] * counted + 4 * U * c
+    _grad_within("grad", xr.grad, leaf.grad, p, c, c_off, E, dtype)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "mean_of_texts"])
+@pytest.mark.parametrize("old,ref,per_token", [(True, True, False), (False, True, True), (True, False, True)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,V", [(1, 1, 30), (4, 9, 1000), (3, 65, 130), (2, 3, 65536), (300, 1, 64)])
+def test_policy_loss(B, T, V, dtype, old, ref, per_token, reduction):
+    print("policy_loss", B, T, V, dtype, old, ref, reduction, flush=True)
+    tau, lo, hi, klw = 0.8, 0.2, 0.28, 0.05
+    x, ids, mask, g = _case(B, T, V, dtype, B + T + V)
+    if B > 1:
+        mask[1] = False
+    leaf, lp, counted, E, p = _lp64(x, ids, mask, tau)
+    d = torch.randn(B, T, generator=g) * 0.2
+    near = ((d.exp() - 1 - hi).abs() < 1e-2) | ((d.exp() - 1 + lo).abs() < 1e-2)
+    d = torch.where(near, torch.zeros(()), d)    # away from the corners of the clipping
+    old_lp = (lp.detach() - d).float() if old else None
+    ref_lp = (lp.detach() + torch.randn(B, T, generator=g) * 0.3).float() if ref else None
+    A = torch.randn(*((B, T) if per_token else (B,)), generator=g)
+    junk = torch.full((B, T), float("nan"))      # what stands where no token counts is not looked at
+    give = lambda v: None if v is None else torch.where(counted, v, junk).cuda()  # noqa: E731
+    A_all = A.double() if per_token else A.double()[:, None].expand(B, T)
+    ratio = torch.exp(lp - old_lp.double()) if old else torch.exp(lp - lp.detach())
+    clipped = torch.where(A_all > 0, ratio > 1 + hi, ratio < 1 - lo)
+    each = -torch.minimum(ratio * A_all, ratio.clamp(1 - lo, 1 + hi) * A_all)
+    e = ref_lp.double() - lp if ref else torch.zeros_like(lp)
+    kl = torch.exp(e) - e - 1
+    n = counted.sum(1, keepdim=True).double()
+    w = counted / (n.clamp(min=1) * (n > 0).sum() if reduction == "mean_of_texts" else counted.sum()).clamp(min=1)
+    loss = ((each + klw * kl) * w).sum()
+    xr = x.clone().requires_grad_(True)
+    args = (ids, mask, give(old_lp), torch.where(counted, A, junk).cuda() if per_token else A.cuda())
+    kw = dict(ref_logps=give(ref_lp), clip_low=lo, clip_high=hi, kl_weight=klw, temperature=tau, reduction=reduction)
+    got, got_lp, means = rwkv_kernel.policy_loss(xr, *args, **kw)
+    with torch.no_grad():
+        again = rwkv_kernel.policy_loss(x, *args, **kw)
+    assert all(torch.equal(a, b.detach()) for a, b in zip(again, (got, got_lp, means))) and not (got_lp.requires_grad or means.requires_grad)
+    lp_off = E + 4 * U * lp.abs()
+    _within("lp", got_lp, lp, lp_off)
+    # a term changes by at most (ratio |A| + klw |1 - exp(e)|) times what lp is off by, and its own arithmetic has some ten roundings
+    rA, far = (ratio * A_all).detach().abs(), (e.exp() - 1).detach().abs()
+    off = (rA + klw * far) * lp_off * 2 + 16 * U * (rA + klw * (e.abs() + kl).detach())
+    _within("loss", got, loss, (off * w).sum() + 2 * U * loss.abs())
+    kl_off = far * lp_off * 2 + 16 * U * (e.abs() + kl).detach()
+    want = torch.stack([(kl * w).sum(), (clipped * w).sum()])
+    _within("means", means, want, torch.stack([(kl_off * w).sum(), 8 * U * (w.sum())]) + 2 * U * want.abs())
+    loss.backward()
+    got.backward()
+    c = (rA + klw * far) * w
+    c_off = (rA + klw * (1 + far)) * w * (2 * lp_off + 16 * U)
+    _grad_within("grad", xr.grad, leaf.grad, p, c, c_off, E, dtype, tau)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_with_banned_tokens_and_far_offsets(dtype):
+    """-inf logits have probability zero and no gradient; an offset of all logits changes nothing but their own rounding."""
+    x, ids, _, _ = _case(2, 4, 3001, dtype, 5)
+    x[:, :, 100:2900] = float("-inf")
+    ids[:] = 7
+    x[1] = (x[1].float() + 900.0).to(dtype)
+    leaf, lp, counted, E, p = _lp64(x, ids, None)
+    xr = x.clone().requires_grad_(True)
+    got = rwkv_kernel.cross_entropy(xr, ids)
+    loss = -lp.mean()
+    _within("loss", got, loss, (E + 4 * U * lp.abs()).mean() + 2 * U * loss.abs())
+    loss.backward()
+    got.backward()
+    c = torch.full(lp.shape, 1.0 / 8).double()
+    _grad_within("grad", xr.grad, torch.nan_to_num(leaf.grad), p, c, 4 * U * c, E, dtype)
+    assert bool((xr.grad[:, :, 100:2900] == 0).all())
+
+
+def test_the_wrong_shows():
+    """NaN or +inf in a row that counts, an id beyond the vocabulary and a row of nothing but -inf give NaN there and nowhere else; a banned
+    token that stands there gives a loss of +inf."""
+    V = 2500
+    for spoil, ids_of in ((lambda r: r.fill_(float("-inf")), 3), (lambda r: r[9:10].fill_(float("nan")), 3), (lambda r: r[V - 1:].fill_(float("inf")), 3), (lambda r: None, V + 5), (lambda r: None, 2 ** 40)):
+        x, ids, _, _ = _case(1, 3, V, torch.bfloat16, 6)
+        spoil(x[0, 1])
+        ids[0, 1] = ids_of
+        xr = x.clone().requires_grad_(True)
+        lp = rwkv_kernel.token_logprobs(xr, ids)
+        assert torch.isnan(lp).tolist() == [[False, True, False]]
+        lp.sum().backward()
+        assert bool(torch.isnan(xr.grad[0, 1]).any()) and bool(torch.isfinite(xr.grad[0, [0, 2]]).all())
+        assert bool(torch.isnan(rwkv_kernel.cross_entropy(x, ids)))
+    x, ids, _, _ = _case(1, 3, V, torch.bfloat16, 6)
+    ids[0, 1] = 8
+    x[0, 1, 8] = float("-inf")
+    assert float(rwkv_kernel.cross_entropy(x, ids)) == float("inf")
+
+
+def test_no_counted_token_is_a_loss_of_zero():
+    x, ids, mask, _ = _case(2, 3, 100, torch.bfloat16, 8)
+    x.fill_(float("nan"))
+    mask[:] = False
+    for call in (lambda v: rwkv_kernel.cross_entropy(v, ids, mask), lambda v: rwkv_kernel.policy_loss(v, ids, mask, None, torch.ones(2).cuda())[0],
+                 lambda v: rwkv_kernel.policy_loss(v, ids, mask, None, torch.ones(2).cuda(), reduction="mean_of_texts")[0]):
+        xr = x.clone().requires_grad_(True)
+        loss = call(xr)
+        loss.backward()
+        assert float(loss) == 0.0 and bool((xr.grad == 0).all())
+    xr = x.clone().requires_grad_(True)
+    loss, s = rwkv_kernel.preference_loss(xr, ids, mask) if x.shape[0] % 2 == 0 else None
+    loss.backward()
+    assert abs(float(loss) - math.log(2.0)) < 1e-6 and s.tolist() == [0.0, 0.0] and bool((xr.grad == 0).all())
+
+
+def test_no_tokens_at_all():
+    x = torch.zeros(2, 0, 50, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    ids = torch.zeros(2, 0, dtype=torch.int64, device="cuda")
+    loss = rwkv_kernel.cross_entropy(x, ids)
+    loss.backward()
+    assert float(loss) == 0.0 and x.grad.shape == x.shape and rwkv_kernel.token_logprobs(x, ids).shape == (2, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_logits(dtype):
+    """A slice of a longer sequence, rows off any alignment, a transposed batch, broadcast rows and a vocabulary that is not the last stride."""
+    g = torch.Generator().manual_seed(3)
+    whole = torch.randn(3, 8, 1031, generator=g).to(dtype).cuda()
+    ids = torch.randint(0, 900, (3, 5), generator=g).cuda()
+    views = [whole[:, 2:7, 1:1000], whole[:, 2:7, 3:1030], whole.transpose(0, 1)[:3, :, :].transpose(1, 2)[:, :1000, :].transpose(1, 2)[:, :3].repeat(1, 2, 1)[:, :5],
+             whole[:1, 2:7, :1003].expand(3, 5, 1003), whole[:, :1, :1003].expand(3, 5, 1003), whole[:, 1:6].transpose(1, 2).contiguous().transpose(1, 2)]
+    for v in views:
+        assert v.shape[:2] == (3, 5)
+        want = v.detach().contiguous().clone().requires_grad_(True)
+        rwkv_kernel.cross_entropy(want, ids).backward()
+        leaf = v.detach()
+        leaf.requires_grad_(True)
+        rwkv_kernel.cross_entropy(leaf, ids).backward()
+        assert torch.equal(leaf.grad, want.grad)
+        assert torch.equal(rwkv_kernel.token_logprobs(v, ids), rwkv_kernel.token_logprobs(v.contiguous(), ids))
+    # through autograd's own views: every element of the base gets its gradient
+    base = whole.clone().requires_grad_(True)
+    rwkv_kernel.cross_entropy(base[:, 2:7, 1:1000], ids).backward()
+    inner = whole[:, 2:7, 1:1000].clone().requires_grad_(True)
+    rwkv_kernel.cross_entropy(inner, ids).backward()
+    assert torch.equal(base.grad[:, 2:7, 1:1000], inner.grad) and float(base.grad.abs().sum()) == pytest.approx(float(inner.grad.abs().sum()), rel=1e-3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_outputs_stay_inside(dtype):
+    """Nothing is written before or behind the gradient's rows: they lie in memory whose surroundings hold a known value (the C entry)."""
+    from rwkv_kernel import _native
+    lib, code = _native.load(), {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    B, T, V, room = 2, 3, 4099, 1024
+    x, ids, mask, _ = _case(B, T, V, dtype, 9)
+    for shift in range(0, 9):
+        grad = torch.full((room + B * T * V + room,), 7.0, dtype=dtype, device="cuda")
+        at = grad[room + shift:]
+        stats, coef, loss = (torch.empty(n, device="cuda") for n in (2 * B * T, B * T, 1))
+        n = lib.wkv6_loss_workspace_bytes(B, T)
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        _native.check(lib.wkv6_cross_entropy(torch.cuda.current_stream().cuda_stream, code, B, T, V, x.data_ptr(), T * V, V, ids.data_ptr(), mask.data_ptr(), 1,
+                                             loss.data_ptr(), stats.data_ptr(), coef.data_ptr(), at.data_ptr(), ws.data_ptr(), n))
+        xr = x.clone().requires_grad_(True)
+        rwkv_kernel.cross_entropy(xr, ids, mask).backward(torch.tensor(1.0).cuda())
+        assert torch.equal(at[:B * T * V], xr.grad.view(-1))
+        assert bool((grad[:room + shift] == 7).all()) and bool((at[B * T * V:] == 7).all())
+
+
+def test_gradient_by_differences():
+    """The policy loss's gradient against central differences of the loss, fp32 logits: steps of 2^-5 in a logit, errors of third order."""
+    x, ids, mask, g = _case(2, 3, 12, torch.float32, 11, std=1.0)
+    mask[:] = True
+    lp = rwkv_kernel.token_logprobs(x, ids)
+    old, ref, A = lp - 0.05, lp + 0.1 * torch.randn(2, 3, generator=g).cuda(), torch.randn(2, generator=g).cuda()
+    f = lambda v: rwkv_kernel.policy_loss(v, ids, mask, old, A, ref_logps=ref, kl_weight=0.3)[0]  # noqa: E731
+    xr = x.clone().requires_grad_(True)
+    f(xr).backward()
+    h = 2.0 ** -5
+    for b, t, j in ((0, 0, 0), (0, 2, 5), (1, 1, 11), (1, 0, int(ids[1, 0]))):
+        up, down = x.clone(), x.clone()
+        up[b, t, j] += h
+        down[b, t, j] -= h
+        with torch.no_grad():
+            slope = (float(f(up)) - float(f(down))) / (2 * h)
+        # |f'''| <= about 4 max|A| / 6 tokens; the loss itself is off by some 2^-22
+        assert abs(slope - float(xr.grad[b, t, j])) <= 4 * 2.5 / 6 * h * h / 6 + 2.0 ** -22 / h
+
+
+def test_backward_twice_and_in_parts():
+    """A graph's second backward gives the first one's gradient anew; gradients add up; one that arrives scaled is scaled."""
+    for dtype in DTYPES:
+        x, ids, mask, _ = _case(2, 5, 700, dtype, 12)
+        xr = x.clone().requires_grad_(True)
+        loss = rwkv_kernel.cross_entropy(xr, ids, mask)
+        first, = torch.autograd.grad(loss, xr, retain_graph=True)
+        kept = first.clone()
+        first.zero_()                         # what was handed out is the caller's
+        second, = torch.autograd.grad(loss, xr, retain_graph=True)
+        assert torch.equal(second, kept)
+        half, = torch.autograd.grad(loss * 0.5, xr, retain_graph=True)
+        if dtype != torch.float16:            # (a power of two: exact but for fp16's subnormal numbers)
+            assert torch.equal(half, kept * 0.5)
+        with pytest.raises(RuntimeError):
+            xr2 = x.clone().requires_grad_(True)
+            y = xr2 * 1
+            loss = rwkv_kernel.cross_entropy(y, ids, mask)
+            y.mul_(2)
+            loss.backward()
+
+
+def test_on_another_stream_and_in_a_graph():
+    """Forward and backward captured together, replayed with other logits between eager calls, each time against the eager result."""
+    x, ids, mask, g = _case(4, 6, 3000, torch.bfloat16, 13)
+    old = rwkv_kernel.token_logprobs(x, ids).clone()
+    A = torch.randn(4, generator=g).cuda()
+    calls = [lambda v: rwkv_kernel.cross_entropy(v, ids, mask), lambda v: rwkv_kernel.policy_loss(v, ids, mask, old, A, ref_logps=old, kl_weight=0.1)[0],
+             lambda v: rwkv_kernel.preference_loss(v, ids, mask, ref_logps=old.sum(1))[0], lambda v: rwkv_kernel.token_logprobs(v, ids, mask).sum()]
+    for call in calls:
+        static = x.clone().requires_grad_(True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = torch.autograd.grad(call(static), static)[0]
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, torch.autograd.grad(call(static), static)[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = call(static)
+            grad, = torch.autograd.grad(loss, static)
+        for seed in range(4):
+            fresh = _case(4, 6, 3000, torch.bfloat16, 20 + seed)[0]
+            with torch.no_grad():
+                static.copy_(fresh)
+            graph.replay()
+            torch.cuda.synchronize()
+            v = fresh.clone().requires_grad_(True)
+            want = call(v)
+            want_grad, = torch.autograd.grad(want, v)
+            assert torch.equal(loss, want.detach()) and torch.equal(grad, want_grad), seed
+
+
+def test_many_rows_and_far_rows():
+    """More tokens than one counting workgroup, and rows beyond 2^31 elements."""
+    x, ids, mask, _ = _case(1, 70000, 24, torch.float32, 14)
+    loss = rwkv_kernel.cross_entropy(x, ids, mask)
+    _, lp, counted, E, _ = _lp64(x, ids, mask)
+    _within("loss", loss, -lp.sum() / counted.sum(), (E + 4 * U * lp.abs()).mean() * 2 + 4 * U * lp.abs().mean())
+    V, T = 65536, 33000                       # 2.16e9 elements
+    big = torch.zeros(1, T, V, dtype=torch.bfloat16, device="cuda")
+    ids = torch.full((1, T), -1, dtype=torch.int64, device="cuda")
+    last = torch.randn(V, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    big[0, T - 1] = last
+    ids[0, T - 1] = 12345
+    big.requires_grad_(True)
+    loss = rwkv_kernel.cross_entropy(big, ids)
+    loss.backward()
+    v = last.clone()[None].requires_grad_(True)
+    want = rwkv_kernel.cross_entropy(v, ids[0, T - 1:])
+    want.backward()
+    assert torch.equal(loss.detach(), want.detach()) and torch.equal(big.grad[0, T - 1], v.grad[0]) and bool((big.grad[0, T - 2] == 0).all())
+
+
+def test_results_do_not_change_from_run_to_run():
+    x, ids, mask, _ = _case(8, 50, 9000, torch.bfloat16, 15)
+    runs = []
+    for _ in range(3):
+        v = x.clone().requires_grad_(True)
+        loss, s = rwkv_kernel.preference_loss(v, ids, mask)
+        loss.backward()
+        runs.append((loss.detach(), s, v.grad))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
