@@ -21,28 +21,115 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFinish = 1024;        // threads of the one workgroup that adds up
 constexpr int kCountBlocks = 256;    // at most
+constexpr int kStream = 1024, kStreamVecs = 4;   // rows that no registers hold: threads, vectors of a thread in flight
+constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
 constexpr double kLog2e = 1.44269504088896340736;
 
 // exp(d / temperature) as a power of two.  log2(e) / temperature rounded to fp32 is off by up to 2^-24 of itself, the same way in
-// every element: lp would be off by as much times the mean of d, over a whole text hundreds of times that.  `low` is what the rounding left.
+// every element: lp would be off by as much times the mean of d, over a whole text hundreds of times that.  `low` is what the
+// rounding left; the gradient, whose elements are rounded one by one, does without.  (`high` is rounded down and `low` positive: with d = -inf
+// the two products are -inf both, and not two infinities of different signs.)
 struct Scale {
     float high, low;
     __device__ __forceinline__ explicit Scale(float inv_temperature) {
         const double s = kLog2e * inv_temperature;
         high = (float)s;
+        if ((double)high >= s) high = __uint_as_float(__float_as_uint(high) - 1);
         low = (float)(s - high);
     }
     __device__ __forceinline__ float exp(float d) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, high, d * low)); }
+    __device__ __forceinline__ float exp_once(float d) const { return __builtin_amdgcn_exp2f(d * high); }
+};
+
+// 16 bytes of a row as they sit in memory, at any element's address.
+template <typename T> struct Vec;
+template <> struct Vec<bf16_t> {
+    typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(2)));
+    static constexpr int kN = 8;
+    static constexpr uint32_t kNone = 0xFF80FF80u;   // -inf
+    static __device__ __forceinline__ void unpack(const uint32_t (&r)[4], float (&o)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[2 * i] = __uint_as_float(r[i] << 16), o[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void pack(const float (&v)[8], uint32_t (&r)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    }
+};
+template <> struct Vec<f16_t> {
+    typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    static constexpr int kN = 8;
+    static constexpr uint32_t kNone = 0xFC00FC00u;
+    static __device__ __forceinline__ void unpack(const uint32_t (&r)[4], float (&o)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const h2 h = __builtin_bit_cast(h2, r[i]);
+            o[2 * i] = (float)h[0], o[2 * i + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ void pack(const float (&v)[8], uint32_t (&r)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, (h2){to_f16(v[2 * i]), to_f16(v[2 * i + 1])});
+    }
+};
+template <> struct Vec<float> {
+    typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(4)));
+    static constexpr int kN = 4;
+    static constexpr uint32_t kNone = 0xFF800000u;
+    static __device__ __forceinline__ void unpack(const uint32_t (&r)[4], float (&o)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(r[i]);
+    }
+    static __device__ __forceinline__ void pack(const float (&v)[4], uint32_t (&r)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
+    }
+};
+template <typename T> struct Bits {
+    uint32_t r[4];
+    __device__ __forceinline__ void load(const T *p) {
+        const auto v = *reinterpret_cast<const typename Vec<T>::raw *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = v[i];
+    }
+    // Keeps the compiler from holding the unpacked values of one pass over the registers for the next, at twice the registers.
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("" : "+v"(r[i]));
+    }
+    __device__ __forceinline__ void none() { r[0] = r[1] = r[2] = r[3] = Vec<T>::kNone; }
+    __device__ __forceinline__ void zero() { r[0] = r[1] = r[2] = r[3] = 0; }
+    __device__ __forceinline__ void store(T *p) const {
+        typename Vec<T>::raw v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = r[i];
+        *reinterpret_cast<typename Vec<T>::raw *>(p) = v;
+    }
 };
 
 __device__ __forceinline__ bool counts(const LossRows &a, int64_t row, int64_t id) {
     return id >= 0 && (a.mask == nullptr || a.mask[row] != 0);
 }
 
+// A wave's folds: across neighbours within 16 lanes by DPP, then over the four rows of lanes.
+template <int kCtrl> __device__ __forceinline__ float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = fmaxf(v, moved<0xB1>(v));    // quad_perm [1,0,3,2]
+    v = fmaxf(v, moved<0x4E>(v));    // quad_perm [2,3,0,1]
+    v = fmaxf(v, moved<0x141>(v));   // row_half_mirror
+    v = fmaxf(v, moved<0x140>(v));   // row_mirror
+    return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += moved<0xB1>(v);
+    v += moved<0x4E>(v);
+    v += moved<0x141>(v);
+    v += moved<0x140>(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 template <typename S> __device__ __forceinline__ S wave_sum(S v) {
 #pragma unroll
@@ -98,6 +185,7 @@ __device__ __forceinline__ float weight_of(const LossCounts &c, int64_t b, int r
 
 // What a loss makes of one token's lp: its weighted terms, for the finishing kernel to add up, and c.
 __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l, int64_t row, double exact, float w) {
+#pragma clang fp contract(off)   // (left to itself the compiler joins other products and sums in the kernel with the gradient than in the one without)
     const int64_t rows = a.B * a.T;
     const float lp = (float)exact;
     if (l.kind == kLossCrossEntropy) {
@@ -121,42 +209,160 @@ __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l
     return by_lp * w;
 }
 
-// top, sum and lp of every row, and what the loss makes of it.
-template <typename T> __global__ __launch_bounds__(kThreads) void rows_kernel(LossRows a, LossCounts n, LossTerms l) {
-    __shared__ float part_max[kWaves], part_sum[kWaves];
+// Zeros over a row of the gradient.
+template <typename T, int kT> __device__ __forceinline__ void zero_row(T *out, int V) {
+    constexpr int kN = Vec<T>::kN;
+    const int full = V / kN;
+    Bits<T> z;
+    z.zero();
+    for (int j = threadIdx.x; j < full; j += kT) z.store(out + (int64_t)j * kN);
+    if ((int)threadIdx.x < V - full * kN) store1(out + full * kN + threadIdx.x, 0.f);
+}
+
+// c / temperature (1[j = id] - p_j) for one vector of a row, from its logits.
+template <typename T> __device__ __forceinline__ void gradient(Bits<T> &b, const Scale &scale, float top, float minus_c_norm) {
+    float v[Vec<T>::kN];
+    Vec<T>::unpack(b.r, v);
+#pragma unroll
+    for (int e = 0; e < Vec<T>::kN; ++e) v[e] = scale.exp_once(v[e] - top) * minus_c_norm;
+    Vec<T>::pack(v, b.r);
+}
+template <typename T> __device__ __forceinline__ float gradient(float x, const Scale &scale, float top, float minus_c_norm) {
+    return scale.exp_once(x - top) * minus_c_norm;
+}
+
+// top, sum and lp of every row, and what the loss makes of it; with kGrad the gradient by the row too, while its logits are at hand.
+// A workgroup takes a row.  kVecs > 0: the row is read once, into registers (kVecs vectors of 16 bytes to a thread); the up to 7 elements
+// behind the last whole vector are one more element each to the first threads.  kVecs = 0: rows of any length, a running maximum and sum
+// to a thread, and a second reading for the gradient.
+template <typename T, int kT, int kVecs, bool kGrad>
+__global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_kernel(LossRows a, LossCounts n, LossTerms l, T *__restrict__ grad) {
+    constexpr int kN = Vec<T>::kN, kW = kT / 64, kHeld = kVecs > 0 ? kVecs : kStreamVecs;
+    __shared__ float part_max[kW], part_sum[kW], part_c;
     const int64_t row = blockIdx.x, b = row / a.T;
     const int64_t id = a.ids[row];
+    const int V = (int)a.V, full = V / kN, tid = threadIdx.x;
+    T *out = kGrad ? grad + row * V : nullptr;
     if (!counts(a, row, id)) {
-        if (threadIdx.x == 0) {
+        if (tid == 0) {
             if (a.logps) a.logps[row] = 0.f;
             if (a.exact) a.exact[row] = 0.;
             if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = 1.f;
             if (l.coef) l.coef[row] = 0.f;
             for (int i = 0; i < l.count; ++i) l.terms[i * a.B * a.T + row] = 0.f;
         }
+        if (kGrad) zero_row<T, kT>(out, V);
         return;
     }
     const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + row % a.T * a.stride_t;
-    float top = -INFINITY;
-    for (int64_t j = threadIdx.x; j < a.V; j += kThreads) top = fmaxf(top, load1(x + j));
-    top = block_max<kWaves>(top, part_max);
     const Scale scale(a.inv_temperature);
-    float sum = 0.f;
-    for (int64_t j = threadIdx.x; j < a.V; j += kThreads) sum += scale.exp(load1(x + j) - top);
-    sum = block_sum<kWaves>(sum, part_sum);
-    if (threadIdx.x < 64) {
-        const double lp = id < a.V ? (double)(load1(x + id) - top) * a.inv_temperature - log((double)sum) : NAN;
-        const float w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
-        if (threadIdx.x == 0) {
+    Bits<T> held[kHeld];
+    float rest = tid < V - full * kN ? load1(x + full * kN + tid) : -INFINITY;
+    float top, sum;
+    if (kVecs > 0) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (i * kT + tid < full) held[i].load(x + (int64_t)(i * kT + tid) * kN);
+            else held[i].none();
+        }
+    }
+    const float w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
+    const float stands = id < V ? load1(x + id) : NAN;
+    if (kVecs > 0) {
+        top = rest;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            float v[kN];
+            Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) top = fmaxf(top, v[e]);
+        }
+        top = block_max<kW>(top, part_max);
+        sum = scale.exp(rest - top);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            float v[kN];
+            held[i].again();
+            Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) sum += scale.exp(v[e] - top);
+        }
+    } else {
+        float mine = rest;
+        sum = rest == -INFINITY ? 0.f : scale.exp(rest - rest);
+        for (int first = tid; first < full; first += kHeld * kT) {
+            float most = mine;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (first + i * kT < full) held[i].load(x + (int64_t)(first + i * kT) * kN);
+                else held[i].none();
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                float v[kN];
+                Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) most = fmaxf(most, v[e]);
+            }
+            const float from = most == -INFINITY ? 0.f : most;   // (-inf less -inf is no number)
+            sum *= scale.exp(mine - from);
+            mine = most;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                float v[kN];
+                held[i].again();
+                Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) sum += scale.exp(v[e] - from);
+            }
+        }
+        top = block_max<kW>(mine, part_max);
+        sum = sum == 0.f && top != -INFINITY ? 0.f : sum * scale.exp(mine - top);   // (a thread without elements)
+    }
+    sum = block_sum<kW>(sum, part_sum);
+    float c = id < V ? -w : NAN;   // the cross entropy's: lp does not come into it
+    if (tid < 64) {
+        const double lp = __builtin_fma((double)(stands - top), (double)a.inv_temperature, -log((double)sum));
+        if (tid == 0) {
+            if (l.kind != kLossNone) c = row_terms(a, l, row, lp, w);
             if (a.logps) a.logps[row] = (float)lp;
             if (a.exact) a.exact[row] = lp;
             if (a.stats) a.stats[2 * row] = top, a.stats[2 * row + 1] = sum;
-            if (l.kind != kLossNone) {
-                const float c = row_terms(a, l, row, lp, w);
-                if (l.coef) l.coef[row] = c;
+            if (l.coef) l.coef[row] = c;
+            part_c = c;
+        }
+    }
+    if (!kGrad) return;
+    if (l.kind != kLossCrossEntropy) {
+        __syncthreads();
+        c = part_c;
+    }
+    c *= a.inv_temperature;
+    const float norm = 1.f / sum, factor = -c * norm;
+    if (kVecs > 0) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            held[i].again();
+            gradient<T>(held[i], scale, top, factor);
+            if (i * kT + tid < full) held[i].store(out + (int64_t)(i * kT + tid) * kN);
+        }
+    } else {
+        for (int first = tid; first < full; first += kHeld * kT) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (first + i * kT < full) held[i].load(x + (int64_t)(first + i * kT) * kN);
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (first + i * kT >= full) continue;
+                gradient<T>(held[i], scale, top, factor);
+                held[i].store(out + (int64_t)(first + i * kT) * kN);
             }
         }
     }
+    if (tid < V - full * kN) store1(out + full * kN + tid, gradient<T>(rest, scale, top, factor));
+    // the element that stands there, by the thread whose store it was in
+    const int owner = id < full * (int64_t)kN ? (int)(id / kN) % kT : (int)(id - full * kN);
+    if (id < V && tid == owner) store1(out + id, c + scale.exp_once(stands - top) * factor);
 }
 
 // The sums of up to three arrays of terms.
@@ -219,25 +425,47 @@ __global__ __launch_bounds__(kFinish) void preference_kernel(LossRows a, Prefere
     if (threadIdx.x == 0) l.loss[0] = (float)(loss / (double)P);
 }
 
-template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g) {
+// The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, `pieces` workgroups to a row.
+template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces) {
+    constexpr int kN = Vec<T>::kN;
     const float up = g.upstream ? *g.upstream : 1.f;
     if (g.is_there && up == 1.f) return;
-    const int64_t row = blockIdx.x, b = row / a.T, t = row % a.T;
+    const int64_t row = blockIdx.x / pieces, b = row / a.T, t = row % a.T;
     const int64_t id = a.ids[row];
-    T *out = static_cast<T *>(g.grad) + row * a.V;
+    const int V = (int)a.V, full = V / kN, first = (int)(blockIdx.x % pieces) * (kGradVecs * kThreads) + threadIdx.x;
+    const int behind = blockIdx.x % pieces == 0 && (int)threadIdx.x < V - full * kN ? full * kN + (int)threadIdx.x : -1;
+    T *out = static_cast<T *>(g.grad) + row * V;
     if (!counts(a, row, id)) {
-        for (int64_t j = threadIdx.x; j < a.V; j += kThreads) store1(out + j, 0.f);
+        Bits<T> z;
+        z.zero();
+#pragma unroll
+        for (int i = 0; i < kGradVecs; ++i)
+            if (first + i * kThreads < full) z.store(out + (int64_t)(first + i * kThreads) * kN);
+        if (behind >= 0) store1(out + behind, 0.f);
         return;
     }
     const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + t * a.stride_t;
-    float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up * a.inv_temperature;
-    if (id >= a.V) c = NAN;
-    const float top = a.stats[2 * row], norm = 1.f / a.stats[2 * row + 1];
+    Bits<T> held[kGradVecs];
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i)
+        if (first + i * kThreads < full) held[i].load(x + (int64_t)(first + i * kThreads) * kN);
+    float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up;
+    if (id >= V) c = NAN;
+    c *= a.inv_temperature;
+    const float top = a.stats[2 * row], norm = 1.f / a.stats[2 * row + 1], factor = -c * norm;
     const Scale scale(a.inv_temperature);
-    for (int64_t j = threadIdx.x; j < a.V; j += kThreads) {
-        const float p = scale.exp(load1(x + j) - top) * norm;
-        store1(out + j, c * ((j == id ? 1.f : 0.f) - p));
+#pragma unroll
+    for (int i = 0; i < kGradVecs; ++i) {
+        if (first + i * kThreads >= full) continue;
+        gradient<T>(held[i], scale, top, factor);
+        held[i].store(out + (int64_t)(first + i * kThreads) * kN);
     }
+    if (behind >= 0) store1(out + behind, gradient<T>(load1(x + behind), scale, top, factor));
+    // the element that stands there, by the thread whose store it was in
+    if (id >= V) return;
+    const int64_t j = id / kN;
+    const bool mine = id < full * (int64_t)kN ? j % kThreads == threadIdx.x && j / (kGradVecs * kThreads) == blockIdx.x % pieces : (int)id == behind;
+    if (mine) store1(out + id, c + scale.exp_once(load1(x + id) - top) * factor);
 }
 
 template <typename F> hipError_t by_type(int dtype, F &&f) {
@@ -254,6 +482,27 @@ size_t loss_workspace_bytes(int64_t B, int64_t T) {
     return (size_t)(3 * B * T) * sizeof(float) + (size_t)(B + 2 * kCountBlocks) * sizeof(int);
 }
 
+namespace {
+
+template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRows &a, const LossCounts &n, const LossTerms &l, void *grad) {
+    const dim3 grid((unsigned)(a.B * a.T));
+    T *out = static_cast<T *>(grad);
+    const int64_t vecs = a.V / Vec<T>::kN;
+    // (the smallest class that holds a row)
+    if (vecs <= 256 * 1) hipLaunchKernelGGL((rows_kernel<T, 256, 1, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
+    else if (vecs <= 256 * 2) hipLaunchKernelGGL((rows_kernel<T, 256, 2, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
+    else if (vecs <= 256 * 4) hipLaunchKernelGGL((rows_kernel<T, 256, 4, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
+    else if (vecs <= 256 * 8) hipLaunchKernelGGL((rows_kernel<T, 256, 8, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
+    else if (vecs <= 1024 * 4) hipLaunchKernelGGL((rows_kernel<T, 1024, 4, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
+    else if (vecs <= 1024 * 8) hipLaunchKernelGGL((rows_kernel<T, 1024, 8, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
+    else if (vecs <= 1024 * 12) hipLaunchKernelGGL((rows_kernel<T, 1024, 12, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
+    else if (vecs <= 1024 * 16) hipLaunchKernelGGL((rows_kernel<T, 1024, 16, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
+    else if (vecs <= 1024 * 20) hipLaunchKernelGGL((rows_kernel<T, 1024, 20, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
+    else hipLaunchKernelGGL((rows_kernel<T, kStream, 0, kGrad>), grid, dim3(kStream), 0, st, a, n, l, out);
+}
+
+}  // namespace
+
 hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *grad, void *workspace) {
     LossCounts n{};
     const int64_t rows = a.B * a.T;
@@ -267,12 +516,12 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kThreads), 0, st, a, n);
     }
     hipError_t e = by_type(dtype, [&](auto t) {
-        hipLaunchKernelGGL((rows_kernel<decltype(t)>), dim3((unsigned)rows), dim3(kThreads), 0, st, a, n, l);
+        if (grad) launch_rows<decltype(t), true>(st, a, n, l, grad);
+        else launch_rows<decltype(t), false>(st, a, n, l, nullptr);
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
     hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(kFinish), 0, st, rows, l);
-    if (!grad) return hipGetLastError();
-    return loss_grad(st, dtype, a, LossGrad{l.coef, a.T, 1, nullptr, 0, grad});
+    return hipGetLastError();
 }
 
 hipError_t loss_preference(hipStream_t st, LossRows a, PreferenceTerms l) {
@@ -282,7 +531,9 @@ hipError_t loss_preference(hipStream_t st, LossRows a, PreferenceTerms l) {
 
 hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g) {
     return by_type(dtype, [&](auto t) {
-        hipLaunchKernelGGL((grad_kernel<decltype(t)>), dim3((unsigned)(a.B * a.T)), dim3(kThreads), 0, st, a, g);
+        using T = decltype(t);
+        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per;
+        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(a.B * a.T * pieces)), dim3(kThreads), 0, st, a, g, (int)pieces);
     });
 }
 

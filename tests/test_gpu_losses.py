@@ -234,6 +234,21 @@ def test_rows_with_banned_tokens_and_far_offsets(dtype):
     assert bool((xr.grad[:, :, 100:2900] == 0).all())
 
 
+@pytest.mark.parametrize("temperature", [0.5, 0.7, 0.8, 1.0, 1.1, 1.3, 2.0, 3.3, 1.0 / 1.44269504])
+def test_banned_tokens_at_any_temperature(temperature):
+    x, ids, _, _ = _case(1, 2, 300, torch.float32, 16)
+    x[:, :, 40:290] = float("-inf")
+    ids[:] = 3
+    leaf, lp, counted, E, p = _lp64(x, ids, None, float(torch.tensor(temperature)))
+    xr = x.clone().requires_grad_(True)
+    got = rwkv_kernel.token_logprobs(xr, ids, temperature=temperature)
+    _within("lp", got, lp, E + 4 * U * lp.abs())
+    lp.sum().backward()
+    got.sum().backward()
+    c = torch.ones(lp.shape).double()
+    _grad_within("grad", xr.grad, torch.nan_to_num(leaf.grad), p, c, 4 * U * c / temperature, E, torch.float32, temperature)
+
+
 def test_the_wrong_shows():
     """NaN or +inf in a row that counts, an id beyond the vocabulary and a row of nothing but -inf give NaN there and nowhere else; a banned
     token that stands there gives a loss of +inf."""
