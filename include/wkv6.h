@@ -372,7 +372,7 @@ int wkv6_backward_with_state(void *stream, int dtype, int algo, int64_t B, int64
  *   stats (B,T,2)  what wkv6_logits_backward needs of each row
  *   coef           dL/dlogp: (B,T), of wkv6_preference_loss (B)
  * stats, coef and grad may be NULL where no gradient is wanted.  grad (B,T,V), contiguous, of `dtype`: the forward call writes
- * the gradient of the loss too, for an arriving gradient of 1, in the pass over the logits that it makes anyway.
+ * the gradient of the loss too, for an arriving gradient of 1, while the logits are at hand.
  * No address needs more than its element's alignment here; workspace: 16 bytes. */
 enum { WKV6_REDUCE_SUM = 0, WKV6_REDUCE_MEAN = 1, WKV6_REDUCE_MEAN_OF_TEXTS = 2 };
 enum { WKV6_PREFERENCE_SIGMOID = 0, WKV6_PREFERENCE_HINGE = 1, WKV6_PREFERENCE_IPO = 2 };
@@ -409,7 +409,7 @@ int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
 int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
                          const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
                          const float *ref_logps, int kind, double beta, double label_smoothing, int average,
-                         float *loss, float *text_logps, float *stats, float *coef,
+                         float *loss, float *text_logps, float *stats, float *coef, void *grad,
                          void *workspace, size_t workspace_bytes);
 
 /* grad = upstream * dL/dlogits from stats and coef[b * coef_stride_b + t * coef_stride_t]; upstream: one value on the device, or

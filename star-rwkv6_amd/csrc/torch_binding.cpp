@@ -434,7 +434,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
     const Tensor ws = bytes(x, n);
     check(wkv6_policy_loss(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(), in_f(given(old_logps)),
-                           in_f(advantages), advantages.stride(0), advantages.stride(1), in_f(given(ref_logps)), static_cast<float>(clip_low),
+                           in_f(advantages), advantages.stride(0), advantages.dim() == 2 ? advantages.stride(1) : 0, in_f(given(ref_logps)), static_cast<float>(clip_low),
                            static_cast<float>(clip_high), static_cast<float>(kl_weight), static_cast<float>(temperature),
                            static_cast<int>(reduction), out_f(loss), out_f(lp), out_f(means), out_f(stats), out_f(coef), out(grad), out(ws), n));
     keep_rows(ctx, l, stats, coef, temperature);
@@ -461,12 +461,15 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const c10::DeviceGuard guard(x.device());
     const Logits l = logits_of(x, ids, mask);
     const Tensor loss = fp32(x, {}), text = fp32(x, {l.B});
+    const Tensor grad = gradient_ahead(l, wanted);
     const Tensor stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor(), coef = wanted ? fp32(x, {l.B}) : Tensor();
     const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
     const Tensor ws = bytes(x, n);
     check(wkv6_preference_loss(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(), in_f(given(ref_logps)),
-                               static_cast<int>(kind), beta, label_smoothing, average, out_f(loss), out_f(text), out_f(stats), out_f(coef), out(ws), n));
+                               static_cast<int>(kind), beta, label_smoothing, average, out_f(loss), out_f(text), out_f(stats), out_f(coef),
+                               out(grad), out(ws), n));
     keep_rows(ctx, l, stats, coef, 1.0);
+    keep(ctx, grad, "grad");
     ctx->mark_non_differentiable({text});
     ctx->set_materialize_grads(false);
     return {loss, text};
@@ -477,7 +480,8 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     if (!grads[0].defined()) return res;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
-    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor());
+    const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad");
+    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), ahead);
     return res;
   }
 };

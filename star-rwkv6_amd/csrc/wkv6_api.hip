@@ -323,7 +323,7 @@ static int check_rows(int dtype, int64_t B, int64_t T, int64_t V, const void *lo
 }
 static wkv6::LossRows rows_of(int64_t B, int64_t T, int64_t V, const void *logits, int64_t stride_b, int64_t stride_t,
                               const int64_t *ids, const uint8_t *mask, float temperature, float *logps, float *stats) {
-    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr};
+    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr, 0, B, 0};
 }
 static bool floats(std::initializer_list<const void *> ps) {
     for (const void *p : ps)
@@ -390,19 +390,19 @@ int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
 int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
                          const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
                          const float *ref_logps, int kind, double beta, double label_smoothing, int average,
-                         float *loss, float *text_logps, float *stats, float *coef, void *workspace, size_t workspace_bytes) {
+                         float *loss, float *text_logps, float *stats, float *coef, void *grad, void *workspace, size_t workspace_bytes) {
     int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, 1.f);
     if (rc != WKV6_OK) return rc;
     if (B % 2 != 0 || !loss || !text_logps || !floats({ref_logps, loss, text_logps, stats, coef})) return WKV6_ERR_ARG;
+    if (!aligned(grad, element_size(dtype)) || (grad && (!stats || !coef))) return WKV6_ERR_ARG;
     if (kind < WKV6_PREFERENCE_SIGMOID || kind > WKV6_PREFERENCE_IPO || !(beta > 0.) || !(label_smoothing >= 0. && label_smoothing < 0.5)) return WKV6_ERR_ARG;
     if (kind != WKV6_PREFERENCE_SIGMOID && label_smoothing != 0.) return WKV6_ERR_ARG;
     rc = check_loss_workspace(B, T, workspace, workspace_bytes);
     if (rc != WKV6_OK) return rc;
     wkv6::LossRows a = rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, 1.f, nullptr, stats);
     a.exact = static_cast<double *>(workspace);
-    const int run = finish(wkv6::loss_rows((hipStream_t)stream, dtype, a, wkv6::LossTerms{}, nullptr, nullptr));
-    if (run != WKV6_OK) return run;
-    return finish(wkv6::loss_preference((hipStream_t)stream, a, wkv6::PreferenceTerms{kind, average, beta, label_smoothing, ref_logps, loss, text_logps, coef}));
+    return finish(wkv6::loss_preference((hipStream_t)stream, dtype, a,
+                                        wkv6::PreferenceTerms{kind, average, beta, label_smoothing, ref_logps, loss, text_logps, coef, nullptr}, grad));
 }
 
 int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t V,

@@ -336,6 +336,7 @@ hipError_t sum_over_batch(hipStream_t st, int out_dtype, int64_t B, int64_t C, c
 
 // --- losses over the logits of a vocabulary (wkv6_loss.hip) ---
 // Rows of V logits at b * stride_b + t * stride_t (elements; any alignment of an element); ids (B,T), mask (B,T) or null.
+// A launch takes texts [first, first + part) and, with jump > 0, as many from first + jump on.
 struct LossRows {
     int64_t B, T, V, stride_b, stride_t;
     const void *logits;
@@ -345,6 +346,7 @@ struct LossRows {
     float *logps;   // (B,T) or null
     float *stats;   // (B,T,2) top and sum of a row, or null
     double *exact;  // (B,T) logps in 64 bits, or null
+    int64_t first, part, jump;
 };
 struct LossCounts {
     int *by_text, *tokens, *texts;   // counted tokens of each text; of each counting workgroup's texts: tokens, texts that have any
@@ -370,6 +372,7 @@ struct PreferenceTerms {
     const float *ref_logps;   // (B) or null
     float *loss, *text_logps; // 1 and (B)
     float *coef;              // (B) or null
+    double *by_pair;          // (B / 2)
 };
 struct LossGrad {
     const float *coef;
@@ -380,7 +383,7 @@ struct LossGrad {
 };
 size_t loss_workspace_bytes(int64_t B, int64_t T);
 hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *grad, void *workspace);   // grad: (B,T,V) or null
-hipError_t loss_preference(hipStream_t st, LossRows a, PreferenceTerms l);   // reads a.exact
+hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l, void *grad);   // with a.exact; grad as above
 hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g);     // reads a.stats
 
 // --- AdamW over many tensors (wkv6_adamw.hip) ---

@@ -23,6 +23,7 @@ constexpr int kFinish = 1024;        // threads of the one workgroup that adds u
 constexpr int kCountBlocks = 256;    // at most
 constexpr int kStream = 1024, kStreamVecs = 4;   // rows that no registers hold: threads, vectors of a thread in flight
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
+constexpr int64_t kPairBytes = 128 << 20;   // logits of the pairs whose gradient is formed before the next pairs' logits are read
 constexpr double kLog2e = 1.44269504088896340736;
 
 // exp(d / temperature) as a power of two.  log2(e) / temperature rounded to fp32 is off by up to 2^-24 of itself, the same way in
@@ -108,6 +109,11 @@ template <typename T> struct Bits {
     }
 };
 
+// The row that a launch's index stands for.
+__device__ __forceinline__ int64_t row_of(const LossRows &a, int64_t index) {
+    return a.first * a.T + index + (a.jump > 0 && index >= a.part * a.T ? (a.jump - a.part) * a.T : 0);
+}
+
 __device__ __forceinline__ bool counts(const LossRows &a, int64_t row, int64_t id) {
     return id >= 0 && (a.mask == nullptr || a.mask[row] != 0);
 }
@@ -156,15 +162,29 @@ template <int kW, typename S> __device__ __forceinline__ S block_sum(S v, S *par
     return v;
 }
 
-// Counted tokens of each text, and of each workgroup's texts together: tokens, and texts that have any.
-__global__ __launch_bounds__(kThreads) void count_kernel(LossRows a, LossCounts c) {
-    __shared__ int part[2][kWaves];
+// Counted tokens of each text, and of each workgroup's texts together: tokens, and texts that have any.  (One token after the other
+// to a thread would wait for two loads each: four go together, 6 us for 8 texts of 1024 tokens before, 3 now.)
+__global__ __launch_bounds__(kFinish) void count_kernel(LossRows a, LossCounts c) {
+    __shared__ int part[2][kFinish / 64];
     int64_t tokens = 0, texts = 0;
     int turn = 0;
     for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x, turn ^= 1) {
+        const int64_t *ids = a.ids + b * a.T;
+        const uint8_t *mask = a.mask ? a.mask + b * a.T : nullptr;
         int n = 0;
-        for (int64_t t = threadIdx.x; t < a.T; t += kThreads) n += counts(a, b * a.T + t, a.ids[b * a.T + t]);
-        n = block_sum<kWaves>(n, part[turn]);
+        for (int64_t t = threadIdx.x; t < a.T; t += 4 * kFinish) {
+            int64_t id[4];
+            uint8_t m[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = t + i * kFinish < a.T;
+                id[i] = in ? ids[t + i * kFinish] : -1;
+                m[i] = in && mask ? mask[t + i * kFinish] : 1;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += id[i] >= 0 && m[i] != 0;
+        }
+        n = block_sum<kFinish / 64>(n, part[turn]);
         if (threadIdx.x == 0) c.by_text[b] = n;
         tokens += n;
         texts += n > 0;
@@ -239,7 +259,7 @@ template <typename T, int kT, int kVecs, bool kGrad>
 __global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_kernel(LossRows a, LossCounts n, LossTerms l, T *__restrict__ grad) {
     constexpr int kN = Vec<T>::kN, kW = kT / 64, kHeld = kVecs > 0 ? kVecs : kStreamVecs;
     __shared__ float part_max[kW], part_sum[kW], part_c;
-    const int64_t row = blockIdx.x, b = row / a.T;
+    const int64_t row = row_of(a, blockIdx.x), b = row / a.T;
     const int64_t id = a.ids[row];
     const int V = (int)a.V, full = V / kN, tid = threadIdx.x;
     T *out = kGrad ? grad + row * V : nullptr;
@@ -365,75 +385,88 @@ __global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_ker
     if (id < V && tid == owner) store1(out + id, c + scale.exp_once(stands - top) * factor);
 }
 
+// v[first], v[first + stride], .. below `end`, added up in 64 bits, eight loads on their way at a time.
+template <typename S> __device__ __forceinline__ double strided_sum(const S *v, int64_t first, int64_t end, int stride) {
+    double s = 0.;
+    for (int64_t r = first; r < end; r += 8 * stride) {
+        S x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = r + i * stride < end ? v[r + i * stride] : S(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += (double)x[i];
+    }
+    return s;
+}
+
 // The sums of up to three arrays of terms.
 __global__ __launch_bounds__(kFinish) void finish_kernel(int64_t rows, LossTerms l) {
-    __shared__ double part[3][kFinish / 64];
-    for (int i = 0; i < l.count; ++i) {
-        double s = 0.;
-        for (int64_t r = threadIdx.x; r < rows; r += kFinish) s += l.terms[i * rows + r];
-        s = block_sum<kFinish / 64>(s, part[i]);
-        if (threadIdx.x == 0) (i == 0 ? l.loss[0] : l.means[i - 1]) = (float)s;
-    }
-}
-
-// Pairs of texts (b and b + P), a wave each: log probabilities of whole texts in 64 bits (sums over thousands of tokens, of
-// which a small difference is wanted), the loss of their difference, and c of either text's tokens.
-__global__ __launch_bounds__(kFinish) void preference_kernel(LossRows a, PreferenceTerms l) {
     __shared__ double part[kFinish / 64];
-    const int lane = threadIdx.x & 63;
-    const int64_t P = a.B / 2;
-    double loss = 0.;
-    for (int64_t b = threadIdx.x >> 6; b < P; b += kFinish / 64) {
-        double s[2], len[2];
-        for (int i = 0; i < 2; ++i) {
-            const int64_t first = (b + i * P) * a.T;
-            double v = 0.;
-            int64_t n = 0;
-            for (int64_t t = lane; t < a.T; t += 64) {
-                v += a.exact[first + t];
-                n += counts(a, first + t, a.ids[first + t]);
-            }
-            n = wave_sum(n);
-            len[i] = l.average && n > 0 ? 1. / (double)n : 1.;
-            s[i] = wave_sum(v) * len[i];
-            if (lane == 0) l.text_logps[b + i * P] = (float)s[i];
-        }
-        double d = s[0] - s[1], by_d;
-        if (l.ref_logps) d -= (double)l.ref_logps[b] - (double)l.ref_logps[b + P];
-        if (l.kind == kPreferenceSigmoid) {
-            const double z = l.beta * d, soft = log1p(exp(-fabs(z))), up = 1. / (1. + exp(-z));
-            // (1 - e) softplus(-z) + e softplus(z)
-            loss += soft + (1. - l.label_smoothing) * fmax(-z, 0.);
-            if (l.label_smoothing > 0.) loss += l.label_smoothing * fmax(z, 0.);
-            by_d = l.beta * (up - (1. - l.label_smoothing));
-        } else if (l.kind == kPreferenceHinge) {
-            const double z = 1. - l.beta * d;
-            loss += z <= 0. ? 0. : z;
-            by_d = z <= 0. ? 0. : -l.beta + 0. * z;
-        } else {
-            const double z = d - 0.5 / l.beta;
-            loss += z * z;
-            by_d = 2. * z;
-        }
-        if (lane == 0 && l.coef) {
-            l.coef[b] = (float)(by_d * len[0] / (double)P);
-            l.coef[b + P] = (float)(-by_d * len[1] / (double)P);
-        }
-    }
-    if (lane != 0) loss = 0.;
-    loss = block_sum<kFinish / 64>(loss, part);
-    if (threadIdx.x == 0) l.loss[0] = (float)(loss / (double)P);
+    const int i = blockIdx.x;
+    const double s = block_sum<kFinish / 64>(strided_sum(l.terms + i * rows, threadIdx.x, rows, kFinish), part);
+    if (threadIdx.x == 0) (i == 0 ? l.loss[0] : l.means[i - 1]) = (float)s;
 }
 
-// The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, `pieces` workgroups to a row.
-template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces) {
+// Pairs of texts (b and b + P), a workgroup each: log probabilities of whole texts in 64 bits (sums over thousands of tokens, of
+// which a small difference is wanted), the loss of their difference, and c of either text's tokens.
+__global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTerms l) {
+    __shared__ double part[2][kFinish / 64];
+    __shared__ int count[2][kFinish / 64];
+    const int half = kFinish / 2, i = threadIdx.x / half;   // the first half of the threads takes the chosen text
+    const int64_t P = a.B / 2, pair = a.first + blockIdx.x, b = pair + i * P, first = b * a.T;
+    double v = wave_sum(strided_sum(a.exact + first, threadIdx.x % half, a.T, half));
+    int n = 0;
+    if (l.average)
+        for (int64_t t = threadIdx.x % half; t < a.T; t += half) n += counts(a, first + t, a.ids[first + t]);
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) part[i][threadIdx.x % half / 64] = v, count[i][threadIdx.x % half / 64] = n;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    double s[2], len[2];
+    for (int k = 0; k < 2; ++k) {
+        v = 0., n = 0;
+        for (int w = 0; w < half / 64; ++w) v += part[k][w], n += count[k][w];
+        len[k] = n > 0 ? 1. / n : 1.;
+        s[k] = v * len[k];
+        l.text_logps[pair + k * P] = (float)s[k];
+    }
+    double d = s[0] - s[1], by_d, loss;
+    if (l.ref_logps) d -= (double)l.ref_logps[pair] - (double)l.ref_logps[pair + P];
+    if (l.kind == kPreferenceSigmoid) {
+        const double z = l.beta * d, soft = log1p(exp(-fabs(z))), up = 1. / (1. + exp(-z));
+        // (1 - e) softplus(-z) + e softplus(z)
+        loss = soft + (1. - l.label_smoothing) * fmax(-z, 0.);
+        if (l.label_smoothing > 0.) loss += l.label_smoothing * fmax(z, 0.);
+        by_d = l.beta * (up - (1. - l.label_smoothing));
+    } else if (l.kind == kPreferenceHinge) {
+        const double z = 1. - l.beta * d;
+        loss = z <= 0. ? 0. : z;
+        by_d = z <= 0. ? 0. : -l.beta + 0. * z;
+    } else {
+        const double z = d - 0.5 / l.beta;
+        loss = z * z;
+        by_d = 2. * z;
+    }
+    l.by_pair[pair] = loss / (double)P;
+    if (l.coef) {
+        l.coef[pair] = (float)(by_d * len[0] / (double)P);
+        l.coef[pair + P] = (float)(-by_d * len[1] / (double)P);
+    }
+}
+
+__global__ __launch_bounds__(kFinish) void pairs_finish_kernel(int64_t P, PreferenceTerms l) {
+    __shared__ double part[kFinish / 64];
+    const double s = block_sum<kFinish / 64>(strided_sum(l.by_pair, threadIdx.x, P, kFinish), part);
+    if (threadIdx.x == 0) l.loss[0] = (float)s;
+}
+
+// The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, `pieces` workgroups to a row.  The last
+// rows come first: those are the ones that a pass over all rows before this one may have left in the last-level cache.
+template <typename T> __device__ __forceinline__ void grad_piece(const LossRows &a, const LossGrad &g, float up, int64_t row, int piece) {
     constexpr int kN = Vec<T>::kN;
-    const float up = g.upstream ? *g.upstream : 1.f;
-    if (g.is_there && up == 1.f) return;
-    const int64_t row = blockIdx.x / pieces, b = row / a.T, t = row % a.T;
+    const int64_t b = row / a.T, t = row % a.T;
     const int64_t id = a.ids[row];
-    const int V = (int)a.V, full = V / kN, first = (int)(blockIdx.x % pieces) * (kGradVecs * kThreads) + threadIdx.x;
-    const int behind = blockIdx.x % pieces == 0 && (int)threadIdx.x < V - full * kN ? full * kN + (int)threadIdx.x : -1;
+    const int V = (int)a.V, full = V / kN, first = piece * (kGradVecs * kThreads) + threadIdx.x;
+    const int behind = piece == 0 && (int)threadIdx.x < V - full * kN ? full * kN + (int)threadIdx.x : -1;
     T *out = static_cast<T *>(g.grad) + row * V;
     if (!counts(a, row, id)) {
         Bits<T> z;
@@ -464,8 +497,14 @@ template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(Lo
     // the element that stands there, by the thread whose store it was in
     if (id >= V) return;
     const int64_t j = id / kN;
-    const bool mine = id < full * (int64_t)kN ? j % kThreads == threadIdx.x && j / (kGradVecs * kThreads) == blockIdx.x % pieces : (int)id == behind;
+    const bool mine = id < full * (int64_t)kN ? j % kThreads == threadIdx.x && j / (kGradVecs * kThreads) == piece : (int)id == behind;
     if (mine) store1(out + id, c + scale.exp_once(load1(x + id) - top) * factor);
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces, int64_t rows) {
+    const float up = g.upstream ? *g.upstream : 1.f;
+    if (g.is_there && up == 1.f) return;
+    for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x) grad_piece<T>(a, g, up, row_of(a, rows - 1 - i / pieces), (int)(i % pieces));
 }
 
 template <typename F> hipError_t by_type(int dtype, F &&f) {
@@ -477,15 +516,17 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
 
 }  // namespace
 
-// three terms for each token and the counts, or lp in 64 bits
+// three terms for each token and the counts, or lp in 64 bits and a loss for each pair
 size_t loss_workspace_bytes(int64_t B, int64_t T) {
     return (size_t)(3 * B * T) * sizeof(float) + (size_t)(B + 2 * kCountBlocks) * sizeof(int);
 }
 
 namespace {
 
+int64_t rows_in(const LossRows &a) { return (a.jump > 0 ? 2 : 1) * a.part * a.T; }
+
 template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRows &a, const LossCounts &n, const LossTerms &l, void *grad) {
-    const dim3 grid((unsigned)(a.B * a.T));
+    const dim3 grid((unsigned)rows_in(a));
     T *out = static_cast<T *>(grad);
     const int64_t vecs = a.V / Vec<T>::kN;
     // (the smallest class that holds a row)
@@ -513,28 +554,44 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         n.tokens = n.by_text + a.B;
         n.texts = n.tokens + kCountBlocks;
         n.blocks = (int)(a.B < kCountBlocks ? a.B : kCountBlocks);
-        hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kThreads), 0, st, a, n);
+        hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n);
     }
     hipError_t e = by_type(dtype, [&](auto t) {
         if (grad) launch_rows<decltype(t), true>(st, a, n, l, grad);
         else launch_rows<decltype(t), false>(st, a, n, l, nullptr);
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
-    hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(kFinish), 0, st, rows, l);
-    return hipGetLastError();
-}
-
-hipError_t loss_preference(hipStream_t st, LossRows a, PreferenceTerms l) {
-    hipLaunchKernelGGL(preference_kernel, dim3(1), dim3(kFinish), 0, st, a, l);
+    hipLaunchKernelGGL(finish_kernel, dim3(l.count), dim3(kFinish), 0, st, rows, l);
     return hipGetLastError();
 }
 
 hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g) {
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per;
-        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(a.B * a.T * pieces)), dim3(kThreads), 0, st, a, g, (int)pieces);
+        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per, all = rows_in(a) * pieces;
+        // (most often there is nothing to do where a forward has written the gradient: 32768 workgroups took 9 us to find that out)
+        const int64_t most = g.is_there ? 2048 : 0x7fffffff;
+        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, rows_in(a));
     });
+}
+
+hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l, void *grad) {
+    const int64_t P = a.B / 2, bytes = 2 * a.T * a.V * (dtype == kF32 ? 4 : 2);
+    int64_t pairs = P;
+    if (grad) pairs = bytes > kPairBytes ? 1 : kPairBytes / bytes;
+    l.by_pair = a.exact + a.B * a.T;
+    a.jump = P;
+    for (int64_t first = 0; first < P; first += pairs) {
+        a.first = first;
+        a.part = P - first < pairs ? P - first : pairs;
+        hipError_t e = loss_rows(st, dtype, a, LossTerms{}, nullptr, nullptr);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)a.part), dim3(kFinish), 0, st, a, l);
+        if (grad) e = loss_grad(st, dtype, a, LossGrad{l.coef, 1, 0, nullptr, 0, grad});
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(kFinish), 0, st, P, l);
+    return hipGetLastError();
 }
 
 }  // namespace wkv6

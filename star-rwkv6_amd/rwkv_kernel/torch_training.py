@@ -50,7 +50,7 @@ def _per_token(x, ids, name):
     if x is None:
         return None
     assert x.shape == ids.shape and x.device == ids.device and x.is_floating_point(), "%s must be (batch, time), on the logits' device" % name
-    return x.detach().to(torch.float32).contiguous()
+    return x if x.dtype == torch.float32 and x.is_contiguous() else x.to(torch.float32).contiguous()
 
 
 def token_logprobs(logits, ids, mask=None, temperature=1.0):
@@ -82,7 +82,7 @@ def preference_loss(logits, ids, mask=None, ref_logps=None, beta=0.1, kind="sigm
         "hinge"    max(0, 1 - beta d)
         "ipo"      (d - 1 / (2 beta))^2
     Returns (loss, s): an fp32 scalar, differentiable in logits, and the 2 P values of s, which carry no gradient.  The coefficient of a
-    token's gradient depends on both whole texts, so the logits are read twice."""
+    token's gradient depends on both whole texts, so a pair's logits are read twice, if they fit its last-level cache once from memory."""
     logits, ids, mask = _rows(logits, ids, mask, False)
     B = logits.shape[0]
     assert B % 2 == 0 and B > 0, "the batch holds the chosen texts, then as many rejected ones"
@@ -92,7 +92,7 @@ def preference_loss(logits, ids, mask=None, ref_logps=None, beta=0.1, kind="sigm
     if ref_logps is not None:
         assert ref_logps.shape == (B,) and ref_logps.device == logits.device and ref_logps.is_floating_point(), \
             "ref_logps must hold one value for each text, on the logits' device"
-        ref_logps = ref_logps.detach().to(torch.float32).contiguous()
+        ref_logps = ref_logps.to(torch.float32).contiguous()
     assert ids.numel() > 0, "the texts are empty"
     return _native.load_torch().preference_loss(logits, ids, mask, ref_logps, _PREFERENCE[kind], float(beta), float(label_smoothing), bool(average))
 
@@ -114,10 +114,8 @@ def policy_loss(logits, ids, mask, old_logps, advantages, ref_logps=None, clip_l
     assert advantages.shape in ((B,), ids.shape) and advantages.device == logits.device and advantages.is_floating_point(), \
         "advantages must be (batch,) or (batch, time), on the logits' device"
     assert ids.numel() > 0, "the texts are empty"
-    advantages = advantages.detach().to(torch.float32)
-    if advantages.dim() == 1:
-        advantages = advantages[:, None]
-    return _native.load_torch().policy_loss(logits, ids, mask, old_logps, advantages.expand(ids.shape), ref_logps, float(clip_low), float(clip_high),
+    advantages = advantages.to(torch.float32)
+    return _native.load_torch().policy_loss(logits, ids, mask, old_logps, advantages, ref_logps, float(clip_low), float(clip_high),
                                             float(kl_weight), float(temperature), _REDUCE[reduction])
 
 

@@ -41,7 +41,7 @@ def _calls(lib, rows, workspace=OK, bytes_=1 << 20, **kw):
         "cross_entropy": lambda: lib.wkv6_cross_entropy(*rows, a["red"], a["loss"], a["stats"], a["coef"], a["grad"], *ws),
         "policy": lambda: lib.wkv6_policy_loss(*rows, None, a["adv"], 1, 0, None, a["lo"], a["hi"], a["klw"], a["temperature"], a["red"], a["loss"], a["logps"], a["means"],
                                                a["stats"], a["coef"], a["grad"], *ws),
-        "preference": lambda: lib.wkv6_preference_loss(*rows, None, a["kind"], a["beta"], a["ls"], 0, a["loss"], a["text"], a["stats"], a["coef"], *ws),
+        "preference": lambda: lib.wkv6_preference_loss(*rows, None, a["kind"], a["beta"], a["ls"], 0, a["loss"], a["text"], a["stats"], a["coef"], a["grad"], *ws),
         "backward": lambda: lib.wkv6_logits_backward(*rows, a["temperature"], a["stats"], a["coef"], 1, 0, a["up"], a["there"], a["grad"]),
     }
 
@@ -58,7 +58,7 @@ def test_rows_of_logits(native):
     for bad, who in ((dict(temperature=0.0), "logprobs policy backward"), (dict(temperature=nan), "logprobs policy backward"),
                      (dict(temperature=float("inf")), "logprobs policy backward"), (dict(logps=None), "logprobs policy"), (dict(loss=None), "cross_entropy policy preference"),
                      (dict(loss=OFF), "cross_entropy policy preference"), (dict(stats=OK + 2), "logprobs cross_entropy policy preference backward"),
-                     (dict(grad=OFF), "cross_entropy policy backward"), (dict(stats=None), "cross_entropy policy backward"), (dict(coef=None), "cross_entropy policy backward"),
+                     (dict(grad=OFF), "cross_entropy policy preference backward"), (dict(stats=None), "cross_entropy policy preference backward"), (dict(coef=None), "cross_entropy policy preference backward"),
                      (dict(grad=None), "backward"), (dict(up=None, there=1), "backward"), (dict(red=3), "cross_entropy policy"), (dict(red=2), "cross_entropy"), (dict(red=0), "policy"),
                      (dict(adv=None), "policy"), (dict(means=None), "policy"), (dict(lo=-0.1), "policy"), (dict(hi=nan), "policy"), (dict(klw=nan), "policy"),
                      (dict(kind=3), "preference"), (dict(beta=0.0), "preference"), (dict(beta=nan), "preference"), (dict(ls=0.5), "preference"),
