@@ -409,7 +409,7 @@ int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
 int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
                          const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
                          const float *ref_logps, int kind, double beta, double label_smoothing, int average,
-                         float *loss, float *text_logps, float *stats, float *coef, void *grad,
+                         float *loss, float *text_logps, float *stats, float *coef,
                          void *workspace, size_t workspace_bytes);
 
 /* grad = upstream * dL/dlogits from stats and coef[b * coef_stride_b + t * coef_stride_t]; upstream: one value on the device, or
@@ -420,7 +420,7 @@ int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t 
                          const float *upstream, int grad_is_there, void *grad);
 
 /* Optimizers.  `tensors` lies in HOST memory and may be freed when the call returns.  Addresses need their element's alignment,
- * scales 8 bytes, workspace 16.  param and grad are of `dtype`, dense and in the same order of elements. */
+ * step and scales 8 bytes, workspace 16.  param and grad are of `dtype`, dense and in the same order of elements. */
 typedef struct wkv6_adamw_tensor {
     void *param;
     const void *grad;
@@ -436,7 +436,7 @@ int wkv6_grad_norm(void *stream, int dtype, int64_t count, const wkv6_adamw_tens
                    void *workspace, size_t workspace_bytes);
 
 /* One step of AdamW over `count` tensors, in place.  With g' = g * max_grad_norm / max(*grad_norm, max_grad_norm) (max_grad_norm 0:
- * g' = g), t = *step + 1 (written back) and lr = *lr_device where that is given:
+ * g' = g), t = *step + 1 (written back; 0 <= *step < 2^32 - 1) and lr = *lr_device where that is given:
  *   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
  * master (fp32) or NULL: the weights that are updated, of which param then is the rounded copy.
@@ -444,11 +444,9 @@ int wkv6_grad_norm(void *stream, int dtype, int64_t count, const wkv6_adamw_tens
  * under scales, fp32 (ceil(numel / 256), 2): m's and sqrt(v)'s for each 256 elements.  They are rounded up or down at random, the
  * mean kept; the random bits are a function of seed, t, the tensor's place in the list and the element's in the tensor.
  * skip_nonfinite: where *grad_norm is no finite number nothing is changed.  grad_norm may be NULL where neither needs it. */
-size_t wkv6_adamw_workspace_bytes(int64_t count);
 int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, const wkv6_adamw_tensor *tensors,
                     int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
-                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed,
-                    void *workspace, size_t workspace_bytes);
+                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed);
 
 /* ---- XLA custom-call surface (replaces the pybind module `gpu_ops`,
  * rwkv_kernel/jax_kernel/gpu_ops.cpp:20-43) ---------------------------------------------- */

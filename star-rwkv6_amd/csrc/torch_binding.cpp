@@ -461,15 +461,12 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const c10::DeviceGuard guard(x.device());
     const Logits l = logits_of(x, ids, mask);
     const Tensor loss = fp32(x, {}), text = fp32(x, {l.B});
-    const Tensor grad = gradient_ahead(l, wanted);
     const Tensor stats = wanted ? fp32(x, {l.B, l.T, 2}) : Tensor(), coef = wanted ? fp32(x, {l.B}) : Tensor();
     const size_t n = wkv6_loss_workspace_bytes(l.B, l.T);
     const Tensor ws = bytes(x, n);
     check(wkv6_preference_loss(stream_of(x), l.code, l.B, l.T, l.V, in(x), x.stride(0), x.stride(1), l.id(), l.counted(), in_f(given(ref_logps)),
-                               static_cast<int>(kind), beta, label_smoothing, average, out_f(loss), out_f(text), out_f(stats), out_f(coef),
-                               out(grad), out(ws), n));
+                               static_cast<int>(kind), beta, label_smoothing, average, out_f(loss), out_f(text), out_f(stats), out_f(coef), out(ws), n));
     keep_rows(ctx, l, stats, coef, 1.0);
-    keep(ctx, grad, "grad");
     ctx->mark_non_differentiable({text});
     ctx->set_materialize_grads(false);
     return {loss, text};
@@ -480,8 +477,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     if (!grads[0].defined()) return res;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
-    const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad");
-    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), ahead);
+    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor());
     return res;
   }
 };
@@ -575,10 +571,8 @@ Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &ex
   std::sort(seen.begin(), seen.end());
   TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "wkv6: a parameter is given twice");
   if (!norm.defined() && (max_grad_norm > 0. || skip_nonfinite)) norm = grad_norm(kept);
-  const size_t n = wkv6_adamw_workspace_bytes(count);
-  const Tensor ws = bytes(first, n);
   check(wkv6_adamw_step(stream_of(first), code_of(type), eight ? 8 : 32, count, rows.data(), static_cast<int64_t *>(out(step)), in_f(lr_device), lr, beta1,
-                        beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, in_f(norm), static_cast<uint32_t>(seed), out(ws), n));
+                        beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, in_f(norm), static_cast<uint32_t>(seed)));
   for (const Tensors *l : {&params, &exp_avgs, &exp_avg_sqs, &scales, &masters})
     for (const Tensor &t : *l)
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // (what autograd saved of them is no longer what it was)

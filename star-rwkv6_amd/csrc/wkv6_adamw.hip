@@ -13,27 +13,38 @@
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
+#include <type_traits>
+
 namespace wkv6 {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kGroup = 48;          // tensors of one launch: they travel in its arguments, which hold 4 KB
-constexpr int kChunk = 4096;        // elements of one workgroup
+constexpr int kGroup = 60;          // tensors of one launch: they travel in its arguments, which hold 4 KB
+constexpr int kChunk = 4096;        // elements that a workgroup takes at a time, 16 to a thread in pieces that lie next to each other
 constexpr int kScaleBlock = 256;    // elements that share a scale
-constexpr int kNormBlocks = 1024;   // of a group, at most
+constexpr int kBlocks = 2048;       // workgroups of a launch at most: eight to a compute unit, which go from chunk to chunk
+constexpr int kFinish = 1024;       // threads of the one workgroup that adds up
+constexpr int64_t kPastBytes = 160 << 20;   // of all tensors of a call
 
 struct Group {
     AdamwTensor t[kGroup];
     int first[kGroup + 1];   // chunk at which a tensor begins
     int count;
     int number;              // of the first tensor in the call's list
+    int last;                // whether nothing of the call follows
+    int past;                // whether tensors are read and written past the caches
 };
 
-// What a step is done with, worked out once on the device.
+// What a step is done with.
 struct Plan {
-    float clip, decay, rate, root, skip;   // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
+    float clip, decay, rate, root;   // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
     uint32_t key;
+    int skip;
 };
+struct Rates {
+    float b1, c1, b2, c2, eps;
+};
+static_assert(sizeof(Group) + sizeof(Rates) + sizeof(AdamwStep) <= 4096, "a launch's arguments");
 
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
     x = (x ^ (x >> 16)) * 0xBB67AE85u;   // (fractions of the roots of 3 and 5, as odd numbers)
@@ -41,26 +52,14 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-template <typename S> __device__ __forceinline__ S block_sum(S v, S *part) {
+template <int kW> __device__ __forceinline__ double block_sum(double v, double *part) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = part[0];
-    for (int i = 1; i < kWaves; ++i) v += part[i];
+    for (int i = 1; i < kW; ++i) v += part[i];
     return v;
-}
-__device__ __forceinline__ float block_top(float v, float *part) {   // of magnitudes; NaN if one is
-    uint32_t b = __float_as_uint(v);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, d));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = __uint_as_float(b);
-    __syncthreads();
-    b = __float_as_uint(part[0]);
-    for (int i = 1; i < kWaves; ++i) b = max(b, __float_as_uint(part[i]));
-    return __uint_as_float(b);
 }
 
 __device__ __forceinline__ int tensor_of(const Group &g, int chunk) {
@@ -72,117 +71,280 @@ __device__ __forceinline__ int tensor_of(const Group &g, int chunk) {
     return lo;
 }
 
+// kEach (4 or 8) elements as they sit in memory, at any element's address; the last ones of a tensor one by one.  S: 4-, 2- or 1-byte elements.
+template <typename S, int kEach> struct Piece {
+    static constexpr int kWords = kEach * sizeof(S) / 4, kAtOnce = kWords < 4 ? kWords : 4;
+    typedef uint32_t vec __attribute__((ext_vector_type(kAtOnce), aligned(sizeof(S))));
+    uint32_t r[kWords];
+    template <bool kPast> __device__ __forceinline__ void load(const S *p, int n) {
+        if (n >= kEach) {
+#pragma unroll
+            for (int k = 0; k < kWords / kAtOnce; ++k) {
+                const vec *at = reinterpret_cast<const vec *>(p) + k;
+                vec v;
+                if (kPast) v = __builtin_nontemporal_load(at);
+                else v = *at;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) r[k * kAtOnce + i] = v[i];
+            }
+            return;
+        }
+        const auto *bits = reinterpret_cast<const unsigned_of *>(p);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) r[i] = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (e < n) r[e * (int)sizeof(S) / 4] |= (uint32_t)bits[e] << (e * 8 * (int)sizeof(S) % 32);
+    }
+    template <bool kPast> __device__ __forceinline__ void store(S *p, int n) const {
+        if (n >= kEach) {
+#pragma unroll
+            for (int k = 0; k < kWords / kAtOnce; ++k) {
+                vec *at = reinterpret_cast<vec *>(p) + k;
+                vec v;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) v[i] = r[k * kAtOnce + i];
+                if (kPast) __builtin_nontemporal_store(v, at);
+                else *at = v;
+            }
+            return;
+        }
+        auto *bits = reinterpret_cast<unsigned_of *>(p);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (e < n) bits[e] = (unsigned_of)(r[e * (int)sizeof(S) / 4] >> (e * 8 * (int)sizeof(S) % 32));
+    }
+    typedef std::conditional_t<sizeof(S) == 4, uint32_t, std::conditional_t<sizeof(S) == 2, uint16_t, uint8_t>> unsigned_of;
+};
+
+template <int kEach> __device__ __forceinline__ void unpack(const Piece<float, kEach> &b, float (&o)[kEach]) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) o[i] = __uint_as_float(b.r[i]);
+}
+template <int kEach> __device__ __forceinline__ void unpack(const Piece<bf16_t, kEach> &b, float (&o)[kEach]) {
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) o[2 * i] = __uint_as_float(b.r[i] << 16), o[2 * i + 1] = __uint_as_float(b.r[i] & 0xffff0000u);
+}
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+template <int kEach> __device__ __forceinline__ void unpack(const Piece<f16_t, kEach> &b, float (&o)[kEach]) {
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) {
+        const h2 h = __builtin_bit_cast(h2, b.r[i]);
+        o[2 * i] = (float)h[0], o[2 * i + 1] = (float)h[1];
+    }
+}
+template <int kEach> __device__ __forceinline__ void unpack(const Piece<uint8_t, kEach> &b, float (&o)[kEach]) {   // float8
+    typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < kEach / 4; ++i) {
+        const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.r[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.r[i], true);
+        o[4 * i] = lo[0], o[4 * i + 1] = lo[1], o[4 * i + 2] = hi[0], o[4 * i + 3] = hi[1];
+    }
+}
+template <int kEach> __device__ __forceinline__ void pack(const float (&v)[kEach], Piece<float, kEach> &b) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) b.r[i] = __float_as_uint(v[i]);
+}
+template <int kEach> __device__ __forceinline__ void pack(const float (&v)[kEach], Piece<bf16_t, kEach> &b) {
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) b.r[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+}
+template <int kEach> __device__ __forceinline__ void pack(const float (&v)[kEach], Piece<f16_t, kEach> &b) {
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) b.r[i] = __builtin_bit_cast(uint32_t, (h2){to_f16(v[2 * i]), to_f16(v[2 * i + 1])});
+}
+
+template <typename F> __device__ __forceinline__ void either(bool which, F &&f) {
+    if (which) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 template <typename T> __global__ __launch_bounds__(kThreads) void norm_kernel(Group g, double *partial) {
+    constexpr int kEach = 16 / sizeof(T), kItems = kChunk / kThreads / kEach;
     __shared__ double part[kWaves];
     double s = 0.;
     for (int chunk = blockIdx.x; chunk < g.first[g.count]; chunk += gridDim.x) {
         const int k = tensor_of(g, chunk);
-        const int64_t first = (int64_t)(chunk - g.first[k]) * kChunk, n = min((int64_t)kChunk, g.t[k].numel - first);
+        const int64_t first = (int64_t)(chunk - g.first[k]) * kChunk;
         const T *x = static_cast<const T *>(g.t[k].grad) + first;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const double v = load1(x + i);
-            s += v * v;
+        const int n = (int)min((int64_t)kChunk, g.t[k].numel - first);
+        Piece<T, kEach> held[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int at = (i * kThreads + threadIdx.x) * kEach;
+            held[i].template load<false>(x + at, n - at);
+        }
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            float v[kEach];
+            unpack(held[i], v);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) s = __builtin_fma((double)v[e], (double)v[e], s);
         }
     }
-    s = block_sum(s, part);
+    s = block_sum<kWaves>(s, part);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(kThreads) void norm_finish_kernel(const double *partial, int64_t partials, float *norm) {
-    __shared__ double part[kWaves];
+__global__ __launch_bounds__(kFinish) void norm_finish_kernel(const double *partial, int64_t partials, float *norm) {
+    __shared__ double part[kFinish / 64];
     double s = 0.;
-    for (int64_t i = threadIdx.x; i < partials; i += kThreads) s += partial[i];
-    s = block_sum(s, part);
+    for (int64_t r = threadIdx.x; r < partials; r += 8 * kFinish) {
+        double x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = r + i * kFinish < partials ? partial[r + i * kFinish] : 0.;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += x[i];
+    }
+    s = block_sum<kFinish / 64>(s, part);
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-__global__ void plan_kernel(AdamwStep a, Plan *plan) {
+__device__ Plan plan_of(const AdamwStep &a) {
     Plan p;
     const double norm = a.grad_norm ? (double)*a.grad_norm : 0.;
     p.clip = a.max_grad_norm > 0. ? (float)(norm <= a.max_grad_norm ? 1. : a.max_grad_norm / norm) : 1.f;
-    p.skip = a.skip_nonfinite && !(norm <= 3.402823466e38) ? 1.f : 0.f;
-    const int64_t t = *a.step + 1;
-    if (p.skip == 0.f) *a.step = t;
+    p.skip = a.skip_nonfinite && !(norm <= 3.402823466e38);
+    // (the upper half counts workgroups while a step is under way, see below)
+    const uint32_t t = (uint32_t)__hip_atomic_load(a.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
     const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
     p.decay = (float)(1. - lr * a.weight_decay);
     p.rate = (float)(lr / (1. - pow(a.beta1, (double)t)));
     p.root = (float)(1. / sqrt(1. - pow(a.beta2, (double)t)));
-    p.key = a.seed * 0x9E3779B9u + (uint32_t)t * 0xBB67AE85u;
-    *plan = p;
+    p.key = a.seed * 0x9E3779B9u + t * 0xBB67AE85u;
+    return p;
 }
 
-struct Rates {
-    float b1, c1, b2, c2, eps;
-};
-
-__device__ __forceinline__ uint8_t to_float8(float x, uint32_t random16) {
-    // 2^-120 brings the exponents of the two formats together, below float8's smallest normal number too
-    const uint32_t bits = __float_as_uint(fabsf(x) * 0x1p-120f) + (random16 << 4);
-    return (uint8_t)min(bits >> 20, 0x7Eu);
-}
-__device__ __forceinline__ float from_float8(uint8_t c) {
-    const float x = __uint_as_float((uint32_t)(c & 0x7F) << 20) * 0x1p120f;
-    return c & 0x80 ? -x : x;
+// The largest of 32 or 64 neighbouring lanes' magnitudes; NaN if one is.
+template <int kLanes> __device__ __forceinline__ float top_of(float v) {
+    uint32_t b = __float_as_uint(v);
+    b = max(b, (uint32_t)__builtin_amdgcn_mov_dpp((int)b, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    b = max(b, (uint32_t)__builtin_amdgcn_mov_dpp((int)b, 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    b = max(b, (uint32_t)__builtin_amdgcn_mov_dpp((int)b, 0x141, 0xF, 0xF, true));   // row_half_mirror
+    b = max(b, (uint32_t)__builtin_amdgcn_mov_dpp((int)b, 0x140, 0xF, 0xF, true));   // row_mirror
+    b = max(b, (uint32_t)__shfl_xor((int)b, 16));
+    if (kLanes == 64) b = max(b, (uint32_t)__shfl_xor((int)b, 32));
+    return __uint_as_float(b);
 }
 
-template <typename T, int kBits> __global__ __launch_bounds__(kThreads) void step_kernel(Group g, Rates r, const Plan *plan) {
-    __shared__ float part[kWaves];
-    const Plan q = *plan;
-    if (q.skip != 0.f) return;
-    const int chunk = blockIdx.x, k = tensor_of(g, chunk);
-    const AdamwTensor t = g.t[k];
-    const uint32_t key = mix(q.key + (uint32_t)(g.number + k));
-    const int64_t first = (int64_t)(chunk - g.first[k]) * kChunk, end = min(first + kChunk, t.numel);
-    T *p = static_cast<T *>(t.param);
-    for (int64_t at = first; at < end; at += kThreads) {
-        const int64_t i = at + threadIdx.x;
-        const bool in = i < end;
-        const float grad = in ? load1(static_cast<const T *>(t.grad) + i) * q.clip : 0.f;
-        float m = 0.f, v = 0.f;
-        float2 scale = make_float2(0.f, 0.f);
-        if (kBits == 8) {
-            scale = *reinterpret_cast<const float2 *>(t.scales + 2 * (at / kScaleBlock));
-            if (in) {
-                m = from_float8(static_cast<const uint8_t *>(t.exp_avg)[i]) * scale.x;
-                v = from_float8(static_cast<const uint8_t *>(t.exp_avg_sq)[i]) * scale.y;
-                v *= v;
+// The float8 below or above |x|, above with the probability that keeps the mean.  2^-120 brings the exponents of the two formats together,
+// below float8's smallest normal number too: what float8 holds are the upper bits, the random number rounds by its carry.
+__device__ __forceinline__ uint32_t to_float8(float x, uint32_t random16) {
+    return min((__float_as_uint(fabsf(x) * 0x1p-120f) + (random16 << 4)) >> 20, 0x7Eu);
+}
+
+template <typename T, int kBits, bool kMaster, bool kPast>
+__device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r, const Plan &q, uint32_t key, int64_t first) {
+    typedef std::conditional_t<kBits == 8, uint8_t, float> M;
+    // Neighbouring lanes' pieces lie next to each other, so what one load of a wave reaches has no gaps if a piece has at most 16 bytes: pieces of
+    // 4 elements where there is something in fp32 (AdamW over 490 M fp32 parameters 2.84 ms with pieces of 8)
+    constexpr int kEach = kBits == 8 && sizeof(T) == 2 && !kMaster ? 8 : 4, kItems = kChunk / kThreads / kEach;
+    Piece<T, kEach> g8[kItems], p8[kItems];
+    Piece<M, kEach> m8[kItems], v8[kItems];
+    Piece<float, kEach> w8[kMaster ? kItems : 1];
+    float2 scale[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int64_t at = first + (i * kThreads + (int)threadIdx.x) * kEach;
+        const int n = (int)min((int64_t)kEach, t.numel - at);
+        g8[i].template load<kPast>(static_cast<const T *>(t.grad) + at, n);
+        if (kMaster) w8[i].template load<kPast>(t.master + at, n);
+        else p8[i].template load<kPast>(static_cast<const T *>(t.param) + at, n);
+        m8[i].template load<kPast>(static_cast<const M *>(t.exp_avg) + at, n);
+        v8[i].template load<kPast>(static_cast<const M *>(t.exp_avg_sq) + at, n);
+        if (kBits == 8) scale[i] = n > 0 ? *reinterpret_cast<const float2 *>(t.scales + 2 * (at / kScaleBlock)) : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int64_t at = first + (i * kThreads + (int)threadIdx.x) * kEach;
+        const int n = (int)min((int64_t)kEach, t.numel - at);
+        float g[kEach], w[kEach], m[kEach], v[kEach], root[kEach];
+        unpack(g8[i], g);
+        unpack(m8[i], m);
+        unpack(v8[i], v);
+        if constexpr (kMaster) unpack(w8[i], w);
+        else unpack(p8[i], w);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (kBits == 8) {
+                m[e] *= scale[i].x;
+                v[e] *= scale[i].y;
+                v[e] *= v[e];
             }
-        } else if (in) {
-            m = static_cast<const float *>(t.exp_avg)[i];
-            v = static_cast<const float *>(t.exp_avg_sq)[i];
+            g[e] *= q.clip;
+            m[e] = m[e] * r.b1 + g[e] * r.c1;
+            v[e] = v[e] * r.b2 + g[e] * g[e] * r.c2;
+            // (root and reciprocal to one unit in the last place of fp32; correctly rounded ones take some twenty operations more)
+            root[e] = __builtin_amdgcn_sqrtf(v[e]);
+            w[e] = w[e] * q.decay - m[e] * q.rate * __builtin_amdgcn_rcpf(root[e] * q.root + r.eps);
         }
-        m = m * r.b1 + grad * r.c1;
-        v = v * r.b2 + grad * grad * r.c2;
-        const float root = sqrtf(v);
-        if (in) {
-            float w = t.master ? t.master[i] : load1(p + i);
-            w = w * q.decay - m * q.rate / (root * q.root + r.eps);
-            if (t.master) t.master[i] = w;
-            store1(p + i, w);
+        if constexpr (kMaster) {
+            pack(w, w8[i]);
+            w8[i].template store<kPast>(t.master + at, n);
         }
-        if (kBits == 8) {
-            const float top_m = block_top(in ? fabsf(m) : 0.f, part), top_r = block_top(in ? root : 0.f, part);
+        pack(w, p8[i]);
+        p8[i].template store<kPast>(static_cast<T *>(t.param) + at, n);
+        if constexpr (kBits == 8) {
+            float top_m = 0.f, top_r = 0.f;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                // (as bits: NaN is the largest; elements behind the tensor's end were loaded as zeros and stay zeros)
+                top_m = __uint_as_float(max(__float_as_uint(top_m), __float_as_uint(m[e]) & 0x7fffffffu));
+                top_r = __uint_as_float(max(__float_as_uint(top_r), __float_as_uint(root[e])));
+            }
+            top_m = top_of<kScaleBlock / kEach>(top_m), top_r = top_of<kScaleBlock / kEach>(top_r);
             const float sm = top_m < 0x1p-100f ? 0x1p-100f : top_m, sr = top_r < 0x1p-100f ? 0x1p-100f : top_r;
-            if (threadIdx.x == 0) *reinterpret_cast<float2 *>(t.scales + 2 * (at / kScaleBlock)) = make_float2(sm * (1.f / 448.f), sr * (1.f / 448.f));
-            if (in) {
-                const uint32_t h = mix((uint32_t)i * 0x9E3779B9u + key);
-                const uint8_t cm = to_float8(m * (448.f / sm), h & 0xFFFF);
-                uint8_t cr = to_float8(root * (448.f / sr), h >> 16);
-                if (cr == 0 && root > 0.f) cr = 1;
-                static_cast<uint8_t *>(t.exp_avg)[i] = cm | (m < 0.f ? 0x80 : 0);
-                static_cast<uint8_t *>(t.exp_avg_sq)[i] = cr;
+            if (threadIdx.x % (kScaleBlock / kEach) == 0 && n > 0)
+                *reinterpret_cast<float2 *>(t.scales + 2 * (at / kScaleBlock)) = make_float2(sm * (1.f / 448.f), sr * (1.f / 448.f));
+            const float im = 448.f / sm, ir = 448.f / sr;
+            const uint32_t start = (uint32_t)at * 0x9E3779B9u + key;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const uint32_t h = mix(start + (uint32_t)e * 0x9E3779B9u);
+                const uint32_t cm = to_float8(m[e] * im, h & 0xFFFF) | (__float_as_uint(m[e]) >> 24 & 0x80u);
+                uint32_t cr = to_float8(root[e] * ir, h >> 16);
+                cr = root[e] > 0.f ? max(cr, 1u) : cr;   // (a denominator is never rounded to zero)
+                if (e % 4 == 0) m8[i].r[e / 4] = cm, v8[i].r[e / 4] = cr;
+                else m8[i].r[e / 4] |= cm << (8 * (e % 4)), v8[i].r[e / 4] |= cr << (8 * (e % 4));
             }
-        } else if (in) {
-            static_cast<float *>(t.exp_avg)[i] = m;
-            static_cast<float *>(t.exp_avg_sq)[i] = v;
+        } else {
+            pack(m, m8[i]);
+            pack(v, v8[i]);
         }
+        m8[i].template store<kPast>(static_cast<M *>(t.exp_avg) + at, n);
+        v8[i].template store<kPast>(static_cast<M *>(t.exp_avg_sq) + at, n);
     }
 }
 
-// The tensors in groups that one launch takes: f(group, its chunks).
+template <typename T, int kBits> __global__ __launch_bounds__(kThreads) void step_kernel(Group g, Rates r, AdamwStep a) {
+    __shared__ Plan plan;
+    if (threadIdx.x == 0) plan = plan_of(a);
+    __syncthreads();
+    const Plan q = plan;
+    if (q.skip) return;
+    for (int chunk = blockIdx.x; chunk < g.first[g.count]; chunk += gridDim.x) {
+        const int k = tensor_of(g, chunk);
+        const AdamwTensor t = g.t[k];
+        const uint32_t key = mix(q.key + (uint32_t)(g.number + k));
+        const int64_t first = (int64_t)(chunk - g.first[k]) * kChunk;
+        either(g.past, [&](auto past) {
+            if constexpr (sizeof(T) == 2) {
+                if (t.master) return step_chunk<T, kBits, true, past.value>(t, r, q, key, first);
+            }
+            step_chunk<T, kBits, false, past.value>(t, r, q, key, first);
+        });
+    }
+    // The step count moves on when the last workgroup has read it: the workgroups that have are counted in its upper half.
+    if (!g.last || threadIdx.x != 0) return;
+    auto *step = reinterpret_cast<unsigned long long *>(a.step);
+    const unsigned long long was = __hip_atomic_fetch_add(step, 1ull << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (was >> 32 == gridDim.x - 1) __hip_atomic_store(step, (was & 0xffffffffull) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The tensors in groups that one launch takes: f(group, workgroups).  At least one group, also where there is nothing in any tensor.
 template <typename F> void by_group(int64_t count, const AdamwTensor *tensors, F &&f) {
-    for (int64_t at = 0; at < count;) {
-        Group g;
+    Group g;
+    for (int64_t at = 0;;) {
         g.number = (int)at;
         g.first[0] = 0;
         for (g.count = 0; g.count < kGroup && at < count; ++g.count, ++at) {
@@ -191,7 +353,10 @@ template <typename F> void by_group(int64_t count, const AdamwTensor *tensors, F
             g.t[g.count] = tensors[at];
             g.first[g.count + 1] = g.first[g.count] + (int)chunks;
         }
-        if (g.first[g.count] > 0) f(g, g.first[g.count]);
+        g.last = at >= count;
+        const int chunks = g.first[g.count];
+        if (chunks > 0 || g.last) f(g, chunks < 1 ? 1 : chunks < kBlocks ? chunks : kBlocks);
+        if (g.last) return;
     }
 }
 
@@ -206,32 +371,30 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
 
 // (a group ends early only before more than 2^30 chunks: twice the groups are more than enough)
 size_t grad_norm_workspace_bytes(int64_t count) {
-    return (size_t)(2 * ((count + kGroup - 1) / kGroup)) * kNormBlocks * sizeof(double);
+    return (size_t)(2 * ((count + kGroup - 1) / kGroup)) * kBlocks * sizeof(double);
 }
 
 hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor *tensors, float *norm, void *workspace) {
     return by_type(dtype, [&](auto t) {
         double *partial = static_cast<double *>(workspace);
         int64_t partials = 0;
-        by_group(count, tensors, [&](const Group &g, int chunks) {
-            const int blocks = chunks < kNormBlocks ? chunks : kNormBlocks;
+        by_group(count, tensors, [&](const Group &g, int blocks) {
             hipLaunchKernelGGL((norm_kernel<decltype(t)>), dim3(blocks), dim3(kThreads), 0, st, g, partial + partials);
             partials += blocks;
         });
-        hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kThreads), 0, st, partial, partials, norm);
+        hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kFinish), 0, st, partial, partials, norm);
     });
 }
 
-size_t adamw_workspace_bytes(int64_t) { return 256; }
-
-hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s, void *workspace) {
-    Plan *plan = static_cast<Plan *>(workspace);
+hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s) {
     const Rates r{(float)s.beta1, (float)(1. - s.beta1), (float)s.beta2, (float)(1. - s.beta2), (float)s.eps};
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < count; ++i) bytes += tensors[i].numel * ((dtype == kF32 ? 4 : 2) * 2 + moment_bits / 4 + (tensors[i].master ? 4 : 0));
     return by_type(dtype, [&](auto t) {
-        hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1), 0, st, s, plan);
-        by_group(count, tensors, [&](const Group &g, int chunks) {
-            if (moment_bits == 8) hipLaunchKernelGGL((step_kernel<decltype(t), 8>), dim3(chunks), dim3(kThreads), 0, st, g, r, plan);
-            else hipLaunchKernelGGL((step_kernel<decltype(t), 32>), dim3(chunks), dim3(kThreads), 0, st, g, r, plan);
+        by_group(count, tensors, [&](Group &g, int blocks) {
+            g.past = bytes >= kPastBytes;
+            if (moment_bits == 8) hipLaunchKernelGGL((step_kernel<decltype(t), 8>), dim3(blocks), dim3(kThreads), 0, st, g, r, s);
+            else hipLaunchKernelGGL((step_kernel<decltype(t), 32>), dim3(blocks), dim3(kThreads), 0, st, g, r, s);
         });
     });
 }

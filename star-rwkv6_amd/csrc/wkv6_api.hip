@@ -323,7 +323,7 @@ static int check_rows(int dtype, int64_t B, int64_t T, int64_t V, const void *lo
 }
 static wkv6::LossRows rows_of(int64_t B, int64_t T, int64_t V, const void *logits, int64_t stride_b, int64_t stride_t,
                               const int64_t *ids, const uint8_t *mask, float temperature, float *logps, float *stats) {
-    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr, 0, B, 0};
+    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr};
 }
 static bool floats(std::initializer_list<const void *> ps) {
     for (const void *p : ps)
@@ -390,11 +390,10 @@ int wkv6_policy_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
 int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
                          const void *logits, int64_t stride_b, int64_t stride_t, const int64_t *ids, const uint8_t *mask,
                          const float *ref_logps, int kind, double beta, double label_smoothing, int average,
-                         float *loss, float *text_logps, float *stats, float *coef, void *grad, void *workspace, size_t workspace_bytes) {
+                         float *loss, float *text_logps, float *stats, float *coef, void *workspace, size_t workspace_bytes) {
     int rc = check_rows(dtype, B, T, V, logits, stride_b, stride_t, ids, 1.f);
     if (rc != WKV6_OK) return rc;
     if (B % 2 != 0 || !loss || !text_logps || !floats({ref_logps, loss, text_logps, stats, coef})) return WKV6_ERR_ARG;
-    if (!aligned(grad, element_size(dtype)) || (grad && (!stats || !coef))) return WKV6_ERR_ARG;
     if (kind < WKV6_PREFERENCE_SIGMOID || kind > WKV6_PREFERENCE_IPO || !(beta > 0.) || !(label_smoothing >= 0. && label_smoothing < 0.5)) return WKV6_ERR_ARG;
     if (kind != WKV6_PREFERENCE_SIGMOID && label_smoothing != 0.) return WKV6_ERR_ARG;
     rc = check_loss_workspace(B, T, workspace, workspace_bytes);
@@ -402,7 +401,7 @@ int wkv6_preference_loss(void *stream, int dtype, int64_t B, int64_t T, int64_t 
     wkv6::LossRows a = rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, 1.f, nullptr, stats);
     a.exact = static_cast<double *>(workspace);
     return finish(wkv6::loss_preference((hipStream_t)stream, dtype, a,
-                                        wkv6::PreferenceTerms{kind, average, beta, label_smoothing, ref_logps, loss, text_logps, coef, nullptr}, grad));
+                                        wkv6::PreferenceTerms{kind, average, beta, label_smoothing, ref_logps, loss, text_logps, coef, nullptr}));
 }
 
 int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
@@ -415,7 +414,7 @@ int wkv6_logits_backward(void *stream, int dtype, int64_t B, int64_t T, int64_t 
     if (!floats({stats, coef, upstream}) || !aligned(grad, element_size(dtype))) return WKV6_ERR_ARG;
     return finish(wkv6::loss_grad((hipStream_t)stream, dtype,
                                   rows_of(B, T, V, logits, stride_b, stride_t, ids, mask, temperature, nullptr, const_cast<float *>(stats)),
-                                  wkv6::LossGrad{coef, coef_stride_b, coef_stride_t, upstream, grad_is_there, grad}));
+                                  wkv6::LossGrad{coef, coef_stride_b, coef_stride_t, upstream, grad_is_there, grad, false}));
 }
 
 static_assert(sizeof(wkv6_adamw_tensor) == sizeof(wkv6::AdamwTensor), "one layout");
@@ -446,22 +445,17 @@ int wkv6_grad_norm(void *stream, int dtype, int64_t count, const wkv6_adamw_tens
     return finish(wkv6::grad_norm((hipStream_t)stream, dtype, count, reinterpret_cast<const wkv6::AdamwTensor *>(tensors), norm, workspace));
 }
 
-size_t wkv6_adamw_workspace_bytes(int64_t count) { return count > 0 && count <= 0x7fffffffLL ? wkv6::adamw_workspace_bytes(count) : 0; }
-
 int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, const wkv6_adamw_tensor *tensors,
                     int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
-                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed,
-                    void *workspace, size_t workspace_bytes) {
+                    double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed) {
     if (moment_bits != 8 && moment_bits != 32) return WKV6_ERR_ARG;
     const int rc = check_tensors(dtype, count, tensors, false, moment_bits);
     if (rc != WKV6_OK) return rc;
     if (!step || !aligned(step, 8) || !floats({lr_device, grad_norm})) return WKV6_ERR_ARG;
     if (!(lr >= 0.) || !(beta1 >= 0. && beta1 < 1.) || !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || !(weight_decay >= 0.) || !(max_grad_norm >= 0.)) return WKV6_ERR_ARG;
     if ((max_grad_norm > 0. || skip_nonfinite) && !grad_norm) return WKV6_ERR_ARG;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < wkv6::adamw_workspace_bytes(count)) return WKV6_ERR_WORKSPACE;
     return finish(wkv6::adamw_step((hipStream_t)stream, dtype, moment_bits, count, reinterpret_cast<const wkv6::AdamwTensor *>(tensors),
-                                   wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed},
-                                   workspace));
+                                   wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed}));
 }
 
 static int check_mix(int dtype, int64_t B, int64_t T, int64_t C, int64_t R) {

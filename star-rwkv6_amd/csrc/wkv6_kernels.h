@@ -336,7 +336,6 @@ hipError_t sum_over_batch(hipStream_t st, int out_dtype, int64_t B, int64_t C, c
 
 // --- losses over the logits of a vocabulary (wkv6_loss.hip) ---
 // Rows of V logits at b * stride_b + t * stride_t (elements; any alignment of an element); ids (B,T), mask (B,T) or null.
-// A launch takes texts [first, first + part) and, with jump > 0, as many from first + jump on.
 struct LossRows {
     int64_t B, T, V, stride_b, stride_t;
     const void *logits;
@@ -346,7 +345,6 @@ struct LossRows {
     float *logps;   // (B,T) or null
     float *stats;   // (B,T,2) top and sum of a row, or null
     double *exact;  // (B,T) logps in 64 bits, or null
-    int64_t first, part, jump;
 };
 struct LossCounts {
     int *by_text, *tokens, *texts;   // counted tokens of each text; of each counting workgroup's texts: tokens, texts that have any
@@ -380,10 +378,11 @@ struct LossGrad {
     const float *upstream;    // one value, or null for 1
     int is_there;             // grad holds the gradient for an upstream of 1
     void *grad;               // (B,T,V)
+    bool past;                // set inside: written past the caches
 };
 size_t loss_workspace_bytes(int64_t B, int64_t T);
 hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *grad, void *workspace);   // grad: (B,T,V) or null
-hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l, void *grad);   // with a.exact; grad as above
+hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l);   // with a.exact
 hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g);     // reads a.stats
 
 // --- AdamW over many tensors (wkv6_adamw.hip) ---
@@ -404,7 +403,6 @@ struct AdamwStep {
 };
 size_t grad_norm_workspace_bytes(int64_t count);
 hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor *tensors, float *norm, void *workspace);
-size_t adamw_workspace_bytes(int64_t count);
-hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s, void *workspace);
+hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s);
 
 }  // namespace wkv6

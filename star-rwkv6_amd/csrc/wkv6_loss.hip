@@ -15,6 +15,8 @@
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
+#include <type_traits>
+
 namespace wkv6 {
 namespace {
 
@@ -23,7 +25,10 @@ constexpr int kFinish = 1024;        // threads of the one workgroup that adds u
 constexpr int kCountBlocks = 256;    // at most
 constexpr int kStream = 1024, kStreamVecs = 4;   // rows that no registers hold: threads, vectors of a thread in flight
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
-constexpr int64_t kPairBytes = 128 << 20;   // logits of the pairs whose gradient is formed before the next pairs' logits are read
+// A gradient of this size and more is written past the caches.  Cross entropy, log probabilities with their backward, and the latter with a reader
+// of the gradient behind it, in us, written into / past them: 128 MiB 63 / 66, 78 / 78, 106 / 120; 192 MiB 89 / 89, 119 / 108, 178 / 171; 2 GiB (8 pairs
+// of texts) 1110 / 1000.
+constexpr int64_t kPastBytes = 160 << 20;
 constexpr double kLog2e = 1.44269504088896340736;
 
 // exp(d / temperature) as a power of two.  log2(e) / temperature rounded to fp32 is off by up to 2^-24 of itself, the same way in
@@ -89,8 +94,11 @@ template <> struct Vec<float> {
 };
 template <typename T> struct Bits {
     uint32_t r[4];
-    __device__ __forceinline__ void load(const T *p) {
-        const auto v = *reinterpret_cast<const typename Vec<T>::raw *>(p);
+    // kPast: past the caches
+    template <bool kPast> __device__ __forceinline__ void load(const T *p) {
+        typename Vec<T>::raw v;
+        if (kPast) v = __builtin_nontemporal_load(reinterpret_cast<const typename Vec<T>::raw *>(p));
+        else v = *reinterpret_cast<const typename Vec<T>::raw *>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = v[i];
     }
@@ -101,18 +109,14 @@ template <typename T> struct Bits {
     }
     __device__ __forceinline__ void none() { r[0] = r[1] = r[2] = r[3] = Vec<T>::kNone; }
     __device__ __forceinline__ void zero() { r[0] = r[1] = r[2] = r[3] = 0; }
-    __device__ __forceinline__ void store(T *p) const {
+    template <bool kPast> __device__ __forceinline__ void store(T *p) const {
         typename Vec<T>::raw v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = r[i];
-        *reinterpret_cast<typename Vec<T>::raw *>(p) = v;
+        if (kPast) __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T>::raw *>(p));
+        else *reinterpret_cast<typename Vec<T>::raw *>(p) = v;
     }
 };
-
-// The row that a launch's index stands for.
-__device__ __forceinline__ int64_t row_of(const LossRows &a, int64_t index) {
-    return a.first * a.T + index + (a.jump > 0 && index >= a.part * a.T ? (a.jump - a.part) * a.T : 0);
-}
 
 __device__ __forceinline__ bool counts(const LossRows &a, int64_t row, int64_t id) {
     return id >= 0 && (a.mask == nullptr || a.mask[row] != 0);
@@ -229,13 +233,19 @@ __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l
     return by_lp * w;
 }
 
+// f(true) or f(false), for code that is compiled for either
+template <typename F> __device__ __forceinline__ void either(bool which, F &&f) {
+    if (which) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 // Zeros over a row of the gradient.
 template <typename T, int kT> __device__ __forceinline__ void zero_row(T *out, int V) {
     constexpr int kN = Vec<T>::kN;
     const int full = V / kN;
     Bits<T> z;
     z.zero();
-    for (int j = threadIdx.x; j < full; j += kT) z.store(out + (int64_t)j * kN);
+    for (int j = threadIdx.x; j < full; j += kT) z.template store<true>(out + (int64_t)j * kN);
     if ((int)threadIdx.x < V - full * kN) store1(out + full * kN + threadIdx.x, 0.f);
 }
 
@@ -255,14 +265,16 @@ template <typename T> __device__ __forceinline__ float gradient(float x, const S
 // A workgroup takes a row.  kVecs > 0: the row is read once, into registers (kVecs vectors of 16 bytes to a thread); the up to 7 elements
 // behind the last whole vector are one more element each to the first threads.  kVecs = 0: rows of any length, a running maximum and sum
 // to a thread, and a second reading for the gradient.
+constexpr int waves_per_simd(int threads, int vecs) { return threads == 1024 && vecs <= 8 ? 8 : 4; }
+
 template <typename T, int kT, int kVecs, bool kGrad>
-__global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_kernel(LossRows a, LossCounts n, LossTerms l, T *__restrict__ grad) {
+__global__ __launch_bounds__(kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g) {
     constexpr int kN = Vec<T>::kN, kW = kT / 64, kHeld = kVecs > 0 ? kVecs : kStreamVecs;
     __shared__ float part_max[kW], part_sum[kW], part_c;
-    const int64_t row = row_of(a, blockIdx.x), b = row / a.T;
+    const int64_t row = blockIdx.x, b = row / a.T;
     const int64_t id = a.ids[row];
     const int V = (int)a.V, full = V / kN, tid = threadIdx.x;
-    T *out = kGrad ? grad + row * V : nullptr;
+    T *out = kGrad ? static_cast<T *>(g.grad) + row * V : nullptr;
     if (!counts(a, row, id)) {
         if (tid == 0) {
             if (a.logps) a.logps[row] = 0.f;
@@ -280,11 +292,13 @@ __global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_ker
     float rest = tid < V - full * kN ? load1(x + full * kN + tid) : -INFINITY;
     float top, sum;
     if (kVecs > 0) {
+        either(kGrad || !a.stats, [&](auto past) {   // (read once, or once more by a backward)
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            if (i * kT + tid < full) held[i].load(x + (int64_t)(i * kT + tid) * kN);
-            else held[i].none();
-        }
+            for (int i = 0; i < kHeld; ++i) {
+                if (i * kT + tid < full) held[i].template load<past.value>(x + (int64_t)(i * kT + tid) * kN);
+                else held[i].none();
+            }
+        });
     }
     const float w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
     const float stands = id < V ? load1(x + id) : NAN;
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_ker
             float most = mine;
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
-                if (first + i * kT < full) held[i].load(x + (int64_t)(first + i * kT) * kN);
+                if (first + i * kT < full) held[i].template load<false>(x + (int64_t)(first + i * kT) * kN);
                 else held[i].none();
             }
 #pragma unroll
@@ -360,22 +374,24 @@ __global__ __launch_bounds__(kT, kT == 1024 && kVecs <= 8 ? 8 : 4) void rows_ker
     c *= a.inv_temperature;
     const float norm = 1.f / sum, factor = -c * norm;
     if (kVecs > 0) {
+        either(g.past, [&](auto past) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            held[i].again();
-            gradient<T>(held[i], scale, top, factor);
-            if (i * kT + tid < full) held[i].store(out + (int64_t)(i * kT + tid) * kN);
-        }
+            for (int i = 0; i < kHeld; ++i) {
+                held[i].again();
+                gradient<T>(held[i], scale, top, factor);
+                if (i * kT + tid < full) held[i].template store<past.value>(out + (int64_t)(i * kT + tid) * kN);
+            }
+        });
     } else {
         for (int first = tid; first < full; first += kHeld * kT) {
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
-                if (first + i * kT < full) held[i].load(x + (int64_t)(first + i * kT) * kN);
+                if (first + i * kT < full) held[i].template load<false>(x + (int64_t)(first + i * kT) * kN);
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
                 if (first + i * kT >= full) continue;
                 gradient<T>(held[i], scale, top, factor);
-                held[i].store(out + (int64_t)(first + i * kT) * kN);
+                held[i].template store<true>(out + (int64_t)(first + i * kT) * kN);
             }
         }
     }
@@ -412,7 +428,7 @@ __global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTe
     __shared__ double part[2][kFinish / 64];
     __shared__ int count[2][kFinish / 64];
     const int half = kFinish / 2, i = threadIdx.x / half;   // the first half of the threads takes the chosen text
-    const int64_t P = a.B / 2, pair = a.first + blockIdx.x, b = pair + i * P, first = b * a.T;
+    const int64_t P = a.B / 2, pair = blockIdx.x, b = pair + i * P, first = b * a.T;
     double v = wave_sum(strided_sum(a.exact + first, threadIdx.x % half, a.T, half));
     int n = 0;
     if (l.average)
@@ -459,8 +475,7 @@ __global__ __launch_bounds__(kFinish) void pairs_finish_kernel(int64_t P, Prefer
     if (threadIdx.x == 0) l.loss[0] = (float)s;
 }
 
-// The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, `pieces` workgroups to a row.  The last
-// rows come first: those are the ones that a pass over all rows before this one may have left in the last-level cache.
+// The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, some workgroups to a row.
 template <typename T> __device__ __forceinline__ void grad_piece(const LossRows &a, const LossGrad &g, float up, int64_t row, int piece) {
     constexpr int kN = Vec<T>::kN;
     const int64_t b = row / a.T, t = row % a.T;
@@ -473,7 +488,7 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
         z.zero();
 #pragma unroll
         for (int i = 0; i < kGradVecs; ++i)
-            if (first + i * kThreads < full) z.store(out + (int64_t)(first + i * kThreads) * kN);
+            if (first + i * kThreads < full) z.template store<true>(out + (int64_t)(first + i * kThreads) * kN);
         if (behind >= 0) store1(out + behind, 0.f);
         return;
     }
@@ -481,18 +496,20 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
     Bits<T> held[kGradVecs];
 #pragma unroll
     for (int i = 0; i < kGradVecs; ++i)
-        if (first + i * kThreads < full) held[i].load(x + (int64_t)(first + i * kThreads) * kN);
+        if (first + i * kThreads < full) held[i].template load<false>(x + (int64_t)(first + i * kThreads) * kN);
     float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up;
     if (id >= V) c = NAN;
     c *= a.inv_temperature;
     const float top = a.stats[2 * row], norm = 1.f / a.stats[2 * row + 1], factor = -c * norm;
     const Scale scale(a.inv_temperature);
+    either(g.past, [&](auto past) {
 #pragma unroll
-    for (int i = 0; i < kGradVecs; ++i) {
-        if (first + i * kThreads >= full) continue;
-        gradient<T>(held[i], scale, top, factor);
-        held[i].store(out + (int64_t)(first + i * kThreads) * kN);
-    }
+        for (int i = 0; i < kGradVecs; ++i) {
+            if (first + i * kThreads >= full) continue;
+            gradient<T>(held[i], scale, top, factor);
+            held[i].template store<past.value>(out + (int64_t)(first + i * kThreads) * kN);
+        }
+    });
     if (behind >= 0) store1(out + behind, gradient<T>(load1(x + behind), scale, top, factor));
     // the element that stands there, by the thread whose store it was in
     if (id >= V) return;
@@ -501,10 +518,12 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
     if (mine) store1(out + id, c + scale.exp_once(load1(x + id) - top) * factor);
 }
 
+// (The last rows come first: those are the ones that a pass over all rows before this one may have left in the last-level cache.)
 template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces, int64_t rows) {
     const float up = g.upstream ? *g.upstream : 1.f;
     if (g.is_there && up == 1.f) return;
-    for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x) grad_piece<T>(a, g, up, row_of(a, rows - 1 - i / pieces), (int)(i % pieces));
+    for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x)
+        grad_piece<T>(a, g, up, rows - 1 - i / pieces, (int)(i % pieces));
 }
 
 template <typename F> hipError_t by_type(int dtype, F &&f) {
@@ -523,23 +542,31 @@ size_t loss_workspace_bytes(int64_t B, int64_t T) {
 
 namespace {
 
-int64_t rows_in(const LossRows &a) { return (a.jump > 0 ? 2 : 1) * a.part * a.T; }
+// Whether the gradient is written past the caches: from the size on that they do not hold for whoever reads it next.
+bool past_the_caches(int dtype, const LossRows &a) { return a.B * a.T * a.V * (dtype == kF32 ? 4 : 2) >= kPastBytes; }
 
-template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRows &a, const LossCounts &n, const LossTerms &l, void *grad) {
-    const dim3 grid((unsigned)rows_in(a));
-    T *out = static_cast<T *>(grad);
-    const int64_t vecs = a.V / Vec<T>::kN;
-    // (the smallest class that holds a row)
-    if (vecs <= 256 * 1) hipLaunchKernelGGL((rows_kernel<T, 256, 1, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
-    else if (vecs <= 256 * 2) hipLaunchKernelGGL((rows_kernel<T, 256, 2, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
-    else if (vecs <= 256 * 4) hipLaunchKernelGGL((rows_kernel<T, 256, 4, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
-    else if (vecs <= 256 * 8) hipLaunchKernelGGL((rows_kernel<T, 256, 8, kGrad>), grid, dim3(256), 0, st, a, n, l, out);
-    else if (vecs <= 1024 * 4) hipLaunchKernelGGL((rows_kernel<T, 1024, 4, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
-    else if (vecs <= 1024 * 8) hipLaunchKernelGGL((rows_kernel<T, 1024, 8, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
-    else if (vecs <= 1024 * 12) hipLaunchKernelGGL((rows_kernel<T, 1024, 12, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
-    else if (vecs <= 1024 * 16) hipLaunchKernelGGL((rows_kernel<T, 1024, 16, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
-    else if (vecs <= 1024 * 20) hipLaunchKernelGGL((rows_kernel<T, 1024, 20, kGrad>), grid, dim3(1024), 0, st, a, n, l, out);
-    else hipLaunchKernelGGL((rows_kernel<T, kStream, 0, kGrad>), grid, dim3(kStream), 0, st, a, n, l, out);
+// f(threads, vectors of a thread) of the smallest class that holds a row
+template <typename T, typename F> void by_length(int64_t V, F &&f) {
+    const auto as = [&](auto threads, auto vecs) { f(threads, vecs); };
+    const int64_t n = V / Vec<T>::kN;
+    std::integral_constant<int, 256> few;
+    std::integral_constant<int, 1024> many;
+    if (n <= 256 * 1) as(few, std::integral_constant<int, 1>{});
+    else if (n <= 256 * 2) as(few, std::integral_constant<int, 2>{});
+    else if (n <= 256 * 4) as(few, std::integral_constant<int, 4>{});
+    else if (n <= 256 * 8) as(few, std::integral_constant<int, 8>{});
+    else if (n <= 1024 * 4) as(many, std::integral_constant<int, 4>{});
+    else if (n <= 1024 * 8) as(many, std::integral_constant<int, 8>{});
+    else if (n <= 1024 * 12) as(many, std::integral_constant<int, 12>{});
+    else if (n <= 1024 * 16) as(many, std::integral_constant<int, 16>{});
+    else if (n <= 1024 * 20) as(many, std::integral_constant<int, 20>{});
+    else as(many, std::integral_constant<int, 0>{});
+}
+
+template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRows &a, const LossCounts &n, const LossTerms &l, const LossGrad &g) {
+    by_length<T>(a.V, [&](auto threads, auto vecs) {
+        hipLaunchKernelGGL((rows_kernel<T, threads.value, vecs.value, kGrad>), dim3((unsigned)(a.B * a.T)), dim3(threads.value), 0, st, a, n, l, g);
+    });
 }
 
 }  // namespace
@@ -557,8 +584,8 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n);
     }
     hipError_t e = by_type(dtype, [&](auto t) {
-        if (grad) launch_rows<decltype(t), true>(st, a, n, l, grad);
-        else launch_rows<decltype(t), false>(st, a, n, l, nullptr);
+        if (grad) launch_rows<decltype(t), true>(st, a, n, l, LossGrad{nullptr, 0, 0, nullptr, 0, grad, past_the_caches(dtype, a)});
+        else launch_rows<decltype(t), false>(st, a, n, l, LossGrad{});
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
     hipLaunchKernelGGL(finish_kernel, dim3(l.count), dim3(kFinish), 0, st, rows, l);
@@ -566,30 +593,22 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
 }
 
 hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g) {
+    g.past = past_the_caches(dtype, a);
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per, all = rows_in(a) * pieces;
+        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per, all = a.B * a.T * pieces;
         // (most often there is nothing to do where a forward has written the gradient: 32768 workgroups took 9 us to find that out)
         const int64_t most = g.is_there ? 2048 : 0x7fffffff;
-        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, rows_in(a));
+        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, a.B * a.T);
     });
 }
 
-hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l, void *grad) {
-    const int64_t P = a.B / 2, bytes = 2 * a.T * a.V * (dtype == kF32 ? 4 : 2);
-    int64_t pairs = P;
-    if (grad) pairs = bytes > kPairBytes ? 1 : kPairBytes / bytes;
+hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerms l) {
+    const int64_t P = a.B / 2;
     l.by_pair = a.exact + a.B * a.T;
-    a.jump = P;
-    for (int64_t first = 0; first < P; first += pairs) {
-        a.first = first;
-        a.part = P - first < pairs ? P - first : pairs;
-        hipError_t e = loss_rows(st, dtype, a, LossTerms{}, nullptr, nullptr);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)a.part), dim3(kFinish), 0, st, a, l);
-        if (grad) e = loss_grad(st, dtype, a, LossGrad{l.coef, 1, 0, nullptr, 0, grad});
-        if (e != hipSuccess) return e;
-    }
+    const hipError_t e = loss_rows(st, dtype, a, LossTerms{}, nullptr, nullptr);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)P), dim3(kFinish), 0, st, a, l);
     hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(kFinish), 0, st, P, l);
     return hipGetLastError();
 }

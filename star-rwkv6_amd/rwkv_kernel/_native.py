@@ -63,10 +63,9 @@ SIGNATURES = {
     "wkv6_loss_workspace_bytes": (_sz, [_i64] * 2),
     "wkv6_cross_entropy": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 2 + [_int] + [_p] * 4 + [_p, _sz]),
     "wkv6_policy_loss": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 4 + [_i64] * 2 + [_p] + [_f] * 4 + [_int] + [_p] * 6 + [_p, _sz]),
-    "wkv6_preference_loss": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 3 + [_int, _d, _d, _int] + [_p] * 6 + [_sz]),
+    "wkv6_preference_loss": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 3 + [_int, _d, _d, _int] + [_p] * 5 + [_sz]),
     "wkv6_logits_backward": (_int, [_p, _int] + [_i64] * 3 + [_p] + [_i64] * 2 + [_p] * 2 + [_f] + [_p] * 2 + [_i64] * 2 + [_p, _int, _p]),
-    "wkv6_adamw_workspace_bytes": (_sz, [_i64]),
-    "wkv6_adamw_step": (_int, [_p, _int, _int, _i64, _p, _p, _p] + [_d] * 6 + [_int, _p, ctypes.c_uint32, _p, _sz]),
+    "wkv6_adamw_step": (_int, [_p, _int, _int, _i64, _p, _p, _p] + [_d] * 6 + [_int, _p, ctypes.c_uint32]),
     "wkv6_grad_norm_workspace_bytes": (_sz, [_i64]),
     "wkv6_grad_norm": (_int, [_p, _int, _i64, _p, _p, _p, _sz]),
     "wkv6_create_descriptor": (_sz, [_int] * 7 + [_p]),

@@ -82,7 +82,7 @@ def preference_loss(logits, ids, mask=None, ref_logps=None, beta=0.1, kind="sigm
         "hinge"    max(0, 1 - beta d)
         "ipo"      (d - 1 / (2 beta))^2
     Returns (loss, s): an fp32 scalar, differentiable in logits, and the 2 P values of s, which carry no gradient.  The coefficient of a
-    token's gradient depends on both whole texts, so a pair's logits are read twice, if they fit its last-level cache once from memory."""
+    token's gradient depends on both whole texts, so the logits are read twice."""
     logits, ids, mask = _rows(logits, ids, mask, False)
     B = logits.shape[0]
     assert B % 2 == 0 and B > 0, "the batch holds the chosen texts, then as many rejected ones"

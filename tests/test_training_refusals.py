@@ -41,7 +41,7 @@ def _calls(lib, rows, workspace=OK, bytes_=1 << 20, **kw):
         "cross_entropy": lambda: lib.wkv6_cross_entropy(*rows, a["red"], a["loss"], a["stats"], a["coef"], a["grad"], *ws),
         "policy": lambda: lib.wkv6_policy_loss(*rows, None, a["adv"], 1, 0, None, a["lo"], a["hi"], a["klw"], a["temperature"], a["red"], a["loss"], a["logps"], a["means"],
                                                a["stats"], a["coef"], a["grad"], *ws),
-        "preference": lambda: lib.wkv6_preference_loss(*rows, None, a["kind"], a["beta"], a["ls"], 0, a["loss"], a["text"], a["stats"], a["coef"], a["grad"], *ws),
+        "preference": lambda: lib.wkv6_preference_loss(*rows, None, a["kind"], a["beta"], a["ls"], 0, a["loss"], a["text"], a["stats"], a["coef"], *ws),
         "backward": lambda: lib.wkv6_logits_backward(*rows, a["temperature"], a["stats"], a["coef"], 1, 0, a["up"], a["there"], a["grad"]),
     }
 
@@ -58,7 +58,7 @@ def test_rows_of_logits(native):
     for bad, who in ((dict(temperature=0.0), "logprobs policy backward"), (dict(temperature=nan), "logprobs policy backward"),
                      (dict(temperature=float("inf")), "logprobs policy backward"), (dict(logps=None), "logprobs policy"), (dict(loss=None), "cross_entropy policy preference"),
                      (dict(loss=OFF), "cross_entropy policy preference"), (dict(stats=OK + 2), "logprobs cross_entropy policy preference backward"),
-                     (dict(grad=OFF), "cross_entropy policy preference backward"), (dict(stats=None), "cross_entropy policy preference backward"), (dict(coef=None), "cross_entropy policy preference backward"),
+                     (dict(grad=OFF), "cross_entropy policy backward"), (dict(stats=None), "cross_entropy policy backward"), (dict(coef=None), "cross_entropy policy backward"),
                      (dict(grad=None), "backward"), (dict(up=None, there=1), "backward"), (dict(red=3), "cross_entropy policy"), (dict(red=2), "cross_entropy"), (dict(red=0), "policy"),
                      (dict(adv=None), "policy"), (dict(means=None), "policy"), (dict(lo=-0.1), "policy"), (dict(hi=nan), "policy"), (dict(klw=nan), "policy"),
                      (dict(kind=3), "preference"), (dict(beta=0.0), "preference"), (dict(beta=nan), "preference"), (dict(ls=0.5), "preference"),
@@ -82,9 +82,9 @@ def test_optimizer(native):
     lib = native.load()
     good = dict(param=OK, grad=OK, exp_avg=OK, exp_avg_sq=OK, scales=OK, master=None, numel=10)
 
-    def step(rows=(good,), dtype=0, bits=32, count=None, step=OK, lr_device=None, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, clip=0.0, skip=0, norm=None, ws=OK, n=1 << 20):
+    def step(rows=(good,), dtype=0, bits=32, count=None, step=OK, lr_device=None, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, clip=0.0, skip=0, norm=None):
         t = _tensors(native, *rows)
-        return lib.wkv6_adamw_step(None, dtype, bits, len(rows) if count is None else count, t if rows else None, step, lr_device, lr, b1, b2, eps, wd, clip, skip, norm, 0, ws, n)
+        return lib.wkv6_adamw_step(None, dtype, bits, len(rows) if count is None else count, t if rows else None, step, lr_device, lr, b1, b2, eps, wd, clip, skip, norm, 0)
 
     nan = float("nan")
     for bad in (dict(dtype=3), dict(bits=16), dict(count=0), dict(count=1 << 31), dict(step=None), dict(step=OK + 4), dict(lr=-1.0), dict(lr=nan), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0),
@@ -93,7 +93,6 @@ def test_optimizer(native):
                 dict(rows=(dict(good, scales=None),), bits=8), dict(rows=(dict(good, scales=OK + 4),), bits=8), dict(rows=(dict(good, master=OFF),)),
                 dict(rows=(dict(good, numel=-1),)), dict(rows=(dict(good, numel=1 << 40),)), dict(rows=(dict(good, param=OFF),)), dict(dtype=2, rows=(dict(good, grad=OK + 2),))):
         assert step(**bad) == 1, bad
-    assert step(ws=None) == 3 and step(ws=OK + 8) == 3 and step(n=lib.wkv6_adamw_workspace_bytes(1) - 1) == 3
     rows = _tensors(native, dict(grad=OK, numel=10))
     n = lib.wkv6_grad_norm_workspace_bytes(1)
     assert n > 0 and lib.wkv6_grad_norm_workspace_bytes(0) == 0
