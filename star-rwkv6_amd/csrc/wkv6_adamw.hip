@@ -13,6 +13,8 @@
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
+#include <math.h>
+
 #include <type_traits>
 
 namespace wkv6 {
@@ -32,7 +34,6 @@ struct Group {
     int count;
     int number;              // of the first tensor in the call's list
     int last;                // whether nothing of the call follows
-    int past;                // whether tensors are read and written past the caches
 };
 
 // What a step is done with.
@@ -154,7 +155,7 @@ template <int kEach> __device__ __forceinline__ void pack(const float (&v)[kEach
     for (int i = 0; i < kEach / 2; ++i) b.r[i] = __builtin_bit_cast(uint32_t, (h2){to_f16(v[2 * i]), to_f16(v[2 * i + 1])});
 }
 
-template <typename F> __device__ __forceinline__ void either(bool which, F &&f) {
+template <typename F> void either(bool which, F &&f) {   // f(true) or f(false), for code that is compiled for either
     if (which) f(std::true_type{});
     else f(std::false_type{});
 }
@@ -209,8 +210,8 @@ __device__ Plan plan_of(const AdamwStep &a) {
     const uint32_t t = (uint32_t)__hip_atomic_load(a.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
     const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
     p.decay = (float)(1. - lr * a.weight_decay);
-    p.rate = (float)(lr / (1. - pow(a.beta1, (double)t)));
-    p.root = (float)(1. / sqrt(1. - pow(a.beta2, (double)t)));
+    p.rate = (float)(lr / -expm1((double)t * a.log_beta1));
+    p.root = (float)(1. / sqrt(-expm1((double)t * a.log_beta2)));
     p.key = a.seed * 0x9E3779B9u + t * 0xBB67AE85u;
     return p;
 }
@@ -264,16 +265,12 @@ __device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r,
         unpack(v8[i], v);
         if constexpr (kMaster) unpack(w8[i], w);
         else unpack(p8[i], w);
+        const float by_m = kBits == 8 ? scale[i].x * r.b1 : r.b1, by_v = kBits == 8 ? scale[i].y * scale[i].y * r.b2 : r.b2;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            if (kBits == 8) {
-                m[e] *= scale[i].x;
-                v[e] *= scale[i].y;
-                v[e] *= v[e];
-            }
             g[e] *= q.clip;
-            m[e] = m[e] * r.b1 + g[e] * r.c1;
-            v[e] = v[e] * r.b2 + g[e] * g[e] * r.c2;
+            m[e] = m[e] * by_m + g[e] * r.c1;
+            v[e] = (kBits == 8 ? v[e] * v[e] : v[e]) * by_v + g[e] * g[e] * r.c2;
             // (root and reciprocal to one unit in the last place of fp32; correctly rounded ones take some twenty operations more)
             root[e] = __builtin_amdgcn_sqrtf(v[e]);
             w[e] = w[e] * q.decay - m[e] * q.rate * __builtin_amdgcn_rcpf(root[e] * q.root + r.eps);
@@ -316,7 +313,9 @@ __device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r,
     }
 }
 
-template <typename T, int kBits> __global__ __launch_bounds__(kThreads) void step_kernel(Group g, Rates r, AdamwStep a) {
+// kMaster: some tensor has a master.
+template <typename T, int kBits, bool kMaster, bool kPast>
+__global__ __launch_bounds__(kThreads) void step_kernel(Group g, Rates r, AdamwStep a) {
     __shared__ Plan plan;
     if (threadIdx.x == 0) plan = plan_of(a);
     __syncthreads();
@@ -327,12 +326,8 @@ template <typename T, int kBits> __global__ __launch_bounds__(kThreads) void ste
         const AdamwTensor t = g.t[k];
         const uint32_t key = mix(q.key + (uint32_t)(g.number + k));
         const int64_t first = (int64_t)(chunk - g.first[k]) * kChunk;
-        either(g.past, [&](auto past) {
-            if constexpr (sizeof(T) == 2) {
-                if (t.master) return step_chunk<T, kBits, true, past.value>(t, r, q, key, first);
-            }
-            step_chunk<T, kBits, false, past.value>(t, r, q, key, first);
-        });
+        if (kMaster && t.master) step_chunk<T, kBits, kMaster, kPast>(t, r, q, key, first);
+        else step_chunk<T, kBits, false, kPast>(t, r, q, key, first);
     }
     // The step count moves on when the last workgroup has read it: the workgroups that have are counted in its upper half.
     if (!g.last || threadIdx.x != 0) return;
@@ -388,13 +383,23 @@ hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor
 
 hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s) {
     const Rates r{(float)s.beta1, (float)(1. - s.beta1), (float)s.beta2, (float)(1. - s.beta2), (float)s.eps};
+    AdamwStep a = s;
+    a.log_beta1 = log(s.beta1), a.log_beta2 = log(s.beta2);   // (of 0: -inf, and the power 0)
     int64_t bytes = 0;
-    for (int64_t i = 0; i < count; ++i) bytes += tensors[i].numel * ((dtype == kF32 ? 4 : 2) * 2 + moment_bits / 4 + (tensors[i].master ? 4 : 0));
+    bool master = false;
+    for (int64_t i = 0; i < count; ++i) {
+        bytes += tensors[i].numel * ((dtype == kF32 ? 4 : 2) * 2 + moment_bits / 4 + (tensors[i].master ? 4 : 0));
+        master |= tensors[i].master != nullptr;
+    }
     return by_type(dtype, [&](auto t) {
-        by_group(count, tensors, [&](Group &g, int blocks) {
-            g.past = bytes >= kPastBytes;
-            if (moment_bits == 8) hipLaunchKernelGGL((step_kernel<decltype(t), 8>), dim3(blocks), dim3(kThreads), 0, st, g, r, s);
-            else hipLaunchKernelGGL((step_kernel<decltype(t), 32>), dim3(blocks), dim3(kThreads), 0, st, g, r, s);
+        either(moment_bits == 8, [&](auto eight) {
+            either(master, [&](auto any) {
+                either(bytes >= kPastBytes, [&](auto past) {
+                    by_group(count, tensors, [&](const Group &g, int blocks) {
+                        hipLaunchKernelGGL((step_kernel<decltype(t), eight.value ? 8 : 32, any.value, past.value>), dim3(blocks), dim3(kThreads), 0, st, g, r, a);
+                    });
+                });
+            });
         });
     });
 }

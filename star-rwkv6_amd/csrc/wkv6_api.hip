@@ -455,7 +455,7 @@ int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, con
     if (!(lr >= 0.) || !(beta1 >= 0. && beta1 < 1.) || !(beta2 >= 0. && beta2 < 1.) || !(eps >= 0.) || !(weight_decay >= 0.) || !(max_grad_norm >= 0.)) return WKV6_ERR_ARG;
     if ((max_grad_norm > 0. || skip_nonfinite) && !grad_norm) return WKV6_ERR_ARG;
     return finish(wkv6::adamw_step((hipStream_t)stream, dtype, moment_bits, count, reinterpret_cast<const wkv6::AdamwTensor *>(tensors),
-                                   wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed}));
+                                   wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed, 0., 0.}));
 }
 
 static int check_mix(int dtype, int64_t B, int64_t T, int64_t C, int64_t R) {

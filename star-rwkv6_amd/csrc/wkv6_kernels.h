@@ -400,6 +400,7 @@ struct AdamwStep {
     int skip_nonfinite;
     const float *grad_norm;       // one value, or null where neither of the two needs it
     uint32_t seed;
+    double log_beta1, log_beta2;  // set inside
 };
 size_t grad_norm_workspace_bytes(int64_t count);
 hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor *tensors, float *norm, void *workspace);
