@@ -214,13 +214,13 @@ def bench_model_step(a):
     JSON line: whole-step tokens/s and the share of the step spent inside the operator."""
     import torch
     import rwkv6_harness as hz
-    from rwkv_kernel import RWKVKernelOperator
+    from rwkv_kernel import AdamW, RWKVKernelOperator
 
     dev = torch.device("cuda:0")
     torch.manual_seed(a.seed)
     B, T = 8, 1024
     model = hz.RWKV6(RWKVKernelOperator(64, T), **hz.CONFIG4).to(dev)
-    opt = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=True)
+    opt = AdamW(model.parameters(), lr=1e-4)
     ids = torch.randint(0, hz.CONFIG4["vocabulary_size"], (B, T + 1), device=dev)
     steps, warm = min(a.steps, 10), min(a.warmup, 3)
     losses = [float(hz.train_step(model, opt, ids, torch.bfloat16)) for _ in range(warm)]

@@ -21,6 +21,7 @@ python loop) anywhere.  Initialisation is random (small normal / uniform decay r
 checkpoint format is read or written here.
 """
 import math
+import os
 
 import torch
 from torch import nn
@@ -181,16 +182,62 @@ class RWKV6(nn.Module):
         return self.output_layer(self.output_ln(x))
 
 
-def train_step(model, optimizer, ids, autocast_dtype=None):
-    """One next-token cross-entropy step: forward, backward, optimizer update.  Returns the loss."""
-    optimizer.zero_grad(set_to_none=True)
+def _kernels(logits):
+    """The operator package where it has losses for these logits (its torch flavour, on the GPU), else None."""
+    if not logits.is_cuda or os.environ.get("KERAS_BACKEND") != "torch":
+        return None
+    import rwkv_kernel
+
+    return rwkv_kernel
+
+
+def _logits(model, ids, autocast_dtype):
+    """The model's logits for every token but the first of each text."""
     dev = ids.device.type
     with torch.autocast(dev, dtype=autocast_dtype, enabled=autocast_dtype is not None):
-        logits = model(ids[:, :-1])
-    loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), ids[:, 1:].reshape(-1))
+        return model(ids[:, :-1])
+
+
+def _update(optimizer, loss):
     loss.backward()
     optimizer.step()
     return loss.detach()
+
+
+def train_step(model, optimizer, ids, autocast_dtype=None):
+    """One next-token cross-entropy step: forward, backward, optimizer update.  Returns the loss."""
+    optimizer.zero_grad(set_to_none=True)
+    logits, target = _logits(model, ids, autocast_dtype), ids[:, 1:]
+    kernels = _kernels(logits)
+    if kernels is not None:
+        return _update(optimizer, kernels.cross_entropy(logits, target))
+    return _update(optimizer, F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), target.reshape(-1)))
+
+
+# Fine-tuning steps on the operator package's losses (its torch flavour, on the GPU).  Texts are ids (B, T+1); mask (B, T) says which of
+# their tokens from the second on count (a prompt's and the padding's do not).
+
+@torch.no_grad()
+def token_logprobs(model, ids, mask, autocast_dtype=None, temperature=1.0):
+    """Log probabilities (B, T) of the texts' tokens: what a reference or a sampling model makes of them."""
+    logits = _logits(model, ids, autocast_dtype)
+    return _kernels(logits).token_logprobs(logits, ids[:, 1:], mask, temperature=temperature)
+
+
+def preference_step(model, optimizer, ids, mask, ref_logps, autocast_dtype=None, **options):
+    """One step on pairs of texts, the chosen ones and then as many rejected ones.  ref_logps (B): sums of the reference model's token_logprobs; options
+    as of rwkv_kernel.preference_loss.  Returns the loss."""
+    optimizer.zero_grad(set_to_none=True)
+    logits = _logits(model, ids, autocast_dtype)
+    return _update(optimizer, _kernels(logits).preference_loss(logits, ids[:, 1:], mask, ref_logps=ref_logps, **options)[0])
+
+
+def policy_step(model, optimizer, ids, mask, old_logps, advantages, autocast_dtype=None, **options):
+    """One step on sampled texts: old_logps (B, T) are the sampling model's token_logprobs, advantages (B,) or (B, T); options as of
+    rwkv_kernel.policy_loss.  Returns the loss."""
+    optimizer.zero_grad(set_to_none=True)
+    logits = _logits(model, ids, autocast_dtype)
+    return _update(optimizer, _kernels(logits).policy_loss(logits, ids[:, 1:], mask, old_logps, advantages, **options)[0])
 
 
 # the layer shape of configuration 4: RWKV6-1.6B (24 layers, d_model 2048, 32 heads of 64, FFN 7168)
