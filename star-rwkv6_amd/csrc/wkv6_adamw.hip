@@ -234,6 +234,33 @@ __device__ __forceinline__ uint32_t to_float8(float x, uint32_t random16) {
     return min((__float_as_uint(fabsf(x) * 0x1p-120f) + (random16 << 4)) >> 20, 0x7Eu);
 }
 
+// The square root rounded to the nearest, of anything from 2^-96 on (below, to one unit in the last place): the instruction's is off by one unit at
+// most, and the sign of x - s t for it and a neighbour t says which one is nearer.
+__device__ __forceinline__ float root_of(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float below = __uint_as_float(__float_as_uint(s) - 1), above = __uint_as_float(__float_as_uint(s) + 1);
+    const float r = __builtin_fmaf(-below, s, x) <= 0.f ? below : s;
+    return __builtin_fmaf(-above, s, x) > 0.f ? above : r;
+}
+
+__device__ __forceinline__ void new_moments32(float g, float &m, float &v, float &root, const Rates &r, float clip) {
+    g *= clip;
+    m = m * r.b1 + g * r.c1;
+    v = v * r.b2 + g * g * r.c2;
+    root = __builtin_amdgcn_sqrtf(v);
+}
+// Moments that will be held in 8 bits: every product, sum and root is rounded by itself, to the nearest.  Where one lies next to a value of float8
+// the last bit decides which one it becomes, and the next step starts from there: so the result is that of the formula's operations
+// in fp32, one after the other, and not of what a compiler joins.
+__device__ __forceinline__ void new_moments8(float g, float &m, float &v, float &root, float2 scale, const Rates &r, float clip) {
+#pragma clang fp contract(off)
+    g *= clip;
+    const float m0 = m * scale.x, r0 = v * scale.y;
+    m = m0 * r.b1 + g * r.c1;
+    v = r0 * r0 * r.b2 + g * g * r.c2;
+    root = root_of(v);
+}
+
 template <typename T, int kBits, bool kMaster, bool kPast>
 __device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r, const Plan &q, uint32_t key, int64_t first) {
     typedef std::conditional_t<kBits == 8, uint8_t, float> M;
@@ -265,14 +292,11 @@ __device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r,
         unpack(v8[i], v);
         if constexpr (kMaster) unpack(w8[i], w);
         else unpack(p8[i], w);
-        const float by_m = kBits == 8 ? scale[i].x * r.b1 : r.b1, by_v = kBits == 8 ? scale[i].y * scale[i].y * r.b2 : r.b2;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            g[e] *= q.clip;
-            m[e] = m[e] * by_m + g[e] * r.c1;
-            v[e] = (kBits == 8 ? v[e] * v[e] : v[e]) * by_v + g[e] * g[e] * r.c2;
+            if constexpr (kBits == 8) new_moments8(g[e], m[e], v[e], root[e], scale[i], r, q.clip);
+            else new_moments32(g[e], m[e], v[e], root[e], r, q.clip);
             // (root and reciprocal to one unit in the last place of fp32; correctly rounded ones take some twenty operations more)
-            root[e] = __builtin_amdgcn_sqrtf(v[e]);
             w[e] = w[e] * q.decay - m[e] * q.rate * __builtin_amdgcn_rcpf(root[e] * q.root + r.eps);
         }
         if constexpr (kMaster) {
@@ -293,7 +317,7 @@ __device__ __forceinline__ void step_chunk(const AdamwTensor &t, const Rates &r,
             const float sm = top_m < 0x1p-100f ? 0x1p-100f : top_m, sr = top_r < 0x1p-100f ? 0x1p-100f : top_r;
             if (threadIdx.x % (kScaleBlock / kEach) == 0 && n > 0)
                 *reinterpret_cast<float2 *>(t.scales + 2 * (at / kScaleBlock)) = make_float2(sm * (1.f / 448.f), sr * (1.f / 448.f));
-            const float im = 448.f / sm, ir = 448.f / sr;
+            const float im = 1.f / sm * 448.f, ir = 1.f / sr * 448.f;
             const uint32_t start = (uint32_t)at * 0x9E3779B9u + key;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
