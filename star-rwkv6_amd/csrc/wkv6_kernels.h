@@ -347,7 +347,7 @@ struct LossRows {
     double *exact;  // (B,T) logps in 64 bits, or null
 };
 struct LossCounts {
-    int *by_text, *tokens, *texts;   // counted tokens of each text; of each counting workgroup's texts: tokens, texts that have any
+    int *by_text, *partial;   // counted tokens of each text; each counting workgroup's tokens, or texts that have any
     int blocks;
 };
 enum { kLossNone = 0, kLossCrossEntropy = 1, kLossPolicy = 2 };

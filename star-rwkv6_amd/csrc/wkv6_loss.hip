@@ -23,7 +23,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFinish = 1024;        // threads of the one workgroup that adds up
 constexpr int kCountBlocks = 256;    // at most
-constexpr int kStream = 1024, kStreamVecs = 4;   // rows that no registers hold: threads, vectors of a thread in flight
+constexpr int kStretches = 256;      // of a great many rows
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
 // A gradient of this size and more is written past the caches.  Cross entropy, log probabilities with their backward, and the latter with a reader
 // of the gradient behind it, in us, written into / past them: 128 MiB 63 / 66, 78 / 78, 106 / 120; 192 MiB 89 / 89, 119 / 108, 178 / 171; 2 GiB (8 pairs
@@ -118,6 +118,21 @@ template <typename T> struct Bits {
     }
 };
 
+// How a row of V elements is taken: `full` vectors from its first 16-byte boundary on (loads across such boundaries are allowed, but slower: cross
+// entropy of 10682 rows of 50257 bf16 488 us with them, 410 without), and up to 14 single elements before and behind, one to a thread.
+template <typename T> struct Cut {
+    int head, full, singles;
+    __device__ __forceinline__ Cut(const T *x, int V) {
+        head = min(V, (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+        full = (V - head) / Vec<T>::kN;
+        singles = V - full * Vec<T>::kN;
+    }
+    __device__ __forceinline__ int single(int i) const { return i < head ? i : full * Vec<T>::kN + i; }
+    // whether element id is a single one, and which; or its vector
+    __device__ __forceinline__ int single_of(int id) const { return id < head ? id : id >= head + full * Vec<T>::kN ? id - full * Vec<T>::kN : -1; }
+    __device__ __forceinline__ int vector_of(int id) const { return (id - head) / Vec<T>::kN; }
+};
+
 __device__ __forceinline__ bool counts(const LossRows &a, int64_t row, int64_t id) {
     return id >= 0 && (a.mask == nullptr || a.mask[row] != 0);
 }
@@ -149,6 +164,7 @@ template <typename S> __device__ __forceinline__ S wave_sum(S v) {
 // Over the workgroup, for every thread; `part`: one value per wave in LDS that nothing else is read from meanwhile.
 template <int kW> __device__ __forceinline__ float block_max(float v, float *part) {
     v = wave_max(v);
+    if (kW == 1) return v;
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = part[0];
@@ -158,6 +174,7 @@ template <int kW> __device__ __forceinline__ float block_max(float v, float *par
 }
 template <int kW, typename S> __device__ __forceinline__ S block_sum(S v, S *part) {
     v = wave_sum(v);
+    if (kW == 1) return v;
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = part[0];
@@ -166,42 +183,52 @@ template <int kW, typename S> __device__ __forceinline__ S block_sum(S v, S *par
     return v;
 }
 
-// Counted tokens of each text, and of each workgroup's texts together: tokens, and texts that have any.  (One token after the other
-// to a thread would wait for two loads each: four go together, 6 us for 8 texts of 1024 tokens before, 3 now.)
-__global__ __launch_bounds__(kFinish) void count_kernel(LossRows a, LossCounts c) {
-    __shared__ int part[2][kFinish / 64];
-    int64_t tokens = 0, texts = 0;
-    int turn = 0;
-    for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x, turn ^= 1) {
-        const int64_t *ids = a.ids + b * a.T;
-        const uint8_t *mask = a.mask ? a.mask + b * a.T : nullptr;
-        int n = 0;
-        for (int64_t t = threadIdx.x; t < a.T; t += 4 * kFinish) {
-            int64_t id[4];
-            uint8_t m[4];
+// Counted tokens among n, by all threads of a workgroup.  (One token after the other to a thread would wait for two loads each: four go
+// together, 6 us for 8 texts of 1024 tokens before, 4 now.)
+__device__ __forceinline__ int count_tokens(const LossRows &a, int64_t first, int64_t n, int *part) {
+    const int64_t *ids = a.ids + first;
+    const uint8_t *mask = a.mask ? a.mask + first : nullptr;
+    int sum = 0;
+    for (int64_t t = threadIdx.x; t < n; t += 4 * kFinish) {
+        int64_t id[4];
+        uint8_t m[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = t + i * kFinish < a.T;
-                id[i] = in ? ids[t + i * kFinish] : -1;
-                m[i] = in && mask ? mask[t + i * kFinish] : 1;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) n += id[i] >= 0 && m[i] != 0;
+        for (int i = 0; i < 4; ++i) {
+            const bool in = t + i * kFinish < n;
+            id[i] = in ? ids[t + i * kFinish] : -1;
+            m[i] = in && mask ? mask[t + i * kFinish] : 1;
         }
-        n = block_sum<kFinish / 64>(n, part[turn]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += id[i] >= 0 && m[i] != 0;
+    }
+    return block_sum<kFinish / 64>(sum, part);
+}
+
+// Counted tokens of each text, and in how many texts of a workgroup's there are any.
+__global__ __launch_bounds__(kFinish) void count_texts_kernel(LossRows a, LossCounts c) {
+    __shared__ int part[2][kFinish / 64];
+    int texts = 0, turn = 0;
+    for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x, turn ^= 1) {
+        const int n = count_tokens(a, b * a.T, a.T, part[turn]);
         if (threadIdx.x == 0) c.by_text[b] = n;
-        tokens += n;
         texts += n > 0;
     }
-    if (threadIdx.x == 0) c.tokens[blockIdx.x] = (int)tokens, c.texts[blockIdx.x] = (int)texts;
+    if (threadIdx.x == 0) c.partial[blockIdx.x] = texts;
+}
+
+// Counted tokens of all texts, a stretch of them to each workgroup.
+__global__ __launch_bounds__(kFinish) void count_kernel(LossRows a, LossCounts c, int64_t stretch) {
+    __shared__ int part[kFinish / 64];
+    const int64_t first = blockIdx.x * stretch, end = a.B * a.T;
+    const int n = count_tokens(a, first, first + stretch < end ? stretch : end - first, part);
+    if (threadIdx.x == 0) c.partial[blockIdx.x] = n;
 }
 
 // The weight of each of text b's tokens in the loss.
 __device__ __forceinline__ float weight_of(const LossCounts &c, int64_t b, int reduction) {
     if (reduction == kLossSum) return 1.f;
-    const int *of = reduction == kLossMean ? c.tokens : c.texts;
     int64_t n = 0;
-    for (int i = threadIdx.x & 63; i < c.blocks; i += 64) n += of[i];
+    for (int i = threadIdx.x & 63; i < c.blocks; i += 64) n += c.partial[i];
     n = wave_sum(n);
     const double all = reduction == kLossMean ? (double)n : (double)n * c.by_text[b];
     return all > 0. ? (float)(1. / all) : 0.f;
@@ -242,11 +269,11 @@ template <typename F> __device__ __forceinline__ void either(bool which, F &&f) 
 // Zeros over a row of the gradient.
 template <typename T, int kT> __device__ __forceinline__ void zero_row(T *out, int V) {
     constexpr int kN = Vec<T>::kN;
-    const int full = V / kN;
+    const Cut<T> cut(out, V);
     Bits<T> z;
     z.zero();
-    for (int j = threadIdx.x; j < full; j += kT) z.template store<true>(out + (int64_t)j * kN);
-    if ((int)threadIdx.x < V - full * kN) store1(out + full * kN + threadIdx.x, 0.f);
+    for (int j = threadIdx.x % kT; j < cut.full; j += kT) z.template store<true>(out + cut.head + (int64_t)j * kN);
+    if ((int)(threadIdx.x % kT) < cut.singles) store1(out + cut.single(threadIdx.x % kT), 0.f);
 }
 
 // c / temperature (1[j = id] - p_j) for one vector of a row, from its logits.
@@ -262,18 +289,19 @@ template <typename T> __device__ __forceinline__ float gradient(float x, const S
 }
 
 // top, sum and lp of every row, and what the loss makes of it; with kGrad the gradient by the row too, while its logits are at hand.
-// A workgroup takes a row.  kVecs > 0: the row is read once, into registers (kVecs vectors of 16 bytes to a thread); the up to 7 elements
-// behind the last whole vector are one more element each to the first threads.  kVecs = 0: rows of any length, a running maximum and sum
-// to a thread, and a second reading for the gradient.
+// kT threads take a row: a workgroup, or each of a workgroup's four waves.  kHold: the row is read once, into registers (kVecs vectors of 16
+// bytes to a thread); otherwise a thread goes through its part of it with a running maximum and sum, kVecs vectors at a time, and the gradient reads it
+// again.  The up to 7 elements behind the last whole vector are one more element each to the first threads.
 constexpr int waves_per_simd(int threads, int vecs) { return threads == 1024 && vecs <= 8 ? 8 : 4; }
 
-template <typename T, int kT, int kVecs, bool kGrad>
-__global__ __launch_bounds__(kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g) {
-    constexpr int kN = Vec<T>::kN, kW = kT / 64, kHeld = kVecs > 0 ? kVecs : kStreamVecs;
+template <typename T, int kT, int kVecs, bool kHold, bool kGrad>
+__global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g) {
+    constexpr int kN = Vec<T>::kN, kW = kT / 64;
     __shared__ float part_max[kW], part_sum[kW], part_c;
-    const int64_t row = blockIdx.x, b = row / a.T;
+    const int64_t row = kT == 64 ? (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : blockIdx.x, b = row / a.T;
+    if (kT == 64 && row >= a.B * a.T) return;
     const int64_t id = a.ids[row];
-    const int V = (int)a.V, full = V / kN, tid = threadIdx.x;
+    const int V = (int)a.V, tid = threadIdx.x % kT;
     T *out = kGrad ? static_cast<T *>(g.grad) + row * V : nullptr;
     if (!counts(a, row, id)) {
         if (tid == 0) {
@@ -287,34 +315,38 @@ __global__ __launch_bounds__(kT, waves_per_simd(kT, kVecs)) void rows_kernel(Los
         return;
     }
     const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + row % a.T * a.stride_t;
+    const Cut<T> cut(x, V);
+    const int full = cut.full;
+    const T *vectors = x + cut.head;
+    T *out_vectors = out + cut.head;
     const Scale scale(a.inv_temperature);
-    Bits<T> held[kHeld];
-    float rest = tid < V - full * kN ? load1(x + full * kN + tid) : -INFINITY;
+    Bits<T> held[kVecs];
+    const float single = tid < cut.singles ? load1(x + cut.single(tid)) : -INFINITY;
     float top, sum;
-    if (kVecs > 0) {
+    if (kHold) {
         either(kGrad || !a.stats, [&](auto past) {   // (read once, or once more by a backward)
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                if (i * kT + tid < full) held[i].template load<past.value>(x + (int64_t)(i * kT + tid) * kN);
+            for (int i = 0; i < kVecs; ++i) {
+                if (i * kT + tid < full) held[i].template load<past.value>(vectors + (int64_t)(i * kT + tid) * kN);
                 else held[i].none();
             }
         });
     }
     const float w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
     const float stands = id < V ? load1(x + id) : NAN;
-    if (kVecs > 0) {
-        top = rest;
+    if (kHold) {
+        top = single;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < kVecs; ++i) {
             float v[kN];
             Vec<T>::unpack(held[i].r, v);
 #pragma unroll
             for (int e = 0; e < kN; ++e) top = fmaxf(top, v[e]);
         }
         top = block_max<kW>(top, part_max);
-        sum = scale.exp(rest - top);
+        sum = scale.exp(single - top);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < kVecs; ++i) {
             float v[kN];
             held[i].again();
             Vec<T>::unpack(held[i].r, v);
@@ -322,34 +354,36 @@ __global__ __launch_bounds__(kT, waves_per_simd(kT, kVecs)) void rows_kernel(Los
             for (int e = 0; e < kN; ++e) sum += scale.exp(v[e] - top);
         }
     } else {
-        float mine = rest;
-        sum = rest == -INFINITY ? 0.f : scale.exp(rest - rest);
-        for (int first = tid; first < full; first += kHeld * kT) {
-            float most = mine;
+        float mine = single;
+        sum = single == -INFINITY ? 0.f : scale.exp(single - single);
+        either(!kGrad && !a.stats, [&](auto past) {
+            for (int first = tid; first < full; first += kVecs * kT) {
+                float most = mine;
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                if (first + i * kT < full) held[i].template load<false>(x + (int64_t)(first + i * kT) * kN);
-                else held[i].none();
+                for (int i = 0; i < kVecs; ++i) {
+                    if (first + i * kT < full) held[i].template load<past.value>(vectors + (int64_t)(first + i * kT) * kN);
+                    else held[i].none();
+                }
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    float v[kN];
+                    Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) most = fmaxf(most, v[e]);
+                }
+                const float from = most == -INFINITY ? 0.f : most;   // (-inf less -inf is no number)
+                sum *= scale.exp(mine - from);
+                mine = most;
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    float v[kN];
+                    held[i].again();
+                    Vec<T>::unpack(held[i].r, v);
+#pragma unroll
+                    for (int e = 0; e < kN; ++e) sum += scale.exp(v[e] - from);
+                }
             }
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                float v[kN];
-                Vec<T>::unpack(held[i].r, v);
-#pragma unroll
-                for (int e = 0; e < kN; ++e) most = fmaxf(most, v[e]);
-            }
-            const float from = most == -INFINITY ? 0.f : most;   // (-inf less -inf is no number)
-            sum *= scale.exp(mine - from);
-            mine = most;
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                float v[kN];
-                held[i].again();
-                Vec<T>::unpack(held[i].r, v);
-#pragma unroll
-                for (int e = 0; e < kN; ++e) sum += scale.exp(v[e] - from);
-            }
-        }
+        });
         top = block_max<kW>(mine, part_max);
         sum = sum == 0.f && top != -INFINITY ? 0.f : sum * scale.exp(mine - top);   // (a thread without elements)
     }
@@ -363,42 +397,47 @@ __global__ __launch_bounds__(kT, waves_per_simd(kT, kVecs)) void rows_kernel(Los
             if (a.exact) a.exact[row] = lp;
             if (a.stats) a.stats[2 * row] = top, a.stats[2 * row + 1] = sum;
             if (l.coef) l.coef[row] = c;
-            part_c = c;
+            if (kT > 64) part_c = c;
         }
     }
     if (!kGrad) return;
     if (l.kind != kLossCrossEntropy) {
-        __syncthreads();
-        c = part_c;
+        if (kT == 64) {
+            c = lane_of(c, 0);
+        } else {
+            __syncthreads();
+            c = part_c;
+        }
     }
     c *= a.inv_temperature;
     const float norm = 1.f / sum, factor = -c * norm;
-    if (kVecs > 0) {
+    if (kHold) {
         either(g.past, [&](auto past) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
+            for (int i = 0; i < kVecs; ++i) {
                 held[i].again();
                 gradient<T>(held[i], scale, top, factor);
-                if (i * kT + tid < full) held[i].template store<past.value>(out + (int64_t)(i * kT + tid) * kN);
+                if (i * kT + tid < full) held[i].template store<past.value>(out_vectors + (int64_t)(i * kT + tid) * kN);
             }
         });
     } else {
-        for (int first = tid; first < full; first += kHeld * kT) {
+        for (int first = tid; first < full; first += kVecs * kT) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                if (first + i * kT < full) held[i].template load<false>(x + (int64_t)(first + i * kT) * kN);
+            for (int i = 0; i < kVecs; ++i)
+                if (first + i * kT < full) held[i].template load<false>(vectors + (int64_t)(first + i * kT) * kN);
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
+            for (int i = 0; i < kVecs; ++i) {
                 if (first + i * kT >= full) continue;
                 gradient<T>(held[i], scale, top, factor);
-                held[i].template store<true>(out + (int64_t)(first + i * kT) * kN);
+                held[i].template store<true>(out_vectors + (int64_t)(first + i * kT) * kN);
             }
         }
     }
-    if (tid < V - full * kN) store1(out + full * kN + tid, gradient<T>(rest, scale, top, factor));
+    if (tid < cut.singles) store1(out + cut.single(tid), gradient<T>(single, scale, top, factor));
     // the element that stands there, by the thread whose store it was in
-    const int owner = id < full * (int64_t)kN ? (int)(id / kN) % kT : (int)(id - full * kN);
-    if (id < V && tid == owner) store1(out + id, c + scale.exp_once(stands - top) * factor);
+    if (id >= V) return;
+    const int lone = cut.single_of((int)id), owner = lone >= 0 ? lone : cut.vector_of((int)id) % kT;
+    if (tid == owner) store1(out + id, c + scale.exp_once(stands - top) * factor);
 }
 
 // v[first], v[first + stride], .. below `end`, added up in 64 bits, eight loads on their way at a time.
@@ -414,11 +453,20 @@ template <typename S> __device__ __forceinline__ double strided_sum(const S *v, 
     return s;
 }
 
-// The sums of up to three arrays of terms.
-__global__ __launch_bounds__(kFinish) void finish_kernel(int64_t rows, LossTerms l) {
+// The sums of up to three arrays of terms: all of an array by one workgroup, or of a great many rows a stretch by each of kStretches, into `sums`.
+__global__ __launch_bounds__(kFinish) void finish_kernel(int64_t rows, LossTerms l, double *sums, int64_t stretch) {
     __shared__ double part[kFinish / 64];
+    const int i = blockIdx.y;
+    const int64_t first = blockIdx.x * stretch, end = first + stretch < rows ? first + stretch : rows;
+    const double s = block_sum<kFinish / 64>(strided_sum(l.terms + i * rows, first + threadIdx.x, end, kFinish), part);
+    if (threadIdx.x != 0) return;
+    if (gridDim.x > 1) sums[i * kStretches + blockIdx.x] = s;
+    else (i == 0 ? l.loss[0] : l.means[i - 1]) = (float)s;
+}
+__global__ __launch_bounds__(kStretches) void finish_stretches_kernel(LossTerms l, const double *sums, int stretches) {
+    __shared__ double part[kStretches / 64];
     const int i = blockIdx.x;
-    const double s = block_sum<kFinish / 64>(strided_sum(l.terms + i * rows, threadIdx.x, rows, kFinish), part);
+    const double s = block_sum<kStretches / 64>((int)threadIdx.x < stretches ? sums[i * kStretches + threadIdx.x] : 0., part);
     if (threadIdx.x == 0) (i == 0 ? l.loss[0] : l.means[i - 1]) = (float)s;
 }
 
@@ -480,23 +528,24 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
     constexpr int kN = Vec<T>::kN;
     const int64_t b = row / a.T, t = row % a.T;
     const int64_t id = a.ids[row];
-    const int V = (int)a.V, full = V / kN, first = piece * (kGradVecs * kThreads) + threadIdx.x;
-    const int behind = piece == 0 && (int)threadIdx.x < V - full * kN ? full * kN + (int)threadIdx.x : -1;
+    const int V = (int)a.V, tid = threadIdx.x, first = piece * (kGradVecs * kThreads) + tid;
+    const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + t * a.stride_t;
     T *out = static_cast<T *>(g.grad) + row * V;
+    const Cut<T> cut(x, V);
+    const bool lone = piece == 0 && tid < cut.singles;
     if (!counts(a, row, id)) {
         Bits<T> z;
         z.zero();
 #pragma unroll
         for (int i = 0; i < kGradVecs; ++i)
-            if (first + i * kThreads < full) z.template store<true>(out + (int64_t)(first + i * kThreads) * kN);
-        if (behind >= 0) store1(out + behind, 0.f);
+            if (first + i * kThreads < cut.full) z.template store<true>(out + cut.head + (int64_t)(first + i * kThreads) * kN);
+        if (lone) store1(out + cut.single(tid), 0.f);
         return;
     }
-    const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + t * a.stride_t;
     Bits<T> held[kGradVecs];
 #pragma unroll
     for (int i = 0; i < kGradVecs; ++i)
-        if (first + i * kThreads < full) held[i].template load<false>(x + (int64_t)(first + i * kThreads) * kN);
+        if (first + i * kThreads < cut.full) held[i].template load<false>(x + cut.head + (int64_t)(first + i * kThreads) * kN);
     float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up;
     if (id >= V) c = NAN;
     c *= a.inv_temperature;
@@ -505,16 +554,16 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
     either(g.past, [&](auto past) {
 #pragma unroll
         for (int i = 0; i < kGradVecs; ++i) {
-            if (first + i * kThreads >= full) continue;
+            if (first + i * kThreads >= cut.full) continue;
             gradient<T>(held[i], scale, top, factor);
-            held[i].template store<past.value>(out + (int64_t)(first + i * kThreads) * kN);
+            held[i].template store<past.value>(out + cut.head + (int64_t)(first + i * kThreads) * kN);
         }
     });
-    if (behind >= 0) store1(out + behind, gradient<T>(load1(x + behind), scale, top, factor));
+    if (lone) store1(out + cut.single(tid), gradient<T>(load1(x + cut.single(tid)), scale, top, factor));
     // the element that stands there, by the thread whose store it was in
     if (id >= V) return;
-    const int64_t j = id / kN;
-    const bool mine = id < full * (int64_t)kN ? j % kThreads == threadIdx.x && j / (kGradVecs * kThreads) == piece : (int)id == behind;
+    const int j = cut.single_of((int)id), v = cut.vector_of((int)id);
+    const bool mine = j >= 0 ? lone && tid == j : v % kThreads == tid && v / (kGradVecs * kThreads) == piece;
     if (mine) store1(out + id, c + scale.exp_once(load1(x + id) - top) * factor);
 }
 
@@ -535,9 +584,9 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
 
 }  // namespace
 
-// three terms for each token and the counts, or lp in 64 bits and a loss for each pair
+// three terms for each token, sums of stretches of them and the counts; or lp in 64 bits and a loss for each pair
 size_t loss_workspace_bytes(int64_t B, int64_t T) {
-    return (size_t)(3 * B * T) * sizeof(float) + (size_t)(B + 2 * kCountBlocks) * sizeof(int);
+    return (size_t)(3 * B * T + 1) / 2 * 2 * sizeof(float) + 3 * kStretches * sizeof(double) + (size_t)(B + kCountBlocks) * sizeof(int);
 }
 
 namespace {
@@ -545,28 +594,50 @@ namespace {
 // Whether the gradient is written past the caches: from the size on that they do not hold for whoever reads it next.
 bool past_the_caches(int dtype, const LossRows &a) { return a.B * a.T * a.V * (dtype == kF32 ? 4 : 2) >= kPastBytes; }
 
-// f(threads, vectors of a thread) of the smallest class that holds a row
-template <typename T, typename F> void by_length(int64_t V, F &&f) {
-    const auto as = [&](auto threads, auto vecs) { f(threads, vecs); };
-    const int64_t n = V / Vec<T>::kN;
-    std::integral_constant<int, 256> few;
-    std::integral_constant<int, 1024> many;
-    if (n <= 256 * 1) as(few, std::integral_constant<int, 1>{});
-    else if (n <= 256 * 2) as(few, std::integral_constant<int, 2>{});
-    else if (n <= 256 * 4) as(few, std::integral_constant<int, 4>{});
-    else if (n <= 256 * 8) as(few, std::integral_constant<int, 8>{});
-    else if (n <= 1024 * 4) as(many, std::integral_constant<int, 4>{});
-    else if (n <= 1024 * 8) as(many, std::integral_constant<int, 8>{});
-    else if (n <= 1024 * 12) as(many, std::integral_constant<int, 12>{});
-    else if (n <= 1024 * 16) as(many, std::integral_constant<int, 16>{});
-    else if (n <= 1024 * 20) as(many, std::integral_constant<int, 20>{});
-    else as(many, std::integral_constant<int, 0>{});
+template <int kT, int kVecs, bool kHold> struct Shape {
+    static constexpr int threads = kT, vecs = kVecs;
+    static constexpr bool hold = kHold;
+};
+
+// f(shape) of the smallest one that holds a row of n vectors
+template <typename F> void by_length(int64_t n, F &&f) {
+    if (n <= 64 * 1) f(Shape<64, 1, true>{});
+    else if (n <= 64 * 2) f(Shape<64, 2, true>{});
+    else if (n <= 64 * 4) f(Shape<64, 4, true>{});
+    else if (n <= 64 * 8) f(Shape<64, 8, true>{});
+    else if (n <= 256 * 4) f(Shape<256, 4, true>{});
+    else if (n <= 256 * 6) f(Shape<256, 6, true>{});
+    else if (n <= 256 * 8) f(Shape<256, 8, true>{});
+    else if (n <= 512 * 6) f(Shape<512, 6, true>{});
+    else if (n <= 512 * 8) f(Shape<512, 8, true>{});
+    else if (n <= 1024 * 5) f(Shape<1024, 5, true>{});
+    else if (n <= 1024 * 6) f(Shape<1024, 6, true>{});
+    else if (n <= 1024 * 7) f(Shape<1024, 7, true>{});
+    else if (n <= 1024 * 8) f(Shape<1024, 8, true>{});
+    else if (n <= 1024 * 10) f(Shape<1024, 10, true>{});
+    else if (n <= 1024 * 13) f(Shape<1024, 13, true>{});
+    else if (n <= 1024 * 16) f(Shape<1024, 16, true>{});
+    else if (n <= 1024 * 20) f(Shape<1024, 20, true>{});
+    else f(Shape<1024, 4, false>{});
+}
+// ... where nothing but the row's sums is wanted of it
+template <typename F> void by_length_alone(int64_t n, F &&f) {
+    if (n <= 64 * 1) f(Shape<64, 1, true>{});
+    else if (n <= 64 * 2) f(Shape<64, 2, true>{});
+    else if (n <= 64 * 4) f(Shape<64, 4, true>{});
+    else if (n <= 64 * 8) f(Shape<64, 8, true>{});
+    else if (n <= 256 * 4) f(Shape<256, 4, true>{});
+    else if (n <= 256 * 6) f(Shape<256, 6, true>{});
+    else if (n <= 256 * 8) f(Shape<256, 8, true>{});
+    else if (n <= 512 * 8) f(Shape<256, 4, false>{});
+    else f(Shape<512, 4, false>{});
 }
 
-template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRows &a, const LossCounts &n, const LossTerms &l, const LossGrad &g) {
-    by_length<T>(a.V, [&](auto threads, auto vecs) {
-        hipLaunchKernelGGL((rows_kernel<T, threads.value, vecs.value, kGrad>), dim3((unsigned)(a.B * a.T)), dim3(threads.value), 0, st, a, n, l, g);
-    });
+template <typename T, typename S, bool kGrad> void launch_rows(hipStream_t st, S, const LossRows &a, const LossCounts &n, const LossTerms &l, const LossGrad &g) {
+    const int64_t rows = a.B * a.T;
+    const bool waves = S::threads == 64;
+    hipLaunchKernelGGL((rows_kernel<T, S::threads, S::vecs, S::hold, kGrad>), dim3((unsigned)(waves ? (rows + kWaves - 1) / kWaves : rows)),
+                       dim3(waves ? kThreads : S::threads), 0, st, a, n, l, g);
 }
 
 }  // namespace
@@ -574,21 +645,36 @@ template <typename T, bool kGrad> void launch_rows(hipStream_t st, const LossRow
 hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *grad, void *workspace) {
     LossCounts n{};
     const int64_t rows = a.B * a.T;
+    double *sums = nullptr;
     if (l.kind != kLossNone) {
         l.terms = static_cast<float *>(workspace);
         l.count = l.kind == kLossPolicy ? 3 : 1;
-        n.by_text = reinterpret_cast<int *>(l.terms + 3 * rows);
-        n.tokens = n.by_text + a.B;
-        n.texts = n.tokens + kCountBlocks;
-        n.blocks = (int)(a.B < kCountBlocks ? a.B : kCountBlocks);
-        hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n);
+        sums = reinterpret_cast<double *>(l.terms + (3 * rows + 1) / 2 * 2);
+        n.partial = reinterpret_cast<int *>(sums + 3 * kStretches);
+        n.by_text = n.partial + kCountBlocks;
+        if (l.reduction == kLossMeanOfTexts) {
+            n.blocks = (int)(a.B < kCountBlocks ? a.B : kCountBlocks);
+            hipLaunchKernelGGL(count_texts_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n);
+        } else if (l.reduction == kLossMean) {
+            int64_t stretch = 2 * kFinish;
+            if (rows > stretch * kCountBlocks) stretch = (rows + kCountBlocks - 1) / kCountBlocks;
+            n.blocks = (int)((rows + stretch - 1) / stretch);
+            hipLaunchKernelGGL(count_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n, stretch);
+        }
     }
     hipError_t e = by_type(dtype, [&](auto t) {
-        if (grad) launch_rows<decltype(t), true>(st, a, n, l, LossGrad{nullptr, 0, 0, nullptr, 0, grad, past_the_caches(dtype, a)});
-        else launch_rows<decltype(t), false>(st, a, n, l, LossGrad{});
+        using T = decltype(t);
+        const int64_t vecs = a.V / Vec<T>::kN;
+        const LossGrad g{nullptr, 0, 0, nullptr, 0, grad, past_the_caches(dtype, a)};
+        if (l.kind == kLossNone) by_length_alone(vecs, [&](auto s) { launch_rows<T, decltype(s), false>(st, s, a, n, l, g); });
+        else if (!grad) by_length(vecs, [&](auto s) { launch_rows<T, decltype(s), false>(st, s, a, n, l, g); });
+        else by_length(vecs, [&](auto s) { launch_rows<T, decltype(s), true>(st, s, a, n, l, g); });
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
-    hipLaunchKernelGGL(finish_kernel, dim3(l.count), dim3(kFinish), 0, st, rows, l);
+    // (one workgroup adds 65536 values in some 10 us, and a great many in proportion)
+    const int64_t stretch = rows <= 65536 ? rows : (rows + kStretches - 1) / kStretches;
+    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)((rows + stretch - 1) / stretch), l.count), dim3(kFinish), 0, st, rows, l, sums, stretch);
+    if (rows > 65536) hipLaunchKernelGGL(finish_stretches_kernel, dim3(l.count), dim3(kStretches), 0, st, l, sums, (int)((rows + stretch - 1) / stretch));
     return hipGetLastError();
 }
 
