@@ -599,28 +599,40 @@ template <int kT, int kVecs, bool kHold> struct Shape {
     static constexpr bool hold = kHold;
 };
 
-// f(shape) of the smallest one that holds a row of n vectors
-template <typename F> void by_length(int64_t n, F &&f) {
-    if (n <= 64 * 1) f(Shape<64, 1, true>{});
-    else if (n <= 64 * 2) f(Shape<64, 2, true>{});
-    else if (n <= 64 * 4) f(Shape<64, 4, true>{});
-    else if (n <= 64 * 8) f(Shape<64, 8, true>{});
-    else if (n <= 256 * 4) f(Shape<256, 4, true>{});
-    else if (n <= 256 * 6) f(Shape<256, 6, true>{});
-    else if (n <= 256 * 8) f(Shape<256, 8, true>{});
-    else if (n <= 512 * 6) f(Shape<512, 6, true>{});
-    else if (n <= 512 * 8) f(Shape<512, 8, true>{});
-    else if (n <= 1024 * 5) f(Shape<1024, 5, true>{});
-    else if (n <= 1024 * 6) f(Shape<1024, 6, true>{});
-    else if (n <= 1024 * 7) f(Shape<1024, 7, true>{});
-    else if (n <= 1024 * 8) f(Shape<1024, 8, true>{});
-    else if (n <= 1024 * 10) f(Shape<1024, 10, true>{});
-    else if (n <= 1024 * 13) f(Shape<1024, 13, true>{});
-    else if (n <= 1024 * 16) f(Shape<1024, 16, true>{});
-    else if (n <= 1024 * 20) f(Shape<1024, 20, true>{});
-    else f(Shape<1024, 4, false>{});
+// f(shape) of the smallest one that holds a row of n vectors.  Cross entropy with its gradient of 1 GiB of bf16 logits, in us, this shape / the next
+// one up: V 20000 411 / 445, 32000 360 / 448 (1024 x 5), 50257 404 / 488 (1024 x 8, rows not from a boundary).  Two workgroups of 512 threads share a compute
+// unit where one of 1024 fills it, so that one reads while the other computes and writes: V 73000 420 / 500 (1024 x 10), 98000 452 / 492 (1024 x
+// 13); fp32 logits, half as many to a byte, gain nothing by it (V 40000 759 / 725).
+template <typename T, typename F> void by_length(int64_t n, F &&f) {
+    if (n <= 64 * 1) return f(Shape<64, 1, true>{});
+    if (n <= 64 * 2) return f(Shape<64, 2, true>{});
+    if (n <= 64 * 4) return f(Shape<64, 4, true>{});
+    if (n <= 64 * 8) return f(Shape<64, 8, true>{});
+    if (n <= 256 * 4) return f(Shape<256, 4, true>{});
+    if (n <= 256 * 6) return f(Shape<256, 6, true>{});
+    if (n <= 256 * 8) return f(Shape<256, 8, true>{});
+    if (n <= 256 * 10) return f(Shape<256, 10, true>{});
+    if (n <= 512 * 6) return f(Shape<512, 6, true>{});
+    if (n <= 512 * 8) return f(Shape<512, 8, true>{});
+    if (n <= 1024 * 5) return f(Shape<1024, 5, true>{});
+    if (n <= 1024 * 6) return f(Shape<1024, 6, true>{});
+    if (n <= 1024 * 7) return f(Shape<1024, 7, true>{});
+    if (n <= 1024 * 8) return f(Shape<1024, 8, true>{});
+    if constexpr (sizeof(T) == 2) {
+        if (n <= 512 * 18) return f(Shape<512, 18, true>{});
+        if (n <= 512 * 20) return f(Shape<512, 20, true>{});
+        if (n <= 512 * 22) return f(Shape<512, 22, true>{});
+        if (n <= 512 * 24) return f(Shape<512, 24, true>{});
+    } else {
+        if (n <= 1024 * 10) return f(Shape<1024, 10, true>{});
+    }
+    if (n <= 1024 * 13) return f(Shape<1024, 13, true>{});
+    if (n <= 1024 * 16) return f(Shape<1024, 16, true>{});
+    if (n <= 1024 * 20) return f(Shape<1024, 20, true>{});
+    f(Shape<1024, 4, false>{});
 }
-// ... where nothing but the row's sums is wanted of it
+// ... where nothing but the row's sums is wanted of it: from 16384 16-bit logits on a row is better gone through than held (8192 rows of 65536 bf16
+// 200 us held by 1024 threads, 157 gone through by 512), down to 4096 the wave that holds a row does without LDS and barriers.
 template <typename F> void by_length_alone(int64_t n, F &&f) {
     if (n <= 64 * 1) f(Shape<64, 1, true>{});
     else if (n <= 64 * 2) f(Shape<64, 2, true>{});
@@ -667,8 +679,8 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         const int64_t vecs = a.V / Vec<T>::kN;
         const LossGrad g{nullptr, 0, 0, nullptr, 0, grad, past_the_caches(dtype, a)};
         if (l.kind == kLossNone) by_length_alone(vecs, [&](auto s) { launch_rows<T, decltype(s), false>(st, s, a, n, l, g); });
-        else if (!grad) by_length(vecs, [&](auto s) { launch_rows<T, decltype(s), false>(st, s, a, n, l, g); });
-        else by_length(vecs, [&](auto s) { launch_rows<T, decltype(s), true>(st, s, a, n, l, g); });
+        else if (!grad) by_length<T>(vecs, [&](auto s) { launch_rows<T, decltype(s), false>(st, s, a, n, l, g); });
+        else by_length<T>(vecs, [&](auto s) { launch_rows<T, decltype(s), true>(st, s, a, n, l, g); });
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
     // (one workgroup adds 65536 values in some 10 us, and a great many in proportion)

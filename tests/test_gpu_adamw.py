@@ -115,6 +115,33 @@ def _check(before, after, norm, clip, bits, t, lr=LR):
             assert bool(((wide.abs() - y).abs() <= 2 * step).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_eight_bits_to_the_last_bit(dtype):
+    """Moments in 8 bits and their scales are what the formula's fp32 operations give one after the other, bit for bit, over several steps."""
+    st = _setup([(70001,), (3000,), (64, 2048)], dtype, 8, False, 21)
+    for t in (11, 12, 13):
+        for x in st["grads"]:
+            x.mul_(0.9).add_(1e-3)
+        before = _clone(st)
+        _step(st)
+        for j, g in enumerate(before["grads"]):
+            n, g = g.numel(), g.reshape(-1).float()
+            sc = before["scales"][j].repeat_interleave(256, 0)[:n]
+            m, r = before["exp_avgs"][j].reshape(-1).float() * sc[:, 0], before["exp_avg_sqs"][j].reshape(-1).float() * sc[:, 1]
+            m, v = m * BETAS[0] + g * (1 - BETAS[0]), r * r * BETAS[1] + g * g * (1 - BETAS[1])
+            key = _mix((7 * 0x9E3779B9 + t * 0xBB67AE85 + j) & 0xFFFFFFFF)
+            h = _mix((torch.arange(n, device="cuda") * 0x9E3779B9 + key) & 0xFFFFFFFF)
+            for column, (name, x, u16) in enumerate((("exp_avgs", m, h & 0xFFFF), ("exp_avg_sqs", torch.sqrt(v), h >> 16))):
+                top = torch.cat([x, x.new_zeros(-n % 256)]).view(-1, 256).abs().amax(1).clamp(min=2.0 ** -100)
+                assert torch.equal(st["scales"][j][:, column], top * (1.0 / 448.0)), (j, name)
+                y = x.abs() * (torch.reciprocal(top) * 448.0).repeat_interleave(256)[:n]
+                code = ((((y * 2.0 ** -120).view(torch.int32).long()) + (u16 << 4)) >> 20).clamp(max=0x7E)
+                if column == 1:
+                    code = torch.where((code == 0) & (x > 0), torch.ones_like(code), code)
+                want = code.to(torch.uint8).view(F8).float() * torch.where(x < 0, -1.0, 1.0)
+                assert torch.equal(st[name][j].reshape(-1).float(), want), (j, name)
+
+
 def _clone(st):
     return {k: [t.clone() for t in v] if isinstance(v, list) else (v.clone() if v is not None else None) for k, v in st.items()}
 

@@ -22,7 +22,8 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 SMALLEST = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
 # vocabularies on either side of what a vector, a wave, a workgroup and the kernels' size classes hold
 VOCABULARIES = [1, 2, 7, 8, 9, 63, 64, 255, 1000, 2047, 2048, 2049, 4100, 8191, 16384, 16392, 32768, 50277, 65536, 65537, 131073, 151936, 170001,
-                512, 513, 1024, 1025, 4096, 4097, 8193, 12288, 12289, 20481, 24576, 24577, 40961, 49153, 57345, 81920, 81921, 106497, 163840, 163841, 163849]
+                512, 513, 1024, 1025, 4096, 4097, 8193, 12288, 12289, 20481, 24576, 24577, 40961, 49153, 57345, 81920, 81921, 106497, 163840, 163841, 163849,
+                20480, 20488, 73000, 73729, 90113, 98304, 98305]
 
 
 def _case(B, T, V, dtype, seed, std=2.0):
