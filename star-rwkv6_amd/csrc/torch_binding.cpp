@@ -566,10 +566,12 @@ Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &ex
     kept.push_back(g);
     row.grad = in(g);
     rows.push_back(row);
-    if (p.numel() > 0) seen.push_back(row.param);
+    for (const void *written : {static_cast<const void *>(row.param), static_cast<const void *>(row.exp_avg), static_cast<const void *>(row.exp_avg_sq),
+                                static_cast<const void *>(row.scales), static_cast<const void *>(row.master)})
+      if (written && p.numel() > 0) seen.push_back(written);
   }
   std::sort(seen.begin(), seen.end());
-  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "wkv6: a parameter is given twice");
+  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "wkv6: a parameter, a moment, its scales or a master is given twice");
   if (!norm.defined() && (max_grad_norm > 0. || skip_nonfinite)) norm = grad_norm(kept);
   check(wkv6_adamw_step(stream_of(first), code_of(type), eight ? 8 : 32, count, rows.data(), static_cast<int64_t *>(out(step)), in_f(lr_device), lr, beta1,
                         beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, in_f(norm), static_cast<uint32_t>(seed)));
@@ -627,6 +629,10 @@ std::pair<Tensor, Tensor> forward_gn_gate(int64_t H, const Tensor &map, const Te
                                 out(ys), out(ws), n));
   return {res, ys};
 }
+
+// A tensor that takes no part in a graph.
+Tensor apart(const Tensor &t) { return t.defined() && t.requires_grad() ? t.detach() : t; }
+std::optional<Tensor> apart(const std::optional<Tensor> &t) { return t.has_value() ? std::optional<Tensor>(apart(*t)) : t; }
 
 // ---- what the Python layer calls ----
 
@@ -747,7 +753,7 @@ PYBIND11_MODULE(_wkv6_torch, m) {
                           double temperature, int64_t reduction) {
     const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
     const variable_list o = unlocked([&] {
-      return PolicyLoss::apply(x, ids, mask, old_logps, advantages, ref_logps, clip_low, clip_high, kl_weight, temperature,
+      return PolicyLoss::apply(x, ids, mask, apart(old_logps), apart(advantages), apart(ref_logps), clip_low, clip_high, kl_weight, temperature,
                                reduction, wanted);
     });
     return py::make_tuple(wrap(o[0]), wrap(o[1]), wrap(o[2]));
@@ -756,7 +762,7 @@ PYBIND11_MODULE(_wkv6_torch, m) {
                               int64_t kind, double beta, double label_smoothing, bool average) {
     const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
     const variable_list o = unlocked([&] {
-      return PreferenceLoss::apply(x, ids, mask, ref_logps, kind, beta, label_smoothing, average, wanted);
+      return PreferenceLoss::apply(x, ids, mask, apart(ref_logps), kind, beta, label_smoothing, average, wanted);
     });
     return py::make_tuple(wrap(o[0]), wrap(o[1]));
   });

@@ -24,6 +24,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFinish = 1024;        // threads of the one workgroup that adds up
 constexpr int kCountBlocks = 256;    // at most
 constexpr int kStretches = 256;      // of a great many rows
+constexpr int64_t kMostBlocks = 1 << 21;   // of a launch: it counts its threads in 32 bits
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
 // A gradient of this size and more is written past the caches.  Cross entropy, log probabilities with their backward, and the latter with a reader
 // of the gradient behind it, in us, written into / past them: 128 MiB 63 / 66, 78 / 78, 106 / 120; 192 MiB 89 / 89, 119 / 108, 178 / 171; 2 GiB (8 pairs
@@ -295,10 +296,10 @@ template <typename T> __device__ __forceinline__ float gradient(float x, const S
 constexpr int waves_per_simd(int threads, int vecs) { return threads == 1024 && vecs <= 8 ? 8 : 4; }
 
 template <typename T, int kT, int kVecs, bool kHold, bool kGrad>
-__global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g) {
+__global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g, int64_t first_block) {
     constexpr int kN = Vec<T>::kN, kW = kT / 64;
     __shared__ float part_max[kW], part_sum[kW], part_c;
-    const int64_t row = kT == 64 ? (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : blockIdx.x, b = row / a.T;
+    const int64_t block = first_block + blockIdx.x, row = kT == 64 ? block * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : block, b = row / a.T;
     if (kT == 64 && row >= a.B * a.T) return;
     const int64_t id = a.ids[row];
     const int V = (int)a.V, tid = threadIdx.x % kT;
@@ -472,11 +473,11 @@ __global__ __launch_bounds__(kStretches) void finish_stretches_kernel(LossTerms 
 
 // Pairs of texts (b and b + P), a workgroup each: log probabilities of whole texts in 64 bits (sums over thousands of tokens, of
 // which a small difference is wanted), the loss of their difference, and c of either text's tokens.
-__global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTerms l) {
+__global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTerms l, int64_t first_pair) {
     __shared__ double part[2][kFinish / 64];
     __shared__ int count[2][kFinish / 64];
     const int half = kFinish / 2, i = threadIdx.x / half;   // the first half of the threads takes the chosen text
-    const int64_t P = a.B / 2, pair = blockIdx.x, b = pair + i * P, first = b * a.T;
+    const int64_t P = a.B / 2, pair = first_pair + blockIdx.x, b = pair + i * P, first = b * a.T;
     double v = wave_sum(strided_sum(a.exact + first, threadIdx.x % half, a.T, half));
     int n = 0;
     if (l.average)
@@ -645,11 +646,16 @@ template <typename F> void by_length_alone(int64_t n, F &&f) {
     else f(Shape<512, 4, false>{});
 }
 
+template <typename F> void in_launches(int64_t blocks, F &&f) {
+    for (int64_t first = 0; first < blocks; first += kMostBlocks) f(first, (unsigned)(blocks - first < kMostBlocks ? blocks - first : kMostBlocks));
+}
+
 template <typename T, typename S, bool kGrad> void launch_rows(hipStream_t st, S, const LossRows &a, const LossCounts &n, const LossTerms &l, const LossGrad &g) {
     const int64_t rows = a.B * a.T;
     const bool waves = S::threads == 64;
-    hipLaunchKernelGGL((rows_kernel<T, S::threads, S::vecs, S::hold, kGrad>), dim3((unsigned)(waves ? (rows + kWaves - 1) / kWaves : rows)),
-                       dim3(waves ? kThreads : S::threads), 0, st, a, n, l, g);
+    in_launches(waves ? (rows + kWaves - 1) / kWaves : rows, [&](int64_t first, unsigned blocks) {
+        hipLaunchKernelGGL((rows_kernel<T, S::threads, S::vecs, S::hold, kGrad>), dim3(blocks), dim3(waves ? kThreads : S::threads), 0, st, a, n, l, g, first);
+    });
 }
 
 }  // namespace
@@ -696,7 +702,7 @@ hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g) {
         using T = decltype(t);
         const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per, all = a.B * a.T * pieces;
         // (most often there is nothing to do where a forward has written the gradient: 32768 workgroups took 9 us to find that out)
-        const int64_t most = g.is_there ? 2048 : 0x7fffffff;
+        const int64_t most = g.is_there ? 2048 : kMostBlocks;
         hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, a.B * a.T);
     });
 }
@@ -706,7 +712,7 @@ hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerm
     l.by_pair = a.exact + a.B * a.T;
     const hipError_t e = loss_rows(st, dtype, a, LossTerms{}, nullptr, nullptr);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(pairs_kernel, dim3((unsigned)P), dim3(kFinish), 0, st, a, l);
+    in_launches(P, [&](int64_t pair, unsigned blocks) { hipLaunchKernelGGL(pairs_kernel, dim3(blocks), dim3(kFinish), 0, st, a, l, pair); });
     hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(kFinish), 0, st, P, l);
     return hipGetLastError();
 }

@@ -103,7 +103,7 @@ def policy_loss(logits, ids, mask, old_logps, advantages, ref_logps=None, clip_l
     sampling model's; None: the sampling model is this one, the ratio 1 with lp's gradient) and e = ref_logps - lp, the loss is the mean of
         kl_weight (exp(e) - e - 1) - min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
     over all tokens that count ("mean"), or over each text's and then over the texts that have any ("mean_of_texts").  `advantages`: (B,)
-    or (B, T).  `ref_logps` (B, T): a reference model's; None: no KL term.
+    or (B, T).  `ref_logps` (B, T): a reference model's; None: no KL term.  None of the three gets a gradient.
     Returns (loss, lp, means): an fp32 scalar, differentiable in logits, and without gradients lp (B, T) and the same means of
     exp(e) - e - 1 and of whether the clamped term was the smaller one (2 values).  With a gradient wanted the logits are read once."""
     logits, ids, mask = _rows(logits, ids, mask, False)
@@ -130,7 +130,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
         g = g * max_grad_norm / max(norm, max_grad_norm)                 (max_grad_norm None: g as it is)
         m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  t = step = step + 1
         p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
-    params, grads: of one dtype (bf16, fp16, fp32), any dense layout.  step: one int64 on the device.  lr: a number, or one fp32 value on the
+    params, grads: of one dtype (bf16, fp16, fp32), any dense layout, none twice.  step: one int64 on the device, that of no other call under way.  lr: a number, or one fp32 value on the
     device (which a captured graph's replays read anew).  masters: fp32 weights that are updated in the params' place, the
     params their rounded copies.  grad_norm: the norm to clip by, one fp32 value on the device; None: that of these gradients.  skip_nonfinite: a
     step whose norm is not finite changes nothing.  Returns the norm, None if nothing asked for it.
@@ -152,7 +152,8 @@ class AdamW(torch.optim.Optimizer):
     launches, without a synchronisation.
 
     moment_bits: 32 or 8 (see adamw_step; a parameter then has 2 bytes of state and a little).  master_weights: 16-bit parameters are
-    updated in fp32 behind their rounded copies.  max_grad_norm: gradients of all groups together are clipped to it;
+    updated in fp32 behind their rounded copies.  max_grad_norm: gradients of all groups
+    together are clipped to it;
     ``last_grad_norm`` is their norm, on the device.  skip_nonfinite: a step whose norm is not finite is left out.  lr of a group may be an
     fp32 tensor on the device.  A step can be captured into a graph once every parameter has its state, after a first step.
 
@@ -171,6 +172,8 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     def _new_state(self, p, step):
+        # (into a graph each replay would begin from nothing again)
+        assert not torch.cuda.is_current_stream_capturing(), "a step is captured after a first one that gave every parameter its state"
         s = self.state[p]
         s["step"] = step
         dtype = torch.float8_e4m3fn if self.moment_bits == 8 else torch.float32
@@ -208,6 +211,7 @@ class AdamW(torch.optim.Optimizer):
                     for q in taking.pop(id(self.state[p]["step"])):
                         key, old = ("after", q.dtype, id(self.state[q]["step"])), self.state[q]["step"]
                         if key not in new:
+                            assert not torch.cuda.is_current_stream_capturing(), "a captured step takes the parameters that the step before it took"
                             new[key] = old.clone()
                         self.state[q]["step"] = new[key]
         return [(key[0], ps) for key, ps in cohorts.items()]

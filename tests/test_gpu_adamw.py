@@ -436,3 +436,80 @@ def test_refusals_on_the_gpu():
             _step(st, **kw)
     with pytest.raises(RuntimeError):
         _step(st, betas=(1.0, 0.9))
+
+
+def test_a_first_step_is_not_captured():
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = rwkv_kernel.AdamW([p])
+    p.grad = torch.ones_like(p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(AssertionError, match="captured"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    torch.cuda.synchronize()
+    opt.step()
+    assert int(opt.state[p]["step"]) == 1
+
+
+def test_a_moment_twice_is_refused():
+    st = _setup([(10,), (10,)], torch.float32, 32, False, 9)
+    with pytest.raises(RuntimeError, match="twice"):
+        _step(dict(st, exp_avgs=[st["exp_avgs"][0]] * 2))
+    with pytest.raises(RuntimeError, match="twice"):
+        _step(dict(st, exp_avg_sqs=st["exp_avgs"]))
+    with pytest.raises(RuntimeError, match="dense"):
+        wide = torch.zeros(10, 4, device="cuda")
+        _step({k: [wide[:, 0].clone().as_strided((10,), (1,)) if k != "params" else wide[:, 0]] if isinstance(v, list) else v for k, v in st.items()})
+
+
+def test_steps_on_two_streams():
+    """Two optimizers side by side, each as if alone."""
+    def run(streams):
+        out = []
+        for i, stream in enumerate(streams):
+            p = torch.nn.Parameter(torch.linspace(-1, 1, 50000 + i).cuda())
+            with torch.cuda.stream(stream):
+                opt = rwkv_kernel.AdamW([p], lr=1e-2, max_grad_norm=1.0, moment_bits=8)
+                for t in range(5):
+                    p.grad = torch.sin(p.detach() * (t + 1))
+                    opt.step()
+            out.append(p)
+        torch.cuda.synchronize()
+        return [p.detach().clone() for p in out]
+
+    torch.cuda.synchronize()
+    alone = run([torch.cuda.current_stream()] * 3)
+    side = [torch.cuda.Stream() for _ in range(3)]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    assert all(torch.equal(a, b) for a, b in zip(alone, run(side)))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_elements_than_32_bits_count(bits):
+    """A tensor of more than 2^31 elements: its last ones go as they do in a tensor of their own (in 8 bits: within the two values that the drawn number chooses from)."""
+    n, tail = (1 << 31) + 4096 + 77, 4096 + 77
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    st = _setup([(tail,)], torch.bfloat16, bits, False, 31)
+    whole = dict(params=[p], grads=[g], masters=None, step=st["step"].clone(), scales=None)
+    p[-tail:], g[-tail:] = st["params"][0], st["grads"][0]
+    for k in ("exp_avgs", "exp_avg_sqs"):
+        m = torch.zeros(n, dtype=torch.uint8 if bits == 8 else torch.float32, device="cuda")
+        m[-tail:] = st[k][0].view(torch.uint8) if bits == 8 else st[k][0]
+        whole[k] = [m.view(F8) if bits == 8 else m]
+    if bits == 8:
+        scales = torch.zeros((n + 255) // 256, 2, device="cuda")
+        scales[-((tail + 255) // 256):] = st["scales"][0]
+        whole["scales"] = [scales]
+    norms = [_step(x, max_grad_norm=0.5) for x in (st, whole)]
+    assert torch.equal(*norms) and torch.equal(p[-tail:], st["params"][0]) and not bool(p[:-tail].any())
+    for k in ("exp_avgs", "exp_avg_sqs"):
+        got, want = whole[k][0][-tail:], st[k][0]
+        if bits == 32:
+            assert torch.equal(got, want)
+        else:
+            got, want = got.view(torch.uint8).int(), want.view(torch.uint8).int()
+            assert int((got - want).abs().max()) <= 1
+    if bits == 8:
+        assert torch.equal(whole["scales"][0][-((tail + 255) // 256):], st["scales"][0])

@@ -452,3 +452,105 @@ def test_results_do_not_change_from_run_to_run():
         runs.append((loss.detach(), s, v.grad))
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_what_stands_beside_the_logits_gets_no_gradient():
+    """Log probabilities of other models and advantages may carry a graph: nothing flows into it, and without logits that want one there is no gradient."""
+    x, ids, mask, g = _case(4, 5, 300, torch.float32, 17)
+    old = rwkv_kernel.token_logprobs(x, ids).requires_grad_(True)
+    ref = (old * 1.5)
+    A = torch.randn(4, generator=g).cuda().requires_grad_(True)
+    for leaf in (x.clone().requires_grad_(True), x):
+        loss = rwkv_kernel.policy_loss(leaf, ids, mask, old, A, ref_logps=ref, kl_weight=0.1)[0] + rwkv_kernel.preference_loss(leaf, ids, mask, ref.sum(1))[0]
+        assert loss.requires_grad == leaf.requires_grad
+        if leaf.requires_grad:
+            loss.backward()
+            assert leaf.grad is not None
+    assert old.grad is None and A.grad is None
+
+
+def test_more_rows_than_a_launch_counts_threads():
+    """2^32 threads and more: rows of 256 threads each, all the same one in memory."""
+    rows, V = (1 << 24) + 5, 4104
+    row = torch.randn(V, generator=torch.Generator().manual_seed(18)).to(torch.bfloat16).cuda()
+    ids = torch.full((1, rows), -1, dtype=torch.int64, device="cuda")
+    ids[0, ::4096] = 3
+    ids[0, rows - 1] = 11
+    lp = rwkv_kernel.token_logprobs(row.expand(1, rows, V), ids)
+    want = rwkv_kernel.token_logprobs(row[None, None].expand(1, 2, V), torch.tensor([[3, 11]]).cuda())
+    assert bool((lp[0, :rows - 1:4096] == want[0, 0]).all()) and bool(lp[0, rows - 1] == want[0, 1])
+    assert int((lp != 0).sum()) == (rows - 2) // 4096 + 2
+
+
+@pytest.mark.parametrize("reduction", ["mean", "mean_of_texts"])
+def test_many_short_texts(reduction):
+    """More texts than counting workgroups, and more rows than one workgroup adds up."""
+    B, T, V = 70000, 2, 40
+    x, ids, mask, g = _case(B, T, V, torch.float32, 19)
+    A = torch.randn(B, generator=g).cuda()
+    got, got_lp, _ = rwkv_kernel.policy_loss(x, ids, mask, None, A, reduction=reduction)
+    _, lp, counted, E, _ = _lp64(x, ids, mask)
+    n = counted.sum(1, keepdim=True).double()
+    w = counted / (n.clamp(min=1) * (n > 0).sum() if reduction == "mean_of_texts" else counted.sum())
+    want = -(A.cpu().double()[:, None] * w).sum()
+    # (the ratio is 1: a term is the advantage times its weight, two roundings)
+    _within("loss", got, want, 4 * U * (A.cpu().double().abs()[:, None] * w).sum())
+    _within("lp", got_lp, lp, E + 2 * U * lp.abs())
+    loss, s = rwkv_kernel.preference_loss(x, ids, mask)
+    want, s64, d = _preference(lp, counted, None, 0.1, "sigmoid", 0.0, False)
+    off = (E * counted).sum(1)
+    _within("preference", loss, want, 0.1 * (off[:B // 2] + off[B // 2:]).mean() + 2 * U * want.abs())
+
+
+def test_two_streams_at_once():
+    """The same logits on two streams, and calls of different sizes side by side: each as if alone."""
+    cases = [_case(3, 40, V, torch.bfloat16, V) for V in (3000, 40000)]
+    alone = []
+    for x, ids, mask, _ in cases:
+        v = x.clone().requires_grad_(True)
+        loss = rwkv_kernel.cross_entropy(v, ids, mask)
+        alone.append((loss.detach(), torch.autograd.grad(loss, v)[0]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for i, s in enumerate(streams):
+        x, ids, mask, _ = cases[i % 2]
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                v = x.clone().requires_grad_(True)
+                loss = rwkv_kernel.cross_entropy(v, ids, mask)
+                got.append((i % 2, loss.detach(), torch.autograd.grad(loss, v)[0]))
+    torch.cuda.synchronize()
+    for which, loss, grad in got:
+        assert torch.equal(loss, alone[which][0]) and torch.equal(grad, alone[which][1])
+
+
+def test_a_backward_captured_after_an_eager_forward():
+    """Its replays give the gradient anew each time, whatever became of the last one, and an eager backward behind them too."""
+    x, ids, mask, _ = _case(2, 9, 1500, torch.bfloat16, 20)
+    y = x.clone().requires_grad_(True)   # (a leaf that only the capturing stream has seen: torch's engine would make any other stream of the graph wait
+    side = torch.cuda.Stream()           # for the captured gradient, and so a part of the capture that nothing joins again)
+    side.wait_stream(torch.cuda.current_stream())
+    up = torch.ones((), device="cuda")
+    with torch.cuda.stream(side):
+        loss = rwkv_kernel.cross_entropy(y, ids, mask)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grad, = torch.autograd.grad(loss, y, up, retain_graph=True)
+    torch.cuda.synchronize()
+    w = x.clone().requires_grad_(True)
+    rwkv_kernel.cross_entropy(w, ids, mask).backward()
+    for scale in (1.0, 1.0, 0.5, 1.0):
+        up.fill_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, w.grad * scale)
+        grad.fill_(float("nan"))
+        torch.cuda.synchronize()
+    up.fill_(1.0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        eager, = torch.autograd.grad(loss, y, up)
+    torch.cuda.synchronize()
+    assert torch.equal(eager, w.grad)
