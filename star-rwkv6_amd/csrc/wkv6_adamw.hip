@@ -10,6 +10,11 @@
 // is for ever; it is rounded to one of its two neighbours with the probabilities that keep the mean instead.  The 16 random
 // bits for each come from a hash of seed, step, tensor and element: the same call gives the same result.  p is formed from
 // the moments before they are rounded, and no r > 0 is rounded to 0.
+//
+// Bound by memory: 28 bytes a parameter with everything in fp32, 10 with bf16 parameters and 8-bit moments (whose some 60 vector operations a parameter
+// take two thirds of the time), and the gradient once more for the norm.  490 M parameters in 150 tensors: step 2.43 ms and norm 0.32 ms in fp32
+// (5.6 and 6.1 TB/s; elements of a wave's load without gaps, past the caches 10 % faster than through them), 0.98 and 0.18 ms in bf16 with 8 bits.
+// Some 1 M parameters in 26 tensors: one launch of 9.5 us.
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
