@@ -740,6 +740,16 @@ PYBIND11_MODULE(_wkv6_torch, m) {
     const ScalarType st = state_code == WKV6_F32 ? at::kFloat : state_code == WKV6_F16 ? at::kHalf : at::kBFloat16;
     return wrap(unlocked([&] { return forward_with_state(H, given(map), r, k, v, w, u, given(s0), algo, st, backward_follows); }));
   }, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg("backward_follows") = false);
+  // Logits, ids and a mask (or None) as the kernels take them, with nothing left for the Python layer to check or to change.
+  m.def("plain_rows", [](const py::object &x_, const py::object &ids_, const py::object &mask_) {
+    const Tensor *x = tensor(x_), *ids = tensor(ids_), *mask = tensor(mask_);
+    if (!x || !ids || !(mask || mask_.is_none()) || !x->is_cuda() || x->dim() != 3 || code_of(x->scalar_type()) < 0 || x->size(2) == 0 || x->stride(2) != 1)
+      return false;
+    const auto beside = [&](const Tensor &t) {
+      return t.device() == x->device() && t.dim() == 2 && t.size(0) == x->size(0) && t.size(1) == x->size(1) && t.is_contiguous();
+    };
+    return ids->scalar_type() == at::kLong && beside(*ids) && (!mask || ((mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte) && beside(*mask)));
+  });
   m.def("token_logprobs", [](const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, double temperature) {
     const bool wanted = at::GradMode::is_enabled() && x.requires_grad();
     return unlocked([&] { return TokenLogprobs::apply(x, ids, mask, temperature, wanted); });

@@ -30,6 +30,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFinish = 1024;        // threads of the one workgroup that adds up
 constexpr int kCountBlocks = 256;    // at most
 constexpr int kStretches = 256;      // of a great many rows
+constexpr int kFewRows = 1024;       // whose tokens every row's threads count for themselves: a launch less (2 us of the card's time and of the host's)
 constexpr int64_t kMostBlocks = 1 << 21;   // of a launch: it counts its threads in 32 bits
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
 // A gradient of this size and more is written past the caches.  Cross entropy, log probabilities with their backward, and the latter with a reader
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(kFinish) void count_kernel(LossRows a, LossCounts c
     if (threadIdx.x == 0) c.partial[blockIdx.x] = n;
 }
 
-// The weight of each of text b's tokens in the loss.
+// The weight of each of text b's tokens in the loss, from counts that were taken ahead.
 __device__ __forceinline__ float weight_of(const LossCounts &c, int64_t b, int reduction) {
     if (reduction == kLossSum) return 1.f;
     int64_t n = 0;
@@ -239,6 +240,13 @@ __device__ __forceinline__ float weight_of(const LossCounts &c, int64_t b, int r
     n = wave_sum(n);
     const double all = reduction == kLossMean ? (double)n : (double)n * c.by_text[b];
     return all > 0. ? (float)(1. / all) : 0.f;
+}
+// The same where no counts were taken: of few tokens in all, every kT threads count for themselves.
+template <int kT> __device__ __forceinline__ float weight_of_few(const LossRows &a, int *part) {
+    int n = 0;
+    for (int t = threadIdx.x % kT; t < (int)(a.B * a.T); t += kT) n += counts(a, t, a.ids[t]);
+    n = block_sum<kT / 64>(n, part);
+    return n > 0 ? (float)(1. / (double)n) : 0.f;
 }
 
 // What a loss makes of one token's lp: its weighted terms, for the finishing kernel to add up, and c.
@@ -307,6 +315,7 @@ template <typename T, int kT, int kVecs, bool kHold, bool kGrad>
 __global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)) void rows_kernel(LossRows a, LossCounts n, LossTerms l, LossGrad g, int64_t first_block) {
     constexpr int kN = Vec<T>::kN, kW = kT / 64;
     __shared__ float part_max[kW], part_sum[kW], part_c;
+    __shared__ int part_n[kW];
     const int64_t block = first_block + blockIdx.x, row = kT == 64 ? block * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : block, b = row / a.T;
     if (kT == 64 && row >= a.B * a.T) return;
     const int64_t id = a.ids[row];
@@ -323,6 +332,9 @@ __global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)
         if (kGrad) zero_row<T, kT>(out, V);
         return;
     }
+    // (before the row is loaded: its registers are not free later)
+    const bool few = l.reduction == kLossMean && n.blocks == 0 && l.kind != kLossNone;
+    float w = few ? weight_of_few<kT>(a, part_n) : 0.f;
     const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + row % a.T * a.stride_t;
     const Cut<T> cut(x, V);
     const int full = cut.full;
@@ -341,7 +353,7 @@ __global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)
             }
         });
     }
-    const float w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
+    if (!few) w = l.kind == kLossNone ? 0.f : weight_of(n, b, l.reduction);
     const float stands = id < V ? load1(x + id) : NAN;
     if (kHold) {
         top = single;
@@ -682,7 +694,7 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         if (l.reduction == kLossMeanOfTexts) {
             n.blocks = (int)(a.B < kCountBlocks ? a.B : kCountBlocks);
             hipLaunchKernelGGL(count_texts_kernel, dim3(n.blocks), dim3(kFinish), 0, st, a, n);
-        } else if (l.reduction == kLossMean) {
+        } else if (l.reduction == kLossMean && rows > kFewRows) {
             int64_t stretch = 2 * kFinish;
             if (rows > stretch * kCountBlocks) stretch = (rows + kCountBlocks - 1) / kCountBlocks;
             n.blocks = (int)((rows + stretch - 1) / stretch);

@@ -29,6 +29,8 @@ SCALE_BLOCK = 256   # elements that share a scale where moments are held in 8 bi
 
 def _rows(logits, ids, mask, flat_allowed):
     """(logits (B,T,V) with rows in one piece, ids (B,T), mask (B,T) bytes or None), checked."""
+    if _native.load_torch().plain_rows(logits, ids, mask):
+        return logits, ids, mask
     assert isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be on the GPU"
     assert logits.dtype in _DTYPES, "logits must be bfloat16, float16 or float32"
     assert logits.dim() == 3 or (flat_allowed and logits.dim() == 2), "logits must be (batch, time, vocabulary)%s" % (
@@ -60,7 +62,8 @@ def token_logprobs(logits, ids, mask=None, temperature=1.0):
     assert temperature > 0
     if ids.numel() == 0:
         return logits.float().sum(-1).reshape(shape)
-    return _native.load_torch().token_logprobs(logits, ids, mask, float(temperature)).reshape(shape)
+    lp = _native.load_torch().token_logprobs(logits, ids, mask, float(temperature))
+    return lp if len(shape) == 2 else lp.reshape(shape)
 
 
 def cross_entropy(logits, ids, mask=None, reduction="mean"):
