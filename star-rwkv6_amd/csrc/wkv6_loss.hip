@@ -622,7 +622,7 @@ template <int kT, int kVecs, bool kHold> struct Shape {
 };
 
 // f(shape) of the smallest one that holds a row of n vectors.  Cross entropy with its gradient of 1 GiB of bf16 logits, in us, this shape / the next
-// one up: V 20000 411 / 445, 32000 360 / 448 (1024 x 5), 50257 404 / 488 (1024 x 8, rows not from a boundary).  Two workgroups of 512 threads share a compute
+// one up: V 20000 411 / 445, 32000 361 / 406 (1024 x 4), 50257 410 / 488 (1024 x 8, rows not from a boundary).  Two workgroups of 512 threads share a compute
 // unit where one of 1024 fills it, so that one reads while the other computes and writes: V 73000 420 / 500 (1024 x 10), 98000 452 / 492 (1024 x
 // 13); fp32 logits, half as many to a byte, gain nothing by it (V 40000 759 / 725).
 template <typename T, typename F> void by_length(int64_t n, F &&f) {
@@ -710,10 +710,10 @@ hipError_t loss_rows(hipStream_t st, int dtype, LossRows a, LossTerms l, void *g
         else by_length<T>(vecs, [&](auto s) { launch_rows<T, decltype(s), true>(st, s, a, n, l, g); });
     });
     if (e != hipSuccess || l.kind == kLossNone) return e;
-    // (one workgroup adds 65536 values in some 10 us, and a great many in proportion)
-    const int64_t stretch = rows <= 65536 ? rows : (rows + kStretches - 1) / kStretches;
+    // (one workgroup adds 65536 values in 19 us; stretches and their sums take 9, at four times as many too)
+    const int64_t stretch = rows <= 32768 ? rows : (rows + kStretches - 1) / kStretches;
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)((rows + stretch - 1) / stretch), l.count), dim3(kFinish), 0, st, rows, l, sums, stretch);
-    if (rows > 65536) hipLaunchKernelGGL(finish_stretches_kernel, dim3(l.count), dim3(kStretches), 0, st, l, sums, (int)((rows + stretch - 1) / stretch));
+    if (rows > 32768) hipLaunchKernelGGL(finish_stretches_kernel, dim3(l.count), dim3(kStretches), 0, st, l, sums, (int)((rows + stretch - 1) / stretch));
     return hipGetLastError();
 }
 
