@@ -531,7 +531,8 @@ __global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTe
         loss = z * z;
         by_d = 2. * z;
     }
-    l.by_pair[pair] = loss / (double)P;
+    if (P == 1) l.loss[0] = (float)loss;
+    else l.by_pair[pair] = loss / (double)P;
     if (l.coef) {
         l.coef[pair] = (float)(by_d * len[0] / (double)P);
         l.coef[pair + P] = (float)(-by_d * len[1] / (double)P);
@@ -734,7 +735,7 @@ hipError_t loss_preference(hipStream_t st, int dtype, LossRows a, PreferenceTerm
     const hipError_t e = loss_rows(st, dtype, a, LossTerms{}, nullptr, nullptr);
     if (e != hipSuccess) return e;
     in_launches(P, [&](int64_t pair, unsigned blocks) { hipLaunchKernelGGL(pairs_kernel, dim3(blocks), dim3(kFinish), 0, st, a, l, pair); });
-    hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(kFinish), 0, st, P, l);
+    if (P > 1) hipLaunchKernelGGL(pairs_finish_kernel, dim3(1), dim3(kFinish), 0, st, P, l);   // (4 us behind a large kernel)
     return hipGetLastError();
 }
 
