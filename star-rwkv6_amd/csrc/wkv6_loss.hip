@@ -547,11 +547,11 @@ __global__ __launch_bounds__(kFinish) void pairs_finish_kernel(int64_t P, Prefer
 
 // The gradient by the logits from stats and c, a pass of its own: kGradVecs vectors of a row to a thread, some workgroups to a row.  No sums, so nothing
 // waits but for its own loads: 12288 rows of 65536 bf16 read and 16384 written in 668 us, 5.6 TB/s.
-template <typename T> __device__ __forceinline__ void grad_piece(const LossRows &a, const LossGrad &g, float up, int64_t row, int piece) {
+template <typename T, int kT> __device__ __forceinline__ void grad_piece(const LossRows &a, const LossGrad &g, float up, int64_t row, int piece) {
     constexpr int kN = Vec<T>::kN;
     const int64_t b = row / a.T, t = row % a.T;
     const int64_t id = a.ids[row];
-    const int V = (int)a.V, tid = threadIdx.x, first = piece * (kGradVecs * kThreads) + tid;
+    const int V = (int)a.V, tid = threadIdx.x % kT, first = piece * (kGradVecs * kT) + tid;
     const T *x = static_cast<const T *>(a.logits) + b * a.stride_b + t * a.stride_t;
     T *out = static_cast<T *>(g.grad) + row * V;
     const Cut<T> cut(x, V);
@@ -561,14 +561,14 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
         z.zero();
 #pragma unroll
         for (int i = 0; i < kGradVecs; ++i)
-            if (first + i * kThreads < cut.full) z.template store<true>(out + cut.head + (int64_t)(first + i * kThreads) * kN);
+            if (first + i * kT < cut.full) z.template store<true>(out + cut.head + (int64_t)(first + i * kT) * kN);
         if (lone) store1(out + cut.single(tid), 0.f);
         return;
     }
     Bits<T> held[kGradVecs];
 #pragma unroll
     for (int i = 0; i < kGradVecs; ++i)
-        if (first + i * kThreads < cut.full) held[i].template load<false>(x + cut.head + (int64_t)(first + i * kThreads) * kN);
+        if (first + i * kT < cut.full) held[i].template load<false>(x + cut.head + (int64_t)(first + i * kT) * kN);
     float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up;
     if (id >= V) c = NAN;
     c *= a.inv_temperature;
@@ -577,25 +577,27 @@ template <typename T> __device__ __forceinline__ void grad_piece(const LossRows 
     either(g.past, [&](auto past) {
 #pragma unroll
         for (int i = 0; i < kGradVecs; ++i) {
-            if (first + i * kThreads >= cut.full) continue;
+            if (first + i * kT >= cut.full) continue;
             gradient<T>(held[i], scale, top, factor);
-            held[i].template store<past.value>(out + cut.head + (int64_t)(first + i * kThreads) * kN);
+            held[i].template store<past.value>(out + cut.head + (int64_t)(first + i * kT) * kN);
         }
     });
     if (lone) store1(out + cut.single(tid), gradient<T>(load1(x + cut.single(tid)), scale, top, factor));
     // the element that stands there, by the thread whose store it was in
     if (id >= V) return;
     const int j = cut.single_of((int)id), v = cut.vector_of((int)id);
-    const bool mine = j >= 0 ? lone && tid == j : v % kThreads == tid && v / (kGradVecs * kThreads) == piece;
+    const bool mine = j >= 0 ? lone && tid == j : v % kT == tid && v / (kGradVecs * kT) == piece;
     if (mine) store1(out + id, c + scale.exp_once(load1(x + id) - top) * factor);
 }
 
-// (The last rows come first: those are the ones that a pass over all rows before this one may have left in the last-level cache.)
-template <typename T> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces, int64_t rows) {
+// kT threads, a workgroup or one of its waves, take a piece.  (The last rows come first: those are the ones that a pass over all rows before this
+// one may have left in the last-level cache.)
+template <typename T, int kT> __global__ __launch_bounds__(kThreads) void grad_kernel(LossRows a, LossGrad g, int pieces, int64_t rows) {
     const float up = g.upstream ? *g.upstream : 1.f;
     if (g.is_there && up == 1.f) return;
-    for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x)
-        grad_piece<T>(a, g, up, rows - 1 - i / pieces, (int)(i % pieces));
+    constexpr int kTogether = kThreads / kT;
+    for (int64_t i = (int64_t)blockIdx.x * kTogether + __builtin_amdgcn_readfirstlane(threadIdx.x / kT); i < rows * pieces; i += (int64_t)gridDim.x * kTogether)
+        grad_piece<T, kT>(a, g, up, rows - 1 - i / pieces, (int)(i % pieces));
 }
 
 template <typename F> hipError_t by_type(int dtype, F &&f) {
@@ -722,10 +724,17 @@ hipError_t loss_grad(hipStream_t st, int dtype, LossRows a, LossGrad g) {
     g.past = past_the_caches(dtype, a);
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t per = (int64_t)kGradVecs * kThreads * Vec<T>::kN, pieces = (a.V + per - 1) / per, all = a.B * a.T * pieces;
-        // (most often there is nothing to do where a forward has written the gradient: 32768 workgroups took 9 us to find that out)
-        const int64_t most = g.is_there ? 2048 : kMostBlocks;
-        hipLaunchKernelGGL((grad_kernel<T>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, a.B * a.T);
+        const auto launch = [&](auto threads) {
+            const int64_t per = (int64_t)kGradVecs * threads.value * Vec<T>::kN, pieces = (a.V + per - 1) / per, rows = a.B * a.T;
+            const int64_t all = (rows * pieces * threads.value + kThreads - 1) / kThreads;
+            // (most often there is nothing to do where a forward has written the gradient: 32768 workgroups took 9 us to find that out)
+            const int64_t most = g.is_there ? 2048 : kMostBlocks;
+            hipLaunchKernelGGL((grad_kernel<T, threads.value>), dim3((unsigned)(all < most ? all : most)), dim3(kThreads), 0, st, a, g, (int)pieces, rows);
+        };
+        // (a short row leaves most of a workgroup idle, a wave with more than four vectors to a lane has few others beside it: 512 MiB of rows by workgroups /
+        // by waves, in us, bf16 V 1000 471 / 186, 2048 245 / 166, 4000 175 / 183; fp32 V 1000 521 / 435, 2048 367 / 421)
+        if (a.V <= 64 * 4 * Vec<T>::kN) launch(std::integral_constant<int, 64>{});
+        else launch(std::integral_constant<int, kThreads>{});
     });
 }
 
