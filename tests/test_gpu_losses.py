@@ -554,3 +554,40 @@ def test_a_backward_captured_after_an_eager_forward():
         eager, = torch.autograd.grad(loss, y, up)
     torch.cuda.synchronize()
     assert torch.equal(eager, w.grad)
+
+
+def test_refusals_on_the_gpu():
+    x, ids, mask, _ = _case(2, 3, 40, torch.bfloat16, 22)
+    A = torch.ones(2, device="cuda")
+    lp = torch.zeros(2, 3, device="cuda")
+    k = rwkv_kernel
+    bad_rows = [(x.double(), ids, mask), (x[0, 0], ids[0, 0], None), (x, ids.int(), mask), (x, ids[:, :2], mask), (x, ids.cpu(), mask), (x, ids, mask.float()),
+                (x, ids, mask[:1]), (x, ids, mask.cpu()), (x[:, :, :0], ids, mask), (x.cpu(), ids, mask)]
+    for rows in bad_rows:
+        for call in (lambda r: k.cross_entropy(*r), lambda r: k.token_logprobs(*r), lambda r: k.preference_loss(*r), lambda r: k.policy_loss(*r, lp, A)):
+            with pytest.raises(AssertionError):
+                call(rows)
+    for call in (lambda: k.cross_entropy(x, ids, reduction="none"), lambda: k.token_logprobs(x, ids, temperature=0.0), lambda: k.preference_loss(x[:1], ids[:1]),
+                 lambda: k.preference_loss(x, ids, kind="other"), lambda: k.preference_loss(x, ids, beta=0.0), lambda: k.preference_loss(x, ids, label_smoothing=0.5),
+                 lambda: k.preference_loss(x, ids, kind="hinge", label_smoothing=0.1), lambda: k.preference_loss(x, ids, ref_logps=lp),
+                 lambda: k.preference_loss(x[0], ids[0]), lambda: k.preference_loss(x[:, :0], ids[:, :0]), lambda: k.policy_loss(x[0], ids[0], None, lp[0], A),
+                 lambda: k.policy_loss(x, ids, mask, lp[:, :2], A), lambda: k.policy_loss(x, ids, mask, lp.cpu(), A), lambda: k.policy_loss(x, ids, mask, lp, A[:1]),
+                 lambda: k.policy_loss(x, ids, mask, lp, A, ref_logps=lp[0]), lambda: k.policy_loss(x, ids, mask, lp, A, reduction="sum"),
+                 lambda: k.policy_loss(x, ids, mask, lp, A, clip_low=-0.1), lambda: k.policy_loss(x, ids, mask, lp, A, kl_weight=-1.0),
+                 lambda: k.policy_loss(x, ids, mask, lp, A, temperature=0.0), lambda: k.policy_loss(x[:, :0], ids[:, :0], None, lp[:, :0], A)):
+        with pytest.raises(AssertionError):
+            call()
+    with pytest.raises(RuntimeError, match="wkv6"):     # 1 / temperature is no number of fp32
+        k.token_logprobs(x, ids, temperature=1e-40)
+
+
+def test_other_types_beside_the_logits():
+    """Masks in bytes, log probabilities and advantages in other types or not contiguous: as their fp32 copies."""
+    x, ids, mask, g = _case(4, 6, 500, torch.float32, 23)
+    old = rwkv_kernel.token_logprobs(x, ids) - 0.05
+    ref, A = old + 0.1, torch.randn(4, 6, generator=g).cuda()
+    want = rwkv_kernel.policy_loss(x, ids, mask, old, A, ref_logps=ref, kl_weight=0.1)
+    wide = lambda t: t.t().contiguous().t()  # noqa: E731
+    for got in (rwkv_kernel.policy_loss(x, wide(ids), wide(mask).to(torch.uint8) * 7, old.double(), wide(A), ref_logps=wide(ref), kl_weight=0.1),
+                rwkv_kernel.policy_loss(wide(x.view(4, -1)).view(4, 6, 500), ids, mask, wide(old), A.double(), ref_logps=ref, kl_weight=0.1)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
