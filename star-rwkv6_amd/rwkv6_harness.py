@@ -183,8 +183,8 @@ class RWKV6(nn.Module):
 
 
 def _kernels(logits):
-    """The operator package where it has losses for these logits (its torch flavour, on the GPU), else None."""
-    if not logits.is_cuda or os.environ.get("KERAS_BACKEND") != "torch":
+    """The operator package where it has losses for these logits (its torch flavour, on the GPU, in 16 or 32 bits), else None."""
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32) or os.environ.get("KERAS_BACKEND") != "torch":
         return None
     import rwkv_kernel
 

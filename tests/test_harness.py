@@ -285,3 +285,16 @@ def test_config4_full_size_train_step(oracle):
     check_composite("goffset", rec["offset_param"].grad, want["goffset"])
     for name, leaf in zip("gr gk gv gw gu".split(), "rkvwu"):
         check_composite(name, rec[leaf].grad, want[name])
+
+
+@pytest.mark.gpu
+def test_train_step_takes_logits_in_64_bits():
+    """A model in double precision trains as it always did: the loss is torch's cross entropy of its logits in fp32."""
+    torch.manual_seed(8)
+    model = torch.nn.Embedding(31, 31).double().cuda()     # (a model whose logits are looked up)
+    ids = torch.randint(0, 31, (3, 9), device="cuda")
+    before = model.weight.detach().clone()
+    with torch.no_grad():
+        want = F.cross_entropy(model(ids[:, :-1]).float().reshape(-1, 31), ids[:, 1:].reshape(-1))
+    loss = hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), ids)
+    assert torch.equal(loss, want) and not torch.equal(model.weight, before) and bool(torch.isfinite(model.weight).all())
