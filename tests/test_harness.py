@@ -298,3 +298,26 @@ def test_train_step_takes_logits_in_64_bits():
         want = F.cross_entropy(model(ids[:, :-1]).float().reshape(-1, 31), ids[:, 1:].reshape(-1))
     loss = hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), ids)
     assert torch.equal(loss, want) and not torch.equal(model.weight, before) and bool(torch.isfinite(model.weight).all())
+
+
+@pytest.mark.gpu
+def test_train_step_takes_logits_of_another_shape():
+    """Rows of logits one behind the other, or with a dimension between, belong to the texts' tokens in order, as torch's cross entropy takes them."""
+    class Shaped(torch.nn.Embedding):
+        def forward(self, ids):
+            return super().forward(ids).reshape(*self.shape_of(ids), self.num_embeddings)
+
+    torch.manual_seed(9)
+    ids = torch.randint(0, 31, (3, 9), device="cuda")
+    weight = torch.randn(31, 31, device="cuda")
+    grads = []
+    for shape_of in (lambda ids: ids.shape, lambda ids: (ids.numel(),), lambda ids: (ids.shape[0], 1, ids.shape[1]), lambda ids: (ids.numel(), 1)):
+        model = Shaped(31, 31).cuda()
+        model.shape_of = shape_of
+        with torch.no_grad():
+            model.weight.copy_(weight)
+        loss = hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), ids)
+        grads.append((loss, model.weight.grad))
+    for loss, grad in grads[1:]:
+        # (the same rows and sums; the embedding's backward may add them up in another order: 27 terms of less than 1 / 24 each)
+        assert torch.equal(loss, grads[0][0]) and float((grad - grads[0][1]).abs().max()) <= 27 * 2.0 ** -24
