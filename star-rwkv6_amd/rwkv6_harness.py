@@ -212,7 +212,7 @@ def train_step(model, optimizer, ids, autocast_dtype=None):
     if kernels is not None:
         if logits.shape[:-1] != target.shape:
             logits, target = logits.reshape(-1, logits.shape[-1]), target.reshape(-1)
-        return _update(optimizer, kernels.cross_entropy(logits, target))
+        return _update(optimizer, kernels.cross_entropy(logits, target.long()))
     return _update(optimizer, F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), target.reshape(-1)))
 
 

@@ -321,3 +321,22 @@ def test_train_step_takes_logits_of_another_shape():
     for loss, grad in grads[1:]:
         # (the same rows and sums; the embedding's backward may add them up in another order: 27 terms of less than 1 / 24 each)
         assert torch.equal(loss, grads[0][0]) and float((grad - grads[0][1]).abs().max()) <= 27 * 2.0 ** -24
+
+
+@pytest.mark.gpu
+def test_train_step_takes_tokens_in_bytes():
+    """A model over bytes whose ids are held as such: as with the same ids in 64 bits."""
+    class Bytes(torch.nn.Embedding):
+        def forward(self, ids):
+            return super().forward(ids.long())
+
+    torch.manual_seed(10)
+    ids = torch.randint(0, 256, (3, 9), device="cuda", dtype=torch.uint8)
+    weight = torch.randn(256, 256, device="cuda")
+    runs = []
+    for tokens in (ids.long(), ids):
+        model = Bytes(256, 256).cuda()
+        with torch.no_grad():
+            model.weight.copy_(weight)
+        runs.append(hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), tokens))
+    assert torch.equal(*runs)
