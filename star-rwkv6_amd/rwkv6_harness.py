@@ -191,6 +191,13 @@ def _kernels(logits):
     return rwkv_kernel
 
 
+def _losses(logits):
+    """The same where there is nothing to fall back on."""
+    kernels = _kernels(logits)
+    assert kernels is not None, "this step is for the package's torch flavour (KERAS_BACKEND=torch) and logits in 16 or 32 bits on the GPU"
+    return kernels
+
+
 def _logits(model, ids, autocast_dtype):
     """The model's logits for every token but the first of each text."""
     dev = ids.device.type
@@ -223,7 +230,7 @@ def train_step(model, optimizer, ids, autocast_dtype=None):
 def token_logprobs(model, ids, mask, autocast_dtype=None, temperature=1.0):
     """Log probabilities (B, T) of the texts' tokens: what a reference or a sampling model makes of them."""
     logits = _logits(model, ids, autocast_dtype)
-    return _kernels(logits).token_logprobs(logits, ids[:, 1:], mask, temperature=temperature)
+    return _losses(logits).token_logprobs(logits, ids[:, 1:], mask, temperature=temperature)
 
 
 def preference_step(model, optimizer, ids, mask, ref_logps, autocast_dtype=None, **options):
@@ -231,7 +238,7 @@ def preference_step(model, optimizer, ids, mask, ref_logps, autocast_dtype=None,
     as of rwkv_kernel.preference_loss.  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
     logits = _logits(model, ids, autocast_dtype)
-    return _update(optimizer, _kernels(logits).preference_loss(logits, ids[:, 1:], mask, ref_logps=ref_logps, **options)[0])
+    return _update(optimizer, _losses(logits).preference_loss(logits, ids[:, 1:], mask, ref_logps=ref_logps, **options)[0])
 
 
 def policy_step(model, optimizer, ids, mask, old_logps, advantages, autocast_dtype=None, **options):
@@ -239,7 +246,7 @@ def policy_step(model, optimizer, ids, mask, old_logps, advantages, autocast_dty
     rwkv_kernel.policy_loss.  Returns the loss."""
     optimizer.zero_grad(set_to_none=True)
     logits = _logits(model, ids, autocast_dtype)
-    return _update(optimizer, _kernels(logits).policy_loss(logits, ids[:, 1:], mask, old_logps, advantages, **options)[0])
+    return _update(optimizer, _losses(logits).policy_loss(logits, ids[:, 1:], mask, old_logps, advantages, **options)[0])
 
 
 # the layer shape of configuration 4: RWKV6-1.6B (24 layers, d_model 2048, 32 heads of 64, FFN 7168)

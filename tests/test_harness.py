@@ -340,3 +340,17 @@ def test_train_step_takes_tokens_in_bytes():
             model.weight.copy_(weight)
         runs.append(hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), tokens))
     assert torch.equal(*runs)
+
+
+def test_fine_tuning_steps_say_what_they_need(monkeypatch):
+    """Off the GPU, or with another flavour of the package, there are no losses to run them on."""
+    model = _toy(OPSKernelOperator(64, 32))
+    opt = torch.optim.SGD(model.parameters(), lr=0.1)
+    ids = torch.randint(0, TOY["vocabulary_size"], (2, 9))
+    mask = torch.ones(2, 8, dtype=torch.bool)
+    for backend in ("torch", "jax"):
+        monkeypatch.setenv("KERAS_BACKEND", backend)
+        for step in (lambda: hz.token_logprobs(model, ids, mask), lambda: hz.preference_step(model, opt, ids, mask, torch.zeros(2)),
+                     lambda: hz.policy_step(model, opt, ids, mask, torch.zeros(2, 8), torch.zeros(2))):
+            with pytest.raises(AssertionError, match="on the GPU"):
+                step()
