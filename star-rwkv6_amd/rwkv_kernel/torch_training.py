@@ -187,7 +187,7 @@ class AdamW(torch.optim.Optimizer):
                 s[name] = torch.zeros_like(p, dtype=dtype, memory_format=torch.preserve_format)
         if self.moment_bits == 8:
             s["scales"] = torch.zeros((p.numel() + SCALE_BLOCK - 1) // SCALE_BLOCK, 2, dtype=torch.float32, device=p.device)
-        if self.master_weights and p.dtype != torch.float32:
+        if self._has_master(p):
             s["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
 
     def _cohorts(self):
@@ -247,13 +247,21 @@ class AdamW(torch.optim.Optimizer):
                            max_grad_norm=self.max_grad_norm, grad_norm=norm, skip_nonfinite=self.skip_nonfinite, seed=self.seed + n)
         return loss
 
+    def _has_master(self, p):
+        return self.master_weights and p.dtype != torch.float32
+
     def load_state_dict(self, state_dict):
-        """As every optimizer's, but states keep their own dtypes, and parameters with one step count share it again."""
-        for s in state_dict["state"].values():
-            assert ("scales" in s) == (self.moment_bits == 8), "the moments were saved in another number of bits"
+        """As every optimizer's, but states keep their own dtypes, and parameters with one step count share it again.  A state with moments in another
+        number of bits, without the masters that this optimizer has or with others, is refused."""
+        theirs = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(theirs, [p for group in self.param_groups for p in group["params"]]):
+            s = state_dict["state"].get(i)
+            if s:
+                assert ("scales" in s) == (self.moment_bits == 8), "the moments were saved in another number of bits"
+                assert ("master" in s) == self._has_master(p), "saved %s master, by an optimizer with other master_weights or parameters of another dtype" % (
+                    "with a" if "master" in s else "without a")
         super().load_state_dict(state_dict)
         ours = [(n, p) for n, group in enumerate(self.param_groups) for p in group["params"]]
-        theirs = [i for group in state_dict["param_groups"] for i in group["params"]]
         shared = {}
         for (n, p), i in zip(ours, theirs):
             if i not in state_dict["state"]:

@@ -120,3 +120,32 @@ def test_python_layer():
         k.adamw_step([p.detach()], [p.grad], [p.grad], [p.grad], torch.zeros((), dtype=torch.int64), 1e-3)
     with pytest.raises(RuntimeError, match="GPU"):
         k.grad_norm([p.grad])
+
+
+def test_masters_are_not_lost_or_gained_by_loading():
+    """A state whose masters are not what the optimizer asks for is refused before anything is taken from it (no GPU needed)."""
+    import rwkv_kernel as k
+    params = lambda: [torch.nn.Parameter(torch.ones(5, dtype=d)) for d in (torch.bfloat16, torch.float32)]  # noqa: E731
+
+    def saved(masters):
+        """What an optimizer over the two has saved behind a step, with or without a master of the first."""
+        state = {i: dict(step=torch.tensor(3), exp_avg=torch.full((5,), 0.5), exp_avg_sq=torch.full((5,), 0.25)) for i in (0, 1)}
+        if masters:
+            state[0]["master"] = torch.full((5,), 1.001)
+        return dict(k.AdamW(params(), master_weights=masters).state_dict(), state=state)
+
+    for has in (False, True):
+        for wants in (False, True):
+            opt = k.AdamW(params(), master_weights=wants)
+            if has != wants:
+                with pytest.raises(AssertionError, match="master"):
+                    opt.load_state_dict(saved(has))
+                assert not opt.state
+                continue
+            opt.load_state_dict(saved(has))
+            a, b = (opt.state[p] for p in opt.param_groups[0]["params"])
+            assert ("master" in a) == wants and "master" not in b and int(a["step"]) == 3
+            assert not wants or (a["master"].dtype == torch.float32 and bool((a["master"] == 1.001).all()))
+    # parameters of 16 bits that became parameters of 32 have no master either
+    with pytest.raises(AssertionError, match="master"):
+        k.AdamW([torch.nn.Parameter(p.detach().float()) for p in params()], master_weights=True).load_state_dict(saved(True))
