@@ -591,3 +591,32 @@ def test_other_types_beside_the_logits():
     for got in (rwkv_kernel.policy_loss(x, wide(ids), wide(mask).to(torch.uint8) * 7, old.double(), wide(A), ref_logps=wide(ref), kl_weight=0.1),
                 rwkv_kernel.policy_loss(wide(x.view(4, -1)).view(4, 6, 500), ids, mask, wide(old), A.double(), ref_logps=ref, kl_weight=0.1)):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _banned_case(dtype, seed, B=2, T=4, V=300):
+    """Logits of which the token that stands at (0, 1) has -inf, with softmax and E of each row in 64 bits."""
+    x, ids, _, g = _case(B, T, V, dtype, seed)
+    ids[0, 1] = 8
+    x[0, 1, 8] = float("-inf")
+    _, lp, _, E, p = _lp64(x, ids, None)
+    return x, ids, lp.detach(), E, p, g
+
+
+def _rows_of(c, ids, p):
+    """c (1[id] - p) of each row, in 64 bits."""
+    return c[..., None] * (torch.zeros_like(p).scatter_(-1, ids.cpu()[..., None], 1.0) - p)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_policy_of_a_banned_token_without_old_logps(dtype):
+    """The ratio is 1 wherever the log probability is a number or -inf: loss and gradient are the advantages'."""
+    x, ids, lp, E, p, g = _banned_case(dtype, 41)
+    A = torch.randn(2, 4, generator=g)
+    xr = x.clone().requires_grad_(True)
+    loss, got_lp, means = rwkv_kernel.policy_loss(xr, ids, None, None, A.cuda())
+    want = -A.double().mean()
+    _within("loss", loss, want, 4 * U * A.double().abs().mean())
+    assert float(got_lp[0, 1]) == float("-inf") and means.tolist() == [0.0, 0.0]
+    loss.backward()
+    c = -A.double() / 8
+    _grad_within("grad", xr.grad, _rows_of(c, ids, p), p, c, 4 * U * c.abs(), E, dtype)
