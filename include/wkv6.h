@@ -389,7 +389,7 @@ int wkv6_cross_entropy(void *stream, int dtype, int64_t B, int64_t T, int64_t V,
                        void *workspace, size_t workspace_bytes);
 
 /* Clipped policy loss: with ratio = exp(logp - old_logps) (1 where old_logps is NULL: the sampling model is this one) and
- * e = ref_logps - logp (no such term where NULL), the mean over counted tokens of
+ * e = ref_logps - logp (no such term where NULL; with a kl_weight of 0 it is in means alone), the mean over counted tokens of
  *   kl_weight (exp(e) - e - 1) - min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A),   A = advantages[b adv_stride_b + t adv_stride_t]
  * WKV6_REDUCE_MEAN: over all tokens; WKV6_REDUCE_MEAN_OF_TEXTS: over each text's tokens, then over the texts that have any.
  * means (2): the same mean of exp(e) - e - 1, and of whether the clamped term was the smaller one. */

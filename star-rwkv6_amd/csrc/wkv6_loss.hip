@@ -266,10 +266,12 @@ __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l
     float kl = 0.f, by_lp = clipped ? 0.f : -free;
     if (l.ref_logps) {
         const float e = l.ref_logps[row] - lp, g = expm1f(e);   // (small where the models agree: neither term is formed from 1)
-        kl = g - e;
-        by_lp -= l.kl_weight * g;
+        kl = g == INFINITY ? g : g - e;                         // (e may be infinite too)
+        // (a weight of 0: the term is reported and takes no part, infinite as it may be)
+        if (l.kl_weight != 0.f) by_lp -= l.kl_weight * g;
     }
-    l.terms[row] = (l.kl_weight * kl - (clipped ? held : free)) * w;
+    const float penalty = l.kl_weight != 0.f ? l.kl_weight * kl : 0.f;
+    l.terms[row] = (penalty - (clipped ? held : free)) * w;
     l.terms[rows + row] = kl * w;
     l.terms[2 * rows + row] = clipped ? w : 0.f;
     return by_lp * w;

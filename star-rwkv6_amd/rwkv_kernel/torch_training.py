@@ -106,7 +106,7 @@ def policy_loss(logits, ids, mask, old_logps, advantages, ref_logps=None, clip_l
     sampling model's; None: the sampling model is this one, the ratio 1 with lp's gradient) and e = ref_logps - lp, the loss is the mean of
         kl_weight (exp(e) - e - 1) - min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
     over all tokens that count ("mean"), or over each text's and then over the texts that have any ("mean_of_texts").  `advantages`: (B,)
-    or (B, T).  `ref_logps` (B, T): a reference model's; None: no KL term.  None of the three gets a gradient.
+    or (B, T).  `ref_logps` (B, T): a reference model's; None: no KL term, and with a kl_weight of 0 it is in the means alone.  None of the three gets a gradient.
     Returns (loss, lp, means): an fp32 scalar, differentiable in logits, and without gradients lp (B, T) and the same means of
     exp(e) - e - 1 and of whether the clamped term was the smaller one (2 values).  With a gradient wanted the logits are read once."""
     logits, ids, mask = _rows(logits, ids, mask, False)

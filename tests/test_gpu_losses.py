@@ -620,3 +620,30 @@ def test_policy_of_a_banned_token_without_old_logps(dtype):
     loss.backward()
     c = -A.double() / 8
     _grad_within("grad", xr.grad, _rows_of(c, ids, p), p, c, 4 * U * c.abs(), E, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_policy_kl_that_is_infinite(dtype):
+    """A KL term beyond fp32's range, or of a banned token, is infinite and no NaN; with a weight of 0 it is only reported, and loss and
+    gradient are those without a reference model, bit for bit."""
+    x, ids, lp, E, p, g = _banned_case(dtype, 42)
+    A = torch.randn(2, generator=g).cuda()
+    ref = torch.where(torch.isfinite(lp), lp, torch.full_like(lp, -3.0)).float().cuda()   # (a number where lp is -inf: exp(e) is infinite there)
+    far = torch.zeros_like(ref)
+    far[1, 2] = 200.0
+    for r, spoilt in ((ref, (0, 1)), (ref + far, (1, 2))):
+        ids_r = ids.clone()
+        if spoilt == (1, 2):
+            ids_r[0, 1] = -1                               # (the banned token does not count)
+        runs = []
+        for kw in (dict(), dict(ref_logps=r, kl_weight=0.0), dict(ref_logps=r, kl_weight=0.1)):
+            xr = x.clone().requires_grad_(True)
+            loss, _, means = rwkv_kernel.policy_loss(xr, ids_r, None, None, A, **kw)
+            loss.backward()
+            runs.append((loss.detach(), xr.grad, means))
+        assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1]) and bool(torch.isfinite(runs[0][1]).all())
+        assert runs[0][2].tolist() == [0.0, 0.0] and runs[1][2].tolist() == [float("inf"), 0.0]
+        assert float(runs[2][0]) == float("inf") and float(runs[2][2][0]) == float("inf")
+        others = torch.ones(2, 4, dtype=torch.bool)
+        others[spoilt] = False
+        assert bool(torch.isfinite(runs[2][1][others.cuda()]).all()) and not bool(torch.isfinite(runs[2][1][spoilt]).all())
