@@ -261,7 +261,9 @@ __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l
     const int64_t b = row / a.T, t = row % a.T;
     const float A = l.advantages[b * l.adv_stride_b + t * l.adv_stride_t];
     const float ratio = l.old_logps ? expf(lp - l.old_logps[row]) : lp == lp ? 1.f : lp;   // (the sampling model is this one: only NaN stays NaN)
-    const float free = ratio * A, held = fminf(fmaxf(ratio, 1.f - l.clip_low), 1.f + l.clip_high) * A;
+    // (exp of a finite difference that fp32 cannot hold, times an advantage of 0: 0 and no NaN)
+    const bool beyond = A == 0.f && ratio == INFINITY && lp - l.old_logps[row] < INFINITY;
+    const float free = beyond ? 0.f : ratio * A, held = fminf(fmaxf(ratio, 1.f - l.clip_low), 1.f + l.clip_high) * A;
     const bool clipped = free > held;
     float kl = 0.f, by_lp = clipped ? 0.f : -free;
     if (l.ref_logps) {

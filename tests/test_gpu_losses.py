@@ -647,3 +647,26 @@ def test_policy_kl_that_is_infinite(dtype):
         others = torch.ones(2, 4, dtype=torch.bool)
         others[spoilt] = False
         assert bool(torch.isfinite(runs[2][1][others.cuda()]).all()) and not bool(torch.isfinite(runs[2][1][spoilt]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_policy_ratio_beyond_the_range_with_an_advantage_of_zero(dtype):
+    """exp(lp - old) of 100 is beyond fp32: times an advantage of 0 it is 0, as the formula's; of a positive one it is clipped, of a negative one infinite."""
+    x, ids, _, g = _case(2, 3, 200, dtype, 43)
+    _, lp, _, E, p = _lp64(x, ids, None)
+    old = lp.detach().float().cuda()
+    old[0, 1] -= 100.0
+    A = torch.tensor([[1.0, 0.0, -0.5], [0.25, 2.0, -1.0]])
+    xr = x.clone().requires_grad_(True)
+    loss, _, means = rwkv_kernel.policy_loss(xr, ids, None, old, A.cuda())
+    loss.backward()
+    # (elsewhere the ratio is 1 but for what lp and its rounding are off by)
+    off = E + 8 * U * (1 + lp.detach().abs())
+    _within("loss", loss, -A.double().mean(), (A.double().abs() * off).mean() * 2)
+    c = -A.double() / 6
+    _grad_within("grad", xr.grad, _rows_of(c, ids, p), p, c, 2 * c.abs() * off, E, dtype)
+    assert bool((xr.grad[0, 1] == 0).all()) and means.tolist() == [0.0, 0.0]
+    for a, want in ((0.5, False), (-0.5, True)):
+        A[0, 1] = a
+        loss = rwkv_kernel.policy_loss(x, ids, None, old, A.cuda())[0]
+        assert bool(torch.isinf(loss)) == want and not bool(torch.isnan(loss))
