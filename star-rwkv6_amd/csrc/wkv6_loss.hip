@@ -529,7 +529,7 @@ __global__ __launch_bounds__(kFinish) void pairs_kernel(LossRows a, PreferenceTe
     } else if (l.kind == kPreferenceHinge) {
         const double z = 1. - l.beta * d;
         loss = z <= 0. ? 0. : z;
-        by_d = z <= 0. ? 0. : -l.beta + 0. * z;
+        by_d = z <= 0. ? 0. : z == z ? -l.beta : z;
     } else {
         const double z = d - 0.5 / l.beta;
         loss = z * z;

@@ -670,3 +670,23 @@ def test_policy_ratio_beyond_the_range_with_an_advantage_of_zero(dtype):
         A[0, 1] = a
         loss = rwkv_kernel.policy_loss(x, ids, None, old, A.cuda())[0]
         assert bool(torch.isinf(loss)) == want and not bool(torch.isnan(loss))
+
+
+@pytest.mark.parametrize("kind", ["hinge", "sigmoid"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_preference_for_a_text_with_a_banned_token(dtype, kind):
+    """A chosen text of probability zero: the loss is infinite, and its slope -beta, as the formula's."""
+    x, ids, lp, E, p, _ = _banned_case(dtype, 44)
+    beta = 0.3
+    xr = x.clone().requires_grad_(True)
+    loss, s = rwkv_kernel.preference_loss(xr, ids, beta=beta, kind=kind)
+    assert float(loss) == float("inf") and float(s[0]) == float("-inf") and math.isfinite(float(s[1]))
+    loss.backward()
+    c = torch.tensor([-beta, beta]).double()[:, None].expand(2, 4)
+    _grad_within("grad", xr.grad, _rows_of(c, ids, p), p, c, 4 * U * c.abs(), E, dtype)
+    # rejected instead, it costs nothing
+    back = torch.tensor([1, 0]).cuda()
+    xr = x[back].clone().requires_grad_(True)
+    loss, _ = rwkv_kernel.preference_loss(xr, ids[back], beta=beta, kind=kind)
+    loss.backward()
+    assert float(loss) == 0.0 and bool((xr.grad == 0).all())
