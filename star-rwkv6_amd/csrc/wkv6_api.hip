@@ -323,7 +323,7 @@ static int check_rows(int dtype, int64_t B, int64_t T, int64_t V, const void *lo
 }
 static wkv6::LossRows rows_of(int64_t B, int64_t T, int64_t V, const void *logits, int64_t stride_b, int64_t stride_t,
                               const int64_t *ids, const uint8_t *mask, float temperature, float *logps, float *stats) {
-    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1.f / temperature, logps, stats, nullptr};
+    return {B, T, V, stride_b, stride_t, logits, ids, mask, 1. / temperature, logps, stats, nullptr};
 }
 static bool floats(std::initializer_list<const void *> ps) {
     for (const void *p : ps)

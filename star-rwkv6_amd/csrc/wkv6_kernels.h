@@ -341,7 +341,7 @@ struct LossRows {
     const void *logits;
     const int64_t *ids;
     const uint8_t *mask;
-    float inv_temperature;
+    double inv_temperature;
     float *logps;   // (B,T) or null
     float *stats;   // (B,T,2) top and sum of a row, or null
     double *exact;  // (B,T) logps in 64 bits, or null

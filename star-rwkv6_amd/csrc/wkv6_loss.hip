@@ -39,13 +39,13 @@ constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's ow
 constexpr int64_t kPastBytes = 160 << 20;
 constexpr double kLog2e = 1.44269504088896340736;
 
-// exp(d / temperature) as a power of two.  log2(e) / temperature rounded to fp32 is off by up to 2^-24 of itself, the same way in
+// exp(d / temperature) as a power of two.  (1 / temperature is in 64 bits, here and in lp.)  log2(e) / temperature rounded to fp32 is off by up to 2^-24 of itself, the same way in
 // every element: lp would be off by as much times the mean of d, over a whole text hundreds of times that.  `low` is what the
 // rounding left; the gradient, whose elements are rounded one by one, does without.  (`high` is rounded down and `low` positive: with d = -inf
 // the two products are -inf both, and not two infinities of different signs.)
 struct Scale {
     float high, low;
-    __device__ __forceinline__ explicit Scale(float inv_temperature) {
+    __device__ __forceinline__ explicit Scale(double inv_temperature) {
         const double s = kLog2e * inv_temperature;
         high = (float)s;
         if ((double)high >= s) high = __uint_as_float(__float_as_uint(high) - 1);
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)
     sum = block_sum<kW>(sum, part_sum);
     float c = id < V ? -w : NAN;   // the cross entropy's: lp does not come into it
     if (tid < 64) {
-        const double lp = __builtin_fma((double)(stands - top), (double)a.inv_temperature, -log((double)sum));
+        const double lp = __builtin_fma((double)(stands - top), a.inv_temperature, -log((double)sum));
         if (tid == 0) {
             if (l.kind != kLossNone) c = row_terms(a, l, row, lp, w);
             if (a.logps) a.logps[row] = (float)lp;
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(kT == 64 ? kThreads : kT, waves_per_simd(kT, kVecs)
             c = part_c;
         }
     }
-    c *= a.inv_temperature;
+    c *= (float)a.inv_temperature;
     const float norm = 1.f / sum, factor = -c * norm;
     if (kHold) {
         either(g.past, [&](auto past) {
@@ -575,7 +575,7 @@ template <typename T, int kT> __device__ __forceinline__ void grad_piece(const L
         if (first + i * kT < cut.full) held[i].template load<false>(x + cut.head + (int64_t)(first + i * kT) * kN);
     float c = g.coef[b * g.coef_stride_b + t * g.coef_stride_t] * up;
     if (id >= V) c = NAN;
-    c *= a.inv_temperature;
+    c *= (float)a.inv_temperature;
     const float top = a.stats[2 * row], norm = 1.f / a.stats[2 * row + 1], factor = -c * norm;
     const Scale scale(a.inv_temperature);
     either(g.past, [&](auto past) {

@@ -12,7 +12,7 @@ slice of a longer sequence is taken as it is).  All arithmetic on them is in fp3
 logits' dtype and is rounded once.  `ids` (int64) names the token that stands at each place: for a model's outputs at
 positions 0 .. T-1 these are the input ids from position 1 on.  A token counts if its `mask` is not zero (None: all do) and its id is not
 negative; the logits of one that does not are never read, and get a gradient of zero.  An id of V or more makes its token's log
-probability, and with it the loss, NaN.
+probability, and with it the loss, NaN.  A temperature is the fp32 number nearest to what is given; logits are divided by it in 64 bits.
 
 Calls go to the current stream of the tensors' device, allocate nothing but their results and workspaces, never
 synchronise, and can be captured into a graph.

@@ -690,3 +690,22 @@ def test_preference_for_a_text_with_a_banned_token(dtype, kind):
     loss, _ = rwkv_kernel.preference_loss(xr, ids[back], beta=beta, kind=kind)
     loss.backward()
     assert float(loss) == 0.0 and bool((xr.grad == 0).all())
+
+
+@pytest.mark.parametrize("temperature", [0.7, 0.9, 1.3, 3.3])
+def test_temperature_has_no_error_of_its_own(temperature):
+    """The log probability is divided by the temperature (as an fp32 number) in 64 bits.  Rows of two logits, 0 and -d with d of 60 and more: the sum of
+    exponentials is 1 to the last bit (exp(-60 / 3.3) < 2^-26), so lp is -d / temperature, once rounded: no rounding of 1 / temperature, which has the same sign in each token, adds up
+    over a text.  (Half of a last place, 2^-24 of the value at most, and 2^-50 for the arithmetic in 64 bits; at 3.3 what the sum of exponentials leaves out.)"""
+    tau = float(torch.tensor(temperature))
+    d = torch.linspace(60, 400, 1999)
+    x = torch.stack([torch.zeros_like(d), -d], 1)[None].cuda()
+    ids = torch.ones(1, d.numel(), dtype=torch.int64, device="cuda")
+    want = -d.double() / tau - torch.log1p(torch.exp(-d.double() / tau))
+    with torch.no_grad():
+        for lp in (rwkv_kernel.token_logprobs(x, ids, temperature=temperature),
+                   rwkv_kernel.policy_loss(x, ids, None, None, torch.ones(1).cuda(), temperature=temperature)[1]):
+            off = lp.cpu().double()[0] - want
+            assert bool((off.abs() <= want.abs() * 2.0 ** -24 * (1 + 2.0 ** -20) + torch.exp(-d.double() / tau)).all()), float((off / want).abs().max())
+            # and the errors' mean is that of roundings, each at most 2^-24 of its value either way: 1999 of them, nine standard deviations of their mean
+            assert abs(float((off / want).mean())) <= 9 * 2.0 ** -24 / math.sqrt(3 * d.numel())
