@@ -49,7 +49,7 @@ struct Scale {
         const double s = kLog2e * inv_temperature;
         high = (float)s;
         if ((double)high >= s) high = __uint_as_float(__float_as_uint(high) - 1);
-        low = (float)(s - high);
+        low = fmaxf((float)(s - high), 0x1p-149f);
     }
     __device__ __forceinline__ float exp(float d) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(d, high, d * low)); }
     __device__ __forceinline__ float exp_once(float d) const { return __builtin_amdgcn_exp2f(d * high); }

@@ -709,3 +709,18 @@ def test_temperature_has_no_error_of_its_own(temperature):
             assert bool((off.abs() <= want.abs() * 2.0 ** -24 * (1 + 2.0 ** -20) + torch.exp(-d.double() / tau)).all()), float((off / want).abs().max())
             # and the errors' mean is that of roundings, each at most 2^-24 of its value either way: 1999 of them, nine standard deviations of their mean
             assert abs(float((off / want).mean())) <= 9 * 2.0 ** -24 / math.sqrt(3 * d.numel())
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e20, 1e29, 3e36, 1e38, 3.4e38])
+def test_banned_tokens_at_temperatures_at_the_ends_of_the_range(temperature):
+    """All tokens that are not banned are as likely as each other, or the largest logit is all there is."""
+    x, ids, _, _ = _case(1, 2, 300, torch.float32, 48)
+    x[:, :, 40:290] = float("-inf")
+    ids[:] = x.argmax(-1)
+    xr = x.clone().requires_grad_(True)
+    lp = rwkv_kernel.token_logprobs(xr, ids, temperature=temperature)
+    lp.sum().backward()
+    want = 0.0 if temperature < 1 else -math.log(50)
+    # (of 50 equal terms the sum is exact; log and its rounding)
+    assert float((lp.detach().double() - want).abs().max()) <= 2 * U * abs(want)
+    assert bool((xr.grad[:, :, 40:290] == 0).all()) and bool(torch.isfinite(xr.grad).all())
