@@ -380,6 +380,21 @@ Tensor logits_backward(const variable_list &saved, double temperature, const Ten
 
 Tensor arriving(const Tensor &g) { return g.to(at::kFloat).contiguous(); }
 
+// Stands for what a gradient depends on where a graph of the backward is wanted (create_graph): the gradient has its value, and a derivative of it
+// is refused, where without a node it would be missing from whatever it is a part of.
+struct FirstOrder : torch::autograd::Function<FirstOrder> {
+  static Tensor forward(AutogradContext *, const Tensor &grad, const Tensor &, const Tensor &) { return grad; }
+  static variable_list backward(AutogradContext *, variable_list) {
+    TORCH_CHECK(false, "wkv6: the losses over logits have no second derivative");
+  }
+};
+
+Tensor first_order(bool graph_wanted, const Tensor &grad, const Tensor &logits, const Tensor &arrived) {
+  if (!graph_wanted) return grad;
+  const at::AutoGradMode on(true);
+  return FirstOrder::apply(grad, logits, arrived);
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &ids, const std::optional<Tensor> &mask, double temperature, bool wanted) {
     const c10::DeviceGuard guard(x.device());
@@ -391,11 +406,13 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return lp;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
     const Tensor coef = arriving(grads[0]);
-    return {logits_backward(s, ctx->saved_data["temperature"].toDouble(), coef, s[0].size(1), 1, Tensor(), Tensor()), Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor grad = logits_backward(s, ctx->saved_data["temperature"].toDouble(), coef, s[0].size(1), 1, Tensor(), Tensor());
+    return {first_order(graph_wanted, grad, s[0], grads[0]), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -414,11 +431,13 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     return loss;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
     const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad"), up = arriving(grads[0]);
-    return {logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead), Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor grad = logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead);
+    return {first_order(graph_wanted, grad, s[0], grads[0]), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -444,13 +463,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     return {loss, lp, means};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     variable_list res(12);
     if (!grads[0].defined()) return res;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
     const Tensor ahead = is_captured() ? Tensor() : take(ctx, "grad"), up = arriving(grads[0]);
-    res[0] = logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead);
+    res[0] = first_order(graph_wanted, logits_backward(s, ctx->saved_data["temperature"].toDouble(), s[4], s[0].size(1), 1, up, ahead), s[0], grads[0]);
     return res;
   }
 };
@@ -472,12 +492,13 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     return {loss, text};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     variable_list res(9);
     if (!grads[0].defined()) return res;
     const auto s = ctx->get_saved_variables();
     const c10::DeviceGuard guard(s[0].device());
-    res[0] = logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor());
+    res[0] = first_order(graph_wanted, logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor()), s[0], grads[0]);
     return res;
   }
 };

@@ -16,6 +16,8 @@ probability, and with it the loss, NaN.  A temperature is the fp32 number neares
 
 Calls go to the current stream of the tensors' device, allocate nothing but their results and workspaces, never
 synchronise, and can be captured into a graph.
+
+The losses have first derivatives.  A gradient taken with create_graph has its value, and a derivative of it is refused.
 """
 import torch
 

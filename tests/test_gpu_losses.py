@@ -724,3 +724,25 @@ def test_banned_tokens_at_temperatures_at_the_ends_of_the_range(temperature):
     # (of 50 equal terms the sum is exact; log and its rounding)
     assert float((lp.detach().double() - want).abs().max()) <= 2 * U * abs(want)
     assert bool((xr.grad[:, :, 40:290] == 0).all()) and bool(torch.isfinite(xr.grad).all())
+
+
+def test_no_second_derivative():
+    """A gradient taken with create_graph has the plain one's values, and whoever differentiates it is told that there is nothing, instead of losing a term."""
+    x, ids, mask, g = _case(2, 5, 300, torch.float32, 45)
+    old = rwkv_kernel.token_logprobs(x, ids)
+    A = torch.randn(2, generator=g).cuda()
+    w = torch.randn(2, 5, generator=g).cuda()
+    for call in (lambda v: (rwkv_kernel.token_logprobs(v, ids, mask) * w).sum(), lambda v: rwkv_kernel.cross_entropy(v, ids, mask),
+                 lambda v: rwkv_kernel.preference_loss(v, ids, mask, old.sum(1))[0], lambda v: rwkv_kernel.policy_loss(v, ids, mask, old, A, ref_logps=old + 0.1, kl_weight=0.1)[0]):
+        leaf = x.clone().requires_grad_(True)
+        logits = leaf * 1.0                                # (a leaf, and logits that something made)
+        plain, = torch.autograd.grad(call(logits), leaf, retain_graph=True)
+        for at in (leaf, logits):
+            loss = call(logits)
+            grad, = torch.autograd.grad(loss, at, create_graph=True)
+            assert torch.equal(grad.detach(), plain) and grad.requires_grad
+            with pytest.raises(RuntimeError, match="second derivative"):
+                (loss + grad.square().sum()).backward()
+        leaf.grad = None
+        call(leaf * 1.0).backward()
+        assert torch.equal(leaf.grad, plain)
