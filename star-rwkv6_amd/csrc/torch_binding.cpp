@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <initializer_list>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "wkv6.h"
@@ -560,7 +561,7 @@ Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &ex
   const c10::DeviceGuard guard(first.device());
   Tensors kept;
   std::vector<wkv6_adamw_tensor> rows;
-  std::vector<const void *> seen;
+  std::vector<std::pair<uintptr_t, uintptr_t>> seen;   // what is written, from and to
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
     for (const Tensor *t : {&p, &grads[i], &m, &v}) {
@@ -587,12 +588,15 @@ Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &ex
     kept.push_back(g);
     row.grad = in(g);
     rows.push_back(row);
-    for (const void *written : {static_cast<const void *>(row.param), static_cast<const void *>(row.exp_avg), static_cast<const void *>(row.exp_avg_sq),
-                                static_cast<const void *>(row.scales), static_cast<const void *>(row.master)})
-      if (written && p.numel() > 0) seen.push_back(written);
+    const int64_t n = p.numel(), moment_bytes = n * (eight ? 1 : 4);
+    for (const auto &[written, size] : {std::pair<void *, int64_t>{row.param, n * p.element_size()}, {row.exp_avg, moment_bytes}, {row.exp_avg_sq, moment_bytes},
+                                        {row.scales, (n + 255) / 256 * 8}, {row.master, n * 4}})
+      if (written && n > 0) seen.emplace_back(reinterpret_cast<uintptr_t>(written), reinterpret_cast<uintptr_t>(written) + size);
   }
+  // (in order of where they begin, one that reaches into another reaches into the next)
   std::sort(seen.begin(), seen.end());
-  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "wkv6: a parameter, a moment, its scales or a master is given twice");
+  for (size_t i = 1; i < seen.size(); ++i)
+    TORCH_CHECK(seen[i - 1].second <= seen[i].first, "wkv6: a parameter, a moment, its scales or a master is given twice, or shares elements with another");
   if (!norm.defined() && (max_grad_norm > 0. || skip_nonfinite)) norm = grad_norm(kept);
   check(wkv6_adamw_step(stream_of(first), code_of(type), eight ? 8 : 32, count, rows.data(), static_cast<int64_t *>(out(step)), in_f(lr_device), lr, beta1,
                         beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, in_f(norm), static_cast<uint32_t>(seed)));

@@ -135,7 +135,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
         g = g * max_grad_norm / max(norm, max_grad_norm)                 (max_grad_norm None: g as it is)
         m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  t = step = step + 1
         p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
-    params, grads: of one dtype (bf16, fp16, fp32), any dense layout, none twice.  step: one int64 on the device, that of no other call under way.  lr: a number, or one fp32 value on the
+    params, grads: of one dtype (bf16, fp16, fp32), any dense layout, none twice and no two with elements in common.  step: one int64 on the device, that of no other call under way.  lr: a number, or one fp32 value on the
     device (which a captured graph's replays read anew).  masters: fp32 weights that are updated in the params' place, the
     params their rounded copies.  grad_norm: the norm to clip by, one fp32 value on the device; None: that of these gradients.  skip_nonfinite: a
     step whose norm is not finite changes nothing.  Returns the norm, None if nothing asked for it.

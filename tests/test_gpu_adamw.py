@@ -513,3 +513,19 @@ def test_more_elements_than_32_bits_count(bits):
             assert int((got - want).abs().max()) <= 1
     if bits == 8:
         assert torch.equal(whole["scales"][0][-((tail + 255) // 256):], st["scales"][0])
+
+
+def test_tensors_that_overlap_are_refused():
+    """Two tensors of a call that share elements would be written by two workgroups at once; neighbours in one buffer are in order."""
+    for bits in (32, 8):
+        for name in ("params", "exp_avgs", "exp_avg_sqs", "masters"):
+            st = _setup([(600,), (600,)], torch.bfloat16, bits, True, 9)
+            room = torch.zeros(1200, device="cuda").to(st[name][0].dtype)
+            before = _clone(st)
+            with pytest.raises(RuntimeError, match="twice"):
+                _step(dict(st, **{name: [room[:600], room[300:900]]}))
+            with pytest.raises(RuntimeError, match="twice"):
+                _step(dict(st, **{name: [room[599:1199], room[:600]]}))
+            assert int(st["step"]) == 10 and all(torch.equal(a.float(), b.float()) for a, b in zip(before["params"], st["params"]))
+            _step(dict(st, **{name: [room[600:], room[:600]]}))
+            assert int(st["step"]) == 11
