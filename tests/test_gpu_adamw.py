@@ -529,3 +529,47 @@ def test_tensors_that_overlap_are_refused():
             assert int(st["step"]) == 10 and all(torch.equal(a.float(), b.float()) for a, b in zip(before["params"], st["params"]))
             _step(dict(st, **{name: [room[600:], room[:600]]}))
             assert int(st["step"]) == 11
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [59, 60, 61, 119, 120, 121])
+def test_as_many_tensors_as_launches_take(count, bits):
+    """On either side of 60 and 120 tensors: one launch, two, three."""
+    test_many_tensors(count, bits)
+
+
+@pytest.mark.parametrize("dtype,bits,master", [(torch.float32, 32, False), (torch.float32, 8, False), (torch.bfloat16, 32, False), (torch.bfloat16, 32, True), (torch.float16, 8, True),
+                                               (torch.bfloat16, 8, False)])
+def test_steps_past_the_caches(dtype, bits, master):
+    """Tensors of 160 MiB and more together are loaded and stored in another way: they become what they do in calls of their own, at the same place of a list."""
+    sizes = [9_000_001, 8_999_743, 9_500_123, 3_000_000, 4097]
+    es = torch.finfo(dtype).bits // 8
+    assert sum(sizes) * (2 * es + bits // 4 + (4 if master else 0)) >= 160 << 20 > max(sizes) * (2 * es + bits // 4 + (4 if master else 0))
+    gen = torch.Generator(device="cuda").manual_seed(47)
+    rand = lambda n, std: torch.randn(n, generator=gen, device="cuda") * std  # noqa: E731
+    st = dict(params=[], grads=[], exp_avgs=[], exp_avg_sqs=[], scales=[] if bits == 8 else None, masters=[] if master else None, step=torch.tensor(10, device="cuda"))
+    for n in sizes:
+        w = rand(n, 0.1)
+        st["params"].append(w.to(dtype))
+        if master:
+            st["masters"].append(w)
+        st["grads"].append(rand(n, 1e-2).to(dtype))
+        if bits == 8:
+            st["scales"].append(torch.rand((n + 255) // 256, 2, generator=gen, device="cuda") * 1e-4 + 1e-6)
+            st["exp_avgs"].append(rand(n, 100.0).clamp(-448, 448).to(F8))
+            st["exp_avg_sqs"].append(rand(n, 100.0).abs().clamp(0, 448).to(F8))
+        else:
+            st["exp_avgs"].append(rand(n, 1e-2))
+            st["exp_avg_sqs"].append(rand(n, 1e-2).square())
+    alone = _clone(st)
+    norm = rwkv_kernel.grad_norm(st["grads"])
+    _step(st, max_grad_norm=0.5, grad_norm=norm)
+    for j in range(len(sizes)):
+        # (empty tensors before it: the place in the list decides what 8-bit moments are rounded to)
+        one = {k: [t[:0].clone() for t in v[:j]] + v[j:j + 1] if isinstance(v, list) else v for k, v in alone.items()}
+        one["step"] = torch.tensor(10, device="cuda")
+        _step(one, max_grad_norm=0.5, grad_norm=norm)
+        for k in ("params", "exp_avgs", "exp_avg_sqs", "scales", "masters"):
+            if st[k]:
+                assert torch.equal(st[k][j].float(), alone[k][j].float()), (j, k)
+        assert not torch.equal(st["exp_avgs"][j].float(), torch.zeros_like(st["exp_avgs"][j]).float())

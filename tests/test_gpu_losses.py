@@ -746,3 +746,87 @@ def test_no_second_derivative():
         leaf.grad = None
         call(leaf * 1.0).backward()
         assert torch.equal(leaf.grad, plain)
+
+
+@pytest.mark.parametrize("rows,V,dtype", [(4500, 4100, torch.bfloat16), (4500, 4100, torch.float32), (2500, 20000, torch.bfloat16), (2500, 20000, torch.float32),
+                                          (17000, 250, torch.bfloat16), (17000, 1000, torch.float32)])
+def test_many_rows_under_a_loss_that_is_scaled(rows, V, dtype):
+    """What the forward wrote for an arriving gradient of 1 is written anew for another one, in every row: more of them than the workgroups that look at what arrived (2048,
+    of one row, of a piece of one, or of four short ones) take at once.  0.5 and 2 are powers of two: exact."""
+    x, ids, mask, g = _case(4, rows // 4, V, dtype, rows + V, std=1.0)
+    old = rwkv_kernel.token_logprobs(x, ids) - 0.05
+    A = torch.randn(4, generator=g).cuda()
+    for call in (lambda v: rwkv_kernel.cross_entropy(v, ids, mask, reduction="sum"), lambda v: rwkv_kernel.policy_loss(v, ids, mask, old, A, ref_logps=old, kl_weight=0.1)[0]):
+        grads = []
+        for up in (1.0, 0.5, 2.0):
+            v = x.clone().requires_grad_(True)
+            grads.append(torch.autograd.grad(call(v), v, torch.tensor(up).cuda())[0])
+        assert torch.equal(grads[1] * 2, grads[0]) and torch.equal(grads[2], grads[0] * 2)
+        assert bool((grads[0][mask].abs().amax(-1) > 0).all()) and bool((grads[0][~mask] == 0).all())
+
+
+@pytest.mark.parametrize("T,V,dtype", [(1400, 65536, torch.bfloat16), (1300, 70001, torch.float16), (700, 65537, torch.float32), (90000, 1003, torch.bfloat16)])
+def test_gradients_past_the_caches(T, V, dtype):
+    """A gradient of 160 MiB and more is stored in another way; its rows are those of calls on parts that stay below."""
+    assert T * V * torch.finfo(dtype).bits // 8 >= 160 << 20
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.empty(1, T, V, dtype=dtype, device="cuda").normal_(0.0, 2.0, generator=gen)
+    ids = torch.randint(0, V, (1, T), generator=gen, device="cuda")
+    mask = torch.rand(1, T, generator=gen, device="cuda") < 0.8
+    w = torch.randn(1, T, generator=gen, device="cuda")
+
+    def logprobs(a, b):
+        v = x[:, a:b].detach().requires_grad_(True)
+        lp = rwkv_kernel.token_logprobs(v, ids[:, a:b], mask[:, a:b], temperature=0.9)
+        return lp.detach(), torch.autograd.grad(lp, v, w[:, a:b])[0]
+
+    def loss(a, b):   # (a forward that writes the gradient too, or leaves it to the backward: fp16)
+        v = x[:, a:b].detach().requires_grad_(True)
+        return torch.autograd.grad(rwkv_kernel.cross_entropy(v, ids[:, a:b], mask[:, a:b], reduction="sum"), v)
+
+    for call in (logprobs, loss):
+        whole, step = call(0, T), (T + 2) // 3
+        for a in range(0, T, step):
+            b = min(T, a + step)
+            for got, part in zip(whole, call(a, b)):
+                assert torch.equal(got[:, a:b], part), (a, b)
+
+
+def test_preference_gradients_past_the_caches():
+    """Two texts of 96 MiB each: the gradient's rows are those that their halves have, of a loss whose slope is the same (the sigmoid's at d = 0, as both texts are one)."""
+    T, V = 768, 65536
+    gen = torch.Generator(device="cuda").manual_seed(46)
+    text = torch.empty(1, T, V, dtype=torch.bfloat16, device="cuda").normal_(0.0, 2.0, generator=gen)
+    ids = torch.randint(0, V, (1, T), generator=gen, device="cuda")
+
+    def grad(a, b):
+        v = text[:, a:b].repeat(2, 1, 1).requires_grad_(True)
+        loss, _ = rwkv_kernel.preference_loss(v, ids[:, a:b].repeat(2, 1), beta=0.25)
+        return torch.autograd.grad(loss, v)[0]
+
+    whole = grad(0, T)
+    assert whole.numel() * 2 >= 160 << 20
+    for a in range(0, T, T // 2):
+        assert torch.equal(whole[:, a:a + T // 2], grad(a, a + T // 2))
+    assert torch.equal(whole[0], -whole[1]) and bool((whole[0].abs().amax(-1) > 0).all())
+
+
+def test_other_ways_to_run_them():
+    """Inference mode, recomputation, and saved tensors kept on the host: as a plain call."""
+    from torch.utils.checkpoint import checkpoint
+    whole = torch.randn(4, 9, 400, generator=torch.Generator().manual_seed(49)).cuda()
+    _, ids, mask, g = _case(4, 6, 390, torch.float32, 49)
+    view = whole[:, 2:8, 3:393]                            # (rows apart: what comes back from the host may lie otherwise)
+    old, A = rwkv_kernel.token_logprobs(view, ids) - 0.05, torch.randn(4, generator=g).cuda()
+    for call in (lambda v: rwkv_kernel.cross_entropy(v, ids, mask), lambda v: rwkv_kernel.token_logprobs(v, ids, mask).sum(),
+                 lambda v: rwkv_kernel.preference_loss(v, ids, mask, old.sum(1))[0], lambda v: rwkv_kernel.policy_loss(v, ids, mask, old, A, ref_logps=old, kl_weight=0.1)[0]):
+        leaf = view.detach().requires_grad_(True)
+        want = call(leaf)
+        want_grad, = torch.autograd.grad(want, leaf)
+        with torch.inference_mode():
+            assert torch.equal(call(view), want) and torch.equal(call(whole.clone()[:, 2:8, 3:393]), want)   # (rows that begin where they did: the sums' order goes by that)
+        with torch.autograd.graph.save_on_cpu():
+            loss = call(leaf)
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want_grad)
+        loss = checkpoint(call, leaf, use_reentrant=False)
+        assert torch.equal(loss, want) and torch.equal(torch.autograd.grad(loss, leaf)[0], want_grad)
