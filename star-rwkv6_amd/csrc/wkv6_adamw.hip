@@ -13,8 +13,8 @@
 //
 // Bound by memory: 28 bytes a parameter with everything in fp32, 10 with bf16 parameters and 8-bit moments (whose some 60 vector operations a parameter
 // take two thirds of the time), and the gradient once more for the norm.  490 M parameters in 150 tensors: step 2.43 ms and norm 0.32 ms in fp32
-// (5.6 and 6.1 TB/s; elements of a wave's load without gaps, past the caches 10 % faster than through them), 0.98 and 0.18 ms in bf16 with 8 bits.
-// Some 1 M parameters in 26 tensors: one launch of 9.5 us.
+// (5.6 and 6.1 TB/s; elements of a wave's load without gaps, past the caches 10 % faster than through them), 0.98 and 0.18 ms in bf16 with 8 bits; steps of
+// bf16 parameters with masters 2.2 ms (6.3 TB/s) and with 8 bits 1.4 (5.5).  Some 1 M parameters in 36 tensors: one launch of 9.5 us.
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
@@ -29,7 +29,10 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kGroup = 60;          // tensors of one launch: they travel in its arguments, which hold 4 KB
 constexpr int kChunk = 4096;        // elements that a workgroup takes at a time, 16 to a thread in pieces that lie next to each other
 constexpr int kScaleBlock = 256;    // elements that share a scale
-constexpr int kBlocks = 2048;       // workgroups of a launch at most: eight to a compute unit, which go from chunk to chunk
+// Workgroups of a launch at most, which go from chunk to chunk.  Of step_kernel four or five stand on a compute unit at a time (84 to 115 registers), of norm_kernel eight:
+// of 2048 some stand at once and the others follow, and launches of no more than stand at once are no faster.  490 M parameters, fp32 / bf16 with 8 bits, clipped, in us: 1024
+// 2824 / 1182, 1280 2762 / 1167, 2048 2760 / 1142, 4096 2748 / 1138, 8192 2738 / 1291.
+constexpr int kBlocks = 2048;
 constexpr int kFinish = 1024;       // threads of the one workgroup that adds up
 constexpr int64_t kPastBytes = 160 << 20;   // of all tensors of a call
 

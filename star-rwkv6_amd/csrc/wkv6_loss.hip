@@ -17,7 +17,7 @@
 // writes its gradient from there: two passes over the logits instead of three (8192 rows of 65536 bf16: 390 us, 5.5 TB/s, where copying as
 // much takes 432).  The preference loss's c needs both whole texts, so its gradient reads the logits again (16 x 1024 rows: 955 us, 5.6 TB/s of three
 // passes; grouping the pairs so that the second reading might find them in the last-level cache, with the next pairs' rows in the same launch or
-// in one of their own, took as long).  Sums alone reach 6.2 to 7 TB/s (8192 rows of 512-token texts: 126 us).
+// in one of their own, took as long).  Sums alone reach 6.2 to 7 TB/s (8192 rows of 65536 bf16, three quarters of which count: 134 us).
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 
@@ -30,7 +30,10 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kFinish = 1024;        // threads of the one workgroup that adds up
 constexpr int kCountBlocks = 256;    // at most
 constexpr int kStretches = 256;      // of a great many rows
-constexpr int kFewRows = 1024;       // whose tokens every row's threads count for themselves: a launch less (2 us of the card's time and of the host's)
+// Of up to so many rows every row's threads count the tokens for themselves, a launch less; beyond, each row's reading of all ids takes longer than the launch.  All
+// kernels of a cross entropy over V 1000, in us, counted by the rows / ahead: 64 rows 10.2 / 14.2, 512 12.2 / 14.2, 1024 14.6 / 14.4 (and the host's 2 us for a launch), 2048
+// 19.5 / 15.6, 8192 71 / 23.
+constexpr int kFewRows = 1024;
 constexpr int64_t kMostBlocks = 1 << 21;   // of a launch: it counts its threads in 32 bits
 constexpr int kGradVecs = 8;         // vectors of a thread in the gradient's own pass
 // A gradient of this size and more is written past the caches.  Cross entropy, log probabilities with their backward, and the latter with a reader
@@ -253,6 +256,7 @@ template <int kT> __device__ __forceinline__ float weight_of_few(const LossRows 
 __device__ __forceinline__ float row_terms(const LossRows &a, const LossTerms &l, int64_t row, double exact, float w) {
 #pragma clang fp contract(off)   // (left to itself the compiler joins other products and sums in the kernel with the gradient than in the one without)
     const int64_t rows = a.B * a.T;
+    // (as this call returns it, in fp32 like the other models': a model beside its own log probabilities has ratios of 1 and a KL term of 0 to the last bit)
     const float lp = (float)exact;
     if (l.kind == kLossCrossEntropy) {
         l.terms[row] = -lp * w;

@@ -15,7 +15,8 @@ negative; the logits of one that does not are never read, and get a gradient of 
 probability, and with it the loss, NaN.  A temperature is the fp32 number nearest to what is given; logits are divided by it in 64 bits.
 
 Calls go to the current stream of the tensors' device, allocate nothing but their results and workspaces, never
-synchronise, and can be captured into a graph.
+synchronise, and can be captured into a graph (a backward only where no graph of its leaves is alive that another stream made: torch's engine
+would make that stream wait for the capture, and the process ends).
 
 The losses have first derivatives.  A gradient taken with create_graph has its value, and a derivative of it is refused.
 """

@@ -830,3 +830,16 @@ def test_other_ways_to_run_them():
         assert torch.equal(torch.autograd.grad(loss, leaf)[0], want_grad)
         loss = checkpoint(call, leaf, use_reentrant=False)
         assert torch.equal(loss, want) and torch.equal(torch.autograd.grad(loss, leaf)[0], want_grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_policy_beside_its_own_log_probabilities(dtype):
+    """The ratio is 1 and the KL term 0 to the last bit, so that the loss and its gradient are those without either."""
+    x, ids, mask, g = _case(3, 7, 1200, dtype, 50)
+    A = torch.randn(3, generator=g).cuda()
+    xr, same = (x.clone().requires_grad_(True) for _ in range(2))
+    plain, lp, _ = rwkv_kernel.policy_loss(xr, ids, mask, None, A, temperature=0.9)
+    loss, _, means = rwkv_kernel.policy_loss(same, ids, mask, lp, A, ref_logps=lp, kl_weight=0.5, clip_low=0.0, clip_high=0.0, temperature=0.9)
+    plain.backward()
+    loss.backward()
+    assert torch.equal(loss, plain) and means.tolist() == [0.0, 0.0] and torch.equal(same.grad, xr.grad)
