@@ -217,7 +217,7 @@ def train_step(model, optimizer, ids, autocast_dtype=None):
     logits, target = _logits(model, ids, autocast_dtype), ids[:, 1:]
     kernels = _kernels(logits)
     if kernels is not None:
-        if logits.shape[:-1] != target.shape:
+        if logits.dim() != 3 or logits.shape[:-1] != target.shape:
             logits, target = logits.reshape(-1, logits.shape[-1]), target.reshape(-1)
         return _update(optimizer, kernels.cross_entropy(logits, target.long()))
     return _update(optimizer, F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), target.reshape(-1)))

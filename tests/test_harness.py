@@ -354,3 +354,16 @@ def test_fine_tuning_steps_say_what_they_need(monkeypatch):
                      lambda: hz.policy_step(model, opt, ids, mask, torch.zeros(2, 8), torch.zeros(2))):
             with pytest.raises(AssertionError, match="on the GPU"):
                 step()
+
+
+@pytest.mark.gpu
+def test_train_step_takes_several_tokens_at_a_place():
+    """Texts of K tokens at each place and logits for each of them: the loss is the mean over all."""
+    torch.manual_seed(11)
+    model = torch.nn.Embedding(31, 31).cuda()
+    ids = torch.randint(0, 31, (3, 9, 4), device="cuda")
+    with torch.no_grad():
+        want = F.cross_entropy(model(ids[:, :-1]).reshape(-1, 31), ids[:, 1:].reshape(-1))
+    loss = hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), ids)
+    # (losses of about 4, each off by some 2^-22 of itself)
+    assert abs(float(loss) - float(want)) <= 2.0 ** -20 * float(want) and bool(torch.isfinite(model.weight).all())
