@@ -448,6 +448,35 @@ int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, con
                     int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
                     double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed);
 
+/* ---- Before and between the layers' own operators -----------------------------------------
+ * No counterpart in the reference, whose model takes both from the framework (rwkv6_model.py:187-208, :259-274). */
+
+/* Layer norm with the residual addition before it.  rows of C channels (at most 32768); x and add of any row stride, everything else
+ * contiguous, addresses aligned to their elements (stats to 8 bytes, workspace to 16).  Where add is given, total = x + add, rounded to
+ * `dtype`, is written and normalised; otherwise x is, and total is NULL.  y = (s - mean) / sqrt(variance + eps) * weight + bias, weight
+ * and bias (C) of param_dtype or NULL.  x, total and their gradients are of `dtype`; add, y and their gradients of branch_dtype: the same,
+ * or BF16 or F16 beside F32.  stats (rows, 2) for the backward, or NULL. */
+int wkv6_layer_norm(void *stream, int dtype, int branch_dtype, int param_dtype, int64_t rows, int64_t C, const void *x, int64_t x_stride,
+                    const void *add, int64_t add_stride, const void *weight, const void *bias, float eps, void *total, void *y, float *stats);
+
+/* gx = dL/d(x + add) from gy and gtotal (what else arrives at the sum, or NULL), gadd the same rounded to branch_dtype; gweight, gbias
+ * (C) of param_dtype.  Any of the four may be NULL; the workspace is for the last two. */
+size_t wkv6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t C);
+int wkv6_layer_norm_backward(void *stream, int dtype, int branch_dtype, int param_dtype, int64_t rows, int64_t C, const void *total, int64_t total_stride,
+                             const float *stats, const void *weight, const void *gy, const void *gtotal, void *gx, void *gadd, void *gweight, void *gbias,
+                             void *workspace, size_t workspace_bytes);
+
+/* out[i] = scale * weight[ids[i]] for N tokens: rows of C values of a table (V, C) of `dtype` with this row stride; out (N, C) of
+ * out_dtype: the same, or BF16 or F16 beside F32.  A negative id gives zeros, an id of V or more NaN.  Addresses need their element's
+ * alignment, the workspace 16 bytes. */
+int wkv6_embedding(void *stream, int dtype, int out_dtype, int64_t N, int64_t V, int64_t C, const int64_t *ids, const void *weight, int64_t stride, float scale, void *out);
+
+/* gweight (V, C), all of it: scale times the sums of gout's rows by token, added up in the order of their places; rows of tokens that do not
+ * occur, or are padding_id (-1: none), are zero.  Ids outside of the table take no part. */
+size_t wkv6_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t C);
+int wkv6_embedding_backward(void *stream, int dtype, int gout_dtype, int64_t N, int64_t V, int64_t C, const int64_t *ids, const void *gout, float scale,
+                            int64_t padding_id, void *gweight, void *workspace, size_t workspace_bytes);
+
 /* ---- XLA custom-call surface (replaces the pybind module `gpu_ops`,
  * rwkv_kernel/jax_kernel/gpu_ops.cpp:20-43) ---------------------------------------------- */
 

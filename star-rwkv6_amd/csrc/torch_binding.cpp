@@ -48,6 +48,8 @@ int code_of(ScalarType t) {
   }
 }
 
+ScalarType type_of(int code) { return code == WKV6_F32 ? at::kFloat : code == WKV6_F16 ? at::kHalf : at::kBFloat16; }
+
 // rwkv_kernel/torch_rwkv_kernel.py:35 of the reference: float16 inputs produce float32 outputs
 ScalarType out_type(ScalarType t) { return t == at::kHalf ? at::kFloat : t; }
 
@@ -390,6 +392,14 @@ struct FirstOrder : torch::autograd::Function<FirstOrder> {
   }
 };
 
+// The same for the layer norm's and the embedding's gradients.
+struct FirstOrderOfLayer : torch::autograd::Function<FirstOrderOfLayer> {
+  static Tensor forward(AutogradContext *, const Tensor &grad, const Tensor &, const Tensor &) { return grad; }
+  static variable_list backward(AutogradContext *, variable_list) {
+    TORCH_CHECK(false, "wkv6: layer_norm and embedding have no second derivative");
+  }
+};
+
 Tensor first_order(bool graph_wanted, const Tensor &grad, const Tensor &logits, const Tensor &arrived) {
   if (!graph_wanted) return grad;
   const at::AutoGradMode on(true);
@@ -501,6 +511,125 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const c10::DeviceGuard guard(s[0].device());
     res[0] = first_order(graph_wanted, logits_backward(s, 1.0, s[4], 1, 0, arriving(grads[0]), Tensor()), s[0], grads[0]);
     return res;
+  }
+};
+
+// ---- layer norm, embedding ----
+
+// Rows of C values, as (rows, stride) if a single stride leads from row to row and a row's values lie next to each other.
+std::optional<int64_t> row_stride(const Tensor &t) {
+  const int64_t d = t.dim(), C = t.size(d - 1);
+  if (C > 1 && t.stride(d - 1) != 1) return std::nullopt;
+  int64_t stride = C, rows = 1;   // (one row: any)
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (rows == 1) stride = t.stride(i);
+    else if (t.stride(i) != stride * rows) return std::nullopt;
+    rows *= t.size(i);
+  }
+  return stride;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x_, const std::optional<Tensor> &add_, const std::optional<Tensor> &weight_,
+                               const std::optional<Tensor> &bias_, double eps, ScalarType branch, bool wanted) {
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = row_stride(x_) ? x_ : x_.contiguous();
+    Tensor add = given(add_), weight = given(weight_), bias = given(bias_);
+    if (add.defined() && !row_stride(add)) add = add.contiguous();
+    const ScalarType params = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : at::kFloat;
+    if (weight.defined()) weight = weight.contiguous();
+    if (bias.defined()) bias = bias.contiguous();
+    const int64_t C = x.size(-1), rows = x.numel() / C;
+    const Tensor y = at::empty(x.sizes(), x.options().dtype(branch)), total = add.defined() ? at::empty(x.sizes(), x.options()) : Tensor();
+    const Tensor stats = wanted ? fp32(x, {rows, 2}) : Tensor();
+    check(wkv6_layer_norm(stream_of(x), code_of(x.scalar_type()), code_of(branch), code_of(params), rows, C, in(x), *row_stride(x), in(add),
+                          add.defined() ? *row_stride(add) : 0, in(weight), in(bias), static_cast<float>(eps), out(total), out(y), out_f(stats)));
+    ctx->saved_data["branch"] = static_cast<int64_t>(branch);
+    ctx->saved_data["params"] = static_cast<int64_t>(params);
+    ctx->saved_data["shapes"] = std::vector<bool>{add.defined(), weight.defined(), bias.defined()};
+    ctx->set_materialize_grads(false);
+    if (wanted) ctx->save_for_backward({add.defined() ? total : x, stats, weight});
+    return add.defined() ? variable_list{y, total} : variable_list{y};
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
+    const auto s = ctx->get_saved_variables();
+    const Tensor &total = s[0], &stats = s[1], &weight = s[2];
+    const c10::DeviceGuard guard(total.device());
+    const ScalarType branch = static_cast<ScalarType>(ctx->saved_data["branch"].toInt()), params = static_cast<ScalarType>(ctx->saved_data["params"].toInt());
+    const auto there = ctx->saved_data["shapes"].toBoolList();
+    const bool added = there[0];
+    variable_list res(7);
+    const bool wants_x = ctx->needs_input_grad(0), wants_add = added && ctx->needs_input_grad(1),
+               wants_weight = there[1] && ctx->needs_input_grad(added ? 2 : 1), wants_bias = there[2] && ctx->needs_input_grad((added ? 2 : 1) + there[1]);
+    const int64_t C = total.size(-1), rows = total.numel() / C;
+    const Tensor gtotal = added && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    if (!grads[0].defined()) {   // (nothing goes through the norm)
+      if (!gtotal.defined()) return res;
+      if (wants_x) res[0] = gtotal;
+      if (wants_add) res[1] = gtotal.to(branch);
+    } else {
+      const Tensor gy = grads[0].contiguous();
+      const ScalarType stream = total.scalar_type();
+      const bool one = stream == branch;   // one gradient is both inputs'
+      const Tensor gx = wants_x || (wants_add && one) ? at::empty(total.sizes(), total.options()) : Tensor();
+      const Tensor gadd = wants_add && !one ? at::empty(total.sizes(), total.options().dtype(branch)) : Tensor();
+      const Tensor gw = wants_weight ? parameter_gradient(total, {C}, params) : Tensor(), gb = wants_bias ? parameter_gradient(total, {C}, params) : Tensor();
+      const size_t n = wants_weight || wants_bias ? wkv6_layer_norm_backward_workspace_bytes(rows, C) : 0;
+      const Tensor ws = bytes(total, n);
+      check(wkv6_layer_norm_backward(stream_of(total), code_of(stream), code_of(branch), code_of(params), rows, C, in(total), *row_stride(total), in_f(stats),
+                                     in(weight), in(gy), in(gtotal), out(gx), out(gadd), out(gw), out(gb), out(ws), n));
+      if (wants_x) res[0] = gx;
+      if (wants_add) res[1] = one ? gx : gadd;
+      res[2] = gw;
+      res[3] = gb;
+    }
+    if (graph_wanted) {
+      const at::AutoGradMode on(true);
+      for (Tensor &t : res)
+        if (t.defined()) t = FirstOrderOfLayer::apply(t, total, grads[0].defined() ? grads[0] : grads[1]);
+    }
+    return res;
+  }
+};
+
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &ids, const Tensor &weight_, double scale, int64_t padding_id, ScalarType type) {
+    const c10::DeviceGuard guard(weight_.device());
+    const Tensor weight = weight_.size(1) > 1 && weight_.stride(1) != 1 ? weight_.contiguous() : weight_;
+    const int64_t V = weight.size(0), C = weight.size(1);
+    at::DimVector shape(ids.sizes().begin(), ids.sizes().end());
+    shape.push_back(C);
+    const Tensor res = at::empty(shape, weight.options().dtype(type));
+    check(wkv6_embedding(stream_of(weight), code_of(weight.scalar_type()), code_of(type), ids.numel(), V, C, static_cast<const int64_t *>(in(ids)), in(weight),
+                         weight.stride(0), static_cast<float>(scale), out(res)));
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_id"] = padding_id;
+    ctx->saved_data["type"] = static_cast<int64_t>(weight.scalar_type());
+    ctx->saved_data["V"] = V;
+    ctx->save_for_backward({ids});
+    return res;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const bool graph_wanted = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
+    const Tensor ids = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+    const c10::DeviceGuard guard(g.device());
+    const int64_t N = ids.numel(), V = ctx->saved_data["V"].toInt(), C = g.size(-1);
+    const ScalarType type = static_cast<ScalarType>(ctx->saved_data["type"].toInt());
+    Tensor gweight = parameter_gradient(g, {V, C}, type);
+    const size_t n = wkv6_embedding_backward_workspace_bytes(N, V, C);
+    const Tensor ws = bytes(g, n);
+    check(wkv6_embedding_backward(stream_of(g), code_of(type), code_of(g.scalar_type()), N, V, C, static_cast<const int64_t *>(in(ids)), in(g),
+                                  static_cast<float>(ctx->saved_data["scale"].toDouble()), ctx->saved_data["padding_id"].toInt(), out(gweight), out(ws), n));
+    if (graph_wanted) {
+      const at::AutoGradMode on(true);
+      gweight = FirstOrderOfLayer::apply(gweight, grads[0], grads[0]);
+    }
+    return {Tensor(), gweight, Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -762,7 +891,7 @@ PYBIND11_MODULE(_wkv6_torch, m) {
   m.def("forward_with_state", [](int64_t H, const std::optional<Tensor> &map, const Tensor &r, const Tensor &k, const Tensor &v,
                                  const Tensor &w, const Tensor &u, const std::optional<Tensor> &s0, int64_t algo, int state_code,
                                  bool backward_follows) {
-    const ScalarType st = state_code == WKV6_F32 ? at::kFloat : state_code == WKV6_F16 ? at::kHalf : at::kBFloat16;
+    const ScalarType st = type_of(state_code);
     return wrap(unlocked([&] { return forward_with_state(H, given(map), r, k, v, w, u, given(s0), algo, st, backward_follows); }));
   }, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg("backward_follows") = false);
   // Logits, ids and a mask (or None) as the kernels take them, with nothing left for the Python layer to check or to change.
@@ -800,6 +929,15 @@ PYBIND11_MODULE(_wkv6_torch, m) {
       return PreferenceLoss::apply(x, ids, mask, apart(ref_logps), kind, beta, label_smoothing, average, wanted);
     });
     return py::make_tuple(wrap(o[0]), wrap(o[1]));
+  });
+  m.def("layer_norm", [](const Tensor &x, const std::optional<Tensor> &add, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps,
+                         int branch_code) {
+    const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || (add && add->requires_grad()) || (weight && weight->requires_grad()) || (bias && bias->requires_grad()));
+    const variable_list o = unlocked([&] { return LayerNorm::apply(x, add, weight, bias, eps, type_of(branch_code), wanted); });
+    return py::make_tuple(wrap(o[0]), o.size() > 1 ? wrap(o[1]) : py::none());
+  });
+  m.def("embedding", [](const Tensor &ids, const Tensor &weight, double scale, int64_t padding_id, int out_code) {
+    return unlocked([&] { return Embedding::apply(ids, weight, scale, padding_id, type_of(out_code)); });
   });
   m.def("grad_norm", [](const Tensors &grads) { return unlocked([&] { return grad_norm(grads); }); });
   m.def("adamw_step", [](const Tensors &params, const Tensors &grads, const Tensors &exp_avgs, const Tensors &exp_avg_sqs, const Tensor &step,

@@ -458,6 +458,79 @@ int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, con
                                    wkv6::AdamwStep{step, lr_device, lr, beta1, beta2, eps, weight_decay, max_grad_norm, skip_nonfinite, grad_norm, seed, 0., 0.}));
 }
 
+// ---- layer norm, embedding ----
+
+static bool is_type(int dtype) { return dtype == WKV6_BF16 || dtype == WKV6_F16 || dtype == WKV6_F32; }
+// a stream or a table, and what goes with it: the same type, or 16 bits beside 32
+static bool goes_with(int dtype, int other) { return is_type(dtype) && is_type(other) && (dtype == other || dtype == WKV6_F32); }
+
+static int check_norm(int dtype, int branch_dtype, int param_dtype, int64_t rows, int64_t C) {
+    if (!goes_with(dtype, branch_dtype) || !is_type(param_dtype) || rows <= 0 || C <= 0) return WKV6_ERR_ARG;
+    if (C > wkv6::kNormMostChannels || rows > 0x7fffffffffffLL / C) return WKV6_ERR_UNSUPPORTED;
+    return WKV6_OK;
+}
+
+int wkv6_layer_norm(void *stream, int dtype, int branch_dtype, int param_dtype, int64_t rows, int64_t C, const void *x, int64_t x_stride,
+                    const void *add, int64_t add_stride, const void *weight, const void *bias, float eps, void *total, void *y, float *stats) {
+    const int rc = check_norm(dtype, branch_dtype, param_dtype, rows, C);
+    if (rc != WKV6_OK) return rc;
+    if (!x || !y || (add != nullptr) != (total != nullptr) || x_stride < 0 || add_stride < 0 || !(eps >= 0.f)) return WKV6_ERR_ARG;
+    if (!aligned(x, element_size(dtype)) || !aligned(total, element_size(dtype)) || !aligned(add, element_size(branch_dtype)) ||
+        !aligned(y, element_size(branch_dtype)) || !aligned(weight, element_size(param_dtype)) || !aligned(bias, element_size(param_dtype)) || !aligned(stats, 8))
+        return WKV6_ERR_ARG;
+    return finish(wkv6::layer_norm((hipStream_t)stream, dtype, branch_dtype,
+                                   wkv6::NormArgs{rows, C, x_stride, add_stride, x, add, weight, bias, param_dtype, eps, total, y, stats}));
+}
+
+size_t wkv6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t C) {
+    return rows > 0 && C > 0 && C <= wkv6::kNormMostChannels ? wkv6::layer_norm_backward_workspace_bytes(rows, C) : 0;
+}
+
+int wkv6_layer_norm_backward(void *stream, int dtype, int branch_dtype, int param_dtype, int64_t rows, int64_t C, const void *total, int64_t total_stride,
+                             const float *stats, const void *weight, const void *gy, const void *gtotal, void *gx, void *gadd, void *gweight, void *gbias,
+                             void *workspace, size_t workspace_bytes) {
+    const int rc = check_norm(dtype, branch_dtype, param_dtype, rows, C);
+    if (rc != WKV6_OK) return rc;
+    if (!total || !stats || !gy || total_stride < 0) return WKV6_ERR_ARG;
+    for (const void *p : {total, gtotal, static_cast<const void *>(gx)})
+        if (!aligned(p, element_size(dtype))) return WKV6_ERR_ARG;
+    for (const void *p : {gy, static_cast<const void *>(gadd)})
+        if (!aligned(p, element_size(branch_dtype))) return WKV6_ERR_ARG;
+    for (const void *p : {weight, static_cast<const void *>(gweight), static_cast<const void *>(gbias)})
+        if (!aligned(p, element_size(param_dtype))) return WKV6_ERR_ARG;
+    if (!aligned(stats, 8)) return WKV6_ERR_ARG;
+    if ((gweight || gbias) && (!workspace || !aligned16(workspace) || workspace_bytes < wkv6::layer_norm_backward_workspace_bytes(rows, C))) return WKV6_ERR_WORKSPACE;
+    return finish(wkv6::layer_norm_backward((hipStream_t)stream, dtype, branch_dtype,
+                                            wkv6::NormGrad{rows, C, total_stride, total, stats, weight, param_dtype, gy, gtotal, gx, gadd, gweight, gbias}, workspace));
+}
+
+static int check_embedding(int dtype, int out_dtype, int64_t N, int64_t V, int64_t C, const int64_t *ids, const void *rows, const void *table) {
+    if (!goes_with(dtype, out_dtype) || N <= 0 || V <= 0 || C <= 0 || !ids || !rows || !table) return WKV6_ERR_ARG;
+    if (!aligned(ids, 8) || !aligned(table, element_size(dtype)) || !aligned(rows, element_size(out_dtype))) return WKV6_ERR_ARG;
+    // (places and tokens are sorted as 32-bit numbers; no offset of an element passes 2^46)
+    if (N > 0x7fffffffLL || V > 0x7fffffffLL || C > (1 << 24) || N > (1LL << 46) / C || V > (1LL << 46) / C) return WKV6_ERR_UNSUPPORTED;
+    return WKV6_OK;
+}
+
+int wkv6_embedding(void *stream, int dtype, int out_dtype, int64_t N, int64_t V, int64_t C, const int64_t *ids, const void *weight, int64_t stride, float scale, void *out) {
+    const int rc = check_embedding(dtype, out_dtype, N, V, C, ids, out, weight);
+    if (rc != WKV6_OK) return rc;
+    if (stride < 0) return WKV6_ERR_ARG;
+    return finish(wkv6::embedding((hipStream_t)stream, dtype, out_dtype, wkv6::EmbeddingArgs{N, V, C, stride, ids, weight, scale, out}));
+}
+
+size_t wkv6_embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t C) {
+    return N > 0 && N <= 0x7fffffffLL && V > 0 && V <= 0x7fffffffLL && C > 0 && C <= (1 << 24) ? wkv6::embedding_backward_workspace_bytes(N, V, C) : 0;
+}
+
+int wkv6_embedding_backward(void *stream, int dtype, int gout_dtype, int64_t N, int64_t V, int64_t C, const int64_t *ids, const void *gout, float scale,
+                            int64_t padding_id, void *gweight, void *workspace, size_t workspace_bytes) {
+    const int rc = check_embedding(dtype, gout_dtype, N, V, C, ids, gout, gweight);
+    if (rc != WKV6_OK) return rc;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < wkv6::embedding_backward_workspace_bytes(N, V, C)) return WKV6_ERR_WORKSPACE;
+    return finish(wkv6::embedding_backward((hipStream_t)stream, dtype, gout_dtype, wkv6::EmbeddingGrad{N, V, C, padding_id, ids, gout, scale, gweight}, workspace));
+}
+
 static int check_mix(int dtype, int64_t B, int64_t T, int64_t C, int64_t R) {
     if (B <= 0 || T <= 0 || C <= 0 || R <= 0) return WKV6_ERR_ARG;
     if (dtype != WKV6_BF16 || !wkv6::shift_mix_supported(C, R)) return WKV6_ERR_UNSUPPORTED;

@@ -406,4 +406,47 @@ size_t grad_norm_workspace_bytes(int64_t count);
 hipError_t grad_norm(hipStream_t st, int dtype, int64_t count, const AdamwTensor *tensors, float *norm, void *workspace);
 hipError_t adamw_step(hipStream_t st, int dtype, int moment_bits, int64_t count, const AdamwTensor *tensors, const AdamwStep &s);
 
+// --- layer norm with a residual addition (wkv6_norm.hip) ---
+constexpr int64_t kNormMostChannels = 32768;
+struct NormArgs {
+    int64_t rows, C, x_stride, add_stride;   // strides in elements
+    const void *x, *add;                     // add may be null
+    const void *weight, *bias;               // (C), of param_type, either may be null
+    int param_type;
+    float eps;
+    void *total, *y;                         // total where add is given
+    float *stats;                            // (rows, 2) mean and 1 / deviation, or null
+};
+struct NormGrad {
+    int64_t rows, C, total_stride;
+    const void *total;                       // x where nothing was added
+    const float *stats;
+    const void *weight;
+    int param_type;
+    const void *gy, *gtotal;                 // gtotal may be null
+    void *gx, *gadd, *gweight, *gbias;       // any may be null
+};
+hipError_t layer_norm(hipStream_t st, int dtype, int branch_dtype, const NormArgs &a);
+size_t layer_norm_backward_workspace_bytes(int64_t rows, int64_t C);
+hipError_t layer_norm_backward(hipStream_t st, int dtype, int branch_dtype, const NormGrad &a, void *workspace);
+
+// --- embedding (wkv6_embed.hip) ---
+struct EmbeddingArgs {
+    int64_t N, V, C, stride;   // stride: of the table's rows, in elements
+    const int64_t *ids;
+    const void *weight;
+    float scale;
+    void *out;                 // (N, C)
+};
+struct EmbeddingGrad {
+    int64_t N, V, C, padding_id;   // padding_id -1: none
+    const int64_t *ids;
+    const void *gout;              // (N, C)
+    float scale;
+    void *gweight;                 // (V, C)
+};
+hipError_t embedding(hipStream_t st, int dtype, int out_dtype, const EmbeddingArgs &a);
+size_t embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t C);
+hipError_t embedding_backward(hipStream_t st, int dtype, int out_dtype, const EmbeddingGrad &a, void *workspace);
+
 }  // namespace wkv6

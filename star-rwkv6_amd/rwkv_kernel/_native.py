@@ -68,6 +68,12 @@ SIGNATURES = {
     "wkv6_adamw_step": (_int, [_p, _int, _int, _i64, _p, _p, _p] + [_d] * 6 + [_int, _p, ctypes.c_uint32]),
     "wkv6_grad_norm_workspace_bytes": (_sz, [_i64]),
     "wkv6_grad_norm": (_int, [_p, _int, _i64, _p, _p, _p, _sz]),
+    "wkv6_layer_norm": (_int, [_p] + [_int] * 3 + [_i64] * 2 + [_p, _i64, _p, _i64, _p, _p, _f, _p, _p, _p]),
+    "wkv6_layer_norm_backward_workspace_bytes": (_sz, [_i64] * 2),
+    "wkv6_layer_norm_backward": (_int, [_p] + [_int] * 3 + [_i64] * 2 + [_p, _i64] + [_p] * 9 + [_sz]),
+    "wkv6_embedding": (_int, [_p, _int, _int] + [_i64] * 3 + [_p, _p, _i64, _f, _p]),
+    "wkv6_embedding_backward_workspace_bytes": (_sz, [_i64] * 3),
+    "wkv6_embedding_backward": (_int, [_p, _int, _int] + [_i64] * 3 + [_p, _p, _f, _i64, _p, _p, _sz]),
     "wkv6_create_descriptor": (_sz, [_int] * 7 + [_p]),
     "wkv_forward": (None, [_p, ctypes.POINTER(_p), ctypes.c_char_p, _sz]),
     "wkv_backward": (None, [_p, ctypes.POINTER(_p), ctypes.c_char_p, _sz]),
