@@ -448,6 +448,33 @@ int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, con
                     int64_t *step, const float *lr_device, double lr, double beta1, double beta2, double eps, double weight_decay,
                     double max_grad_norm, int skip_nonfinite, const float *grad_norm, uint32_t seed);
 
+/* Orthogonalized updates.  `matrices` and coefficients lie in HOST memory and may be freed when the call returns.  grad and out are of
+ * `dtype`, row-major and contiguous like the rest; addresses need their element's alignment, the workspace 256 bytes.  A matrix without elements is
+ * left out. */
+typedef struct wkv6_muon_matrix {
+    const void *grad;
+    float *momentum;   /* wkv6_muon_step: the mean of gradients; otherwise NULL */
+    void *out;         /* the weights, or where the orthogonalized matrix goes */
+    float *master;     /* the weights in fp32, of which out then is the rounded copy, or NULL */
+    int64_t rows, columns;
+    double rate;       /* of the step, over lr */
+} wkv6_muon_matrix;
+
+/* What lets all of them go through together, or a part at a time where they are very large; more than the largest alone needs is not
+ * necessary. */
+size_t wkv6_muon_workspace_bytes(int64_t count, const wkv6_muon_matrix *matrices);
+
+/* out = X after X = grad / (|grad| + eps) and, with A = X X^T, `steps` times X = a X + b A X + c A A X; coefficients (steps, 3): a, b, c of each step.  (Of
+ * a matrix with more rows than columns, its transpose's, transposed.)  All products have 22 bits.  Entries of X, A and of a I + b A + c A A
+ * have to stay below 64; what leaves that range ends as NaN. */
+int wkv6_orthogonalize(void *stream, int dtype, int64_t count, const wkv6_muon_matrix *matrices, int steps, const double *coefficients, double eps,
+                       void *workspace, size_t workspace_bytes);
+
+/* In place: momentum = mu momentum + (1 - mu) grad; of (1 - mu) grad + mu momentum (nesterov) or of momentum the above;
+ * out = out (1 - lr weight_decay) - lr rate X.  lr_device: one value on the device in lr's place, or NULL. */
+int wkv6_muon_step(void *stream, int dtype, int64_t count, const wkv6_muon_matrix *matrices, int steps, const double *coefficients, double eps, double momentum,
+                   int nesterov, double lr, const float *lr_device, double weight_decay, void *workspace, size_t workspace_bytes);
+
 /* ---- Before and between the layers' own operators -----------------------------------------
  * No counterpart in the reference, whose model takes both from the framework (rwkv6_model.py:187-208, :259-274). */
 

@@ -736,6 +736,91 @@ Tensor adamw_step(const Tensors &params, const Tensors &grads, const Tensors &ex
   return norm;
 }
 
+// ---- orthogonalized updates ----
+
+// The matrices of tensors (.., rows, columns), each in one piece.
+void add_matrices(std::vector<wkv6_muon_matrix> &to, const Tensor &grad, const Tensor &out_, const Tensor &momentum, const Tensor &master, double rate) {
+  const int64_t rows = grad.size(-2), columns = grad.size(-1), n = rows * columns, es = static_cast<int64_t>(grad.element_size());
+  if (grad.numel() == 0) return;
+  for (int64_t i = 0; i < grad.numel() / n; ++i)
+    to.push_back({static_cast<const char *>(in(grad)) + i * n * es, momentum.defined() ? out_f(momentum) + i * n : nullptr, static_cast<char *>(out(out_)) + i * n * es,
+                  master.defined() ? out_f(master) + i * n : nullptr, rows, columns, rate});
+}
+
+void check_matrix(const Tensor &t, const Tensor &first, const char *what) {
+  on_one_device(t, first, what);
+  TORCH_CHECK(t.layout() == at::kStrided && t.dim() >= 2 && t.scalar_type() == first.scalar_type() && code_of(t.scalar_type()) >= 0, "wkv6: ", what,
+              " are matrices of one dtype, bf16, fp16 or fp32, on the GPU");
+}
+
+Tensors orthogonalize(const Tensors &matrices, const std::vector<double> &coefficients, double eps) {
+  Tensors res;
+  if (matrices.empty()) return res;
+  const Tensor &first = matrices[0];
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(first.device());
+  Tensors kept;
+  std::vector<wkv6_muon_matrix> rows;
+  for (const Tensor &m : matrices) check_matrix(m, first, "matrices");
+  for (const Tensor &m : matrices) {
+    kept.push_back(m.contiguous());
+    res.push_back(at::empty(m.sizes(), m.options()));
+    add_matrices(rows, kept.back(), res.back(), Tensor(), Tensor(), 0.);
+  }
+  if (rows.empty()) return res;
+  const size_t n = wkv6_muon_workspace_bytes(rows.size(), rows.data());
+  const Tensor ws = bytes(first, n);
+  check(wkv6_orthogonalize(stream_of(first), code_of(first.scalar_type()), rows.size(), rows.data(), static_cast<int>(coefficients.size() / 3), coefficients.data(), eps,
+                           out(ws), n));
+  return res;
+}
+
+void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momenta, const Tensors &masters, const std::vector<double> &rates,
+               const std::vector<double> &coefficients, double eps, double momentum, bool nesterov, double lr, const Tensor &lr_device, double weight_decay) {
+  const size_t count = params.size();
+  TORCH_CHECK(count > 0 && grads.size() == count && momenta.size() == count && rates.size() == count, "wkv6: one gradient and one momentum for each parameter");
+  const Tensor &first = params[0];
+  TORCH_CHECK(masters.empty() || (masters.size() == count && first.scalar_type() != at::kFloat), "wkv6: one master for each parameter of 16 bits");
+  if (lr_device.defined()) {
+    on_one_device(lr_device, first, "lr");
+    TORCH_CHECK(lr_device.scalar_type() == at::kFloat && lr_device.numel() == 1, "wkv6: lr is one float32");
+  }
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(first.device());
+  Tensors kept;
+  std::vector<wkv6_muon_matrix> rows;
+  std::vector<std::pair<uintptr_t, uintptr_t>> seen;   // what is written, from and to
+  for (size_t i = 0; i < count; ++i) {
+    check_matrix(params[i], first, "parameters");
+    check_matrix(grads[i], first, "gradients");
+    TORCH_CHECK(grads[i].sizes() == params[i].sizes() && params[i].is_contiguous(), "wkv6: parameters are contiguous, gradients of their shapes");
+    const Tensor master = masters.empty() ? Tensor() : masters[i];
+    for (const Tensor *t : {&momenta[i], &master}) {
+      if (!t->defined()) continue;
+      on_one_device(*t, first, "momenta and masters");
+      TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->sizes() == params[i].sizes(), "wkv6: momenta and masters are float32, contiguous, of the parameters' shapes");
+    }
+    kept.push_back(grads[i].contiguous());
+    add_matrices(rows, kept.back(), params[i], momenta[i], master, rates[i]);
+    for (const Tensor *t : {&params[i], &momenta[i], &master}) {
+      if (!t->defined() || t->numel() == 0) continue;
+      const auto at = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+      seen.emplace_back(at, at + t->nbytes());
+    }
+  }
+  std::sort(seen.begin(), seen.end());
+  for (size_t i = 1; i < seen.size(); ++i)
+    TORCH_CHECK(seen[i - 1].second <= seen[i].first, "wkv6: a parameter, a momentum or a master is given twice, or shares elements with another");
+  if (rows.empty()) return;
+  const size_t n = wkv6_muon_workspace_bytes(rows.size(), rows.data());
+  const Tensor ws = bytes(first, n);
+  check(wkv6_muon_step(stream_of(first), code_of(first.scalar_type()), rows.size(), rows.data(), static_cast<int>(coefficients.size() / 3), coefficients.data(), eps, momentum,
+                       nesterov, lr, in_f(lr_device), weight_decay, out(ws), n));
+  for (const Tensors *l : {&params, &momenta, &masters})
+    for (const Tensor &t : *l)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // (B, H, N, N)
 at::DimVector state_shape(const Dims &d) {
   TORCH_CHECK(d.H > 0, "wkv6: tensors without channels have no state");   // (the size per head below divides by it)
@@ -948,6 +1033,17 @@ PYBIND11_MODULE(_wkv6_torch, m) {
       return adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, scales, masters, given(lr_device), lr, beta1, beta2, eps, weight_decay,
                         max_grad_norm, skip_nonfinite, given(norm), seed);
     }));
+  });
+  m.def("orthogonalize", [](const Tensors &matrices, const std::vector<double> &coefficients, double eps) {
+    const Tensors res = unlocked([&] { return orthogonalize(matrices, coefficients, eps); });
+    py::list l;
+    for (const Tensor &t : res) l.append(wrap(t));
+    return l;
+  });
+  m.def("muon_step", [](const Tensors &params, const Tensors &grads, const Tensors &momenta, const Tensors &masters, const std::vector<double> &rates,
+                        const std::vector<double> &coefficients, double eps, double momentum, bool nesterov, double lr, const std::optional<Tensor> &lr_device,
+                        double weight_decay) {
+    unlocked([&] { muon_step(params, grads, momenta, masters, rates, coefficients, eps, momentum, nesterov, lr, given(lr_device), weight_decay); });
   });
   m.def("forward_gn_gate", [](int64_t H, const std::optional<Tensor> &map, const Tensor &r, const Tensor &k, const Tensor &v, const Tensor &w,
                               const Tensor &u, const std::optional<Tensor> &s0, const Tensor &gate, const Tensor &scale,

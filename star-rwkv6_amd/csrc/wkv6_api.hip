@@ -531,6 +531,63 @@ int wkv6_embedding_backward(void *stream, int dtype, int gout_dtype, int64_t N, 
     return finish(wkv6::embedding_backward((hipStream_t)stream, dtype, gout_dtype, wkv6::EmbeddingGrad{N, V, C, padding_id, ids, gout, scale, gweight}, workspace));
 }
 
+// ---- orthogonalized updates ----
+
+static_assert(sizeof(wkv6_muon_matrix) == sizeof(wkv6::MuonMatrix), "one layout");
+
+static int check_muon(int dtype, int64_t count, const wkv6_muon_matrix *matrices, bool update, int steps, const double *coefficients, double eps) {
+    if (!is_type(dtype) || count <= 0 || count > 0x7fffffffLL || !matrices) return WKV6_ERR_ARG;
+    if (steps <= 0 || steps > 100 || !coefficients || !(eps >= 0.)) return WKV6_ERR_ARG;
+    for (int64_t i = 0; i < count; ++i) {
+        const wkv6_muon_matrix &t = matrices[i];
+        if (t.rows < 0 || t.columns < 0) return WKV6_ERR_ARG;
+        if (t.rows == 0 || t.columns == 0) continue;
+        if (!t.grad || !t.out || !aligned(t.grad, element_size(dtype)) || !aligned(t.out, element_size(dtype))) return WKV6_ERR_ARG;
+        if (update && (!t.momentum || !(t.rate >= 0.))) return WKV6_ERR_ARG;
+        if (!aligned(t.momentum, 4) || !aligned(t.master, 4) || (!update && (t.momentum || t.master))) return WKV6_ERR_ARG;
+        if (!wkv6::muon_supported(t.rows, t.columns)) return WKV6_ERR_UNSUPPORTED;
+    }
+    return WKV6_OK;
+}
+
+// Room for all matrices at once, up to a size at which a launch fills the chip many times over; a larger one alone.
+static size_t muon_bytes(int64_t count, const wkv6_muon_matrix *matrices, bool least) {
+    size_t all = 0, most = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (matrices[i].rows <= 0 || matrices[i].columns <= 0 || !wkv6::muon_supported(matrices[i].rows, matrices[i].columns)) continue;
+        const size_t n = wkv6::muon_matrix_bytes(matrices[i].rows, matrices[i].columns);
+        all += n;
+        most = n > most ? n : most;
+    }
+    constexpr size_t kEnough = (size_t)2 << 30;
+    return least ? most : all < kEnough ? all : most > kEnough ? most : kEnough;
+}
+
+size_t wkv6_muon_workspace_bytes(int64_t count, const wkv6_muon_matrix *matrices) {
+    return count > 0 && count <= 0x7fffffffLL && matrices ? muon_bytes(count, matrices, false) : 0;
+}
+
+static int muon(void *stream, int dtype, int64_t count, const wkv6_muon_matrix *matrices, const wkv6::MuonStep &step, void *workspace, size_t workspace_bytes) {
+    if (muon_bytes(count, matrices, true) == 0) return WKV6_OK;   // (no elements)
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < muon_bytes(count, matrices, true)) return WKV6_ERR_WORKSPACE;
+    return finish(wkv6::muon((hipStream_t)stream, dtype, count, reinterpret_cast<const wkv6::MuonMatrix *>(matrices), step, workspace, workspace_bytes));
+}
+
+int wkv6_orthogonalize(void *stream, int dtype, int64_t count, const wkv6_muon_matrix *matrices, int steps, const double *coefficients, double eps,
+                       void *workspace, size_t workspace_bytes) {
+    const int rc = check_muon(dtype, count, matrices, false, steps, coefficients, eps);
+    if (rc != WKV6_OK) return rc;
+    return muon(stream, dtype, count, matrices, wkv6::MuonStep{steps, coefficients, eps, 0, 0., 0, 0., nullptr, 0.}, workspace, workspace_bytes);
+}
+
+int wkv6_muon_step(void *stream, int dtype, int64_t count, const wkv6_muon_matrix *matrices, int steps, const double *coefficients, double eps, double momentum,
+                   int nesterov, double lr, const float *lr_device, double weight_decay, void *workspace, size_t workspace_bytes) {
+    const int rc = check_muon(dtype, count, matrices, true, steps, coefficients, eps);
+    if (rc != WKV6_OK) return rc;
+    if (!(momentum >= 0. && momentum < 1.) || !(lr >= 0.) || !(weight_decay >= 0.) || !aligned(lr_device, 4)) return WKV6_ERR_ARG;
+    return muon(stream, dtype, count, matrices, wkv6::MuonStep{steps, coefficients, eps, 1, momentum, nesterov, lr, lr_device, weight_decay}, workspace, workspace_bytes);
+}
+
 static int check_mix(int dtype, int64_t B, int64_t T, int64_t C, int64_t R) {
     if (B <= 0 || T <= 0 || C <= 0 || R <= 0) return WKV6_ERR_ARG;
     if (dtype != WKV6_BF16 || !wkv6::shift_mix_supported(C, R)) return WKV6_ERR_UNSUPPORTED;

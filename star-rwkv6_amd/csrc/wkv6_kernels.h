@@ -449,4 +449,32 @@ hipError_t embedding(hipStream_t st, int dtype, int out_dtype, const EmbeddingAr
 size_t embedding_backward_workspace_bytes(int64_t N, int64_t V, int64_t C);
 hipError_t embedding_backward(hipStream_t st, int dtype, int out_dtype, const EmbeddingGrad &a, void *workspace);
 
+// --- orthogonalized updates, the optimizer with them (wkv6_muon.hip) ---
+struct MuonMatrix {
+    const void *grad;
+    float *momentum;      // null: what is orthogonalized is grad
+    void *out;            // the weights, or where the orthogonalized matrix goes
+    float *master;        // or null
+    int64_t rows, columns;
+    double rate;          // of the step, over lr
+};
+struct MuonStep {
+    int steps;
+    const double *coefficients;   // (steps, 3), in host memory: of X, A X and A A X
+    double eps;
+    int update;                   // the step; 0: only the orthogonalized matrices, and nothing below
+    double momentum;
+    int nesterov;
+    double lr;
+    const float *lr_device;       // one value in lr's place, or null
+    double weight_decay;
+};
+// (rows are addressed with 32-bit byte offsets, tiles counted in 32 bits)
+inline bool muon_supported(int64_t rows, int64_t columns) {
+    return rows < (1 << 26) && columns < (1 << 26) && rows * ((columns + 31) / 32 * 128) < (1LL << 32) && columns * ((rows + 31) / 32 * 128) < (1LL << 32);
+}
+size_t muon_matrix_bytes(int64_t rows, int64_t columns);
+// The matrices go through in groups that fit the workspace; one alone has to.
+hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matrices, const MuonStep &a, void *workspace, size_t workspace_bytes);
+
 }  // namespace wkv6

@@ -1,0 +1,489 @@
+// Weight updates brought near to the nearest matrix with orthonormal rows or columns, by Newton-Schulz products, and the optimizer's step with them.
+//
+//   X = U / (|U| + eps)              (|U|: the 2-norm of all elements; transposed if U has more rows than columns, so that X is m x n with m <= n)
+//   steps times:  A = X X^T,   B = a I + b A + c A A,   X = B X
+//   the step: buf = mu buf + (1 - mu) g,   U = (1 - mu) g + mu buf, or buf,   p = p (1 - lr wd) - rate X
+//
+// Precision.  The polynomial takes a singular value s to about a s while it is small, so five steps multiply what is lost in the small ones by up to a^5 = 485: with the
+// matrices in bf16 throughout the result is off by 1 to 16 % of its size, with fp16 by 0.1 to 2 %.  Here every matrix is a pair of fp16 numbers hi + lo,
+// 22 bits, and a product the three matrix instructions hi hi + hi lo + lo hi, which accumulate in fp32: about 1.6 times the error of fp32 throughout, at
+// 5 times the rate of the fp32 matrix instructions.  Values are held times 1024: those of X, A and B stay below some 4, so the pairs' range of
+// 64 is not left by coefficients of any use, and lo keeps its bits down to 2^-13 of 1 (below, the pair is exact to 2^-35).
+//
+// A pair's row of K numbers: for every 32 of them 64 bytes of hi, then 64 of lo; zeros behind the last.  So what the matrix instructions take of a row
+// in one stage is one line of 128 bytes.  All products are of rows by rows (X is kept beside its transpose): C_ij = sum_k P_ik Q_jk.  A and
+// A A are symmetric: only the tiles on and above the diagonal are computed, and each is written to both of its places.  B has a I in it, so that B X is the whole step.
+#include "wkv6_common.h"
+#include "wkv6_kernels.h"
+#include "wkv6_mfma.h"
+#include "wkv6_pieces.h"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace wkv6 {
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef float f16x __attribute__((ext_vector_type(16)));
+
+constexpr float kHeld = 1024.f;     // what values are multiplied by in a pair
+constexpr int kThreads = 256;
+constexpr int kGroup = 56;          // matrices of one launch: they travel in its arguments, which hold 4 KB
+constexpr int kChunk = 16384;       // elements of a matrix that a workgroup squares and adds up
+constexpr int kLine = 128;          // bytes of 32 numbers of a pair
+
+struct Item {
+    const void *grad;
+    float *momentum;      // null: U is the gradient
+    void *out;            // the weights, or the orthogonalized matrix
+    float *master;
+    int64_t at;           // of this matrix in the workspace, in bytes
+    int m, n;             // m <= n
+    float rate;           // of the step, over lr
+    int tall;             // it has n rows and m columns
+};
+struct Group {
+    Item t[kGroup];
+    int first[kGroup + 1];   // unit of work (chunk, tile) at which a matrix begins
+    int count;
+};
+struct Step {
+    float momentum, kept;    // kept = 1 - momentum
+    int nesterov, update;    // update: the last product is applied to weights
+    float eps, weight_decay, lr;
+    const float *lr_device;  // one value in lr's place, or null
+    float a, b, c;
+    char *workspace;
+};
+static_assert(sizeof(Group) + sizeof(Step) + 64 <= 4096, "a launch's arguments");
+
+__host__ __device__ inline int64_t pitch_of(int k) { return (int64_t)((k + 31) / 32) * kLine; }
+// What a matrix has in the workspace: X, its transpose twice (one is read while the other is written), A, B, sums of squares.
+struct Layout {
+    int64_t x, xt, xt_other, a, b, sums, end;
+};
+__host__ __device__ inline Layout layout_of(int m, int n) {
+    Layout l;
+    l.x = 0;
+    l.xt = l.x + m * pitch_of(n);
+    l.xt_other = l.xt + n * pitch_of(m);
+    l.a = l.xt_other + n * pitch_of(m);
+    l.b = l.a + m * pitch_of(m);
+    l.sums = l.b + m * pitch_of(m);
+    l.end = l.sums + ((int64_t)m * n + kChunk - 1) / kChunk * 8;
+    l.end = (l.end + 255) / 256 * 256;
+    return l;
+}
+
+__device__ __forceinline__ int item_of(const Group &g, int unit) {
+    int lo = 0, hi = g.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (g.first[mid] <= unit) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double block_sum(double v, double *part) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+    for (int i = 1; i < kThreads / 64; ++i) v += part[i];
+    return v;
+}
+
+// The momentum's update, and sums of squares of U by chunk.
+template <typename G> __global__ __launch_bounds__(kThreads) void momentum_kernel(Group g, Step s) {
+    constexpr int kE = 4;
+    __shared__ double part[kThreads / 64];
+    const int k = item_of(g, blockIdx.x);
+    const Item &t = g.t[k];
+    const int64_t numel = (int64_t)t.m * t.n;
+    const int chunk = blockIdx.x - g.first[k];
+    double sum = 0.;
+#pragma unroll 4
+    for (int i = 0; i < kChunk / kThreads / kE; ++i) {
+        const int64_t at = (int64_t)chunk * kChunk + (i * kThreads + (int)threadIdx.x) * kE;
+        const int n = (int)max((int64_t)0, min((int64_t)kE, numel - at));
+        Piece<G, kE> p;
+        p.template load<false>(static_cast<const G *>(t.grad) + at, n);
+        float v[kE];
+        unpack(p, v);
+        if (t.momentum) {
+            Piece<float, kE> q;
+            q.template load<false>(t.momentum + at, n);
+            float b[kE];
+            unpack(q, b);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+                b[e] = b[e] * s.momentum + v[e] * s.kept;
+                v[e] = s.nesterov ? v[e] * s.kept + b[e] * s.momentum : b[e];
+            }
+            pack(b, q);
+            q.template store<false>(t.momentum + at, n);
+        }
+#pragma unroll
+        for (int e = 0; e < kE; ++e) sum = __builtin_fma((double)v[e], (double)v[e], sum);
+    }
+    sum = block_sum(sum, part);
+    if (threadIdx.x == 0) reinterpret_cast<double *>(s.workspace + t.at + layout_of(t.m, t.n).sums)[chunk] = sum;
+}
+
+__device__ __forceinline__ void split(float v, f16_t &hi, f16_t &lo) {
+    hi = to_f16(v);
+    lo = to_f16(v - (float)hi);
+}
+
+// Eight values (times kHeld) into a pair's row.
+__device__ __forceinline__ void store_pair8(char *row, int k, const float (&v)[8]) {
+    h8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f16_t x, y;
+        split(v[e], x, y);
+        hi[e] = x, lo[e] = y;
+    }
+    char *p = row + (int64_t)(k / 32) * kLine + k % 32 * 2;
+    *reinterpret_cast<h8 *>(p) = hi;
+    *reinterpret_cast<h8 *>(p + 64) = lo;
+}
+
+constexpr int kSpread = 64;   // rows and columns of U that a workgroup takes
+
+// U over its norm as a pair, and its transpose.
+template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(Group g, Step s) {
+    __shared__ double part[kThreads / 64];
+    __shared__ float tile[kSpread][kSpread + 1];
+    const int k = item_of(g, blockIdx.x);
+    const Item &t = g.t[k];
+    const Layout l = layout_of(t.m, t.n);
+    const int rows = t.tall ? t.n : t.m, columns = t.tall ? t.m : t.n;
+    char *base = s.workspace + t.at;
+    const double *sums = reinterpret_cast<const double *>(base + l.sums);
+    const int chunks = (int)(((int64_t)t.m * t.n + kChunk - 1) / kChunk);
+    double sum = 0.;
+    for (int i = threadIdx.x; i < chunks; i += kThreads) sum += sums[i];
+    const float scale = (float)(kHeld / (sqrt(block_sum(sum, part)) + s.eps));
+    const int across = (columns + kSpread - 1) / kSpread, number = blockIdx.x - g.first[k], r0 = number / across * kSpread, c0 = number % across * kSpread;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll 4
+    for (int i = 0; i < kSpread / 4; ++i) {
+        const int r = r0 + i * 4 + wave, c = c0 + lane;
+        float v = 0.f;
+        if (r < rows && c < columns) {
+            const int64_t at = (int64_t)r * columns + c;
+            v = load1(static_cast<const G *>(t.grad) + at);
+            if (t.momentum) {
+                const float b = t.momentum[at];
+                v = s.nesterov ? v * s.kept + b * s.momentum : b;
+            }
+        }
+        tile[i * 4 + wave][lane] = v * scale;
+    }
+    __syncthreads();
+    char *straight = base + (t.tall ? l.xt : l.x), *across_to = base + (t.tall ? l.x : l.xt);
+#pragma unroll
+    for (int i = 0; i < kSpread * 8 / kThreads; ++i) {
+        const int which = i * kThreads + threadIdx.x, q = which % 8 * 8, r = which / 8;
+        float v[8];
+        if (r0 + r < rows && c0 + q < (columns + 31) / 32 * 32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[r][q + e];
+            store_pair8(straight + (r0 + r) * pitch_of(columns), c0 + q, v);
+        }
+        if (c0 + r < columns && r0 + q < (rows + 31) / 32 * 32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[q + e][r];
+            store_pair8(across_to + (c0 + r) * pitch_of(rows), r0 + q, v);
+        }
+    }
+}
+
+enum { kGram = 0, kPoly = 1, kApply = 2, kLast = 3 };   // A = X X^T; B = a I + b A + c A A; X = B X; the same into the result
+
+// Product tiles of kT x kT.  kWM x kWN waves share a tile's rows and columns, kKS of such sets its stages of 32 k.
+template <int T, int WM, int WN, int KS> struct TileShape {
+    static constexpr int tile = T, wm = WM, wn = WN, ks = KS, threads = 64 * WM * WN * KS;
+    static constexpr int set_bytes = 2 * T * kLine, stage_bytes = KS * set_bytes;
+};
+
+__device__ __forceinline__ f16x product(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+template <typename O> __device__ __forceinline__ void store_last(const Item &t, bool update, float decay, float rate, int64_t at, float v) {
+    O *out = static_cast<O *>(t.out) + at;
+    if (update) {
+        const float w = (t.master ? t.master[at] : load1(out)) * decay - rate * v;
+        if (t.master) t.master[at] = w;
+        store1(out, w);
+    } else {
+        store1(out, v);
+    }
+}
+
+template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::threads) void product_kernel(Group g, Step s, int turn, int total) {
+    constexpr int T = S::tile, kSet = S::wm * S::wn, kMT = T / S::wm / 32, kNT = T / S::wn / 32, kOctets = 2 * T / 8 / kSet;
+    __shared__ __align__(1024) char lds[2 * S::stage_bytes];
+    // neighbouring tiles, which read the same rows, to one of the eight caches: workgroups go to those in turn
+    const int unit = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    if (unit >= total) return;
+    const int item = item_of(g, unit);
+    const Item &t = g.t[item];
+    const Layout l = layout_of(t.m, t.n);
+    char *base = s.workspace + t.at;
+    int number = unit - g.first[item], ti, tj;
+    // rows of P and Q, and the length of either
+    int I, J, K;
+    const char *P, *Q;
+    if (kMode == kGram || kMode == kPoly) {
+        I = J = t.m, K = kMode == kGram ? t.n : t.m;
+        P = Q = base + (kMode == kGram ? l.x : l.a);
+        int wide = (t.m + T - 1) / T;
+        ti = 0;
+        while (number >= wide) number -= wide--, ++ti;
+        tj = ti + number;
+    } else {
+        I = t.m, J = t.n, K = t.m;
+        P = base + l.b, Q = base + (turn ? l.xt_other : l.xt);
+        const int down = (t.m + T - 1) / T;
+        ti = number % down, tj = number / down;
+        if (kMode == kLast && t.tall) {   // (the result's rows are X's columns)
+            I = t.n, J = t.m;
+            const char *q = P;
+            P = Q, Q = q;
+            const int swap = ti;
+            ti = tj, tj = swap;
+        }
+    }
+    const int64_t pitch = pitch_of(K);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / kSet, in_set = wave % kSet;
+    const int stages = (int)(pitch / kLine), rounds = (stages + S::ks - 1) / S::ks;
+
+    // This wave's part of a stage: rows 8 at a time, each row's line with its eight pieces of 16 bytes in an order of its own (piece p of row r at
+    // p ^ (r & 7)), so that the rows that eight lanes read next lie in different banks.
+    uint32_t from[kOctets];
+#pragma unroll
+    for (int q = 0; q < kOctets; ++q) {
+        const int octet = in_set * kOctets + q, r = octet * 8 + (lane >> 3);
+        const int row = r < T ? min(ti * T + r, I - 1) : min(tj * T + r - T, J - 1);
+        from[q] = (uint32_t)(row * pitch) + (uint32_t)(((lane & 7) ^ ((lane >> 3) & 7)) * 16);
+    }
+    const uint32_t to = lds_address(lds) + set * S::set_bytes + in_set * kOctets * 1024;
+    const auto load_stage = [&](int round) {
+        const int stage = round * S::ks + set;
+        if (stage >= stages) return;
+#pragma unroll
+        for (int q = 0; q < kOctets; ++q) {
+            const bool rows_of_p = (in_set * kOctets + q) * 8 < T;
+            load_rows8_to_lds((rows_of_p ? P : Q) + (int64_t)stage * kLine, from[q], to + (round & 1) * S::stage_bytes + q * 1024);
+        }
+    };
+    f16x acc[kMT][kNT];
+#pragma unroll
+    for (int a = 0; a < kMT; ++a)
+#pragma unroll
+        for (int b = 0; b < kNT; ++b) acc[a][b] = (f16x)(0.f);
+    const int row_i = (in_set / S::wn) * (T / S::wm), row_j = (in_set % S::wn) * (T / S::wn);
+    load_stage(0);
+    for (int round = 0; round < rounds; ++round) {
+        wait_loads<0>();
+        __syncthreads();
+        if (round + 1 < rounds) load_stage(round + 1);
+        if (round * S::ks + set < stages) {
+            const char *p = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (row_i + (lane & 31)) * kLine;
+            const char *q = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (T + row_j + (lane & 31)) * kLine;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int hi_at = ((half * 2 + (lane >> 5)) ^ (lane & 7)) * 16, lo_at = hi_at ^ 64;
+                h8 ph[kMT], pl[kMT], qh[kNT], ql[kNT];
+#pragma unroll
+                for (int a = 0; a < kMT; ++a) {
+                    ph[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + hi_at);
+                    pl[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + lo_at);
+                }
+#pragma unroll
+                for (int b = 0; b < kNT; ++b) {
+                    qh[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + hi_at);
+                    ql[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + lo_at);
+                }
+#pragma unroll
+                for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(ph[a], qh[b], acc[a][b]);
+#pragma unroll
+                for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(ph[a], ql[b], acc[a][b]);
+#pragma unroll
+                for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(pl[a], qh[b], acc[a][b]);
+            }
+        }
+    }
+    if constexpr (S::ks > 1) {
+        // the sets' sums, to the first
+        static_assert(2 * S::stage_bytes >= (S::ks - 1) * T * T * 4, "room for the sums");
+        float *sums = reinterpret_cast<float *>(lds);
+        __syncthreads();
+        if (set > 0) {
+#pragma unroll
+            for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums[((((set - 1) * kSet + in_set) * kMT + a) * kNT + b) * 1024 + r * 64 + lane] = acc[a][b][r];
+        }
+        __syncthreads();
+        if (set > 0) return;
+#pragma unroll
+        for (int other = 0; other < S::ks - 1; ++other)
+#pragma unroll
+            for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[a][b][r] += sums[(((other * kSet + in_set) * kMT + a) * kNT + b) * 1024 + r * 64 + lane];
+    }
+
+    // Lane l has column l % 32 of a 32 x 32 tile, and rows 8 k + 4 (l / 32) + (0 .. 3).
+    const float lr = kMode != kLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
+    const int64_t out_pitch = pitch_of(J), across_pitch = pitch_of(I);
+    char *out = base + (kMode == kGram ? l.a : kMode == kPoly ? l.b : l.x), *across = kMode == kApply ? base + (turn ? l.xt : l.xt_other) : out;
+#pragma unroll
+    for (int a = 0; a < kMT; ++a)
+#pragma unroll
+        for (int b = 0; b < kNT; ++b) {
+            const int i0 = ti * T + row_i + a * 32, j0 = tj * T + row_j + b * 32, j = j0 + (lane & 31);
+            if (i0 >= I || j0 >= J) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = i0 + q * 8 + (lane >> 5) * 4;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[a][b][q * 4 + e];
+                if constexpr (kMode == kLast) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + e < I && j < J) store_last<O>(t, s.update, decay, rate, (int64_t)(i + e) * J + j, v[e] * (1.f / (kHeld * kHeld)));
+                } else {
+                    char *line = across + (int64_t)min(j, J - 1) * across_pitch + (int64_t)(i0 / 32) * kLine + (i - i0) * 2;
+                    if constexpr (kMode == kPoly) {
+                        // (A is symmetric: four of a row instead of a column's)
+                        const char *gram = base + l.a + (line - across);
+                        const h4 hi = *reinterpret_cast<const h4 *>(gram), lo = *reinterpret_cast<const h4 *>(gram + 64);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = v[e] * (s.c / kHeld) + s.b * ((float)hi[e] + (float)lo[e]) + (i + e == j ? s.a * kHeld : 0.f);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] *= 1.f / kHeld;
+                    }
+                    h4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f16_t x, y;
+                        split(i + e < I && j < J ? v[e] : 0.f, x, y);
+                        hi[e] = x, lo[e] = y;
+                    }
+                    if (j < J) {
+                        *reinterpret_cast<h4 *>(line) = hi;
+                        *reinterpret_cast<h4 *>(line + 64) = lo;
+                    }
+                    if (kMode == kApply || ti != tj) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (i + e >= I) continue;
+                            char *p = out + (int64_t)(i + e) * out_pitch + (int64_t)(j0 / 32) * kLine + (lane & 31) * 2;
+                            *reinterpret_cast<f16_t *>(p) = hi[e];
+                            *reinterpret_cast<f16_t *>(p + 64) = lo[e];
+                        }
+                    }
+                }
+            }
+        }
+}
+
+template <typename F> hipError_t by_type(int dtype, F &&f) {
+    if (dtype == kBF16) f(bf16_t{});
+    else if (dtype == kF16) f(f16_t{});
+    else f(float{});
+    return hipGetLastError();
+}
+
+int tiles(int k, int tile) { return (k + tile - 1) / tile; }
+
+template <typename S, typename O> void launch_products(hipStream_t st, Group &g, Step s, int steps, const double *coefficients) {
+    const auto units = [&](bool symmetric) {
+        int total = 0;
+        for (int i = 0; i < g.count; ++i) {
+            g.first[i] = total;
+            const int down = tiles(g.t[i].m, S::tile);
+            total += symmetric ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
+        }
+        g.first[g.count] = total;
+        return total;
+    };
+    const auto launch = [&](auto kernel, int total, int turn) {
+        hipLaunchKernelGGL(kernel, dim3((total + 7) / 8 * 8), dim3(S::threads), 0, st, g, s, turn, total);
+    };
+    for (int step = 0; step < steps; ++step) {
+        s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
+        const int half = units(true);
+        launch(product_kernel<S, kGram, float>, half, 0);
+        launch(product_kernel<S, kPoly, float>, half, 0);
+        const int all = units(false);
+        if (step + 1 < steps) launch(product_kernel<S, kApply, float>, all, step & 1);
+        else launch(product_kernel<S, kLast, O>, all, step & 1);
+    }
+}
+
+}  // namespace
+
+size_t muon_matrix_bytes(int64_t rows, int64_t columns) {
+    return (size_t)layout_of((int)std::min(rows, columns), (int)std::max(rows, columns)).end;
+}
+
+hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matrices, const MuonStep &a, void *workspace, size_t workspace_bytes) {
+    const Step s{(float)a.momentum, (float)(1. - a.momentum), a.nesterov, a.update, (float)a.eps, (float)a.weight_decay, (float)a.lr, a.lr_device, 0.f, 0.f, 0.f,
+                 static_cast<char *>(workspace)};
+    for (int64_t at = 0; at < count;) {
+        Group g{};
+        size_t used = 0;
+        for (; at < count && g.count < kGroup; ++at) {
+            const MuonMatrix &t = matrices[at];
+            if (t.rows == 0 || t.columns == 0) continue;
+            const size_t bytes = muon_matrix_bytes(t.rows, t.columns);
+            if (g.count > 0 && used + bytes > workspace_bytes) break;
+            g.t[g.count++] = Item{t.grad, t.momentum, t.out, t.master, (int64_t)used, (int)std::min(t.rows, t.columns), (int)std::max(t.rows, t.columns), (float)t.rate,
+                                  t.rows > t.columns};
+            used += bytes;
+        }
+        if (g.count == 0) break;
+        const hipError_t e = by_type(dtype, [&](auto type) {
+            using O = decltype(type);
+            int total = 0;
+            for (int i = 0; i < g.count; ++i) g.first[i] = total, total += (int)(((int64_t)g.t[i].m * g.t[i].n + kChunk - 1) / kChunk);
+            g.first[g.count] = total;
+            hipLaunchKernelGGL((momentum_kernel<O>), dim3(total), dim3(kThreads), 0, st, g, s);
+            total = 0;
+            for (int i = 0; i < g.count; ++i) g.first[i] = total, total += tiles(g.t[i].m, kSpread) * tiles(g.t[i].n, kSpread);
+            g.first[g.count] = total;
+            hipLaunchKernelGGL((spread_kernel<O>), dim3(total), dim3(kThreads), 0, st, g, s);
+            int64_t large = 0;
+            for (int i = 0; i < g.count; ++i) large += (int64_t)tiles(g.t[i].m, 256) * tiles(g.t[i].n, 256);
+            if (large >= 256) launch_products<TileShape<256, 2, 4, 1>, O>(st, g, s, a.steps, a.coefficients);
+            else if (large >= 32) launch_products<TileShape<128, 2, 2, 1>, O>(st, g, s, a.steps, a.coefficients);
+            else launch_products<TileShape<64, 1, 1, 4>, O>(st, g, s, a.steps, a.coefficients);
+        });
+        if (e != hipSuccess) return e;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace wkv6

@@ -20,7 +20,7 @@ State arguments (reference doc, rwkv_kernel/__init__.py:14-38):
 Returns (y, final_state or None).
 
 The torch flavour also has what a training step does behind the model's last layer (torch_training.py): cross_entropy, token_logprobs,
-preference_loss, policy_loss, grad_norm, adamw_step and the optimizer AdamW; and before and between the layers (torch_layers.py) embedding and
+preference_loss, policy_loss, grad_norm, adamw_step and the optimizer AdamW; the optimizer Muon with orthogonalize and muon_step (torch_muon.py); and before and between the layers (torch_layers.py) embedding and
 layer_norm.
 """
 import os
@@ -32,6 +32,7 @@ if os.environ["KERAS_BACKEND"] == "jax":
 elif os.environ["KERAS_BACKEND"] == "torch":
     from .torch_rwkv_kernel import RWKVKernelOperator
     from .torch_layers import embedding, layer_norm
+    from .torch_muon import Muon, muon_step, orthogonalize
     from .torch_training import AdamW, adamw_step, cross_entropy, grad_norm, policy_loss, preference_loss, token_logprobs
 else:
     from .ops_rwkv_kernal import RWKVKernelOperator
@@ -40,4 +41,5 @@ from .ops_rwkv_kernal import RWKVKernelOperator as OPSKernelOperator
 
 __all__ = ["RWKVKernelOperator", "OPSKernelOperator"]
 if os.environ["KERAS_BACKEND"] == "torch":
-    __all__ += ["AdamW", "adamw_step", "cross_entropy", "embedding", "grad_norm", "layer_norm", "policy_loss", "preference_loss", "token_logprobs"]
+    __all__ += ["AdamW", "adamw_step", "cross_entropy", "embedding", "grad_norm", "layer_norm", "policy_loss", "preference_loss", "token_logprobs", "Muon",
+                "muon_step", "orthogonalize"]

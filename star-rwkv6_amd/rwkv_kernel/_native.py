@@ -68,6 +68,9 @@ SIGNATURES = {
     "wkv6_adamw_step": (_int, [_p, _int, _int, _i64, _p, _p, _p] + [_d] * 6 + [_int, _p, ctypes.c_uint32]),
     "wkv6_grad_norm_workspace_bytes": (_sz, [_i64]),
     "wkv6_grad_norm": (_int, [_p, _int, _i64, _p, _p, _p, _sz]),
+    "wkv6_muon_workspace_bytes": (_sz, [_i64, _p]),
+    "wkv6_orthogonalize": (_int, [_p, _int, _i64, _p, _int, _p, _d, _p, _sz]),
+    "wkv6_muon_step": (_int, [_p, _int, _i64, _p, _int, _p, _d, _d, _int, _d, _p, _d, _p, _sz]),
     "wkv6_layer_norm": (_int, [_p] + [_int] * 3 + [_i64] * 2 + [_p, _i64, _p, _i64, _p, _p, _f, _p, _p, _p]),
     "wkv6_layer_norm_backward_workspace_bytes": (_sz, [_i64] * 2),
     "wkv6_layer_norm_backward": (_int, [_p] + [_int] * 3 + [_i64] * 2 + [_p, _i64] + [_p] * 9 + [_sz]),
@@ -88,6 +91,11 @@ SIGNATURES = {
 class AdamwTensor(ctypes.Structure):
     """wkv6_adamw_tensor"""
     _fields_ = [(name, _p) for name in ("param", "grad", "exp_avg", "exp_avg_sq", "scales", "master")] + [("numel", _i64)]
+
+
+class MuonMatrix(ctypes.Structure):
+    """wkv6_muon_matrix"""
+    _fields_ = [(name, _p) for name in ("grad", "momentum", "out", "master")] + [("rows", _i64), ("columns", _i64), ("rate", _d)]
 
 
 _lib = None

@@ -1,0 +1,263 @@
+"""orthogonalize, muon_step and the optimizer against the formula in float64.
+
+Tolerances: the iteration multiplies what is lost in small singular values by up to 485, by how much depends on the matrix.  So the same iteration in float32 gives the
+measure: a pair of fp16 numbers has 22 bits where float32 has 24, each rounding is at most 4 times as large and there are as many of them, and the results may differ from
+float64 by 8 times what float32's does, in the 2-norm and in the largest element (beside 2^-19 of it, or 2^-16 of matrices so small that float32 may
+happen to be exact: five steps of some six roundings of 2^-22, doubled on the way).  The result's rounding to its type comes on top."""
+import math
+
+import pytest
+import torch
+
+import rwkv_kernel
+from rwkv_kernel.torch_muon import COEFFICIENTS
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = 2.0 ** -24
+
+
+def _iterate(g, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=torch.float64):
+    """One matrix, in this dtype, on its device."""
+    rows = coefficients if hasattr(coefficients[0], "__len__") else [coefficients] * steps
+    x = (g.double() / (g.double().norm() + eps)).to(dtype)
+    tall = x.shape[0] > x.shape[1]
+    x = x.t().contiguous() if tall else x
+    for a, b, c in rows:
+        gram = x @ x.t().contiguous()
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.t() if tall else x
+
+
+def _off(g, **kw):
+    """(the value in float64, what each element may be off by, and the 2-norm of all)"""
+    want, single = _iterate(g, **kw), _iterate(g, dtype=F32, **kw).double()
+    floor = 2.0 ** (-16 if min(g.shape) <= 4 else -19)
+    return want, 8 * float((single - want).abs().max()) + floor * float(want.abs().max()), 8 * float((single - want).norm()) + floor * float(want.norm())
+
+
+def _check(got, g, **kw):
+    assert got.shape == g.shape and got.dtype == g.dtype and got.is_contiguous()
+    want, each, all_ = _off(g, **kw)
+    half = torch.finfo(got.dtype).eps / 2
+    rounding = want.abs() * half + torch.finfo(got.dtype).smallest_normal * half
+    error = (got.double() - want).abs()
+    assert bool((error <= each + rounding + each * half).all()), (tuple(g.shape), float(error.max()), each)
+    assert float(error.norm()) <= all_ + float(rounding.norm()) * (1 + half), (tuple(g.shape), float(error.norm()), all_)
+
+
+def _matrix(m, n, seed, kind="gradient", dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, n, generator=g)
+    if kind == "gradient":     # a few strong directions and many weak ones
+        r = min(m, n, 8)
+        x = (torch.randn(m, r, generator=g) * torch.exp(-torch.arange(r) / 2.0)) @ torch.randn(r, n, generator=g) + 0.2 * x
+    elif kind == "deficient":  # rows that repeat
+        x = x[torch.arange(m) // 2]
+    elif kind == "sparse":
+        x = x * (torch.rand(m, n, generator=g) < 0.01)
+        x[0, 0] = 1.0
+    return (x * 1e-3).to(dtype).cuda()
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 3), (3, 2), (16, 16), (31, 33), (33, 31), (32, 32), (32, 64), (64, 32), (63, 65), (64, 64), (65, 129), (96, 100), (128, 128), (129, 300),
+          (300, 129), (256, 256), (257, 1000), (32, 2048), (2048, 32), (777, 1311), (1500, 600)]
+
+
+@pytest.mark.parametrize("m,n", SHAPES)
+def test_shapes(m, n):
+    print("orthogonalize", m, n, flush=True)
+    for dtype in (F32, BF16, F16):
+        x = _matrix(m, n, m + n, dtype=dtype)
+        out = rwkv_kernel.orthogonalize(x)
+        _check(out, x)
+        assert torch.equal(out, rwkv_kernel.orthogonalize(x))
+
+
+@pytest.mark.parametrize("kind", ["gradient", "normal", "deficient", "sparse"])
+def test_kinds(kind):
+    print("orthogonalize", kind, flush=True)
+    for m, n in ((100, 300), (300, 100), (200, 200)):
+        x = _matrix(m, n, 5, kind)
+        _check(rwkv_kernel.orthogonalize(x), x)
+        _check(rwkv_kernel.orthogonalize(x, steps=1), x, steps=1)
+        triples = [(3.0, -3.2, 1.2), (1.875, -1.25, 0.375)] * 2
+        _check(rwkv_kernel.orthogonalize(x, steps=4, coefficients=triples, eps=1e-3), x, steps=4, coefficients=triples, eps=1e-3)
+
+
+def test_singular_values():
+    """What the operator is for: those of a well-conditioned matrix come to 0.65 .. 1.25."""
+    x = _matrix(120, 400, 3, "normal")
+    s = torch.linalg.svdvals(rwkv_kernel.orthogonalize(x).double().cpu())
+    assert 0.65 < float(s.min()) and float(s.max()) < 1.25
+
+
+def test_lists_and_batches():
+    print("orthogonalize, lists", flush=True)
+    shapes = [(64, 64), (3, 200, 70), (1, 1), (32, 300), (2, 2, 40, 40), (300, 32), (0, 5), (256, 700), (4, 0, 8)] + [(24 + i, 40) for i in range(70)]
+    xs = [_matrix(math.prod(s[:-1]), s[-1], i).view(s) if math.prod(s) else torch.zeros(s, device="cuda") for i, s in enumerate(shapes)]
+    out = rwkv_kernel.orthogonalize(xs)
+    for x, o in zip(xs, out):
+        assert o.shape == x.shape
+        if x.numel():
+            for a, b in zip(x.reshape(-1, *x.shape[-2:]), o.reshape(-1, *o.shape[-2:])):
+                _check(b, a)
+    assert rwkv_kernel.orthogonalize([]) == []
+
+
+@pytest.mark.parametrize("count,m,n", [(4, 2048, 2048), (1, 2048, 2048), (1, 1024, 4096), (2, 4096, 1024), (9, 1000, 1500), (1, 300, 20000)])
+def test_large(count, m, n):
+    """(in float64 and float32 on the GPU)"""
+    print("orthogonalize", count, m, n, flush=True)
+    xs = [_matrix(m, n, i, dtype=BF16 if i % 2 else F32) for i in range(count)]
+    for dtype in (F32, BF16):
+        mine = [x for x in xs if x.dtype == dtype]
+        for x, o in zip(mine, rwkv_kernel.orthogonalize(mine)):
+            _check(o, x)
+
+
+def test_views():
+    x = _matrix(50, 120, 1)
+    big = torch.zeros(60, 130, device="cuda")
+    big[3:53, 7:127] = x
+    flat = torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(50, 120)
+    assert torch.equal(rwkv_kernel.orthogonalize(big[3:53, 7:127]), rwkv_kernel.orthogonalize(x))
+    assert torch.equal(rwkv_kernel.orthogonalize(flat), rwkv_kernel.orthogonalize(x))
+    _check(rwkv_kernel.orthogonalize(x.t()), x.t())
+
+
+def test_sizes_of_the_values():
+    """Only eps knows how large the elements are: from 1e-18 to 1e18 (their squares leave fp32), and nothing at all."""
+    x = _matrix(40, 60, 2, "normal")
+    for scale in (1e-18, 1e-10, 1e10, 1e18):
+        y = x * scale
+        _check(rwkv_kernel.orthogonalize(y, eps=0.0), y, eps=0.0)
+    assert not bool(rwkv_kernel.orthogonalize(torch.zeros(40, 60, device="cuda")).any())
+    y = x.clone()
+    y[3, 3] = float("nan")
+    assert bool(rwkv_kernel.orthogonalize(y).isnan().all())
+    out = rwkv_kernel.orthogonalize([x, y, x])
+    assert torch.equal(out[0], rwkv_kernel.orthogonalize(x)) and torch.equal(out[0], out[2])
+
+
+def _step_inputs(shapes, dtype, seed, masters):
+    ps = [_matrix(math.prod(s[:-1]), s[-1], seed + i, "normal").view(s) * 300 for i, s in enumerate(shapes)]
+    gs = [_matrix(math.prod(s[:-1]), s[-1], seed + 100 + i).view(s).to(dtype) for i, s in enumerate(shapes)]
+    bufs = [_matrix(math.prod(s[:-1]), s[-1], seed + 200 + i).view(s) * 0.3 for i, s in enumerate(shapes)]
+    return [p.to(dtype) for p in ps], gs, bufs, ps if masters else None
+
+
+def _check_step(before, after, lr, momentum, nesterov, decay, scale):
+    params, grads, bufs, masters = before
+    for i in range(len(params)):
+        g, b = grads[i].double(), bufs[i].double()
+        new = momentum * b + (1 - momentum) * g
+        off = 4 * U * (momentum * b.abs() + (1 - momentum) * g.abs())
+        assert bool(((after[2][i].double() - new).abs() <= off).all())
+        u = (1 - momentum) * g + momentum * new if nesterov else new
+        w = (masters or params)[i].double()
+        shape = w.shape
+        rate = {"shape": math.sqrt(max(1, shape[-2] / shape[-1])), "rms": 0.2 * math.sqrt(max(shape[-2:]))}.get(scale, scale)
+        for j in range(math.prod(shape[:-2])):
+            at = lambda t: t.reshape(-1, *shape[-2:])[j]  # noqa: E731
+            o, each, _ = _off(at(u))
+            want = at(w) * (1 - lr * decay) - lr * rate * o
+            off = lr * rate * each + 4 * U * (at(w).abs() + lr * rate * o.abs())
+            if masters:
+                assert bool(((at(after[3][i]).double() - want).abs() <= off).all())
+                assert torch.equal(after[0][i], after[3][i].to(after[0][i].dtype))
+            half = torch.finfo(after[0][i].dtype).eps / 2
+            off = off + (want.abs() + off) * half
+            error = (at(after[0][i]).double() - want).abs()
+            assert bool((error <= off).all()), (shape, float((error / off).max()))
+
+
+@pytest.mark.parametrize("dtype,masters", [(F32, False), (BF16, False), (BF16, True), (F16, True)])
+def test_steps(dtype, masters):
+    print("muon step", dtype, masters, flush=True)
+    shapes = [(64, 64), (300, 70), (70, 300), (2, 40, 50), (1, 9), (128, 256), (33, 33)]
+    for momentum, nesterov, decay, scale in ((0.95, True, 0.1, "shape"), (0.9, False, 0.0, "rms"), (0.0, True, 0.5, 0.7)):
+        before = _step_inputs(shapes, dtype, 7, masters)
+        after = tuple(None if l is None else [t.clone() for t in l] for l in before)
+        rwkv_kernel.muon_step(after[0], after[1], after[2], lr=0.02, momentum=momentum, nesterov=nesterov, weight_decay=decay, scale=scale, masters=after[3])
+        assert all(torch.equal(a, b) for a, b in zip(before[1], after[1]))
+        _check_step(before, after, 0.02, momentum, nesterov, decay, scale)
+        again = tuple(None if l is None else [t.clone() for t in l] for l in before)
+        rate = torch.tensor(0.02, device="cuda")
+        rwkv_kernel.muon_step(again[0], again[1], again[2], lr=rate, momentum=momentum, nesterov=nesterov, weight_decay=decay, scale=scale, masters=again[3])
+        assert all(torch.equal(a, b) for a, b in zip(after[0] + after[2], again[0] + again[2]))
+
+
+def test_optimizer():
+    print("Muon", flush=True)
+    g = torch.Generator().manual_seed(1)
+    make = lambda: [torch.nn.Parameter(p.clone()) for p in _step_inputs([(64, 32), (32, 64)], BF16, 3, False)[0]] + [torch.nn.Parameter(torch.ones(8, 8, device="cuda"))]  # noqa: E731
+    ps, qs = make(), make()
+    a, b = (rwkv_kernel.Muon([{"params": x[:2]}, {"params": x[2:], "lr": torch.tensor(0.1, device="cuda")}], lr=0.05, weight_decay=0.1, master_weights=True) for x in (ps, qs))
+    for step in range(4):
+        for p, q in zip(ps, qs):
+            p.grad = torch.randn(p.shape, generator=g).to(p.dtype).cuda() if step != 1 or p.shape != (8, 8) else None
+            q.grad = p.grad
+        before = [[p.detach().clone() for p in ps[:2]], [p.grad for p in ps[:2]], [a.state[p]["momentum"].clone() for p in ps[:2]] if step else [torch.zeros(p.shape, device="cuda") for p in ps[:2]],
+                  [a.state[p]["master"].clone() for p in ps[:2]] if step else [p.detach().float() for p in ps[:2]]]
+        last = ps[2].detach().clone()
+        a.step()
+        _check_step(before, [[p.detach() for p in ps[:2]], None, [a.state[p]["momentum"] for p in ps[:2]], [a.state[p]["master"] for p in ps[:2]]], 0.05, 0.95, True, 0.1, "shape")
+        assert torch.equal(last, ps[2].detach()) == (step == 1)
+        assert a.state[ps[0]]["momentum"].dtype == F32 and "master" not in a.state.get(ps[2], {})
+        if step == 1:   # the twin goes on from what was saved
+            b.load_state_dict(a.state_dict())
+            for p, q in zip(ps, qs):
+                q.data.copy_(p.data)
+        if step > 1:
+            b.step()
+            assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+            assert b.state[qs[0]]["momentum"].dtype == F32 and b.state[qs[0]]["master"].dtype == F32
+    with pytest.raises(AssertionError, match="master"):
+        rwkv_kernel.Muon([{"params": qs[:2]}, {"params": qs[2:]}], lr=0.05).load_state_dict(a.state_dict())
+
+
+def test_refused():
+    w = torch.zeros(8, 8, device="cuda")
+    step = lambda p=w, g=w.clone(), m=w.clone(), lr=0.1, **kw: rwkv_kernel.muon_step([p], [g], [m], lr, **kw)  # noqa: E731
+    for call in (lambda: rwkv_kernel.orthogonalize(w, steps=0), lambda: rwkv_kernel.orthogonalize(w, coefficients=(1, 2)), lambda: rwkv_kernel.orthogonalize(w, eps=-1.0),
+                 lambda: rwkv_kernel.orthogonalize(w, steps=2, coefficients=[(1, 2, 3)] * 3), lambda: rwkv_kernel.orthogonalize(w, coefficients=(1.0, 2.0, float("nan"))),
+                 lambda: step(lr=-1.0), lambda: step(momentum=1.0), lambda: step(scale="other"), lambda: step(scale=-1.0), lambda: step(p=w[0], g=w[0], m=w[0]),
+                 lambda: rwkv_kernel.Muon([torch.nn.Parameter(w[0])])):
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: rwkv_kernel.orthogonalize(w.double()), lambda: rwkv_kernel.orthogonalize(w[0]), lambda: rwkv_kernel.orthogonalize([w, w.to(BF16)]),
+                 lambda: rwkv_kernel.orthogonalize([w, w.cpu()]), lambda: step(p=w.t()[:, :4], g=w[:, :4], m=w[:, :4].contiguous()), lambda: step(m=w.to(BF16)),
+                 lambda: step(g=w.to(BF16)), lambda: step(m=w), lambda: rwkv_kernel.muon_step([w, w.clone()], [w.clone()] * 2, [w.clone(), w], 0.1),
+                 lambda: step(masters=[w.clone()]), lambda: step(lr=torch.ones(1)), lambda: rwkv_kernel.muon_step([], [], [], 0.1)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_captured_and_on_another_stream():
+    print("muon step, captured", flush=True)
+    shapes = [(64, 64), (300, 70), (16, 20)]
+    state = _step_inputs(shapes, BF16, 9, True)
+    twin = tuple([t.clone() for t in l] for l in state)
+    rate = torch.tensor(0.02, device="cuda")
+    run = lambda s: rwkv_kernel.muon_step(s[0], s[1], s[2], lr=rate, weight_decay=0.1, masters=s[3])  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(state)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run(state)
+    torch.cuda.current_stream().wait_stream(side)
+    run(twin)
+    for k in range(3):
+        rate.fill_(0.01 * (k + 1))
+        for a, b in zip(state[1], twin[1]):
+            new = _matrix(*a.shape, 50 + k, dtype=BF16)
+            a.copy_(new)
+            b.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        run(twin)
+        for x, y in zip(state, twin):
+            assert all(torch.equal(a, b) for a, b in zip(x, y))
