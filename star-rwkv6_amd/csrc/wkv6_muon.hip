@@ -215,22 +215,12 @@ template <int T, int WM, int WN, int KS> struct TileShape {
 
 __device__ __forceinline__ f16x product(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-template <typename O> __device__ __forceinline__ void store_last(const Item &t, bool update, float decay, float rate, int64_t at, float v) {
-    O *out = static_cast<O *>(t.out) + at;
-    if (update) {
-        const float w = (t.master ? t.master[at] : load1(out)) * decay - rate * v;
-        if (t.master) t.master[at] = w;
-        store1(out, w);
-    } else {
-        store1(out, v);
-    }
-}
-
-template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::threads) void product_kernel(Group g, Step s, int turn, int total) {
+template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::threads) void product_kernel(Group g, Step s, int turn, int total, int run) {
     constexpr int T = S::tile, kSet = S::wm * S::wn, kMT = T / S::wm / 32, kNT = T / S::wn / 32, kOctets = 2 * T / 8 / kSet;
     __shared__ __align__(1024) char lds[2 * S::stage_bytes];
-    // neighbouring tiles, which read the same rows, to one of the eight caches: workgroups go to those in turn
-    const int unit = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    // Workgroups go to the eight caches in turn: `run` neighbouring tiles, which read the same rows, to one, the next ones to the next, so that each gets as
+    // many of the long ones.
+    const int turn_of = blockIdx.x / 8, unit = (turn_of / run * 8 + (int)blockIdx.x % 8) * run + turn_of % run;
     if (unit >= total) return;
     const int item = item_of(g, unit);
     const Item &t = g.t[item];
@@ -265,13 +255,13 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     const int stages = (int)(pitch / kLine), rounds = (stages + S::ks - 1) / S::ks;
 
     // This wave's part of a stage: rows 8 at a time, each row's line with its eight pieces of 16 bytes in an order of its own (piece p of row r at
-    // p ^ (r & 7)), so that the rows that eight lanes read next lie in different banks.
+    // p ^ (r / 2 & 7)), so that what 16 lanes read of as many rows lies in different ones of the 64 banks.
     uint32_t from[kOctets];
 #pragma unroll
     for (int q = 0; q < kOctets; ++q) {
         const int octet = in_set * kOctets + q, r = octet * 8 + (lane >> 3);
         const int row = r < T ? min(ti * T + r, I - 1) : min(tj * T + r - T, J - 1);
-        from[q] = (uint32_t)(row * pitch) + (uint32_t)(((lane & 7) ^ ((lane >> 3) & 7)) * 16);
+        from[q] = (uint32_t)(row * pitch) + (uint32_t)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
     }
     const uint32_t to = lds_address(lds) + set * S::set_bytes + in_set * kOctets * 1024;
     const auto load_stage = [&](int round) {
@@ -289,42 +279,57 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
 #pragma unroll
         for (int b = 0; b < kNT; ++b) acc[a][b] = (f16x)(0.f);
     const int row_i = (in_set / S::wn) * (T / S::wm), row_j = (in_set % S::wn) * (T / S::wn);
+    // A stage is two halves of 16 k.  While a half's products run, the rows of the next are read; between the two halves of a stage all waves have read all of
+    // it, and what was loaded during the stage before is there: so the loads have the time of a whole stage, and no wave waits with empty hands.
+    struct Half {
+        h8 ph[kMT], pl[kMT], qh[kNT], ql[kNT];
+    };
+    const auto read_half = [&](Half &h, int round, int half) {
+        const char *p = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (row_i + (lane & 31)) * kLine;
+        const char *q = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (T + row_j + (lane & 31)) * kLine;
+        const int hi_at = ((half * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16, lo_at = hi_at ^ 64;
+#pragma unroll
+        for (int a = 0; a < kMT; ++a) {
+            h.ph[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + hi_at);
+            h.pl[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + lo_at);
+        }
+#pragma unroll
+        for (int b = 0; b < kNT; ++b) {
+            h.qh[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + hi_at);
+            h.ql[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + lo_at);
+        }
+    };
+    const auto multiply = [&](const Half &h) {
+#pragma unroll
+        for (int a = 0; a < kMT; ++a)
+#pragma unroll
+            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.ph[a], h.qh[b], acc[a][b]);
+#pragma unroll
+        for (int a = 0; a < kMT; ++a)
+#pragma unroll
+            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.ph[a], h.ql[b], acc[a][b]);
+#pragma unroll
+        for (int a = 0; a < kMT; ++a)
+#pragma unroll
+            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.pl[a], h.qh[b], acc[a][b]);
+    };
+    const auto mine = [&](int round) { return S::ks == 1 || round * S::ks + set < stages; };   // (the last round may leave a set without a stage)
+    Half first, second;
     load_stage(0);
+    wait_loads<0>();
+    __syncthreads();
+    if (rounds > 1) load_stage(1);
+    if (mine(0)) read_half(first, 0, 0);
     for (int round = 0; round < rounds; ++round) {
+        if (mine(round)) {
+            read_half(second, round, 1);
+            multiply(first);
+        }
         wait_loads<0>();
         __syncthreads();
-        if (round + 1 < rounds) load_stage(round + 1);
-        if (round * S::ks + set < stages) {
-            const char *p = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (row_i + (lane & 31)) * kLine;
-            const char *q = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (T + row_j + (lane & 31)) * kLine;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int hi_at = ((half * 2 + (lane >> 5)) ^ (lane & 7)) * 16, lo_at = hi_at ^ 64;
-                h8 ph[kMT], pl[kMT], qh[kNT], ql[kNT];
-#pragma unroll
-                for (int a = 0; a < kMT; ++a) {
-                    ph[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + hi_at);
-                    pl[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + lo_at);
-                }
-#pragma unroll
-                for (int b = 0; b < kNT; ++b) {
-                    qh[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + hi_at);
-                    ql[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + lo_at);
-                }
-#pragma unroll
-                for (int a = 0; a < kMT; ++a)
-#pragma unroll
-                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(ph[a], qh[b], acc[a][b]);
-#pragma unroll
-                for (int a = 0; a < kMT; ++a)
-#pragma unroll
-                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(ph[a], ql[b], acc[a][b]);
-#pragma unroll
-                for (int a = 0; a < kMT; ++a)
-#pragma unroll
-                    for (int b = 0; b < kNT; ++b) acc[a][b] = product(pl[a], qh[b], acc[a][b]);
-            }
-        }
+        if (round + 2 < rounds) load_stage(round + 2);
+        if (round + 1 < rounds && mine(round + 1)) read_half(first, round + 1, 0);
+        if (mine(round)) multiply(second);
     }
     if constexpr (S::ks > 1) {
         // the sets' sums, to the first
@@ -351,35 +356,67 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                     for (int r = 0; r < 16; ++r) acc[a][b][r] += sums[(((other * kSet + in_set) * kMT + a) * kNT + b) * 1024 + r * 64 + lane];
     }
 
-    // Lane l has column l % 32 of a 32 x 32 tile, and rows 8 k + 4 (l / 32) + (0 .. 3).
+    // Lane l has column l % 32 of a 32 x 32 tile, and rows 8 k + 4 (l / 32) + (0 .. 3).  A tile goes out through 4 KB of LDS of the wave's own, so that stores
+    // are of 16 bytes to a lane and 64 or 128 to a line.
     const float lr = kMode != kLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
     const int64_t out_pitch = pitch_of(J), across_pitch = pitch_of(I);
     char *out = base + (kMode == kGram ? l.a : kMode == kPoly ? l.b : l.x), *across = kMode == kApply ? base + (turn ? l.xt : l.xt_other) : out;
+    __syncthreads();   // (all waves have read their stages)
+    char *stage = lds + in_set * 4096;
 #pragma unroll
     for (int a = 0; a < kMT; ++a)
 #pragma unroll
         for (int b = 0; b < kNT; ++b) {
-            const int i0 = ti * T + row_i + a * 32, j0 = tj * T + row_j + b * 32, j = j0 + (lane & 31);
+            const int i0 = ti * T + row_i + a * 32, j0 = tj * T + row_j + b * 32;
             if (i0 >= I || j0 >= J) continue;
+            if constexpr (kMode == kLast) {
+                float *rows = reinterpret_cast<float *>(stage);   // [i][j]
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int i = i0 + q * 8 + (lane >> 5) * 4;
-                float v[4];
+                for (int r = 0; r < 16; ++r) rows[(r / 4 * 8 + (lane >> 5) * 4 + r % 4) * 32 + (lane & 31)] = acc[a][b][r] * (1.f / (kHeld * kHeld));
+                constexpr int kE = 4;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[a][b][q * 4 + e];
-                if constexpr (kMode == kLast) {
+                for (int q = 0; q < 4; ++q) {
+                    const int i = i0 + q * 8 + (lane >> 3), j = j0 + (lane & 7) * kE, n = i < I ? min(J - j, kE) : 0;
+                    const int64_t at = (int64_t)i * J + j;
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(rows + (q * 8 + (lane >> 3)) * 32 + (lane & 7) * kE);
+                    float v[kE] = {x[0], x[1], x[2], x[3]};
+                    Piece<O, kE> w;
+                    if (s.update) {
+                        Piece<float, kE> master;
+                        float old[kE];
+                        if (t.master) {
+                            master.template load<false>(t.master + at, n);
+                            unpack(master, old);
+                        } else {
+                            w.template load<false>(static_cast<const O *>(t.out) + at, n);
+                            unpack(w, old);
+                        }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (i + e < I && j < J) store_last<O>(t, s.update, decay, rate, (int64_t)(i + e) * J + j, v[e] * (1.f / (kHeld * kHeld)));
-                } else {
-                    char *line = across + (int64_t)min(j, J - 1) * across_pitch + (int64_t)(i0 / 32) * kLine + (i - i0) * 2;
+                        for (int e = 0; e < kE; ++e) v[e] = old[e] * decay - rate * v[e];
+                        if (t.master) {
+                            pack(v, master);
+                            master.template store<false>(t.master + at, n);
+                        }
+                    }
+                    pack(v, w);
+                    w.template store<false>(static_cast<O *>(t.out) + at, n);
+                }
+            } else {
+                // rows of `across`, j, with their pieces in the order that stages have too
+                const int j = j0 + (lane & 31), turned = (lane >> 1) & 7;
+                char *row = stage + (lane & 31) * kLine;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int i = i0 + q * 8 + (lane >> 5) * 4;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[a][b][q * 4 + e];
                     if constexpr (kMode == kPoly) {
                         // (A is symmetric: four of a row instead of a column's)
-                        const char *gram = base + l.a + (line - across);
+                        const char *gram = base + l.a + min(j, J - 1) * across_pitch + (int64_t)(i0 / 32) * kLine + (i - i0) * 2;
                         const h4 hi = *reinterpret_cast<const h4 *>(gram), lo = *reinterpret_cast<const h4 *>(gram + 64);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = v[e] * (s.c / kHeld) + s.b * ((float)hi[e] + (float)lo[e]) + (i + e == j ? s.a * kHeld : 0.f);
+                        for (int e = 0; e < 4; ++e) v[e] = v[e] * (s.c / kHeld) + s.b * ((float)hi[e] + (float)lo[e]) + (i + e == j ? s.a * kHeld : 0.f);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] *= 1.f / kHeld;
@@ -391,17 +428,32 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                         split(i + e < I && j < J ? v[e] : 0.f, x, y);
                         hi[e] = x, lo[e] = y;
                     }
-                    if (j < J) {
-                        *reinterpret_cast<h4 *>(line) = hi;
-                        *reinterpret_cast<h4 *>(line + 64) = lo;
-                    }
-                    if (kMode == kApply || ti != tj) {
+                    *reinterpret_cast<h4 *>(row + (q ^ turned) * 16 + (lane >> 5) * 8) = hi;
+                    *reinterpret_cast<h4 *>(row + ((q + 4) ^ turned) * 16 + (lane >> 5) * 8) = lo;
+                }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (i + e >= I) continue;
-                            char *p = out + (int64_t)(i + e) * out_pitch + (int64_t)(j0 / 32) * kLine + (lane & 31) * 2;
-                            *reinterpret_cast<f16_t *>(p) = hi[e];
-                            *reinterpret_cast<f16_t *>(p + 64) = lo[e];
+                for (int q = 0; q < 4; ++q) {
+                    const int r = q * 8 + (lane >> 3), piece = lane & 7;
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(stage + r * kLine + ((piece ^ (r >> 1)) & 7) * 16);
+                    if (j0 + r < J) *reinterpret_cast<u32x4 *>(across + (j0 + r) * across_pitch + (int64_t)(i0 / 32) * kLine + piece * 16) = x;
+                }
+                if (kMode == kApply || ti != tj) {
+                    // rows of `out`, i: the transposing read hands lane l of 16 lanes the l-th element of each of four rows j
+                    const int group = lane >> 4, l16 = lane & 15;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int i = i0 + half * 16 + l16;
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) {   // hi, lo
+                            s16x4 x[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int r = group * 8 + k * 4 + (l16 >> 2), piece = part * 4 + half * 2 + (l16 >> 1 & 1);
+                                const char *p = stage + r * kLine + ((piece ^ (r >> 1)) & 7) * 16 + (l16 & 1) * 8;
+                                x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)p);
+                            }
+                            const u32x2 y = __builtin_bit_cast(u32x2, x[0]), z = __builtin_bit_cast(u32x2, x[1]);
+                            if (i < I) *reinterpret_cast<u32x4 *>(out + i * out_pitch + (int64_t)(j0 / 32) * kLine + part * 64 + group * 16) = (u32x4){y[0], y[1], z[0], z[1]};
                         }
                     }
                 }
@@ -418,8 +470,12 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
 
 int tiles(int k, int tile) { return (k + tile - 1) / tile; }
 
-template <typename S, typename O> void launch_products(hipStream_t st, Group &g, Step s, int steps, const double *coefficients) {
-    const auto units = [&](bool symmetric) {
+template <typename S, typename O> void launch_products(hipStream_t st, Group &by_n, Step s, int steps, const double *coefficients) {
+    // (the longest products first: what is begun last is done soon)
+    Group by_m = by_n;
+    std::sort(by_n.t, by_n.t + by_n.count, [](const Item &x, const Item &y) { return x.n != y.n ? x.n > y.n : x.at < y.at; });
+    std::sort(by_m.t, by_m.t + by_m.count, [](const Item &x, const Item &y) { return x.m != y.m ? x.m > y.m : x.at < y.at; });
+    const auto units = [](Group &g, bool symmetric) {
         int total = 0;
         for (int i = 0; i < g.count; ++i) {
             g.first[i] = total;
@@ -427,19 +483,21 @@ template <typename S, typename O> void launch_products(hipStream_t st, Group &g,
             total += symmetric ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
         }
         g.first[g.count] = total;
-        return total;
     };
-    const auto launch = [&](auto kernel, int total, int turn) {
-        hipLaunchKernelGGL(kernel, dim3((total + 7) / 8 * 8), dim3(S::threads), 0, st, g, s, turn, total);
+    const auto launch = [&](auto kernel, const Group &g, int turn) {
+        const int total = g.first[g.count];
+        const int run = std::max(1, std::min(32, total / 16));
+        hipLaunchKernelGGL(kernel, dim3((total + 8 * run - 1) / (8 * run) * 8 * run), dim3(S::threads), 0, st, g, s, turn, total, run);
     };
     for (int step = 0; step < steps; ++step) {
         s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
-        const int half = units(true);
-        launch(product_kernel<S, kGram, float>, half, 0);
-        launch(product_kernel<S, kPoly, float>, half, 0);
-        const int all = units(false);
-        if (step + 1 < steps) launch(product_kernel<S, kApply, float>, all, step & 1);
-        else launch(product_kernel<S, kLast, O>, all, step & 1);
+        units(by_n, true);
+        launch(product_kernel<S, kGram, float>, by_n, 0);
+        units(by_m, true);
+        launch(product_kernel<S, kPoly, float>, by_m, 0);
+        units(by_m, false);
+        if (step + 1 < steps) launch(product_kernel<S, kApply, float>, by_m, step & 1);
+        else launch(product_kernel<S, kLast, O>, by_m, step & 1);
     }
 }
 
