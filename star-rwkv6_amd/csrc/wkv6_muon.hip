@@ -68,7 +68,8 @@ struct Layout {
 __host__ __device__ inline Layout layout_of(int m, int n) {
     Layout l;
     l.x = 0;
-    l.xt = l.x + m * pitch_of(n);
+    // (of a matrix of at most 64 rows: the parts of A instead of X, two times 16 of 4 KB for each 32 x 32)
+    l.xt = l.x + (m <= 64 ? (int64_t)((m + 31) / 32) * ((m + 31) / 32) * (2 * 16 * 4096) : m * pitch_of(n));
     l.xt_other = l.xt + n * pitch_of(m);
     l.a = l.xt_other + n * pitch_of(m);
     l.b = l.a + m * pitch_of(m);
@@ -78,13 +79,13 @@ __host__ __device__ inline Layout layout_of(int m, int n) {
     return l;
 }
 
+__host__ inline int tiles(int k, int tile) { return (k + tile - 1) / tile; }
+
+// (by all lanes at once: each step of a search would wait for its own load of an argument)
 __device__ __forceinline__ int item_of(const Group &g, int unit) {
-    int lo = 0, hi = g.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (g.first[mid] <= unit) lo = mid; else hi = mid;
-    }
-    return lo;
+    static_assert(kGroup <= 64, "one lane to a matrix");
+    const int lane = threadIdx.x & 63;
+    return __popcll(__ballot(lane < g.count && g.first[min(lane, kGroup - 1)] <= unit)) - 1;
 }
 
 __device__ __forceinline__ double block_sum(double v, double *part) {
@@ -207,9 +208,9 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
 
 enum { kGram = 0, kPoly = 1, kApply = 2, kLast = 3 };   // A = X X^T; B = a I + b A + c A A; X = B X; the same into the result
 
-// Product tiles of kT x kT.  kWM x kWN waves share a tile's rows and columns, kKS of such sets its stages of 32 k.
-template <int T, int WM, int WN, int KS> struct TileShape {
-    static constexpr int tile = T, wm = WM, wn = WN, ks = KS, threads = 64 * WM * WN * KS;
+// Product tiles of T x T.  WM x WN waves share a tile's rows and columns, KS of such sets its stages of 32 k, of which LDS holds NB (to a set) at a time.
+template <int T, int WM, int WN, int KS, int NB> struct TileShape {
+    static constexpr int tile = T, wm = WM, wn = WN, ks = KS, buffers = NB, threads = 64 * WM * WN * KS;
     static constexpr int set_bytes = 2 * T * kLine, stage_bytes = KS * set_bytes;
 };
 
@@ -217,7 +218,7 @@ __device__ __forceinline__ f16x product(h8 a, h8 b, f16x c) { return __builtin_a
 
 template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::threads) void product_kernel(Group g, Step s, int turn, int total, int run) {
     constexpr int T = S::tile, kSet = S::wm * S::wn, kMT = T / S::wm / 32, kNT = T / S::wn / 32, kOctets = 2 * T / 8 / kSet;
-    __shared__ __align__(1024) char lds[2 * S::stage_bytes];
+    __shared__ __align__(1024) char lds[S::buffers * S::stage_bytes];
     // Workgroups go to the eight caches in turn: `run` neighbouring tiles, which read the same rows, to one, the next ones to the next, so that each gets as
     // many of the long ones.
     const int turn_of = blockIdx.x / 8, unit = (turn_of / run * 8 + (int)blockIdx.x % 8) * run + turn_of % run;
@@ -264,14 +265,14 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         from[q] = (uint32_t)(row * pitch) + (uint32_t)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
     }
     const uint32_t to = lds_address(lds) + set * S::set_bytes + in_set * kOctets * 1024;
+    const auto load = [&](int round, int q) {
+        const int stage = min(round * S::ks + set, stages - 1);   // (what the last round may be short of is loaded all the same, and not used)
+        const bool rows_of_p = (in_set * kOctets + q) * 8 < T;
+        load_rows8_to_lds((rows_of_p ? P : Q) + (int64_t)stage * kLine, from[q], to + round % S::buffers * S::stage_bytes + q * 1024);
+    };
     const auto load_stage = [&](int round) {
-        const int stage = round * S::ks + set;
-        if (stage >= stages) return;
 #pragma unroll
-        for (int q = 0; q < kOctets; ++q) {
-            const bool rows_of_p = (in_set * kOctets + q) * 8 < T;
-            load_rows8_to_lds((rows_of_p ? P : Q) + (int64_t)stage * kLine, from[q], to + (round & 1) * S::stage_bytes + q * 1024);
-        }
+        for (int q = 0; q < kOctets; ++q) load(round, q);
     };
     f16x acc[kMT][kNT];
 #pragma unroll
@@ -279,61 +280,83 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
 #pragma unroll
         for (int b = 0; b < kNT; ++b) acc[a][b] = (f16x)(0.f);
     const int row_i = (in_set / S::wn) * (T / S::wm), row_j = (in_set % S::wn) * (T / S::wn);
-    // A stage is two halves of 16 k.  While a half's products run, the rows of the next are read; between the two halves of a stage all waves have read all of
-    // it, and what was loaded during the stage before is there: so the loads have the time of a whole stage, and no wave waits with empty hands.
+    // A stage is two halves of 16 k.  While a half's products run, the rows of the next are read and, in the second half, the stage after the next ones is
+    // loaded; between the two halves of a stage all waves have read all of it, and what was loaded before is there.  Reads and loads stand between the
+    // products, in this order: put before them, they hold the wave up for as long as the products take (a tile of 128 x 128 alone on its compute
+    // unit: 0.88 us a stage).
     struct Half {
-        h8 ph[kMT], pl[kMT], qh[kNT], ql[kNT];
+        h8 ph[kMT], qh[kNT], ql[kNT], pl[kMT];
     };
-    const auto read_half = [&](Half &h, int round, int half) {
-        const char *p = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (row_i + (lane & 31)) * kLine;
-        const char *q = lds + (round & 1) * S::stage_bytes + set * S::set_bytes + (T + row_j + (lane & 31)) * kLine;
+    constexpr int kReads = 2 * (kMT + kNT), kProducts = 3 * kMT * kNT;
+    const auto read = [&](Half &h, int round, int half, int which) {
+        const char *stage = lds + round % S::buffers * S::stage_bytes + set * S::set_bytes;
+        const char *p = stage + (row_i + (lane & 31)) * kLine, *q = stage + (T + row_j + (lane & 31)) * kLine;
         const int hi_at = ((half * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16, lo_at = hi_at ^ 64;
-#pragma unroll
-        for (int a = 0; a < kMT; ++a) {
-            h.ph[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + hi_at);
-            h.pl[a] = *reinterpret_cast<const h8 *>(p + a * 32 * kLine + lo_at);
-        }
-#pragma unroll
-        for (int b = 0; b < kNT; ++b) {
-            h.qh[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + hi_at);
-            h.ql[b] = *reinterpret_cast<const h8 *>(q + b * 32 * kLine + lo_at);
-        }
+        if (which < kMT) h.ph[which] = *reinterpret_cast<const h8 *>(p + which * 32 * kLine + hi_at);
+        else if (which < kMT + kNT) h.qh[which - kMT] = *reinterpret_cast<const h8 *>(q + (which - kMT) * 32 * kLine + hi_at);
+        else if (which < kMT + 2 * kNT) h.ql[which - kMT - kNT] = *reinterpret_cast<const h8 *>(q + (which - kMT - kNT) * 32 * kLine + lo_at);
+        else h.pl[which - kMT - 2 * kNT] = *reinterpret_cast<const h8 *>(p + (which - kMT - 2 * kNT) * 32 * kLine + lo_at);
     };
-    const auto multiply = [&](const Half &h) {
-#pragma unroll
-        for (int a = 0; a < kMT; ++a)
-#pragma unroll
-            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.ph[a], h.qh[b], acc[a][b]);
-#pragma unroll
-        for (int a = 0; a < kMT; ++a)
-#pragma unroll
-            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.ph[a], h.ql[b], acc[a][b]);
-#pragma unroll
-        for (int a = 0; a < kMT; ++a)
-#pragma unroll
-            for (int b = 0; b < kNT; ++b) acc[a][b] = product(h.pl[a], h.qh[b], acc[a][b]);
+    const auto multiply = [&](const Half &h, int which) {
+        const int a = which % (kMT * kNT) / kNT, b = which % kNT;
+        if (which < kMT * kNT) acc[a][b] = product(h.ph[a], h.qh[b], acc[a][b]);
+        else if (which < 2 * kMT * kNT) acc[a][b] = product(h.ph[a], h.ql[b], acc[a][b]);
+        else acc[a][b] = product(h.pl[a], h.qh[b], acc[a][b]);
     };
-    const auto mine = [&](int round) { return S::ks == 1 || round * S::ks + set < stages; };   // (the last round may leave a set without a stage)
-    Half first, second;
-    load_stage(0);
-    wait_loads<0>();
-    __syncthreads();
-    if (rounds > 1) load_stage(1);
-    if (mine(0)) read_half(first, 0, 0);
-    for (int round = 0; round < rounds; ++round) {
-        if (mine(round)) {
-            read_half(second, round, 1);
-            multiply(first);
-        }
-        wait_loads<0>();
+    const auto wait_for_all = [&](bool more) {   // more: the loads of buffers - 2 stages may stay under way
+        if (more) wait_loads<(S::buffers - 2) * kOctets>();
+        else wait_loads<0>();
         __syncthreads();
-        if (round + 2 < rounds) load_stage(round + 2);
-        if (round + 1 < rounds && mine(round + 1)) read_half(first, round + 1, 0);
-        if (mine(round)) multiply(second);
+    };
+    Half first, second;
+#pragma unroll
+    for (int k = 0; k < S::buffers - 1; ++k)
+        if (k < rounds) load_stage(k);
+    wait_for_all(S::buffers - 1 <= rounds);
+    if (S::buffers - 1 < rounds) load_stage(S::buffers - 1);
+#pragma unroll
+    for (int k = 0; k < kReads; ++k) read(first, 0, 0, k);
+    int round = 0;
+    for (; round + S::buffers < rounds; ++round) {
+#pragma unroll
+        for (int o = 0; o < kProducts; ++o) {
+#pragma unroll
+            for (int k = o * kReads / kProducts; k < (o + 1) * kReads / kProducts; ++k) read(second, round, 1, k);
+            multiply(first, o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_for_all(true);
+#pragma unroll
+        for (int o = 0; o < kProducts; ++o) {
+#pragma unroll
+            for (int k = o * kReads / kProducts; k < (o + 1) * kReads / kProducts; ++k) read(first, round + 1, 0, k);
+#pragma unroll
+            for (int k = o * kOctets / kProducts; k < (o + 1) * kOctets / kProducts; ++k) load(round + S::buffers, k);
+            multiply(second, o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    for (; round < rounds; ++round) {   // nothing more to load
+        const bool mine = S::ks == 1 || round * S::ks + set < stages;
+        if (mine) {
+#pragma unroll
+            for (int k = 0; k < kReads; ++k) read(second, round, 1, k);
+#pragma unroll
+            for (int o = 0; o < kProducts; ++o) multiply(first, o);
+        }
+        if (round + 1 < rounds) {
+            wait_for_all(false);
+#pragma unroll
+            for (int k = 0; k < kReads; ++k) read(first, round + 1, 0, k);
+        }
+        if (mine) {
+#pragma unroll
+            for (int o = 0; o < kProducts; ++o) multiply(second, o);
+        }
     }
     if constexpr (S::ks > 1) {
         // the sets' sums, to the first
-        static_assert(2 * S::stage_bytes >= (S::ks - 1) * T * T * 4, "room for the sums");
+        static_assert(S::buffers * S::stage_bytes >= (S::ks - 1) * T * T * 4, "room for the sums");
         float *sums = reinterpret_cast<float *>(lds);
         __syncthreads();
         if (set > 0) {
@@ -461,6 +484,215 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         }
 }
 
+// ---- matrices of at most 64 rows (or columns) ----
+//
+// A and B are one tile, and what a step costs is launches and latency.  So a step is one launch: a workgroup adds up the parts of A that the launch before left,
+// forms B (each for itself), multiplies its columns of X by it 64 at a time, and leaves its part of the new A.  10 matrices of 32 x 2048: 17 launches of
+// the general form 150 us of kernels.
+constexpr int kThin = 64, kThinParts = 16;
+constexpr int kThinRegion = 2 * kThin * kLine;   // 64 rows of 64 k
+
+// LDS operands: 64 rows of kThin k as lines of 32 k, pieces in the order that stages have.
+__device__ __forceinline__ char *thin_piece(char *region, int row, int block, int piece) {
+    return region + (block * kThin + row) * kLine + ((piece ^ (row >> 1)) & 7) * 16;
+}
+__device__ __forceinline__ h8 thin_read(char *region, int row, int k, bool lo) {   // k: a multiple of 8
+    return *reinterpret_cast<const h8 *>(thin_piece(region, row, k / 32, k % 32 / 8 + (lo ? 4 : 0)));
+}
+// 32 x 32 of P Q^T from row_i of P and row_j of Q on, over `blocks` times 32 k
+__device__ __forceinline__ void thin_product(char *p, char *q, int row_i, int row_j, int blocks, int lane, f16x &acc) {
+    for (int block = 0; block < blocks; ++block)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = block * 32 + half * 16 + (lane >> 5) * 8;
+            const h8 ph = thin_read(p, row_i + (lane & 31), k, false), pl = thin_read(p, row_i + (lane & 31), k, true);
+            const h8 qh = thin_read(q, row_j + (lane & 31), k, false), ql = thin_read(q, row_j + (lane & 31), k, true);
+            acc = product(ph, qh, acc);
+            acc = product(ph, ql, acc);
+            acc = product(pl, qh, acc);
+        }
+}
+// A 32 x 32 tile (lane l has column l % 32, rows 8 k + 4 (l / 32) + (0 .. 3); values times kHeld) as rows of its columns.
+__device__ __forceinline__ void thin_put(char *region, int row_i, int row_j, int lane, const float (&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        h4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f16_t x, y;
+            split(v[q * 4 + e], x, y);
+            hi[e] = x, lo[e] = y;
+        }
+        *reinterpret_cast<h4 *>(thin_piece(region, row_j + (lane & 31), row_i / 32, q) + (lane >> 5) * 8) = hi;
+        *reinterpret_cast<h4 *>(thin_piece(region, row_j + (lane & 31), row_i / 32, q + 4) + (lane >> 5) * 8) = lo;
+    }
+}
+
+enum { kThinFirst = 0, kThinStep = 1, kThinLast = 2 };   // X0 and its part of A; a step; the last step, into the result
+
+// turn: which of two sets of parts of A is written (the other is read).
+template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void thin_kernel(Group g, Step s, int turn) {
+    __shared__ __align__(1024) char ra[kThinRegion], rb[kThinRegion], rx[kThinRegion], rr[kThinRegion];
+    __shared__ float tile[kPhase == kThinFirst ? kThin : 1][kThin + 1];
+    __shared__ double part[kThreads / 64];
+    const int item = item_of(g, blockIdx.x);
+    const Item &t = g.t[item];
+    const Layout l = layout_of(t.m, t.n);
+    char *base = s.workspace + t.at, *xt = base + l.xt;
+    const int m = t.m, n = t.n, number = blockIdx.x - g.first[item], parts = g.first[item + 1] - g.first[item];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bi = wave / 2 * 32, bj = wave % 2 * 32, down = (m + 31) / 32;   // this wave's 32 x 32 of a tile; 32s of m
+    const int64_t pitch = pitch_of(m);
+    f32x4 *sums = reinterpret_cast<f32x4 *>(base + l.x);
+    const int part_size = down * down * 256;   // f32x4s: 4 to a lane of each 32 x 32
+    const int my_part = (bi / 32 * down + bj / 32) * 256 + lane;
+    const bool of_a = bi < m && bj < m;
+
+    float scale = 0.f;
+    if constexpr (kPhase == kThinFirst) {
+        const double *squares = reinterpret_cast<const double *>(base + l.sums);
+        const int chunks = (int)(((int64_t)m * n + kChunk - 1) / kChunk);
+        double sum = 0.;
+        for (int i = threadIdx.x; i < chunks; i += kThreads) sum += squares[i];
+        scale = (float)(kHeld / (sqrt(block_sum(sum, part)) + s.eps));
+    } else {
+        float a[16];
+        if (of_a) {
+            f32x4 v[4];
+            const f32x4 *from = sums + (int64_t)(turn ^ 1) * kThinParts * part_size + my_part;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = from[q * 64];
+#pragma unroll 5
+            for (int p = 1; p < parts; ++p)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] += from[(int64_t)p * part_size + q * 64];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) a[r] = v[r / 4][r % 4] * (1.f / kHeld);
+            thin_put(ra, bi, bj, lane, a);   // (symmetric)
+        }
+        __syncthreads();
+        if (of_a) {
+            f16x acc = (f16x)(0.f);
+            thin_product(ra, ra, bi, bj, down, lane, acc);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = bi + r / 4 * 8 + (lane >> 5) * 4 + r % 4, j = bj + (lane & 31);
+                a[r] = i < m && j < m ? acc[r] * (s.c / kHeld) + s.b * a[r] + (i == j ? s.a * kHeld : 0.f) : 0.f;
+            }
+            thin_put(rb, bi, bj, lane, a);
+        }
+    }
+
+    f16x gram = (f16x)(0.f);
+    const int across = (n + kThin - 1) / kThin;
+    const float lr = kPhase != kThinLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
+    for (int block = number; block < across; block += parts) {
+        const int j0 = block * kThin;
+        __syncthreads();   // (the last block's rows have been read)
+        if constexpr (kPhase == kThinFirst) {
+            // U's rows are X's, or its columns
+            const int rows = t.tall ? n : m, columns = t.tall ? m : n, r0 = t.tall ? j0 : 0, c0 = t.tall ? 0 : j0;
+#pragma unroll 4
+            for (int k = 0; k < kThin / 4; ++k) {
+                const int r = r0 + k * 4 + wave, c = c0 + lane;
+                float v = 0.f;
+                if (r < rows && c < columns) {
+                    const int64_t at = (int64_t)r * columns + c;
+                    v = load1(static_cast<const O *>(t.grad) + at);
+                    if (t.momentum) {
+                        const float b = t.momentum[at];
+                        v = s.nesterov ? v * s.kept + b * s.momentum : b;
+                    }
+                }
+                tile[k * 4 + wave][lane] = v * scale;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kThin * 8 / kThreads; ++k) {
+                const int which = k * kThreads + threadIdx.x, q = which % 8 * 8, r = which / 8;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = t.tall ? tile[r][q + e] : tile[q + e][r];   // column j0 + r of X
+                if (j0 + r < n && q < down * 32) store_pair8(xt + (j0 + r) * pitch, q, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = t.tall ? tile[q + e][r] : tile[r][q + e];   // row r of X
+                h8 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f16_t x, y;
+                    split(v[e], x, y);
+                    hi[e] = x, lo[e] = y;
+                }
+                *reinterpret_cast<h8 *>(thin_piece(rr, r, q / 32, q % 32 / 8)) = hi;
+                *reinterpret_cast<h8 *>(thin_piece(rr, r, q / 32, q % 32 / 8 + 4)) = lo;
+            }
+        } else {
+            for (int k = threadIdx.x; k < kThin * down * 8; k += kThreads) {
+                const int piece = k & 7, q = k / 8 % down, r = k / 8 / down;
+                *reinterpret_cast<u32x4 *>(thin_piece(rx, r, q, piece)) = *reinterpret_cast<const u32x4 *>(xt + min(j0 + r, n - 1) * pitch + q * kLine + piece * 16);
+            }
+            __syncthreads();
+            f16x acc = (f16x)(0.f);
+            if (bi < m) thin_product(rb, rx, bi, bj, down, lane, acc);
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = bi + r / 4 * 8 + (lane >> 5) * 4 + r % 4;
+                v[r] = i < m && j0 + bj + (lane & 31) < n ? acc[r] * (1.f / kHeld) : 0.f;
+            }
+            if constexpr (kPhase == kThinLast) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = bi + r / 4 * 8 + (lane >> 5) * 4 + r % 4, j = j0 + bj + (lane & 31);
+                    if (i >= m || j >= n) continue;
+                    const int64_t at = t.tall ? (int64_t)j * m + i : (int64_t)i * n + j;
+                    O *out = static_cast<O *>(t.out) + at;
+                    float x = v[r] * (1.f / kHeld);
+                    if (s.update) {
+                        x = (t.master ? t.master[at] : load1(out)) * decay - rate * x;
+                        if (t.master) t.master[at] = x;
+                    }
+                    store1(out, x);
+                }
+            } else {
+                __syncthreads();   // (rx has been read, its rows are the new ones from here on)
+                if (bi < down * 32) {
+                    thin_put(rx, bi, bj, lane, v);
+                    // the same as rows of X: the transposing read hands lane l of 16 lanes the l-th element of each of four rows
+                    const int group = lane >> 4, l16 = lane & 15;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int lo = 0; lo < 2; ++lo) {
+                            s16x4 x[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const char *p = thin_piece(rx, bj + group * 8 + k * 4 + (l16 >> 2), bi / 32, lo * 4 + half * 2 + (l16 >> 1 & 1)) + (l16 & 1) * 8;
+                                x[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)p);
+                            }
+                            const u32x2 y = __builtin_bit_cast(u32x2, x[0]), z = __builtin_bit_cast(u32x2, x[1]);
+                            *reinterpret_cast<u32x4 *>(thin_piece(rr, bi + half * 16 + l16, bj / 32, group + lo * 4)) = (u32x4){y[0], y[1], z[0], z[1]};
+                        }
+                }
+                __syncthreads();
+                for (int k = threadIdx.x; k < kThin * down * 8; k += kThreads) {
+                    const int piece = k & 7, q = k / 8 % down, r = k / 8 / down;
+                    if (j0 + r < n) *reinterpret_cast<u32x4 *>(xt + (j0 + r) * pitch + q * kLine + piece * 16) = *reinterpret_cast<const u32x4 *>(thin_piece(rx, r, q, piece));
+                }
+            }
+        }
+        if constexpr (kPhase != kThinLast) {
+            if (kPhase == kThinFirst) __syncthreads();
+            if (of_a) thin_product(rr, rr, bi, bj, 2, lane, gram);
+        }
+    }
+    if (kPhase != kThinLast && of_a) {
+        f32x4 *to = sums + ((int64_t)turn * kThinParts + number) * part_size + my_part;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) to[q * 64] = (f32x4){gram[q * 4], gram[q * 4 + 1], gram[q * 4 + 2], gram[q * 4 + 3]};
+    }
+}
+
 template <typename F> hipError_t by_type(int dtype, F &&f) {
     if (dtype == kBF16) f(bf16_t{});
     else if (dtype == kF16) f(f16_t{});
@@ -468,36 +700,70 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
     return hipGetLastError();
 }
 
-int tiles(int k, int tile) { return (k + tile - 1) / tile; }
+template <typename O> void launch_thin(hipStream_t st, Group &g, Step s, int steps, const double *coefficients) {
+    // (workgroups to a matrix: each of them reads all of their parts; 16 while there are few matrices)
+    int total = 0;
+    for (int i = 0; i < g.count; ++i) {
+        g.first[i] = total;
+        total += std::min({tiles(g.t[i].n, kThin), kThinParts, std::max(4, 512 / g.count)});
+    }
+    g.first[g.count] = total;
+    hipLaunchKernelGGL((thin_kernel<kThinFirst, O>), dim3(total), dim3(kThreads), 0, st, g, s, 0);
+    for (int step = 0; step < steps; ++step) {
+        s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
+        if (step + 1 < steps) hipLaunchKernelGGL((thin_kernel<kThinStep, O>), dim3(total), dim3(kThreads), 0, st, g, s, step & 1 ^ 1);
+        else hipLaunchKernelGGL((thin_kernel<kThinLast, O>), dim3(total), dim3(kThreads), 0, st, g, s, step & 1 ^ 1);
+    }
+}
 
-template <typename S, typename O> void launch_products(hipStream_t st, Group &by_n, Step s, int steps, const double *coefficients) {
+// One launch of products over all matrices of a group.
+template <typename S, int kMode, typename O> void launch_tiles(hipStream_t st, Group &g, const Step &s, int turn) {
+    int total = 0;
+    for (int i = 0; i < g.count; ++i) {
+        g.first[i] = total;
+        const int down = tiles(g.t[i].m, S::tile);
+        total += kMode <= kPoly ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
+    }
+    g.first[g.count] = total;
+    const int run = std::max(1, std::min(32, total / 16));
+    hipLaunchKernelGGL((product_kernel<S, kMode, O>), dim3((total + 8 * run - 1) / (8 * run) * 8 * run), dim3(S::threads), 0, st, g, s, turn, total, run);
+}
+
+int64_t tiles_of(const Group &g, int tile, bool symmetric) {
+    int64_t all = 0;
+    for (int i = 0; i < g.count; ++i) {
+        const int64_t down = tiles(g.t[i].m, tile);
+        all += symmetric ? down * (down + 1) / 2 : down * tiles(g.t[i].n, tile);
+    }
+    return all;
+}
+
+// The largest tiles of which there are enough.  Per operation a tile of 256 moves half of what one of 128 does, which counts where the chip's power sets the clock
+// (A, A A and B X of 12 matrices of 2048 x 2048 and 4 of 2048 x 7168 by 256 / by 128, in us: 833 529 1190 / 682 434 1250: the first two have 768 tiles of 256, the last 1856).
+// Of 128, two workgroups of two buffers to a compute unit; where there is no second, one of four (2048 x 2048, in us: 52 56 60 two, 47 50 54
+// one).  Fewer leave units idle: tiles of 64 (777 x 1311, in us: 25 21 20 by 128, 14 11 19 by 64 with eight buffers, 18 14 15 with four,
+// of which two workgroups fit).
+template <int kMode, typename O> void launch_products(hipStream_t st, Group &g, const Step &s, int turn) {
+    const bool symmetric = kMode <= kPoly;
+    const int64_t of_128 = tiles_of(g, 128, symmetric);
+    if (tiles_of(g, 256, symmetric) >= 1024) launch_tiles<TileShape<256, 2, 4, 1, 2>, kMode, O>(st, g, s, turn);
+    else if (of_128 > 256) launch_tiles<TileShape<128, 2, 2, 1, 2>, kMode, O>(st, g, s, turn);
+    else if (of_128 >= 128) launch_tiles<TileShape<128, 2, 2, 1, 4>, kMode, O>(st, g, s, turn);
+    else if (tiles_of(g, 64, symmetric) <= 256) launch_tiles<TileShape<64, 2, 2, 1, 8>, kMode, O>(st, g, s, turn);
+    else launch_tiles<TileShape<64, 2, 1, 2, 2>, kMode, O>(st, g, s, turn);
+}
+
+template <typename O> void launch_steps(hipStream_t st, Group &by_n, Step s, int steps, const double *coefficients) {
     // (the longest products first: what is begun last is done soon)
     Group by_m = by_n;
     std::sort(by_n.t, by_n.t + by_n.count, [](const Item &x, const Item &y) { return x.n != y.n ? x.n > y.n : x.at < y.at; });
     std::sort(by_m.t, by_m.t + by_m.count, [](const Item &x, const Item &y) { return x.m != y.m ? x.m > y.m : x.at < y.at; });
-    const auto units = [](Group &g, bool symmetric) {
-        int total = 0;
-        for (int i = 0; i < g.count; ++i) {
-            g.first[i] = total;
-            const int down = tiles(g.t[i].m, S::tile);
-            total += symmetric ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
-        }
-        g.first[g.count] = total;
-    };
-    const auto launch = [&](auto kernel, const Group &g, int turn) {
-        const int total = g.first[g.count];
-        const int run = std::max(1, std::min(32, total / 16));
-        hipLaunchKernelGGL(kernel, dim3((total + 8 * run - 1) / (8 * run) * 8 * run), dim3(S::threads), 0, st, g, s, turn, total, run);
-    };
     for (int step = 0; step < steps; ++step) {
         s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
-        units(by_n, true);
-        launch(product_kernel<S, kGram, float>, by_n, 0);
-        units(by_m, true);
-        launch(product_kernel<S, kPoly, float>, by_m, 0);
-        units(by_m, false);
-        if (step + 1 < steps) launch(product_kernel<S, kApply, float>, by_m, step & 1);
-        else launch(product_kernel<S, kLast, O>, by_m, step & 1);
+        launch_products<kGram, float>(st, by_n, s, 0);
+        launch_products<kPoly, float>(st, by_m, s, 0);
+        if (step + 1 < steps) launch_products<kApply, float>(st, by_m, s, step & 1);
+        else launch_products<kLast, O>(st, by_m, s, step & 1);
     }
 }
 
@@ -510,34 +776,40 @@ size_t muon_matrix_bytes(int64_t rows, int64_t columns) {
 hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matrices, const MuonStep &a, void *workspace, size_t workspace_bytes) {
     const Step s{(float)a.momentum, (float)(1. - a.momentum), a.nesterov, a.update, (float)a.eps, (float)a.weight_decay, (float)a.lr, a.lr_device, 0.f, 0.f, 0.f,
                  static_cast<char *>(workspace)};
-    for (int64_t at = 0; at < count;) {
+    // groups of either kind, as they fit into a launch's arguments and the workspace
+    int64_t next[2] = {0, 0};
+    for (int thin = 0; thin < 2;) {
         Group g{};
         size_t used = 0;
+        int64_t &at = next[thin];
         for (; at < count && g.count < kGroup; ++at) {
             const MuonMatrix &t = matrices[at];
-            if (t.rows == 0 || t.columns == 0) continue;
+            if (t.rows == 0 || t.columns == 0 || (std::min(t.rows, t.columns) <= kThin) != (thin == 1)) continue;
             const size_t bytes = muon_matrix_bytes(t.rows, t.columns);
             if (g.count > 0 && used + bytes > workspace_bytes) break;
             g.t[g.count++] = Item{t.grad, t.momentum, t.out, t.master, (int64_t)used, (int)std::min(t.rows, t.columns), (int)std::max(t.rows, t.columns), (float)t.rate,
                                   t.rows > t.columns};
             used += bytes;
         }
-        if (g.count == 0) break;
+        if (g.count == 0) {
+            ++thin;
+            continue;
+        }
         const hipError_t e = by_type(dtype, [&](auto type) {
             using O = decltype(type);
             int total = 0;
             for (int i = 0; i < g.count; ++i) g.first[i] = total, total += (int)(((int64_t)g.t[i].m * g.t[i].n + kChunk - 1) / kChunk);
             g.first[g.count] = total;
             hipLaunchKernelGGL((momentum_kernel<O>), dim3(total), dim3(kThreads), 0, st, g, s);
+            if (thin) {
+                launch_thin<O>(st, g, s, a.steps, a.coefficients);
+                return;
+            }
             total = 0;
             for (int i = 0; i < g.count; ++i) g.first[i] = total, total += tiles(g.t[i].m, kSpread) * tiles(g.t[i].n, kSpread);
             g.first[g.count] = total;
             hipLaunchKernelGGL((spread_kernel<O>), dim3(total), dim3(kThreads), 0, st, g, s);
-            int64_t large = 0;
-            for (int i = 0; i < g.count; ++i) large += (int64_t)tiles(g.t[i].m, 256) * tiles(g.t[i].n, 256);
-            if (large >= 256) launch_products<TileShape<256, 2, 4, 1>, O>(st, g, s, a.steps, a.coefficients);
-            else if (large >= 32) launch_products<TileShape<128, 2, 2, 1>, O>(st, g, s, a.steps, a.coefficients);
-            else launch_products<TileShape<64, 1, 1, 4>, O>(st, g, s, a.steps, a.coefficients);
+            launch_steps<O>(st, g, s, a.steps, a.coefficients);
         });
         if (e != hipSuccess) return e;
     }
