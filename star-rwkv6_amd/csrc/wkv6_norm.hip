@@ -4,7 +4,7 @@
 //   y = (s - m) q w + b
 //   backward, with h = (s - m) q and g' = g w:  ds = q (g' - mean(g') - h mean(g' h)) + what arrives at s,   dw = sum over tokens of g h,   db = sum of g
 //
-// A row is held in registers, by a wave up to 32 channels to a lane, by 256 or 1024 threads beyond: it is read once, and the squares are of differences from the mean
+// A row is held in registers, by a wave up to 16 channels to a lane, by 256 to 1024 threads beyond: it is read once, and the squares are of differences from the mean
 // that is already known (a sum of squares less the square of the sum loses what is small beside the mean).  Sums are fp32 within a row; those over
 // rows are fp32 within the rows that a wave takes one after the other, fp64 over the workgroups, always in the same order.
 #include "wkv6_common.h"
@@ -199,22 +199,20 @@ __global__ __launch_bounds__(kT == 64 ? kThreads : kT) void norm_backward_kernel
     if (!partial) return;
     float *out = partial + (int64_t)blockIdx.x * 2 * C;
     if constexpr (kT == 64) {
-        // the four waves' sums, one after the other
-        extern __shared__ float sums[];
-        for (int turn = 0; turn < kRows; ++turn) {
-            if (wave == turn) {
+        extern __shared__ float sums[];   // of the four waves
 #pragma unroll
-                for (int i = 0; i < kVecs; ++i)
+        for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-                    for (int e = 0; e < kE; ++e) {
-                        const int at = (i * 64 + tid) * kE + e;
-                        if (at >= C) continue;
-                        if (turn > 0) dw[i][e] += sums[at], db[i][e] += sums[C + at];
-                        if (turn < kRows - 1) sums[at] = dw[i][e], sums[C + at] = db[i][e];
-                        else out[at] = dw[i][e], out[C + at] = db[i][e];
-                    }
+            for (int e = 0; e < kE; ++e) {
+                const int at = (i * 64 + tid) * kE + e;
+                if (at < C) sums[wave * 2 * C + at] = dw[i][e], sums[wave * 2 * C + C + at] = db[i][e];
             }
-            __syncthreads();
+        __syncthreads();
+        for (int at = threadIdx.x; at < 2 * C; at += kThreads) {
+            float v = sums[at];
+#pragma unroll
+            for (int k = 1; k < kRows; ++k) v += sums[k * 2 * C + at];
+            out[at] = v;
         }
     } else {
 #pragma unroll
@@ -233,32 +231,42 @@ __device__ __forceinline__ void store_param(void *p, int type, int64_t at, float
     else store1(static_cast<f16_t *>(p) + at, v);
 }
 
-// The sums over workgroups of 64 columns of (weight's gradient, bias's gradient).
+// The sums over workgroups of 64 columns of (weight's gradient, bias's gradient): 4 columns to a lane, 64 workgroups' sums at a time.
 __global__ __launch_bounds__(kFinish) void norm_finish_kernel(NormGrad a, const float *partial, int blocks) {
-    __shared__ double part[kFinish / 64][64];
+    constexpr int kW = kFinish / 64, kAtOnce = 4, kEach = 4;
+    __shared__ double part[kW][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t column = (int64_t)blockIdx.x * 64 + lane, width = 2 * a.C;
-    double s = 0.;
-    if (column < width) {
-        constexpr int kStep = 8 * (kFinish / 64);
-        for (int first = wave; first < blocks; first += kStep) {
-            float v[8];
+    const int64_t width = 2 * a.C, column = (int64_t)blockIdx.x * 64 + lane % 16 * kEach;
+    const int n = (int)min(width - column, (int64_t)kEach);
+    double s[kEach] = {};
+    for (int first = wave * 4 + lane / 16; first < blocks; first += kAtOnce * kW * 4) {
+        Piece<float, kEach> b[kAtOnce];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int b = first + k * (kFinish / 64);
-                v[k] = b < blocks ? partial[b * width + column] : 0.f;
-            }
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int row = first + k * kW * 4;
+            b[k].template load<false>(partial + min(row, blocks - 1) * width + column, row < blocks ? n : 0);
+        }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += v[k];
+        for (int k = 0; k < kAtOnce; ++k) {
+            float v[kEach];
+            unpack(b[k], v);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) s[e] += v[e];
         }
     }
-    part[wave][lane] = s;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        s[e] += __shfl_xor(s[e], 16);
+        s[e] += __shfl_xor(s[e], 32);
+        if (lane < 16) part[wave][lane * kEach + e] = s[e];
+    }
     __syncthreads();
-    if (wave != 0 || column >= width) return;
-    s = 0.;
-    for (int i = 0; i < kFinish / 64; ++i) s += part[i][lane];
-    void *out = column < a.C ? a.gweight : a.gbias;
-    if (out) store_param(out, a.param_type, column < a.C ? column : column - a.C, (float)s);
+    const int64_t mine = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || mine >= width) return;
+    double sum = 0.;
+    for (int i = 0; i < kW; ++i) sum += part[i][threadIdx.x];
+    void *out = mine < a.C ? a.gweight : a.gbias;
+    if (out) store_param(out, a.param_type, mine < a.C ? mine : mine - a.C, (float)sum);
 }
 
 template <int T, int V, bool W> struct Shape {
@@ -266,11 +274,13 @@ template <int T, int V, bool W> struct Shape {
     static constexpr bool whole = W;
 };
 
-// By the number of channels: threads that a row is spread over, and 16-byte pieces of the stream's type to a thread.
+// By the number of channels: threads that a row is spread over, and 16-byte pieces of the stream's type to a thread.  (Few to a thread: the backward's sums and the
+// weights take three registers a channel, and four workgroups or more to a compute unit keep the memory busy.  8192 rows of 2048, a stream in fp32 and branches in bf16,
+// backward, in us: 64 threads to a row 61 to 74, 128 49, 256 47.)
 template <int kE, bool kWhole, typename F> void by_width(int64_t C, F &&f) {
     if (C <= 64 * 8) f(Shape<64, 8 / kE, kWhole>{});
     else if (C <= 64 * 16) f(Shape<64, 16 / kE, kWhole>{});
-    else if (C <= 64 * 32) f(Shape<64, 32 / kE, kWhole>{});
+    else if (C <= 256 * 8) f(Shape<256, 8 / kE, kWhole>{});
     else if (C <= 256 * 16) f(Shape<256, 16 / kE, kWhole>{});
     else if (C <= 256 * 32) f(Shape<256, 32 / kE, kWhole>{});
     else if (C <= 512 * 32) f(Shape<512, 32 / kE, kWhole>{});
@@ -293,7 +303,7 @@ template <typename F> hipError_t by_types(int stream, int branch, F &&f) {
 }
 
 int backward_blocks(int64_t rows, int64_t C) {
-    const int64_t at_once = C <= 64 * 32 ? kThreads / 64 : 1, all = (rows + at_once - 1) / at_once;
+    const int64_t at_once = C <= 64 * 16 ? kThreads / 64 : 1, all = (rows + at_once - 1) / at_once;
     return (int)(all < 512 ? all : 512);
 }
 
@@ -321,7 +331,7 @@ hipError_t layer_norm_backward(hipStream_t st, int dtype, int branch_dtype, cons
         by_width<decltype(s)>(a.C, [&](auto shape) {
             constexpr int kT = decltype(shape)::threads;
             hipLaunchKernelGGL((norm_backward_kernel<decltype(s), decltype(y), kT, decltype(shape)::vecs, decltype(shape)::whole>), dim3(blocks),
-                               dim3(kT == 64 ? kThreads : kT), kT == 64 ? 2 * a.C * sizeof(float) : 0, st, a, partial);
+                               dim3(kT == 64 ? kThreads : kT), kT == 64 ? kThreads / 64 * 2 * a.C * sizeof(float) : 0, st, a, partial);
         });
     });
     if (e != hipSuccess || !params) return e;

@@ -62,7 +62,7 @@ def _formula(x, add, weight, bias, eps, gy, gtotal):
     if gtotal is not None:
         t = gtotal.detach().cpu().double().reshape(rows, C)
         gx, off = gx + t, off + 2 * U * (gx.abs() + t.abs())
-    steps = rows / (2048 if C <= 2048 else 512) + 16
+    steps = rows / (2048 if C <= 1024 else 512) + 16
     out["gx"] = out["gadd"] = (gx, off)
     out["gweight"] = ((g * h).sum(0), (g.abs() * h_off).sum(0) + steps * U * (g * h).abs().sum(0))
     out["gbias"] = (g.sum(0), steps * U * g.abs().sum(0))
