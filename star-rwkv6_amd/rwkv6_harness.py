@@ -33,6 +33,33 @@ def time_shift(x):
     return F.pad(x, (0, 0, 1, 0))[:, :-1, :] - x
 
 
+def _kernels(x):
+    """The operator package where it has kernels for this tensor (its torch flavour, on the GPU, in 16 or 32 bits), else None."""
+    if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or os.environ.get("KERAS_BACKEND") != "torch":
+        return None
+    import rwkv_kernel
+
+    return rwkv_kernel
+
+
+def _bf16_autocast():
+    return torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16
+
+
+def add_norm(x, branch, norm, rounded=False):
+    """(x + branch, the norm of it), in one kernel where the package has it; branch None: (x, the norm of x).  rounded: under bf16 autocast the norm's readers
+    round it to bf16, and it comes out so there."""
+    kernels, autocast = _kernels(x), torch.is_autocast_enabled('cuda')
+    if kernels is None or type(norm) is not nn.LayerNorm or (x.dtype != torch.float32 and (autocast or (branch is not None and branch.dtype != x.dtype))):
+        x = x if branch is None else x + branch
+        return x, norm(x)
+    dtype = torch.bfloat16 if rounded and _bf16_autocast() else x.dtype
+    if branch is None:
+        return x, kernels.layer_norm(x, norm.weight, norm.bias, norm.eps, dtype=dtype)
+    h, x = kernels.layer_norm(x, norm.weight, norm.bias, norm.eps, add=branch, dtype=dtype)
+    return x, h
+
+
 class DecomposerDense(nn.Module):
     def __init__(self, hidden_size, decomposer_size, use_bias=False):
         super().__init__()
@@ -84,6 +111,10 @@ class TimeMix(nn.Module):
         with torch.no_grad():
             self.dense_w.dense_b.bias.uniform_(-6.0, 1.0)
 
+    def rounds_its_input(self):
+        """Whether the input is only read in bf16 under bf16 autocast on the GPU: by the library's input side."""
+        return hasattr(self.rwkv_kernel, "shift_mix") and self.hidden_size % 64 == 0 and self.dense_xr.dense_a.out_features in (32, 64)
+
     def _mixed_inputs(self, x):
         """xr, xk, xv, xw, xg of rwkv6_model.py:134-145."""
         mixers = (self.dense_xr, self.dense_xk, self.dense_xv, self.dense_xw, self.dense_xg)
@@ -134,6 +165,9 @@ class ChannelMix(nn.Module):
         self.dense_value = nn.Linear(expand_size, hidden_size, bias=False)
         self.dense_receptance = nn.Linear(hidden_size, hidden_size, bias=False)
 
+    def rounds_its_input(self):
+        return hasattr(self.rwkv_kernel, "shift_mix_x") and self.time_mix_k.numel() % 64 == 0
+
     def forward(self, x):
         fused = getattr(self.rwkv_kernel, "shift_mix_x", None)
         if fused is not None and x.is_cuda and torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16 \
@@ -156,9 +190,15 @@ class Block(nn.Module):
         self.time_mix = TimeMix(rwkv_kernel, hidden_size, decomposer_size, head_size)
         self.channel_mix = ChannelMix(hidden_size, expand_size, rwkv_kernel)
 
+    def stages(self, x, branch, mask=None):
+        """From the stream and the branch that the layer before leaves (or None) to those of this one: each addition goes with the norm that follows it."""
+        x, h = add_norm(x, branch, self.layer_norm_att, self.time_mix.rounds_its_input())
+        x, h = add_norm(x, self.time_mix(h, mask), self.layer_norm_ffn, self.channel_mix.rounds_its_input())
+        return x, self.channel_mix(h)
+
     def forward(self, x, mask=None):
-        x = x + self.time_mix(self.layer_norm_att(x), mask)
-        return x + self.channel_mix(self.layer_norm_ffn(x))
+        x, branch = self.stages(x, None, mask)
+        return x + branch
 
 
 class RWKV6(nn.Module):
@@ -176,19 +216,14 @@ class RWKV6(nn.Module):
         nn.init.normal_(self.embedding.weight, std=0.02)
 
     def forward(self, ids, mask=None):
-        x = self.embedding_ln(self.embedding(ids))
+        table = self.embedding
+        plain = type(table) is nn.Embedding and table.padding_idx is None and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq
+        kernels = _kernels(table.weight) if plain else None
+        x = table(ids) if kernels is None else kernels.embedding(ids.long(), table.weight)
+        x, branch = add_norm(x, None, self.embedding_ln)[1], None
         for blk in self.blocks:
-            x = blk(x, mask)
-        return self.output_layer(self.output_ln(x))
-
-
-def _kernels(logits):
-    """The operator package where it has losses for these logits (its torch flavour, on the GPU, in 16 or 32 bits), else None."""
-    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32) or os.environ.get("KERAS_BACKEND") != "torch":
-        return None
-    import rwkv_kernel
-
-    return rwkv_kernel
+            x, branch = blk.stages(x, branch, mask)
+        return self.output_layer(add_norm(x, branch, self.output_ln, rounded=True)[1])
 
 
 def _losses(logits):
@@ -221,6 +256,32 @@ def train_step(model, optimizer, ids, autocast_dtype=None):
             logits, target = logits.reshape(-1, logits.shape[-1]), target.reshape(-1)
         return _update(optimizer, kernels.cross_entropy(logits, target.long()))
     return _update(optimizer, F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), target.reshape(-1)))
+
+
+class Optimizers:
+    """Several optimizers, of a model's parameters each a part, as one."""
+
+    def __init__(self, *optimizers):
+        self.optimizers = optimizers
+
+    def zero_grad(self, set_to_none=True):
+        for optimizer in self.optimizers:
+            optimizer.zero_grad(set_to_none=set_to_none)
+
+    def step(self):
+        for optimizer in self.optimizers:
+            optimizer.step()
+
+
+def muon_and_adamw(model, lr=0.02, weight_decay=0.0, adamw_lr=1e-4, **options):
+    """The package's Muon for the weight matrices of the model's layers and its AdamW for the rest (embedding, norms, biases, mixes, output layer), as one
+    optimizer for the steps here.  options as of rwkv_kernel.Muon."""
+    from rwkv_kernel import AdamW, Muon
+
+    matrices = [m.weight for m in model.blocks.modules() if isinstance(m, nn.Linear)]
+    others = {id(p) for p in matrices}
+    others = [p for p in model.parameters() if id(p) not in others]
+    return Optimizers(Muon(matrices, lr=lr, weight_decay=weight_decay, **options), AdamW(others, lr=adamw_lr, weight_decay=weight_decay))
 
 
 # Fine-tuning steps on the operator package's losses (its torch flavour, on the GPU).  Texts are ids (B, T+1); mask (B, T) says which of

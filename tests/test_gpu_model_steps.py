@@ -1,0 +1,144 @@
+"""The model with the package's embedding and layer norms, trained with its losses and Muon: against the same model in float64 on the CPU, whose operator is the python loop."""
+import copy
+
+import pytest
+import torch
+
+import rwkv6_harness as hz
+import rwkv_kernel
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+B, T, V = 2, 40, 300
+CONFIG = dict(num_layers=2, vocabulary_size=V, hidden_size=128, decomposer_size=32, head_size=64, expand_size=256)
+
+
+def _models(seed=1):
+    torch.manual_seed(seed)
+    plain = hz.RWKV6(rwkv_kernel.OPSKernelOperator(64, T), **CONFIG)
+    ours = hz.RWKV6(rwkv_kernel.RWKVKernelOperator(64, T), **CONFIG)
+    ours.load_state_dict(plain.state_dict())
+    return plain.double(), ours.cuda()
+
+
+def _ids(seed=2):
+    return torch.randint(0, V, (B, T + 1), generator=torch.Generator().manual_seed(seed))
+
+
+def _calls(monkeypatch):
+    """How often the model's steps call the package's functions."""
+    seen = {}
+    for name in ("embedding", "layer_norm", "cross_entropy"):
+        def counted(*a, _f=getattr(rwkv_kernel, name), _n=name, **k):
+            seen[_n] = seen.get(_n, 0) + 1
+            return _f(*a, **k)
+        monkeypatch.setattr(rwkv_kernel, name, counted)
+    return seen
+
+
+def test_forward_and_gradients_in_fp32(monkeypatch):
+    """Everything in fp32: values and gradients of a loss within 2^-12 of the largest of a tensor (some 100 roundings of 2^-24 on the way, and the operator's own
+    1e-4 of its largest value)."""
+    seen = _calls(monkeypatch)
+    plain, ours = _models()
+    ids = _ids()
+    w = torch.randn(B, T, V, generator=torch.Generator().manual_seed(3)).double()
+    a, b = plain(ids[:, :-1]), ours(ids[:, :-1].cuda())
+    assert seen == {"embedding": 1, "layer_norm": 2 + 2 * CONFIG["num_layers"]}
+    assert float((b.cpu().double() - a).detach().abs().max()) <= 2.0 ** -12 * float(a.detach().abs().max())
+    (a * w).sum().backward()
+    (b * w.float().cuda()).sum().backward()
+    for (name, p), q in zip(plain.named_parameters(), ours.parameters()):
+        assert float((q.grad.cpu().double() - p.grad).abs().max()) <= 2.0 ** -10 * float(p.grad.abs().max()) + 1e-9, name
+
+
+def test_blocks_are_the_stages():
+    _, ours = _models()
+    x = torch.randn(B, T, 128, generator=torch.Generator().manual_seed(5)).cuda()
+    with torch.no_grad():
+        y, branch = ours.blocks[0].stages(x, None)
+        assert torch.equal(ours.blocks[0](x), y + branch)
+        z, branch = ours.blocks[1].stages(y, branch)
+        want = ours.blocks[1](ours.blocks[0](x))
+    assert float((z + branch - want).abs().max()) <= 2.0 ** -20 * float(want.abs().max())   # (one kernel adds what two added)
+
+
+def test_norms_under_autocast():
+    """The norms come out in bf16 where their readers round them: the logits are those of the model whose norms are torch's, to the bit wherever no fp32 value lies next
+    to the middle between two of bf16; half a step of bf16 (2^-9) of the largest value is left for those."""
+    _, ours = _models()
+    plain = copy.deepcopy(ours)
+
+    class Own(torch.nn.LayerNorm):   # (not the class that the package's kernel stands in for)
+        pass
+
+    for module in list(plain.modules()):
+        for name, child in list(module.named_children()):
+            if type(child) is torch.nn.LayerNorm:
+                own = Own(child.normalized_shape, eps=child.eps).cuda()
+                own.load_state_dict(child.state_dict())
+                setattr(module, name, own)
+    ids = _ids().cuda()[:, :-1]
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16):
+        a, b = ours(ids).float(), plain(ids).float()
+    assert float((a - b).abs().max()) <= 2.0 ** -6 * float(b.abs().max())
+    assert float((a - b).norm()) <= 2.0 ** -8 * float(b.norm())
+
+
+@pytest.mark.parametrize("dtype", [None, BF16])
+def test_steps_with_muon(dtype, monkeypatch):
+    """Three steps: each matrix of the layers gets the step that muon_step makes of its gradient and momentum, everything else AdamW's, and the loss is finite."""
+    seen = _calls(monkeypatch)
+    _, ours = _models()
+    opt = hz.muon_and_adamw(ours, lr=0.01, weight_decay=0.1, adamw_lr=1e-3)
+    muon, adamw = opt.optimizers
+    matrices = [p for g in muon.param_groups for p in g["params"]]
+    others = [p for g in adamw.param_groups for p in g["params"]]
+    assert len(matrices) + len(others) == len(list(ours.parameters())) and all(p.dim() == 2 for p in matrices)
+    assert any(p is ours.embedding.weight for p in others) and any(p is ours.output_layer.weight for p in others)
+    for step in range(3):
+        before = [p.detach().clone() for p in matrices]
+        bufs = [muon.state[p]["momentum"].clone() if step else torch.zeros_like(p) for p in matrices]
+        rest = [p.detach().clone() for p in others]
+        loss = hz.train_step(ours, opt, _ids(10 + step).cuda(), dtype)
+        assert bool(loss.isfinite())
+        rwkv_kernel.muon_step(before, [p.grad for p in matrices], bufs, 0.01, weight_decay=0.1)
+        assert all(torch.equal(p, q) for p, q in zip(before, matrices))
+        assert not any(torch.equal(p, q) for p, q in zip(rest, others) if p.numel() > 1)
+    assert seen == {"embedding": 3, "layer_norm": 3 * (2 + 2 * CONFIG["num_layers"]), "cross_entropy": 3}
+
+
+def test_a_captured_step():
+    """Forward, backward and both optimizers in one graph, replayed, against the same steps taken one by one."""
+    print("training step with Muon, captured", flush=True)
+    _, ours = _models()
+    twin = copy.deepcopy(ours)
+    opts = [hz.muon_and_adamw(m, lr=0.01) for m in (ours, twin)]
+    ids = [_ids(20).cuda() for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step(model, opt, x):
+        for p in model.parameters():
+            p.grad = None
+        loss = rwkv_kernel.cross_entropy(model(x[:, :-1]), x[:, 1:])
+        loss.backward()
+        opt.step()
+        return loss
+
+    with torch.cuda.stream(side):
+        step(ours, opts[0], ids[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = step(ours, opts[0], ids[0])
+    torch.cuda.current_stream().wait_stream(side)
+    step(twin, opts[1], ids[1])
+    for k in range(3):
+        for x in ids:
+            x.copy_(_ids(30 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(twin, opts[1], ids[1])
+        assert torch.equal(loss, want)
+        for (name, p), q in zip(ours.named_parameters(), twin.parameters()):
+            assert torch.equal(p, q), name
