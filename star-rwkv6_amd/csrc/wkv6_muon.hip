@@ -288,6 +288,8 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         h8 ph[kMT], qh[kNT], ql[kNT], pl[kMT];
     };
     constexpr int kReads = 2 * (kMT + kNT), kProducts = 3 * kMT * kNT;
+    // (reads in the first two thirds: what comes last has to arrive before the half ends; loads in the last two)
+    constexpr int kMost = kProducts * 2 / 3;
     const auto read = [&](Half &h, int round, int half, int which) {
         const char *stage = lds + round % S::buffers * S::stage_bytes + set * S::set_bytes;
         const char *p = stage + (row_i + (lane & 31)) * kLine, *q = stage + (T + row_j + (lane & 31)) * kLine;
@@ -321,7 +323,8 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
 #pragma unroll
         for (int o = 0; o < kProducts; ++o) {
 #pragma unroll
-            for (int k = o * kReads / kProducts; k < (o + 1) * kReads / kProducts; ++k) read(second, round, 1, k);
+            for (int k = 0; k < kReads; ++k)
+                if (k * kProducts / kReads == o) read(second, round, 1, k);
             multiply(first, o);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -329,9 +332,11 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
 #pragma unroll
         for (int o = 0; o < kProducts; ++o) {
 #pragma unroll
-            for (int k = o * kReads / kProducts; k < (o + 1) * kReads / kProducts; ++k) read(first, round + 1, 0, k);
+            for (int k = 0; k < kReads; ++k)
+                if (k * kProducts / kReads == o) read(first, round + 1, 0, k);
 #pragma unroll
-            for (int k = o * kOctets / kProducts; k < (o + 1) * kOctets / kProducts; ++k) load(round + S::buffers, k);
+            for (int k = 0; k < kOctets; ++k)
+                if (k * kMost / kOctets == o) load(round + S::buffers, k);
             multiply(second, o);
             __builtin_amdgcn_sched_barrier(0);
         }
