@@ -757,11 +757,15 @@ Tensors orthogonalize(const Tensors &matrices, const std::vector<double> &coeffi
   Tensors res;
   if (matrices.empty()) return res;
   const Tensor &first = matrices[0];
+  const bool graph_wanted = at::GradMode::is_enabled();
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(first.device());
   Tensors kept;
   std::vector<wkv6_muon_matrix> rows;
-  for (const Tensor &m : matrices) check_matrix(m, first, "matrices");
+  for (const Tensor &m : matrices) {
+    check_matrix(m, first, "matrices");
+    TORCH_CHECK(!graph_wanted || !m.requires_grad(), "wkv6: orthogonalize has no derivative: detach what requires a gradient");
+  }
   for (const Tensor &m : matrices) {
     kept.push_back(m.contiguous());
     res.push_back(at::empty(m.sizes(), m.options()));

@@ -29,7 +29,8 @@ def _coefficients(coefficients, steps):
 
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """X = G / (|G| + eps) with |G| the 2-norm of all elements, then `steps` times X = a X + b A X + c A A X with A = X X^T (of a matrix with more rows than columns its
-    transpose's, transposed): the singular vectors of G with singular values near 1.  Not differentiable.
+    transpose's, transposed): the singular vectors of G with singular values near 1.  Without a
+    derivative: a matrix that requires a gradient is refused where gradients are recorded.
 
     matrices: a tensor (.., rows, columns), or a list of such, of one dtype and any shapes; they go through together.  Returns the same in new tensors of
     their dtype.  coefficients: (a, b, c), or one such triple for each step; what leaves the range of +-64 on the way (not with coefficients that keep singular

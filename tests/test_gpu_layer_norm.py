@@ -253,6 +253,41 @@ def test_empty_and_refused():
         g.sum().backward()
 
 
+def test_added_to_itself():
+    """layer_norm(x, add=x): x gets both gradients."""
+    for dtype in (F32, BF16):
+        x, _, w, b, gy, gt = _inputs((21, 200), dtype, dtype, F32, True, 3)
+        want = _formula(x, x, w, b, 1e-5, gy, gt)
+        leaf = x.detach().requires_grad_(True)
+        gx, = torch.autograd.grad(rwkv_kernel.layer_norm(leaf, w, b, add=leaf), leaf, [gy, gt])
+        value, off = want["gx"]
+        _check("gx", gx, 2 * value, 2 * (off + _round(value.abs() + off, dtype)))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows are those of a call of their own, and the sums over rows those of its parts."""
+    print("layer norm, 2^31 elements", flush=True)
+    rows, C = 70000, 32768
+    x = torch.zeros(rows, C, dtype=BF16, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    x[-3:], x[0] = torch.randn(3, C, generator=g).to(BF16).cuda(), torch.randn(C, generator=g).to(BF16).cuda()
+    w = torch.randn(C, generator=g).cuda()
+    gy = torch.zeros(rows, C, dtype=BF16, device="cuda")
+    gy[-3:] = torch.randn(3, C, generator=g).to(BF16).cuda()
+    some = [0, rows - 3, rows - 2, rows - 1]
+
+    def run(x, gy):
+        leaf, weight = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = rwkv_kernel.layer_norm(leaf, weight)
+        return (y.detach(), *torch.autograd.grad(y, (leaf, weight), gy))
+
+    y, gx, gw = run(x, gy)
+    y4, gx4, gw4 = run(x[some], gy[some])
+    assert torch.equal(y[some], y4) and torch.equal(gx[some], gx4)
+    assert float((gw - gw4).abs().max()) <= 8 * U * float((gy[some].float().abs() * 8).sum(0).max())
+    assert not bool(y[1:-3].view(-1).view(torch.int16).any())
+
+
 def test_captured_and_on_another_stream():
     print("layer norm, captured", flush=True)
     x, a, w, b, gy, gt = _inputs((300, 512), F32, BF16, F32, True, 7)

@@ -116,6 +116,60 @@ def test_large(count, m, n):
             _check(o, x)
 
 
+@pytest.mark.parametrize("m,n", [(1, 50000), (20, 70001), (64, 100000), (60000, 33), (65, 60000)])
+def test_long_and_thin(m, n):
+    print("orthogonalize", m, n, flush=True)
+    x = _matrix(m, n, 4, "normal")
+    _check(rwkv_kernel.orthogonalize(x), x)
+
+
+def test_more_than_the_workspace_holds_at_once():
+    """30 matrices of 2048 x 2048 go through in parts; and matrices through the C interface with room for one at a time, or for two."""
+    print("orthogonalize, in parts", flush=True)
+    xs = [_matrix(2048, 2048, i, "normal", BF16) for i in range(3)] * 10
+    out = rwkv_kernel.orthogonalize(xs)
+    for i in range(3):
+        _check(out[i], xs[i])
+        assert torch.equal(out[27 + i], rwkv_kernel.orthogonalize(xs)[27 + i])
+    del xs, out
+    from rwkv_kernel import _native
+
+    lib = _native.load()
+    ys = [_matrix(200, 300, 1), _matrix(300, 100, 2), _matrix(40, 500, 3), _matrix(200, 300, 4), _matrix(3, 3, 5)]
+    rows = (_native.MuonMatrix * len(ys))()
+    outs = [torch.zeros_like(y) for y in ys]
+    for r, y, o in zip(rows, ys, outs):
+        r.grad, r.out, r.rows, r.columns = y.data_ptr(), o.data_ptr(), y.shape[0], y.shape[1]
+    import ctypes
+    triples = (ctypes.c_double * 15)(*(list(COEFFICIENTS) * 5))
+    all_ = lib.wkv6_muon_workspace_bytes(len(ys), rows)
+    one = max(lib.wkv6_muon_workspace_bytes(1, ctypes.byref(r)) for r in rows)
+    assert one < all_
+    for n in (all_, one, (one + all_) // 2):
+        ws = torch.full((n + 4096,), 0x7F, dtype=torch.uint8, device="cuda")
+        assert lib.wkv6_orthogonalize(torch.cuda.current_stream().cuda_stream, 2, len(ys), rows, 5, triples, 1e-7, ws.data_ptr(), n) == 0
+        torch.cuda.synchronize()
+        assert bool((ws[n:] == 0x7F).all())
+        for y, o in zip(ys, outs):
+            _check(o, y)
+            o.zero_()
+
+
+def test_two_streams_at_once():
+    print("orthogonalize, two streams", flush=True)
+    xs = [_matrix(300, 500, i) for i in range(2)]
+    want = [rwkv_kernel.orthogonalize(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(rwkv_kernel.orthogonalize(xs[k]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for g, w in zip(got, want) for o in g)
+
+
 def test_views():
     x = _matrix(50, 120, 1)
     big = torch.zeros(60, 130, device="cuda")
@@ -227,7 +281,7 @@ def test_refused():
         with pytest.raises(AssertionError):
             call()
     for call in (lambda: rwkv_kernel.orthogonalize(w.double()), lambda: rwkv_kernel.orthogonalize(w[0]), lambda: rwkv_kernel.orthogonalize([w, w.to(BF16)]),
-                 lambda: rwkv_kernel.orthogonalize([w, w.cpu()]), lambda: step(p=w.t()[:, :4], g=w[:, :4], m=w[:, :4].contiguous()), lambda: step(m=w.to(BF16)),
+                 lambda: rwkv_kernel.orthogonalize([w, w.cpu()]), lambda: rwkv_kernel.orthogonalize(w.clone().requires_grad_(True)), lambda: step(p=w.t()[:, :4], g=w[:, :4], m=w[:, :4].contiguous()), lambda: step(m=w.to(BF16)),
                  lambda: step(g=w.to(BF16)), lambda: step(m=w), lambda: rwkv_kernel.muon_step([w, w.clone()], [w.clone()] * 2, [w.clone(), w], 0.1),
                  lambda: step(masters=[w.clone()]), lambda: step(lr=torch.ones(1)), lambda: rwkv_kernel.muon_step([], [], [], 0.1)):
         with pytest.raises(RuntimeError):
