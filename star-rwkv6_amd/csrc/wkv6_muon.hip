@@ -11,8 +11,9 @@
 // 64 is not left by coefficients of any use, and lo keeps its bits down to 2^-13 of 1 (below, the pair is exact to 2^-35).
 //
 // A pair's row of K numbers: for every 32 of them 64 bytes of hi, then 64 of lo; zeros behind the last.  So what the matrix instructions take of a row
-// in one stage is one line of 128 bytes.  All products are of rows by rows (X is kept beside its transpose): C_ij = sum_k P_ik Q_jk.  A and
-// A A are symmetric: only the tiles on and above the diagonal are computed, and each is written to both of its places.  B has a I in it, so that B X is the whole step.
+// in one stage is one line of 128 bytes.  A and A A are products of rows by rows, C_ij = sum_k P_ik Q_jk, and symmetric: only the tiles on and above the diagonal are
+// computed, and each is written to both of its places.  Of B X the columns of X are multiplied with rows of B; LDS hands them out across its rows.
+// B has a I in it, so that B X is the whole step.
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 #include "wkv6_mfma.h"
@@ -61,17 +62,17 @@ struct Step {
 static_assert(sizeof(Group) + sizeof(Step) + 64 <= 4096, "a launch's arguments");
 
 __host__ __device__ inline int64_t pitch_of(int k) { return (int64_t)((k + 31) / 32) * kLine; }
-// What a matrix has in the workspace: X, its transpose twice (one is read while the other is written), A, B, sums of squares.
+// What a matrix has in the workspace: X twice (one is read while the other is written), with zeros in rows up to a multiple of 32, A, B, sums of squares.  Of a matrix of at
+// most 64 rows: the parts of A, two times 16 of 4 KB for each 32 x 32, and X's transpose.
 struct Layout {
-    int64_t x, xt, xt_other, a, b, sums, end;
+    int64_t x, x_other, a, b, sums, end;
 };
 __host__ __device__ inline Layout layout_of(int m, int n) {
     Layout l;
+    const int down = (m + 31) / 32;
     l.x = 0;
-    // (of a matrix of at most 64 rows: the parts of A instead of X, two times 16 of 4 KB for each 32 x 32)
-    l.xt = l.x + (m <= 64 ? (int64_t)((m + 31) / 32) * ((m + 31) / 32) * (2 * 16 * 4096) : m * pitch_of(n));
-    l.xt_other = l.xt + n * pitch_of(m);
-    l.a = l.xt_other + n * pitch_of(m);
+    l.x_other = l.x + (m <= 64 ? (int64_t)down * down * (2 * 16 * 4096) : down * 32 * pitch_of(n));
+    l.a = l.x_other + (m <= 64 ? n * pitch_of(m) : down * 32 * pitch_of(n));
     l.b = l.a + m * pitch_of(m);
     l.sums = l.b + m * pitch_of(m);
     l.end = l.sums + ((int64_t)m * n + kChunk - 1) / kChunk * 8;
@@ -157,7 +158,7 @@ __device__ __forceinline__ void store_pair8(char *row, int k, const float (&v)[8
 
 constexpr int kSpread = 64;   // rows and columns of U that a workgroup takes
 
-// U over its norm as a pair, and its transpose.
+// U over its norm as a pair: X, or of a matrix with more rows than columns its transpose.
 template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(Group g, Step s) {
     __shared__ double part[kThreads / 64];
     __shared__ float tile[kSpread][kSpread + 1];
@@ -188,21 +189,18 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
         tile[i * 4 + wave][lane] = v * scale;
     }
     __syncthreads();
-    char *straight = base + (t.tall ? l.xt : l.x), *across_to = base + (t.tall ? l.x : l.xt);
+    // rows from x0 of X on, pieces of 8 columns from y0 on; the rows behind the last are zero here and in the other X
+    const int x0 = t.tall ? c0 : r0, y0 = t.tall ? r0 : c0;
+    const int64_t pitch = pitch_of(t.n);
 #pragma unroll
     for (int i = 0; i < kSpread * 8 / kThreads; ++i) {
         const int which = i * kThreads + threadIdx.x, q = which % 8 * 8, r = which / 8;
+        if (x0 + r >= (t.m + 31) / 32 * 32 || y0 + q >= (t.n + 31) / 32 * 32) continue;
         float v[8];
-        if (r0 + r < rows && c0 + q < (columns + 31) / 32 * 32) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[r][q + e];
-            store_pair8(straight + (r0 + r) * pitch_of(columns), c0 + q, v);
-        }
-        if (c0 + r < columns && r0 + q < (rows + 31) / 32 * 32) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[q + e][r];
-            store_pair8(across_to + (c0 + r) * pitch_of(rows), r0 + q, v);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = t.tall ? tile[q + e][r] : tile[r][q + e];
+        store_pair8(base + l.x + (x0 + r) * pitch, y0 + q, v);
+        if (x0 + r >= t.m) store_pair8(base + l.x_other + (x0 + r) * pitch, y0 + q, v);
     }
 }
 
@@ -233,34 +231,35 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     const char *P, *Q;
     if (kMode == kGram || kMode == kPoly) {
         I = J = t.m, K = kMode == kGram ? t.n : t.m;
-        P = Q = base + (kMode == kGram ? l.x : l.a);
+        P = Q = base + (kMode == kPoly ? l.a : turn ? l.x_other : l.x);
         int wide = (t.m + T - 1) / T;
         ti = 0;
         while (number >= wide) number -= wide--, ++ti;
         tj = ti + number;
     } else {
-        I = t.m, J = t.n, K = t.m;
-        P = base + l.b, Q = base + (turn ? l.xt_other : l.xt);
+        I = t.n, J = K = t.m;
+        P = base + (turn ? l.x_other : l.x), Q = base + l.b;
         const int down = (t.m + T - 1) / T;
-        ti = number % down, tj = number / down;
-        if (kMode == kLast && t.tall) {   // (the result's rows are X's columns)
-            I = t.n, J = t.m;
-            const char *q = P;
-            P = Q, Q = q;
-            const int swap = ti;
-            ti = tj, tj = swap;
-        }
+        tj = number % down, ti = number / down;
     }
-    const int64_t pitch = pitch_of(K);
+    constexpr bool kColumns = kMode >= kApply;   // P's rows are X's columns: its stages are 32 rows of X
+    const int64_t pitch = pitch_of(K), x_pitch = pitch_of(t.n);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / kSet, in_set = wave % kSet;
     const int stages = (int)(pitch / kLine), rounds = (stages + S::ks - 1) / S::ks;
 
-    // This wave's part of a stage: rows 8 at a time, each row's line with its eight pieces of 16 bytes in an order of its own (piece p of row r at
-    // p ^ (r / 2 & 7)), so that what 16 lanes read of as many rows lies in different ones of the 64 banks.
+    // This wave's part of a stage: lines 8 at a time, each with its eight pieces of 16 bytes in an order of its own, so that what the lanes of one read want lies in
+    // different ones of the 64 banks.  Of a line of row r, piece p is at p ^ (r / 2 & 7): 16 lanes read as many rows.  Of T columns of row k of X (T / 32 lines), line
+    // l is at l ^ (k & 1), and piece p at p ^ 4 (k / 2 & 1): 32 lanes read 64 bytes of each of four rows.
+    constexpr int kWide = T / 32;
     uint32_t from[kOctets];
 #pragma unroll
     for (int q = 0; q < kOctets; ++q) {
         const int octet = in_set * kOctets + q, r = octet * 8 + (lane >> 3);
+        if (kColumns && octet * 8 < T) {
+            const int k = r / kWide, line = (r % kWide) ^ (k & 1);
+            from[q] = (uint32_t)(k * x_pitch) + (uint32_t)(min(ti * kWide + line, (I + 31) / 32 - 1) * kLine + ((lane & 7) ^ ((k >> 1 & 1) * 4)) * 16);
+            continue;
+        }
         const int row = r < T ? min(ti * T + r, I - 1) : min(tj * T + r - T, J - 1);
         from[q] = (uint32_t)(row * pitch) + (uint32_t)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
     }
@@ -268,7 +267,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     const auto load = [&](int round, int q) {
         const int stage = min(round * S::ks + set, stages - 1);   // (what the last round may be short of is loaded all the same, and not used)
         const bool rows_of_p = (in_set * kOctets + q) * 8 < T;
-        load_rows8_to_lds((rows_of_p ? P : Q) + (int64_t)stage * kLine, from[q], to + round % S::buffers * S::stage_bytes + q * 1024);
+        load_rows8_to_lds((rows_of_p ? P : Q) + stage * (kColumns && rows_of_p ? 32 * x_pitch : (int64_t)kLine), from[q], to + round % S::buffers * S::stage_bytes + q * 1024);
     };
     const auto load_stage = [&](int round) {
 #pragma unroll
@@ -288,16 +287,32 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         h8 ph[kMT], qh[kNT], ql[kNT], pl[kMT];
     };
     constexpr int kReads = 2 * (kMT + kNT), kProducts = 3 * kMT * kNT;
-    // (reads in the first two thirds: what comes last has to arrive before the half ends; loads in the last two)
+    // (reads evenly among the products, loads in the first two thirds: later, or reads earlier, 2 % more)
     constexpr int kMost = kProducts * 2 / 3;
+    const auto read_p = [&](const char *stage, int half, int a, bool lo) {
+        if constexpr (kColumns) {
+            // (the transposing read hands lane l of 16 lanes the l-th element of each of four rows: 8 k of 16 columns in two)
+            s16x4 x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int k = half * 16 + (lane >> 5) * 8 + e * 4 + (lane >> 2 & 3), piece = (lane >> 4 & 1) * 2 + (lane >> 1 & 1) + (lo ? 4 : 0);
+                const char *p = stage + (k * kWide + ((row_i / 32 + a) ^ (k & 1))) * kLine + (piece ^ ((k >> 1 & 1) * 4)) * 16 + (lane & 1) * 8;
+                x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3))) *)p);
+            }
+            const u32x2 y = __builtin_bit_cast(u32x2, x[0]), z = __builtin_bit_cast(u32x2, x[1]);
+            return __builtin_bit_cast(h8, (u32x4){y[0], y[1], z[0], z[1]});
+        } else {
+            return *reinterpret_cast<const h8 *>(stage + (row_i + a * 32 + (lane & 31)) * kLine + (((half * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 ^ (lo ? 64 : 0)));
+        }
+    };
     const auto read = [&](Half &h, int round, int half, int which) {
         const char *stage = lds + round % S::buffers * S::stage_bytes + set * S::set_bytes;
-        const char *p = stage + (row_i + (lane & 31)) * kLine, *q = stage + (T + row_j + (lane & 31)) * kLine;
+        const char *q = stage + (T + row_j + (lane & 31)) * kLine;
         const int hi_at = ((half * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16, lo_at = hi_at ^ 64;
-        if (which < kMT) h.ph[which] = *reinterpret_cast<const h8 *>(p + which * 32 * kLine + hi_at);
+        if (which < kMT) h.ph[which] = read_p(stage, half, which, false);
         else if (which < kMT + kNT) h.qh[which - kMT] = *reinterpret_cast<const h8 *>(q + (which - kMT) * 32 * kLine + hi_at);
         else if (which < kMT + 2 * kNT) h.ql[which - kMT - kNT] = *reinterpret_cast<const h8 *>(q + (which - kMT - kNT) * 32 * kLine + lo_at);
-        else h.pl[which - kMT - 2 * kNT] = *reinterpret_cast<const h8 *>(p + (which - kMT - 2 * kNT) * 32 * kLine + lo_at);
+        else h.pl[which - kMT - 2 * kNT] = read_p(stage, half, which - kMT - 2 * kNT, true);
     };
     const auto multiply = [&](const Half &h, int which) {
         const int a = which % (kMT * kNT) / kNT, b = which % kNT;
@@ -388,7 +403,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     // are of 16 bytes to a lane and 64 or 128 to a line.
     const float lr = kMode != kLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
     const int64_t out_pitch = pitch_of(J), across_pitch = pitch_of(I);
-    char *out = base + (kMode == kGram ? l.a : kMode == kPoly ? l.b : l.x), *across = kMode == kApply ? base + (turn ? l.xt : l.xt_other) : out;
+    char *out = base + (kMode == kGram ? l.a : kMode == kPoly ? l.b : turn ? l.x : l.x_other), *across = out;
     __syncthreads();   // (all waves have read their stages)
     char *stage = lds + in_set * 4096;
 #pragma unroll
@@ -398,15 +413,27 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
             const int i0 = ti * T + row_i + a * 32, j0 = tj * T + row_j + b * 32;
             if (i0 >= I || j0 >= J) continue;
             if constexpr (kMode == kLast) {
-                float *rows = reinterpret_cast<float *>(stage);   // [i][j]
-#pragma unroll
-                for (int r = 0; r < 16; ++r) rows[(r / 4 * 8 + (lane >> 5) * 4 + r % 4) * 32 + (lane & 31)] = acc[a][b][r] * (1.f / (kHeld * kHeld));
+                // rows of the result: X's columns i, or its rows j
+                float *rows = reinterpret_cast<float *>(stage);
                 constexpr int kE = 4;
+                if (t.tall) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) rows[(r / 4 * 8 + (lane >> 5) * 4 + r % 4) * 32 + (lane & 31)] = acc[a][b][r] * (1.f / (kHeld * kHeld));
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4 x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = acc[a][b][q * 4 + e] * (1.f / (kHeld * kHeld));
+                        *reinterpret_cast<f32x4 *>(rows + (lane & 31) * 32 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 4)) = x;   // (in an order that spreads them over the banks)
+                    }
+                }
+                const int r0 = t.tall ? i0 : j0, c0 = t.tall ? j0 : i0, R = t.tall ? I : J, C = t.tall ? J : I;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int i = i0 + q * 8 + (lane >> 3), j = j0 + (lane & 7) * kE, n = i < I ? min(J - j, kE) : 0;
-                    const int64_t at = (int64_t)i * J + j;
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(rows + (q * 8 + (lane >> 3)) * 32 + (lane & 7) * kE);
+                    const int r = q * 8 + (lane >> 3), n = r0 + r < R ? min(C - c0 - (lane & 7) * kE, kE) : 0;
+                    const int64_t at = (int64_t)(r0 + r) * C + c0 + (lane & 7) * kE;
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(rows + r * 32 + (t.tall ? (lane & 7) : (lane & 7) ^ (r & 7)) * kE);
                     float v[kE] = {x[0], x[1], x[2], x[3]};
                     Piece<O, kE> w;
                     if (s.update) {
@@ -465,7 +492,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                     const u32x4 x = *reinterpret_cast<const u32x4 *>(stage + r * kLine + ((piece ^ (r >> 1)) & 7) * 16);
                     if (j0 + r < J) *reinterpret_cast<u32x4 *>(across + (j0 + r) * across_pitch + (int64_t)(i0 / 32) * kLine + piece * 16) = x;
                 }
-                if (kMode == kApply || ti != tj) {
+                if (kMode != kApply && ti != tj) {
                     // rows of `out`, i: the transposing read hands lane l of 16 lanes the l-th element of each of four rows j
                     const int group = lane >> 4, l16 = lane & 15;
 #pragma unroll
@@ -543,7 +570,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
     const int item = item_of(g, blockIdx.x);
     const Item &t = g.t[item];
     const Layout l = layout_of(t.m, t.n);
-    char *base = s.workspace + t.at, *xt = base + l.xt;
+    char *base = s.workspace + t.at, *xt = base + l.x_other;
     const int m = t.m, n = t.n, number = blockIdx.x - g.first[item], parts = g.first[item + 1] - g.first[item];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bi = wave / 2 * 32, bj = wave % 2 * 32, down = (m + 31) / 32;   // this wave's 32 x 32 of a tile; 32s of m
@@ -765,7 +792,7 @@ template <typename O> void launch_steps(hipStream_t st, Group &by_n, Step s, int
     std::sort(by_m.t, by_m.t + by_m.count, [](const Item &x, const Item &y) { return x.m != y.m ? x.m > y.m : x.at < y.at; });
     for (int step = 0; step < steps; ++step) {
         s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
-        launch_products<kGram, float>(st, by_n, s, 0);
+        launch_products<kGram, float>(st, by_n, s, step & 1);
         launch_products<kPoly, float>(st, by_m, s, 0);
         if (step + 1 < steps) launch_products<kApply, float>(st, by_m, s, step & 1);
         else launch_products<kLast, O>(st, by_m, s, step & 1);
