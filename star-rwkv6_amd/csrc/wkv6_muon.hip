@@ -173,34 +173,49 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
     for (int i = threadIdx.x; i < chunks; i += kThreads) sum += sums[i];
     const float scale = (float)(kHeld / (sqrt(block_sum(sum, part)) + s.eps));
     const int across = (columns + kSpread - 1) / kSpread, number = blockIdx.x - g.first[k], r0 = number / across * kSpread, c0 = number % across * kSpread;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 4
-    for (int i = 0; i < kSpread / 4; ++i) {
-        const int r = r0 + i * 4 + wave, c = c0 + lane;
-        float v = 0.f;
-        if (r < rows && c < columns) {
-            const int64_t at = (int64_t)r * columns + c;
-            v = load1(static_cast<const G *>(t.grad) + at);
-            if (t.momentum) {
-                const float b = t.momentum[at];
-                v = s.nesterov ? v * s.kept + b * s.momentum : b;
-            }
-        }
-        tile[i * 4 + wave][lane] = v * scale;
-    }
-    __syncthreads();
-    // rows from x0 of X on, pieces of 8 columns from y0 on; the rows behind the last are zero here and in the other X
+    // pieces of 8 of a row; rows of X as they are, columns through LDS.  Behind X's last row there are zeros, here and in the other X.
+    constexpr int kE = 8, kPieces = kSpread * kSpread / kE / kThreads;
     const int x0 = t.tall ? c0 : r0, y0 = t.tall ? r0 : c0;
     const int64_t pitch = pitch_of(t.n);
-#pragma unroll
-    for (int i = 0; i < kSpread * 8 / kThreads; ++i) {
-        const int which = i * kThreads + threadIdx.x, q = which % 8 * 8, r = which / 8;
-        if (x0 + r >= (t.m + 31) / 32 * 32 || y0 + q >= (t.n + 31) / 32 * 32) continue;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = t.tall ? tile[q + e][r] : tile[r][q + e];
+    const auto store = [&](int r, int q, const float (&v)[kE]) {
+        if (x0 + r >= (t.m + 31) / 32 * 32 || y0 + q >= (t.n + 31) / 32 * 32) return;
         store_pair8(base + l.x + (x0 + r) * pitch, y0 + q, v);
         if (x0 + r >= t.m) store_pair8(base + l.x_other + (x0 + r) * pitch, y0 + q, v);
+    };
+    Piece<G, kE> grad[kPieces];
+    Piece<float, kE> momentum[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int which = i * kThreads + threadIdx.x, r = r0 + which / 8, c = c0 + which % 8 * kE, n = r < rows ? columns - c : 0;
+        grad[i].template load<false>(static_cast<const G *>(t.grad) + (int64_t)r * columns + c, n);
+        if (t.momentum) momentum[i].template load<false>(t.momentum + (int64_t)r * columns + c, n);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int which = i * kThreads + threadIdx.x;
+        float v[kE], m[kE];
+        unpack(grad[i], v);   // (zero where there is nothing)
+        if (t.momentum) {
+            unpack(momentum[i], m);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v[e] = s.nesterov ? v[e] * s.kept + m[e] * s.momentum : m[e];
+        }
+#pragma unroll
+        for (int e = 0; e < kE; ++e) v[e] *= scale;
+        if (!t.tall) store(which / 8, which % 8 * kE, v);
+        else
+#pragma unroll
+            for (int e = 0; e < kE; ++e) tile[which / 8][which % 8 * kE + e] = v[e];
+    }
+    if (!t.tall) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int which = i * kThreads + threadIdx.x, q = which % 8 * kE, r = which / 8;
+        float v[kE];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) v[e] = tile[q + e][r];
+        store(r, q, v);
     }
 }
 
