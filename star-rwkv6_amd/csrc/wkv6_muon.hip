@@ -247,15 +247,31 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     if (kMode == kGram || kMode == kPoly) {
         I = J = t.m, K = kMode == kGram ? t.n : t.m;
         P = Q = base + (kMode == kPoly ? l.a : turn ? l.x_other : l.x);
-        int wide = (t.m + T - 1) / T;
-        ti = 0;
-        while (number >= wide) number -= wide--, ++ti;
-        tj = ti + number;
+        // blocks of 4 x 4 tiles, row by row of blocks: what follows each other shares rows of either side
+        const int N = (t.m + T - 1) / T;
+        int row = 0, rows, diagonal, beyond;
+        for (;; row += 4) {
+            rows = min(4, N - row), diagonal = rows * (rows + 1) / 2, beyond = N - row - rows;
+            const int all = diagonal + rows * beyond;
+            if (number < all) break;
+            number -= all;
+        }
+        if (number < diagonal) {
+            int wide = rows;
+            ti = row;
+            while (number >= wide) number -= wide--, ++ti;
+            tj = ti + number;
+        } else {
+            number -= diagonal;
+            const int block = number / (4 * rows), inside = number % (4 * rows), width = min(4, beyond - block * 4);
+            ti = row + inside / width, tj = row + rows + block * 4 + inside % width;
+        }
     } else {
         I = t.n, J = K = t.m;
         P = base + (turn ? l.x_other : l.x), Q = base + l.b;
-        const int down = (t.m + T - 1) / T;
-        tj = number % down, ti = number / down;
+        // (eight columns of tiles at a time, for the same reason)
+        const int down = (t.m + T - 1) / T, side = number / (8 * down), inside = number % (8 * down), width = min(8, (t.n + T - 1) / T - side * 8);
+        ti = side * 8 + inside % width, tj = inside / width;
     }
     constexpr bool kColumns = kMode >= kApply;   // P's rows are X's columns: its stages are 32 rows of X
     const int64_t pitch = pitch_of(K), x_pitch = pitch_of(t.n);
@@ -772,7 +788,7 @@ template <typename S, int kMode, typename O> void launch_tiles(hipStream_t st, G
         total += kMode <= kPoly ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
     }
     g.first[g.count] = total;
-    const int run = std::max(1, std::min(32, total / 16));
+    const int run = std::min(32, (total + 7) / 8);
     hipLaunchKernelGGL((product_kernel<S, kMode, O>), dim3((total + 8 * run - 1) / (8 * run) * 8 * run), dim3(S::threads), 0, st, g, s, turn, total, run);
 }
 
@@ -795,9 +811,9 @@ template <int kMode, typename O> void launch_products(hipStream_t st, Group &g, 
     const int64_t of_128 = tiles_of(g, 128, symmetric);
     if (tiles_of(g, 256, symmetric) >= 1024) launch_tiles<TileShape<256, 2, 4, 1, 2>, kMode, O>(st, g, s, turn);
     else if (of_128 > 256) launch_tiles<TileShape<128, 2, 2, 1, 2>, kMode, O>(st, g, s, turn);
-    else if (of_128 >= 128) launch_tiles<TileShape<128, 2, 2, 1, 4>, kMode, O>(st, g, s, turn);
-    else if (tiles_of(g, 64, symmetric) <= 256) launch_tiles<TileShape<64, 2, 2, 1, 8>, kMode, O>(st, g, s, turn);
-    else launch_tiles<TileShape<64, 2, 1, 2, 2>, kMode, O>(st, g, s, turn);
+    else if (of_128 >= 128) launch_tiles<TileShape<128, 2, 4, 1, 4>, kMode, O>(st, g, s, turn);
+    else if (tiles_of(g, 64, symmetric) <= 256) launch_tiles<TileShape<64, 2, 2, 2, 4>, kMode, O>(st, g, s, turn);
+    else launch_tiles<TileShape<64, 2, 2, 2, 2>, kMode, O>(st, g, s, turn);
 }
 
 template <typename O> void launch_steps(hipStream_t st, Group &by_n, Step s, int steps, const double *coefficients) {
