@@ -14,6 +14,12 @@
 // in one stage is one line of 128 bytes.  A and A A are products of rows by rows, C_ij = sum_k P_ik Q_jk, and symmetric: only the tiles on and above the diagonal are
 // computed, and each is written to both of its places.  Of B X the columns of X are multiplied with rows of B; LDS hands them out across its rows.
 // B has a I in it, so that B X is the whole step.
+//
+// What bounds it: 12 matrices of 2048 x 2048 and 4 of 2048 x 7168 together, 1140 to 1260 TFLOP/s of fp16 products in B X (1.06 ms) and 1030 in A and A A (0.65 and 0.41 ms), where a library's
+// product of 8192^3 fp16 runs at 1445: the chip's power lowers its clock to 1.6 to 1.8 GHz while the matrix units are busy 53 to 60 % of the time, so that
+// fewer waits give fewer cycles a second, and what costs energy (LDS and cache traffic: tiles of 256) counts.  One matrix of 2048 x 2048: 36 to 49 us a product, of which the matrix
+// units need 20; its tiles of 128 read 285 to 537 MB out of the caches at 8 to 11 TB/s, and half of the units have no tile of A.  Dividing the stages
+// evenly among 256 workgroups instead, parts exchanged through memory: the same time for it, twice as long for many matrices.  Small ones: 17 launches of 10 to 14 us.
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 #include "wkv6_mfma.h"
