@@ -9,8 +9,8 @@
 // no token of the call: it is set to zero by other workgroups of the launch that sorts.
 //
 // Bound by memory, the table's zeros before all: 8192 tokens, 65536 x 2048 in fp32: rows 19 us (7.0 TB/s), zeros with the sorting behind them 91 (5.9 TB/s), sums 19, what reaches over
-// stretches 7.  1665 tokens of 50277 x 777 fp16: 6, 18, 10 and 4.  One token: a launch of 4 us.  All 8192 tokens alike: the parts of 512 stretches are one
-// after the other.
+// stretches 7.  1665 tokens of 50277 x 777 fp16: 6, 18, 10 and 4.  One token: a launch of 4 us.  All 8192 tokens alike: the parts of 512 stretches are added one
+// after the other, 50 us more.
 #include "wkv6_common.h"
 #include "wkv6_kernels.h"
 #include "wkv6_pieces.h"
@@ -359,7 +359,7 @@ template <typename G, typename W, int kT, int kVecs> __global__ __launch_bounds_
 
 // The runs that reach over an end of a stretch, by the stretch that they begin in.
 template <typename W> __global__ __launch_bounds__(kThreads) void join_kernel(EmbeddingGrad a, Sorted s, int64_t first_block) {
-    constexpr int kE = 4, kAhead = 8;
+    constexpr int kE = 4, kAhead = 32;
     const int64_t number = first_block + blockIdx.x, begin = number * s.stretch, end = begin + s.stretch;
     if (end >= a.N) return;
     const uint32_t run = s.keys[end];

@@ -4,6 +4,8 @@ Tolerances: with u = 2^-24 a sum over a row is added up in at most 64 steps (32 
 by 64 u mean|s|, the variance by 64 u of itself and by the square of the mean's error, 1 / deviation by some 36 u; products and differences
 add a few u of themselves.  A result is rounded once more, by half a step of its type.  Sums over rows: a wave adds at most rows / 2048 + 1 rows (where a
 workgroup takes a row, rows / 512 + 1), then four waves, then workgroups in fp64."""
+import gc
+
 import pytest
 import torch
 
@@ -251,6 +253,28 @@ def test_empty_and_refused():
     g, = torch.autograd.grad(rwkv_kernel.layer_norm(leaf).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+
+
+def test_nothing_is_kept_of_a_forward_that_is_dropped():
+    x, a, w, b, _, _ = _inputs((500, 1024), F32, BF16, F32, True, 3)
+    leaves = [t.detach().requires_grad_(True) for t in (x, a, w, b)]
+    gc.collect()   # (what other tests have left may go meanwhile)
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        y, total = rwkv_kernel.layer_norm(leaves[0], leaves[2], leaves[3], add=leaves[1], dtype=BF16)
+        del y, total
+    assert torch.cuda.memory_allocated() <= before
+
+
+def test_a_sum_that_is_changed_is_noticed():
+    """The backward reads the sum that was returned: changed in place, it is refused."""
+    x, a, w, b, gy, _ = _inputs((5, 64), F32, F32, F32, True, 3)
+    leaf = x.detach().requires_grad_(True)
+    y, total = rwkv_kernel.layer_norm(leaf, w, b, add=a)
+    with torch.no_grad():
+        total.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaf, gy)
 
 
 def test_added_to_itself():
