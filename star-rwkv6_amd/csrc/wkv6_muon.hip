@@ -807,11 +807,12 @@ int64_t tiles_of(const Group &g, int tile, bool symmetric) {
     return all;
 }
 
-// The largest tiles of which there are enough.  Per operation a tile of 256 moves half of what one of 128 does, which counts where the chip's power sets the clock
-// (A, A A and B X of 12 matrices of 2048 x 2048 and 4 of 2048 x 7168 by 256 / by 128, in us: 833 529 1190 / 682 434 1250: the first two have 768 tiles of 256, the last 1856).
-// Of 128, two workgroups of two buffers to a compute unit; where there is no second, one of four (2048 x 2048, in us: 52 56 60 two, 47 50 54
-// one).  Fewer leave units idle: tiles of 64 (777 x 1311, in us: 25 21 20 by 128, 14 11 19 by 64 with eight buffers, 18 14 15 with four,
-// of which two workgroups fit).
+// The largest tiles of which there are enough.  Per operation a tile of 256 moves half of what one of 128 does, which counts where the chip's power sets the clock; of
+// 128, two workgroups of two buffers fit a compute unit, and where there is no second, one of eight waves and four buffers is faster; fewer leave units idle, and tiles of
+// 64 have the same two forms.  By 256 / 128 twice / 128 alone / 64 twice / 64 alone, a whole call in us, what is taken in brackets:
+//   8 of 2048 x 2048  4644 [4161] 4481 6062 6805     16 of 1024 x 1024  1294 [1303] 1447 1610 1854     1 of 512 x 2048    905 403 327 226 [180]
+//   4 of 1024 x 1024   952 461 [423] 538 568          8 of 512 x 512      596 273 244 [212] 251         1 of 1024 x 1024   918 409 332 235 [188]
+// and 256 for B X of 16 of 2048 x 2048 and more (1190 for 1250 of 12 with 4 of 2048 x 7168, whose A and A A, 768 tiles, take 833 and 529 for 682 and 434).
 template <int kMode, typename O> void launch_products(hipStream_t st, Group &g, const Step &s, int turn) {
     const bool symmetric = kMode <= kPoly;
     const int64_t of_128 = tiles_of(g, 128, symmetric);
