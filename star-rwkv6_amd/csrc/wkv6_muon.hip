@@ -68,25 +68,36 @@ struct Step {
 static_assert(sizeof(Group) + sizeof(Step) + 64 <= 4096, "a launch's arguments");
 
 __host__ __device__ inline int64_t pitch_of(int k) { return (int64_t)((k + 31) / 32) * kLine; }
-// What a matrix has in the workspace: X twice (one is read while the other is written), with zeros in rows up to a multiple of 32, A, B, sums of squares.  Of a matrix of at
-// most 64 rows: the parts of A, two times 16 of 4 KB for each 32 x 32, and X's transpose.
+__host__ __device__ inline int tiles(int k, int tile) { return (k + tile - 1) / tile; }
+
+// Kinds of matrices, which go through in launches of their own.  kThinMatrix: m <= 64, see thin_kernel.  kLongMatrix: A has so few tiles, of so long a k, that workgroups share them.
+constexpr int kThin = 64, kLongTile = 64;
+enum { kGeneral = 0, kThinMatrix = 1, kLongMatrix = 2, kKinds = 3 };
+__host__ __device__ inline int kind_of(int m, int n) { return m <= kThin ? kThinMatrix : m <= 512 && n >= 8192 && n >= 16 * m ? kLongMatrix : kGeneral; }
+__host__ __device__ inline int half_of(int across) { return across * (across + 1) / 2; }   // tiles on and above the diagonal
+// Workgroups that share a tile of a long matrix's A: 512 of them to all of its tiles, with 16 stages or more each.
+__host__ __device__ inline int shares_of(int m, int n) { return max(1, min((n + 31) / 32 / 16, 512 / half_of(tiles(m, kLongTile)))); }
+// Parts of a thin matrix's A at most: all workgroups of a launch read all of them, so not as many as there are blocks of 64 columns where those are many.
+__host__ __device__ inline int thin_parts_of(int n) { return min(tiles(n, kThin), n <= 64 * 1024 / 4 ? 16 : 64); }
+
+// What a matrix has in the workspace: X twice (one is read while the other is written), with zeros in rows up to a multiple of 32, A, B, the parts of a long matrix's A, sums of
+// squares.  Of a thin matrix: the parts of A for two launches, 4 KB for each 32 x 32 of a part, and X's transpose.
 struct Layout {
-    int64_t x, x_other, a, b, sums, end;
+    int64_t x, x_other, a, b, parts, sums, end;
 };
 __host__ __device__ inline Layout layout_of(int m, int n) {
     Layout l;
-    const int down = (m + 31) / 32;
+    const int down = (m + 31) / 32, kind = kind_of(m, n);
     l.x = 0;
-    l.x_other = l.x + (m <= 64 ? (int64_t)down * down * (2 * 16 * 4096) : down * 32 * pitch_of(n));
-    l.a = l.x_other + (m <= 64 ? n * pitch_of(m) : down * 32 * pitch_of(n));
+    l.x_other = l.x + (kind == kThinMatrix ? (int64_t)down * down * 2 * thin_parts_of(n) * 4096 : down * 32 * pitch_of(n));
+    l.a = l.x_other + (kind == kThinMatrix ? n * pitch_of(m) : down * 32 * pitch_of(n));
     l.b = l.a + m * pitch_of(m);
-    l.sums = l.b + m * pitch_of(m);
+    l.parts = l.b + m * pitch_of(m);
+    l.sums = l.parts + (kind == kLongMatrix ? (int64_t)shares_of(m, n) * half_of(tiles(m, kLongTile)) * (kLongTile * kLongTile * 4) : 0);
     l.end = l.sums + ((int64_t)m * n + kChunk - 1) / kChunk * 8;
     l.end = (l.end + 255) / 256 * 256;
     return l;
 }
-
-__host__ inline int tiles(int k, int tile) { return (k + tile - 1) / tile; }
 
 // (by all lanes at once: each step of a search would wait for its own load of an argument)
 __device__ __forceinline__ int item_of(const Group &g, int unit) {
@@ -225,7 +236,9 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
     }
 }
 
-enum { kGram = 0, kPoly = 1, kApply = 2, kLast = 3 };   // A = X X^T; B = a I + b A + c A A; X = B X; the same into the result
+// A = X X^T; B = a I + b A + c A A; X = B X; the same into the result; of long matrices a workgroup's part of A, and A from the parts
+enum { kGram = 0, kPoly = 1, kApply = 2, kLast = 3, kGramPart = 4, kGramJoin = 5 };
+constexpr bool is_symmetric(int mode) { return mode != kApply && mode != kLast; }
 
 // Product tiles of T x T.  WM x WN waves share a tile's rows and columns, KS of such sets its stages of 32 k, of which LDS holds NB (to a set) at a time.
 template <int T, int WM, int WN, int KS, int NB> struct TileShape {
@@ -247,11 +260,14 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     const Layout l = layout_of(t.m, t.n);
     char *base = s.workspace + t.at;
     int number = unit - g.first[item], ti, tj;
+    constexpr bool kShare = kMode == kGramPart;
+    const int half = half_of((t.m + T - 1) / T), share = kShare ? number / half : 0, tile_number = kShare ? number % half : number;
+    number = tile_number;
     // rows of P and Q, and the length of either
     int I, J, K;
     const char *P, *Q;
-    if (kMode == kGram || kMode == kPoly) {
-        I = J = t.m, K = kMode == kGram ? t.n : t.m;
+    if (is_symmetric(kMode)) {
+        I = J = t.m, K = kMode == kPoly ? t.m : t.n;
         P = Q = base + (kMode == kPoly ? l.a : turn ? l.x_other : l.x);
         // blocks of 4 x 4 tiles, row by row of blocks: what follows each other shares rows of either side
         const int N = (t.m + T - 1) / T;
@@ -279,10 +295,12 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         const int down = (t.m + T - 1) / T, side = number / (8 * down), inside = number % (8 * down), width = min(8, (t.n + T - 1) / T - side * 8);
         ti = side * 8 + inside % width, tj = inside / width;
     }
-    constexpr bool kColumns = kMode >= kApply;   // P's rows are X's columns: its stages are 32 rows of X
+    constexpr bool kColumns = !is_symmetric(kMode);   // P's rows are X's columns: its stages are 32 rows of X
     const int64_t pitch = pitch_of(K), x_pitch = pitch_of(t.n);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / kSet, in_set = wave % kSet;
-    const int stages = (int)(pitch / kLine), rounds = (stages + S::ks - 1) / S::ks;
+    const int lines = (int)(pitch / kLine), shares = kShare ? shares_of(t.m, t.n) : 1;
+    const int begin = kShare ? (int)((int64_t)lines * share / shares) : 0, end = kShare ? (int)((int64_t)lines * (share + 1) / shares) : lines;
+    const int stages = kMode == kGramJoin ? 0 : end - begin, rounds = (stages + S::ks - 1) / S::ks;
 
     // This wave's part of a stage: lines 8 at a time, each with its eight pieces of 16 bytes in an order of its own, so that what the lanes of one read want lies in
     // different ones of the 64 banks.  Of a line of row r, piece p is at p ^ (r / 2 & 7): 16 lanes read as many rows.  Of T columns of row k of X (T / 32 lines), line
@@ -302,7 +320,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
     }
     const uint32_t to = lds_address(lds) + set * S::set_bytes + in_set * kOctets * 1024;
     const auto load = [&](int round, int q) {
-        const int stage = min(round * S::ks + set, stages - 1);   // (what the last round may be short of is loaded all the same, and not used)
+        const int stage = begin + min(round * S::ks + set, stages - 1);   // (what the last round may be short of is loaded all the same, and not used)
         const bool rows_of_p = (in_set * kOctets + q) * 8 < T;
         load_rows8_to_lds((rows_of_p ? P : Q) + stage * (kColumns && rows_of_p ? 32 * x_pitch : (int64_t)kLine), from[q], to + round % S::buffers * S::stage_bytes + q * 1024);
     };
@@ -362,6 +380,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
         else wait_loads<0>();
         __syncthreads();
     };
+    if constexpr (kMode != kGramJoin) {
     Half first, second;
 #pragma unroll
     for (int k = 0; k < S::buffers - 1; ++k)
@@ -411,6 +430,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
             for (int o = 0; o < kProducts; ++o) multiply(second, o);
         }
     }
+    }
     if constexpr (S::ks > 1) {
         // the sets' sums, to the first
         static_assert(S::buffers * S::stage_bytes >= (S::ks - 1) * T * T * 4, "room for the sums");
@@ -436,11 +456,34 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                     for (int r = 0; r < 16; ++r) acc[a][b][r] += sums[(((other * kSet + in_set) * kMT + a) * kNT + b) * 1024 + r * 64 + lane];
     }
 
+    // (a part as the lanes hold it: 64 of a register next to each other)
+    float *part = kMode == kGramPart || kMode == kGramJoin ? reinterpret_cast<float *>(base + l.parts) + (int64_t)tile_number * (T * T) + in_set * (kMT * kNT * 1024) + lane : nullptr;
+    if constexpr (kMode == kGramPart) {
+#pragma unroll
+        for (int a = 0; a < kMT; ++a)
+#pragma unroll
+            for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) part[(int64_t)share * half * (T * T) + (a * kNT + b) * 1024 + r * 64] = acc[a][b][r];
+        return;
+    }
+    if constexpr (kMode == kGramJoin) {
+        const int all = shares_of(t.m, t.n);
+#pragma unroll 4
+        for (int k = 0; k < all; ++k)
+#pragma unroll
+            for (int a = 0; a < kMT; ++a)
+#pragma unroll
+                for (int b = 0; b < kNT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[a][b][r] += part[(int64_t)k * half * (T * T) + (a * kNT + b) * 1024 + r * 64];
+    }
+
     // Lane l has column l % 32 of a 32 x 32 tile, and rows 8 k + 4 (l / 32) + (0 .. 3).  A tile goes out through 4 KB of LDS of the wave's own, so that stores
     // are of 16 bytes to a lane and 64 or 128 to a line.
     const float lr = kMode != kLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
     const int64_t out_pitch = pitch_of(J), across_pitch = pitch_of(I);
-    char *out = base + (kMode == kGram ? l.a : kMode == kPoly ? l.b : turn ? l.x : l.x_other), *across = out;
+    char *out = base + (kMode == kGram || kMode == kGramJoin ? l.a : kMode == kPoly ? l.b : turn ? l.x : l.x_other), *across = out;
     __syncthreads();   // (all waves have read their stages)
     char *stage = lds + in_set * 4096;
 #pragma unroll
@@ -558,7 +601,6 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
 // A and B are one tile, and what a step costs is launches and latency.  So a step is one launch: a workgroup adds up the parts of A that the launch before left,
 // forms B (each for itself), multiplies its columns of X by it 64 at a time, and leaves its part of the new A.  10 matrices of 32 x 2048: 17 launches of
 // the general form 150 us of kernels.
-constexpr int kThin = 64, kThinParts = 16;
 constexpr int kThinRegion = 2 * kThin * kLine;   // 64 rows of 64 k
 
 // LDS operands: 64 rows of kThin k as lines of 32 k, pieces in the order that stages have.
@@ -613,7 +655,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
     const int bi = wave / 2 * 32, bj = wave % 2 * 32, down = (m + 31) / 32;   // this wave's 32 x 32 of a tile; 32s of m
     const int64_t pitch = pitch_of(m);
     f32x4 *sums = reinterpret_cast<f32x4 *>(base + l.x);
-    const int part_size = down * down * 256;   // f32x4s: 4 to a lane of each 32 x 32
+    const int part_size = down * down * 256, most_parts = thin_parts_of(n);   // f32x4s: 4 to a lane of each 32 x 32
     const int my_part = (bi / 32 * down + bj / 32) * 256 + lane;
     const bool of_a = bi < m && bj < m;
 
@@ -628,7 +670,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
         float a[16];
         if (of_a) {
             f32x4 v[4];
-            const f32x4 *from = sums + (int64_t)(turn ^ 1) * kThinParts * part_size + my_part;
+            const f32x4 *from = sums + (int64_t)(turn ^ 1) * most_parts * part_size + my_part;
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[q] = from[q * 64];
 #pragma unroll 5
@@ -756,7 +798,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
         }
     }
     if (kPhase != kThinLast && of_a) {
-        f32x4 *to = sums + ((int64_t)turn * kThinParts + number) * part_size + my_part;
+        f32x4 *to = sums + ((int64_t)turn * most_parts + number) * part_size + my_part;
 #pragma unroll
         for (int q = 0; q < 4; ++q) to[q * 64] = (f32x4){gram[q * 4], gram[q * 4 + 1], gram[q * 4 + 2], gram[q * 4 + 3]};
     }
@@ -774,7 +816,7 @@ template <typename O> void launch_thin(hipStream_t st, Group &g, Step s, int ste
     int total = 0;
     for (int i = 0; i < g.count; ++i) {
         g.first[i] = total;
-        total += std::min({tiles(g.t[i].n, kThin), kThinParts, std::max(4, 512 / g.count)});
+        total += std::min(thin_parts_of(g.t[i].n), std::max(4, 512 / g.count));
     }
     g.first[g.count] = total;
     hipLaunchKernelGGL((thin_kernel<kThinFirst, O>), dim3(total), dim3(kThreads), 0, st, g, s, 0);
@@ -791,7 +833,7 @@ template <typename S, int kMode, typename O> void launch_tiles(hipStream_t st, G
     for (int i = 0; i < g.count; ++i) {
         g.first[i] = total;
         const int down = tiles(g.t[i].m, S::tile);
-        total += kMode <= kPoly ? down * (down + 1) / 2 : down * tiles(g.t[i].n, S::tile);
+        total += is_symmetric(kMode) ? half_of(down) * (kMode == kGramPart ? shares_of(g.t[i].m, g.t[i].n) : 1) : down * tiles(g.t[i].n, S::tile);
     }
     g.first[g.count] = total;
     const int run = std::min(32, (total + 7) / 8);
@@ -814,7 +856,7 @@ int64_t tiles_of(const Group &g, int tile, bool symmetric) {
 //   4 of 1024 x 1024   952 461 [423] 538 568          8 of 512 x 512      596 273 244 [212] 251         1 of 1024 x 1024   918 409 332 235 [188]
 // and 256 for B X of 16 of 2048 x 2048 and more (1190 for 1250 of 12 with 4 of 2048 x 7168, whose A and A A, 768 tiles, take 833 and 529 for 682 and 434).
 template <int kMode, typename O> void launch_products(hipStream_t st, Group &g, const Step &s, int turn) {
-    const bool symmetric = kMode <= kPoly;
+    constexpr bool symmetric = is_symmetric(kMode);
     const int64_t of_128 = tiles_of(g, 128, symmetric);
     if (tiles_of(g, 256, symmetric) >= 1024) launch_tiles<TileShape<256, 2, 4, 1, 2>, kMode, O>(st, g, s, turn);
     else if (of_128 > 256) launch_tiles<TileShape<128, 2, 2, 1, 2>, kMode, O>(st, g, s, turn);
@@ -830,7 +872,12 @@ template <typename O> void launch_steps(hipStream_t st, Group &by_n, Step s, int
     std::sort(by_m.t, by_m.t + by_m.count, [](const Item &x, const Item &y) { return x.m != y.m ? x.m > y.m : x.at < y.at; });
     for (int step = 0; step < steps; ++step) {
         s.a = (float)coefficients[3 * step], s.b = (float)coefficients[3 * step + 1], s.c = (float)coefficients[3 * step + 2];
-        launch_products<kGram, float>(st, by_n, s, step & 1);
+        if (kind_of(by_n.t[0].m, by_n.t[0].n) == kLongMatrix) {   // (a group is of one kind)
+            launch_tiles<TileShape<kLongTile, 2, 2, 2, 4>, kGramPart, float>(st, by_n, s, step & 1);
+            launch_tiles<TileShape<kLongTile, 2, 2, 1, 2>, kGramJoin, float>(st, by_n, s, step & 1);
+        } else {
+            launch_products<kGram, float>(st, by_n, s, step & 1);
+        }
         launch_products<kPoly, float>(st, by_m, s, 0);
         if (step + 1 < steps) launch_products<kApply, float>(st, by_m, s, step & 1);
         else launch_products<kLast, O>(st, by_m, s, step & 1);
@@ -846,15 +893,15 @@ size_t muon_matrix_bytes(int64_t rows, int64_t columns) {
 hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matrices, const MuonStep &a, void *workspace, size_t workspace_bytes) {
     const Step s{(float)a.momentum, (float)(1. - a.momentum), a.nesterov, a.update, (float)a.eps, (float)a.weight_decay, (float)a.lr, a.lr_device, 0.f, 0.f, 0.f,
                  static_cast<char *>(workspace)};
-    // groups of either kind, as they fit into a launch's arguments and the workspace
-    int64_t next[2] = {0, 0};
-    for (int thin = 0; thin < 2;) {
+    // groups of each kind, as they fit into a launch's arguments and the workspace
+    int64_t next[kKinds] = {};
+    for (int kind = 0; kind < kKinds;) {
         Group g{};
         size_t used = 0;
-        int64_t &at = next[thin];
+        int64_t &at = next[kind];
         for (; at < count && g.count < kGroup; ++at) {
             const MuonMatrix &t = matrices[at];
-            if (t.rows == 0 || t.columns == 0 || (std::min(t.rows, t.columns) <= kThin) != (thin == 1)) continue;
+            if (t.rows == 0 || t.columns == 0 || kind_of((int)std::min(t.rows, t.columns), (int)std::max(t.rows, t.columns)) != kind) continue;
             const size_t bytes = muon_matrix_bytes(t.rows, t.columns);
             if (g.count > 0 && used + bytes > workspace_bytes) break;
             g.t[g.count++] = Item{t.grad, t.momentum, t.out, t.master, (int64_t)used, (int)std::min(t.rows, t.columns), (int)std::max(t.rows, t.columns), (float)t.rate,
@@ -862,7 +909,7 @@ hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matr
             used += bytes;
         }
         if (g.count == 0) {
-            ++thin;
+            ++kind;
             continue;
         }
         const hipError_t e = by_type(dtype, [&](auto type) {
@@ -871,7 +918,7 @@ hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matr
             for (int i = 0; i < g.count; ++i) g.first[i] = total, total += (int)(((int64_t)g.t[i].m * g.t[i].n + kChunk - 1) / kChunk);
             g.first[g.count] = total;
             hipLaunchKernelGGL((momentum_kernel<O>), dim3(total), dim3(kThreads), 0, st, g, s);
-            if (thin) {
+            if (kind == kThinMatrix) {
                 launch_thin<O>(st, g, s, a.steps, a.coefficients);
                 return;
             }

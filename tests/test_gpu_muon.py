@@ -116,11 +116,15 @@ def test_large(count, m, n):
             _check(o, x)
 
 
-@pytest.mark.parametrize("m,n", [(1, 50000), (20, 70001), (64, 100000), (60000, 33), (65, 60000)])
+@pytest.mark.parametrize("m,n", [(1, 50000), (20, 70001), (64, 100000), (60000, 33), (65, 60000), (9000, 300), (512, 8192), (513, 8300), (130, 8191), (200, 33333)])
 def test_long_and_thin(m, n):
     print("orthogonalize", m, n, flush=True)
     x = _matrix(m, n, 4, "normal")
     _check(rwkv_kernel.orthogonalize(x), x)
+    few = [x, _matrix(100, 9000, 5), _matrix(40, 20000, 6), _matrix(90, 90, 7), x]
+    out = rwkv_kernel.orthogonalize(few)
+    for y, o in zip(few, out):
+        _check(o, y)
 
 
 def test_more_than_the_workspace_holds_at_once():
