@@ -33,8 +33,9 @@ def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     derivative: a matrix that requires a gradient is refused where gradients are recorded.
 
     matrices: a tensor (.., rows, columns), or a list of such, of one dtype and any shapes; they go through together.  Returns the same in new tensors of
-    their dtype.  coefficients: (a, b, c), or one such triple for each step; what leaves the range of +-64 on the way (not with coefficients that keep singular
-    values of 0 .. 1.2 in it) ends as NaN."""
+    their dtype.  Of a G whose norm is far below eps, and so of a result far below 1, an element is good to some 2^-26, and not to its own size.  coefficients:
+    (a, b, c), or one such triple for each step; what leaves the range of +-64 on the way (not with coefficients that keep singular values of 0 .. 1.2
+    in it) ends as NaN."""
     flat = _coefficients(coefficients, steps)
     assert eps >= 0
     single = isinstance(matrices, torch.Tensor)

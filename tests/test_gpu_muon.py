@@ -198,6 +198,17 @@ def test_sizes_of_the_values():
     assert torch.equal(out[0], rwkv_kernel.orthogonalize(x)) and torch.equal(out[0], out[2])
 
 
+def test_norms_far_below_eps():
+    """X begins with entries down to 1e-12, where the pairs hold them to 2^-35 (half of fp16's smallest number, 2^-25, over 1024), which grows with the small singular
+    values, by 3.4445^5 < 486, like they do: in the 2-norm 486 * 2^-35 * sqrt(number of elements), beside the relative part."""
+    x = _matrix(40, 60, 2, "normal")
+    for scale in (1e-7, 1e-9, 1e-11):
+        y = x * scale
+        want, _, all_ = _off(y)
+        error = rwkv_kernel.orthogonalize(y).double() - want
+        assert float(error.norm()) <= all_ + 2.0 ** -18 * float(want.norm()) + 486 * 2.0 ** -35 * math.sqrt(y.numel()), (scale, float(error.norm()), float(want.norm()))
+
+
 def _step_inputs(shapes, dtype, seed, masters):
     ps = [_matrix(math.prod(s[:-1]), s[-1], seed + i, "normal").view(s) * 300 for i, s in enumerate(shapes)]
     gs = [_matrix(math.prod(s[:-1]), s[-1], seed + 100 + i).view(s).to(dtype) for i, s in enumerate(shapes)]
