@@ -549,6 +549,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     ctx->saved_data["params"] = static_cast<int64_t>(params);
     ctx->saved_data["shapes"] = std::vector<bool>{add.defined(), weight.defined(), bias.defined()};
     ctx->set_materialize_grads(false);
+    if (add.defined() && !x_.requires_grad() && !add_->requires_grad()) ctx->mark_non_differentiable({total});   // (the weights have no part in it)
     if (wanted) ctx->save_for_backward({add.defined() ? total : x, stats, weight});
     return add.defined() ? variable_list{y, total} : variable_list{y};
   }

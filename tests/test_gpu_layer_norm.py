@@ -192,6 +192,9 @@ def test_some_gradients_only():
         outs, arriving = ((y, total), (gy, gt)) if total.requires_grad and ("x" in names or "add" in names) else ((y,), (gy,))
         for k, got in zip(names, torch.autograd.grad(outs, [leaves[k] for k in names], arriving)):
             _check("g" + k, got.reshape(want["g" + k][0].shape), *want["g" + k])
+    # a sum of what needs no gradient needs none, whatever the weights do
+    y, total = rwkv_kernel.layer_norm(x, w.detach().requires_grad_(True), b, add=a, dtype=BF16)
+    assert y.requires_grad and not total.requires_grad
     # one of the two outputs alone
     leaves = [t.detach().requires_grad_(True) for t in (x, a)]
     y, total = rwkv_kernel.layer_norm(leaves[0], w, b, add=leaves[1], dtype=BF16)
