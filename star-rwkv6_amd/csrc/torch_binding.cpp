@@ -531,10 +531,10 @@ std::optional<int64_t> row_stride(const Tensor &t) {
 }
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
-  static variable_list forward(AutogradContext *ctx, const Tensor &x_, const std::optional<Tensor> &add_, const std::optional<Tensor> &weight_,
+  // x has a row stride: it is what is kept where nothing is added, and a copy that is made in here would have no graph for the gradient to hang on.
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &add_, const std::optional<Tensor> &weight_,
                                const std::optional<Tensor> &bias_, double eps, ScalarType branch, bool wanted) {
-    const c10::DeviceGuard guard(x_.device());
-    const Tensor x = row_stride(x_) ? x_ : x_.contiguous();
+    const c10::DeviceGuard guard(x.device());
     Tensor add = given(add_), weight = given(weight_), bias = given(bias_);
     if (add.defined() && !row_stride(add)) add = add.contiguous();
     const ScalarType params = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : at::kFloat;
@@ -549,7 +549,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     ctx->saved_data["params"] = static_cast<int64_t>(params);
     ctx->saved_data["shapes"] = std::vector<bool>{add.defined(), weight.defined(), bias.defined()};
     ctx->set_materialize_grads(false);
-    if (add.defined() && !x_.requires_grad() && !add_->requires_grad()) ctx->mark_non_differentiable({total});   // (the weights have no part in it)
+    if (add.defined() && !x.requires_grad() && !add_->requires_grad()) ctx->mark_non_differentiable({total});   // (the weights have no part in it)
     if (wanted) ctx->save_for_backward({add.defined() ? total : x, stats, weight});
     return add.defined() ? variable_list{y, total} : variable_list{y};
   }
@@ -1023,7 +1023,7 @@ PYBIND11_MODULE(_wkv6_torch, m) {
   m.def("layer_norm", [](const Tensor &x, const std::optional<Tensor> &add, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps,
                          int branch_code) {
     const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || (add && add->requires_grad()) || (weight && weight->requires_grad()) || (bias && bias->requires_grad()));
-    const variable_list o = unlocked([&] { return LayerNorm::apply(x, add, weight, bias, eps, type_of(branch_code), wanted); });
+    const variable_list o = unlocked([&] { return LayerNorm::apply(row_stride(x) ? x : x.contiguous(), add, weight, bias, eps, type_of(branch_code), wanted); });
     return py::make_tuple(wrap(o[0]), o.size() > 1 ? wrap(o[1]) : py::none());
   });
   m.def("embedding", [](const Tensor &ids, const Tensor &weight, double scale, int64_t padding_id, int out_code) {

@@ -335,3 +335,21 @@ def test_captured_and_on_another_stream():
         eager = _run(x, a, w, b, gy, gt, BF16)
         assert all(torch.equal(res[k], eager[k]) for k in res)
         _all_within(res, _formula(x, a, w, b, 1e-5, gy, gt))
+
+
+def test_second_derivatives_are_refused_for_any_layout():
+    """A derivative of a gradient that was taken with create_graph is refused, and not left out, for inputs that the kernels read as they are and for those that are copied."""
+    big = _inputs((6, 4, 32), F32, F32, F32, False, 8)[0]
+    w = torch.ones(16, device="cuda")
+    for view in (lambda t: t, lambda t: t.transpose(0, 1), lambda t: t[:, :, ::2], lambda t: t.permute(2, 0, 1), lambda t: t[1::2, 1:3, :16], lambda t: t[0, 0].expand(3, 32)):
+        for how in ("alone", "added", "added to"):
+            leaf = big.clone().requires_grad_(True)
+            x = view(leaf)
+            if how == "alone":
+                y = rwkv_kernel.layer_norm(x, w if x.shape[-1] == 16 else None)
+            else:
+                y, _ = rwkv_kernel.layer_norm(*((x,) if how == "added to" else (torch.ones_like(x),)), add=torch.ones_like(x) if how == "added to" else x)
+            g, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+            assert g.requires_grad, how
+            with pytest.raises(RuntimeError, match="second derivative"):
+                (y.sum() + g.square().sum()).backward()
