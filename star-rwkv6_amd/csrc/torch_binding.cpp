@@ -765,7 +765,7 @@ Tensors orthogonalize(const Tensors &matrices, const std::vector<double> &coeffi
   std::vector<wkv6_muon_matrix> rows;
   for (const Tensor &m : matrices) {
     check_matrix(m, first, "matrices");
-    TORCH_CHECK(!graph_wanted || !m.requires_grad(), "wkv6: orthogonalize has no derivative: detach what requires a gradient");
+    TORCH_CHECK((!graph_wanted || !m.requires_grad()) && !m._fw_grad(0).defined(), "wkv6: orthogonalize has no derivative: detach what requires a gradient or has a tangent");
   }
   for (const Tensor &m : matrices) {
     kept.push_back(m.contiguous());

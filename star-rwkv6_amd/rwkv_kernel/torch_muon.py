@@ -30,7 +30,7 @@ def _coefficients(coefficients, steps):
 def orthogonalize(matrices, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """X = G / (|G| + eps) with |G| the 2-norm of all elements, then `steps` times X = a X + b A X + c A A X with A = X X^T (of a matrix with more rows than columns its
     transpose's, transposed): the singular vectors of G with singular values near 1.  Without a
-    derivative: a matrix that requires a gradient is refused where gradients are recorded.
+    derivative: a matrix that requires a gradient is refused where gradients are recorded, and one with a tangent (forward mode).
 
     matrices: a tensor (.., rows, columns), or a list of such, of one dtype and any shapes; they go through together.  Returns the same in new tensors of
     their dtype.  Of a G whose norm is far below eps, and so of a result far below 1, an element is good to some 2^-26, and not to its own size.  coefficients:

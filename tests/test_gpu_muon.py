@@ -330,3 +330,16 @@ def test_captured_and_on_another_stream():
         run(twin)
         for x, y in zip(state, twin):
             assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+def test_tangents_are_refused():
+    """orthogonalize has no derivative in forward mode either."""
+    import torch.autograd.forward_ad as fwd
+
+    x = _matrix(40, 60, 2)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: rwkv_kernel.orthogonalize(dual), lambda: rwkv_kernel.orthogonalize([x, dual])):
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call()
+        assert torch.equal(rwkv_kernel.orthogonalize(fwd.unpack_dual(dual).primal), rwkv_kernel.orthogonalize(x))
