@@ -60,7 +60,8 @@ struct Group {
 struct Step {
     float momentum, kept;    // kept = 1 - momentum
     int nesterov, update;    // update: the last product is applied to weights
-    float eps, weight_decay, lr;
+    float weight_decay, lr;
+    double eps;
     const float *lr_device;  // one value in lr's place, or null
     float a, b, c;
     char *workspace;
@@ -116,6 +117,17 @@ __device__ __forceinline__ double block_sum(double v, double *part) {
     for (int i = 1; i < kThreads / 64; ++i) v += part[i];
     return v;
 }
+
+// kHeld / (|U| + eps), which leaves fp32 at either end where |U| and what is multiplied do not: a power of two, and the rest.
+struct Scale {
+    float power, rest;
+    __device__ __forceinline__ Scale(double squares, double eps) {
+        const double norm = sqrt(squares), s = kHeld / (norm + eps);
+        power = s > 0x1p64 ? 0x1p100f : s < 0x1p-64 ? 0x1p-100f : 1.f;
+        rest = norm == 0. && eps > 0. ? 0.f : (float)(s / power);   // (of zeros and a small eps s may be more than any factor)
+    }
+    __device__ __forceinline__ float operator()(float v) const { return v * power * rest; }
+};
 
 // The momentum's update, and sums of squares of U by chunk.
 template <typename G> __global__ __launch_bounds__(kThreads) void momentum_kernel(Group g, Step s) {
@@ -188,7 +200,7 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
     const int chunks = (int)(((int64_t)t.m * t.n + kChunk - 1) / kChunk);
     double sum = 0.;
     for (int i = threadIdx.x; i < chunks; i += kThreads) sum += sums[i];
-    const float scale = (float)(kHeld / (sqrt(block_sum(sum, part)) + s.eps));
+    const Scale scale(block_sum(sum, part), s.eps);
     const int across = (columns + kSpread - 1) / kSpread, number = blockIdx.x - g.first[k], r0 = number / across * kSpread, c0 = number % across * kSpread;
     // pieces of 8 of a row; rows of X as they are, columns through LDS.  Behind X's last row there are zeros, here and in the other X.
     constexpr int kE = 8, kPieces = kSpread * kSpread / kE / kThreads;
@@ -218,7 +230,7 @@ template <typename G> __global__ __launch_bounds__(kThreads) void spread_kernel(
             for (int e = 0; e < kE; ++e) v[e] = s.nesterov ? v[e] * s.kept + m[e] * s.momentum : m[e];
         }
 #pragma unroll
-        for (int e = 0; e < kE; ++e) v[e] *= scale;
+        for (int e = 0; e < kE; ++e) v[e] = scale(v[e]);
         if (!t.tall) store(which / 8, which % 8 * kE, v);
         else
 #pragma unroll
@@ -659,13 +671,13 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
     const int my_part = (bi / 32 * down + bj / 32) * 256 + lane;
     const bool of_a = bi < m && bj < m;
 
-    float scale = 0.f;
+    double norm2 = 0.;
     if constexpr (kPhase == kThinFirst) {
         const double *squares = reinterpret_cast<const double *>(base + l.sums);
         const int chunks = (int)(((int64_t)m * n + kChunk - 1) / kChunk);
         double sum = 0.;
         for (int i = threadIdx.x; i < chunks; i += kThreads) sum += squares[i];
-        scale = (float)(kHeld / (sqrt(block_sum(sum, part)) + s.eps));
+        norm2 = block_sum(sum, part);
     } else {
         float a[16];
         if (of_a) {
@@ -694,6 +706,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
         }
     }
 
+    const Scale scale(norm2, s.eps);
     f16x gram = (f16x)(0.f);
     const int across = (n + kThin - 1) / kThin;
     const float lr = kPhase != kThinLast ? 0.f : s.lr_device ? *s.lr_device : s.lr, decay = 1.f - lr * s.weight_decay, rate = lr * t.rate;
@@ -715,7 +728,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
                         v = s.nesterov ? v * s.kept + b * s.momentum : b;
                     }
                 }
-                tile[k * 4 + wave][lane] = v * scale;
+                tile[k * 4 + wave][lane] = scale(v);
             }
             __syncthreads();
 #pragma unroll
@@ -891,7 +904,7 @@ size_t muon_matrix_bytes(int64_t rows, int64_t columns) {
 }
 
 hipError_t muon(hipStream_t st, int dtype, int64_t count, const MuonMatrix *matrices, const MuonStep &a, void *workspace, size_t workspace_bytes) {
-    const Step s{(float)a.momentum, (float)(1. - a.momentum), a.nesterov, a.update, (float)a.eps, (float)a.weight_decay, (float)a.lr, a.lr_device, 0.f, 0.f, 0.f,
+    const Step s{(float)a.momentum, (float)(1. - a.momentum), a.nesterov, a.update, (float)a.weight_decay, (float)a.lr, a.eps, a.lr_device, 0.f, 0.f, 0.f,
                  static_cast<char *>(workspace)};
     // groups of each kind, as they fit into a launch's arguments and the workspace
     int64_t next[kKinds] = {};

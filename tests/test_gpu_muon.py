@@ -343,3 +343,20 @@ def test_tangents_are_refused():
             with pytest.raises(RuntimeError, match="no derivative"):
                 call()
         assert torch.equal(rwkv_kernel.orthogonalize(fwd.unpack_dual(dual).primal), rwkv_kernel.orthogonalize(x))
+
+
+@pytest.mark.parametrize("m,n", [(40, 60), (60, 40), (100, 130), (130, 100), (33, 9000), (100, 9000)])
+def test_norms_at_the_ends_of_fp32(m, n):
+    """1024 over the norm leaves fp32 at either end where the norm and X do not; an eps below fp32's smallest number is an eps."""
+    print("orthogonalize, ends of fp32", m, n, flush=True)
+    x = _matrix(m, n, 2, "normal") * 1e3   # of a size of 1
+    for scale in (1e-41, 1e-37, 3e-30, 1e30, 3e37):
+        y = x * scale
+        assert bool(y.isfinite().all()) and bool(y.any())
+        _check(rwkv_kernel.orthogonalize(y, eps=0.0), y, eps=0.0)
+    y = x * 1e-40
+    _check(rwkv_kernel.orthogonalize(y, eps=1e-39), y, eps=1e-39)
+    _check(rwkv_kernel.orthogonalize(y, eps=1e-60), y, eps=1e-60)
+    for eps in (1e-7, 1e-40, 1e-46, 1e-300):
+        assert not bool(rwkv_kernel.orthogonalize(torch.zeros(m, n, device="cuda"), eps=eps).any()), eps
+    assert bool(rwkv_kernel.orthogonalize(torch.zeros(m, n, device="cuda"), eps=0.0).isnan().all())
