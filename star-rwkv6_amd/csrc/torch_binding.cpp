@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <iterator>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -816,6 +817,12 @@ void muon_step(const Tensors &params, const Tensors &grads, const Tensors &momen
   std::sort(seen.begin(), seen.end());
   for (size_t i = 1; i < seen.size(); ++i)
     TORCH_CHECK(seen[i - 1].second <= seen[i].first, "wkv6: a parameter, a momentum or a master is given twice, or shares elements with another");
+  // (gradients are read again after the momenta are written, and after another launch's matrices are; copies of what is not contiguous are made before)
+  for (const Tensor &g : kept) {
+    const auto from = reinterpret_cast<uintptr_t>(g.const_data_ptr()), to = from + g.nbytes();
+    const auto next = std::lower_bound(seen.begin(), seen.end(), std::make_pair(to, uintptr_t{0}));   // the first that begins behind it
+    TORCH_CHECK(from == to || next == seen.begin() || std::prev(next)->second <= from, "wkv6: a gradient shares elements with a parameter, a momentum or a master");
+  }
   if (rows.empty()) return;
   const size_t n = wkv6_muon_workspace_bytes(rows.size(), rows.data());
   const Tensor ws = bytes(first, n);

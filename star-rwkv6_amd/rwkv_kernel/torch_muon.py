@@ -57,7 +57,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         buf = momentum buf + (1 - momentum) g
         u = (1 - momentum) g + momentum buf if nesterov else buf
         p = p (1 - lr weight_decay) - lr rate orthogonalize(u)
-    params, grads: of one dtype (bf16, fp16, fp32); params contiguous, none twice and no two with elements in common.  momenta: buf, fp32.  lr: a number, or one
+    params, grads: of one dtype (bf16, fp16, fp32); params contiguous, none twice and no two with elements in common, and a gradient with none of what is written.  momenta: buf, fp32.  lr: a number, or one
     fp32 value on the device (which a captured graph's replays read anew).  scale: rate is sqrt(max(1, rows / columns)) ("shape"), 0.2
     sqrt(max(rows, columns)) ("rms": an update's elements are then as large as AdamW's), or a number.  masters: fp32 weights that are updated in the params'
     place, the params their rounded copies."""

@@ -360,3 +360,20 @@ def test_norms_at_the_ends_of_fp32(m, n):
     for eps in (1e-7, 1e-40, 1e-46, 1e-300):
         assert not bool(rwkv_kernel.orthogonalize(torch.zeros(m, n, device="cuda"), eps=eps).any()), eps
     assert bool(rwkv_kernel.orthogonalize(torch.zeros(m, n, device="cuda"), eps=0.0).isnan().all())
+
+
+def test_gradients_in_what_is_written_are_refused():
+    """Momenta are written before the gradients are read for the second time."""
+    w = _matrix(40, 60, 1)
+    buf = torch.zeros(3 * 2400, device="cuda")
+    g, m, other = (buf[i * 2400:(i + 1) * 2400].view(40, 60) for i in range(3))
+    shifted = buf[2500:4900].view(40, 60)
+    for call in (lambda: rwkv_kernel.muon_step([w], [g], [g], 0.1), lambda: rwkv_kernel.muon_step([w], [shifted], [m], 0.1), lambda: rwkv_kernel.muon_step([w, g], [w.clone(), g], [m, other], 0.1),
+                 lambda: rwkv_kernel.muon_step([w, g], [g, w.clone()], [m, other], 0.1),
+                 lambda: rwkv_kernel.muon_step([w.to(BF16)], [g.view(-1).view(BF16)[:2400].view(40, 60)], [m], 0.1, masters=[g])):
+        with pytest.raises(RuntimeError, match="gradient shares elements"):
+            call()
+    assert not bool(buf.any()) and torch.equal(w, _matrix(40, 60, 1))
+    g.copy_(_matrix(40, 60, 3))
+    rwkv_kernel.muon_step([w, m], [g, g], [other, torch.zeros_like(w)], 0.1)   # (one gradient may be two parameters')
+    rwkv_kernel.muon_step([w], [m.view(60, 40).t()], [m], 0.1)                 # (and one that is not contiguous is copied before)
