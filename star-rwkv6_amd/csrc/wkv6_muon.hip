@@ -258,6 +258,14 @@ template <int T, int WM, int WN, int KS, int NB> struct TileShape {
     static constexpr int set_bytes = 2 * T * kLine, stage_bytes = KS * set_bytes;
 };
 
+// Between what the lanes of a wave write to LDS and what others of them read there, and before it is written anew: the hardware takes a wave's LDS accesses in
+// their order, the compiler would be free to exchange those that are at different addresses for each lane.
+__device__ __forceinline__ void between_lanes() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ __forceinline__ f16x product(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::threads) void product_kernel(Group g, Step s, int turn, int total, int run) {
@@ -520,6 +528,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                         *reinterpret_cast<f32x4 *>(rows + (lane & 31) * 32 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 4)) = x;   // (in an order that spreads them over the banks)
                     }
                 }
+                between_lanes();
                 const int r0 = t.tall ? i0 : j0, c0 = t.tall ? j0 : i0, R = t.tall ? I : J, C = t.tall ? J : I;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -578,6 +587,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                     *reinterpret_cast<h4 *>(row + (q ^ turned) * 16 + (lane >> 5) * 8) = hi;
                     *reinterpret_cast<h4 *>(row + ((q + 4) ^ turned) * 16 + (lane >> 5) * 8) = lo;
                 }
+                between_lanes();
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int r = q * 8 + (lane >> 3), piece = lane & 7;
@@ -605,6 +615,7 @@ template <typename S, int kMode, typename O> __global__ __launch_bounds__(S::thr
                     }
                 }
             }
+            between_lanes();   // (the next tile goes out through the same 4 KB)
         }
 }
 
@@ -782,6 +793,7 @@ template <int kPhase, typename O> __global__ __launch_bounds__(kThreads) void th
                 __syncthreads();   // (rx has been read, its rows are the new ones from here on)
                 if (bi < down * 32) {
                     thin_put(rx, bi, bj, lane, v);
+                    between_lanes();
                     // the same as rows of X: the transposing read hands lane l of 16 lanes the l-th element of each of four rows
                     const int group = lane >> 4, l16 = lane & 15;
 #pragma unroll
