@@ -42,6 +42,14 @@ def _kernels(x):
     return rwkv_kernel
 
 
+def _as_built(module, cls):
+    """Whether a call of this module is its class's forward and nothing else, so that what stands in for it is the same: no hooks, no wrapper or
+    subclass, no forward of its own, not compiled."""
+    return type(module) is cls and "forward" not in module.__dict__ and getattr(module, "_compiled_call_impl", None) is None \
+        and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks) \
+        and not nn.modules.module._has_any_global_hook()
+
+
 def _bf16_autocast():
     return torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16
 
@@ -222,7 +230,10 @@ class RWKV6(nn.Module):
         x = table(ids) if kernels is None else kernels.embedding(ids.long(), table.weight)
         x, branch = add_norm(x, None, self.embedding_ln)[1], None
         for blk in self.blocks:
-            x, branch = blk.stages(x, branch, mask)
+            if _as_built(blk, Block):
+                x, branch = blk.stages(x, branch, mask)
+            else:
+                x, branch = blk(x if branch is None else x + branch, mask), None
         return self.output_layer(add_norm(x, branch, self.output_ln, rounded=True)[1])
 
 

@@ -7,6 +7,7 @@ import sys
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "star-rwkv6_amd"))
@@ -367,3 +368,73 @@ def test_train_step_takes_several_tokens_at_a_place():
     loss = hz.train_step(model, torch.optim.SGD(model.parameters(), lr=0.1), ids)
     # (losses of about 4, each off by some 2^-22 of itself)
     assert abs(float(loss) - float(want)) <= 2.0 ** -20 * float(want) and bool(torch.isfinite(model.weight).all())
+
+
+class _Wrapped(torch.nn.Module):
+    """A block whose activations are computed again in the backward pass."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x, mask=None):
+        return torch.utils.checkpoint.checkpoint(self.inner, x, mask, use_reentrant=False)
+
+
+class _Doubled(hz.Block):
+    def forward(self, x, mask=None):
+        return 2.0 * super().forward(x, mask)
+
+
+def _blocks_are_called(op, device):
+    """Hooks of a block run, and a wrapped block, a subclass's and an instance's own forward are what is called.  (On the GPU an addition may be made by another
+    kernel: of 2^-24 each, some 100 roundings behind each other, and 16 for how far two layers spread them: 2^-13 of the largest.)"""
+    model = _toy(op).to(device)
+    ids = torch.randint(0, TOY["vocabulary_size"], (2, 20), generator=torch.Generator().manual_seed(4)).to(device)
+    want = model(ids)
+    want.square().mean().backward()
+    grads = [p.grad.clone() for p in model.parameters()]
+
+    def close(a, b):
+        return float((a - b).detach().abs().max()) <= 2.0 ** -13 * float(b.detach().abs().max())
+
+    seen = []
+    for k, blk in enumerate(model.blocks):
+        blk.register_forward_pre_hook(lambda m, a, k=k: seen.append(("before", k, a[0].shape)))
+        blk.register_forward_hook(lambda m, a, out, k=k: seen.append(("after", k, out.shape)))
+    shape = (2, 20, TOY["hidden_size"])
+    assert close(model(ids), want) and seen == [(when, k, shape) for k in range(2) for when in ("before", "after")]
+    model.blocks[1].register_forward_hook(lambda m, a, out: torch.zeros_like(out))
+    assert not close(model(ids), want)
+    for which in ([0], [1], [0, 1]):
+        model = _toy(op).to(device)
+        for k in which:
+            model.blocks[k] = _Wrapped(model.blocks[k])
+        model(ids).square().mean().backward()
+        got = [p.grad for p in model.parameters()]
+        assert len(got) == len(grads) and all(close(a, b) for a, b in zip(got, grads))
+    model = _toy(op).to(device)
+    model.blocks[1].__class__ = _Doubled
+    other = _toy(op).to(device)
+    other.blocks[1].forward = lambda x, mask=None: 2.0 * hz.Block.forward(other.blocks[1], x, mask)
+    third = _toy(op).to(device)
+    third.blocks[1].register_forward_hook(lambda m, a, out: 2.0 * out)
+    assert close(model(ids), third(ids)) and close(other(ids), third(ids))
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: seen.append(type(m)))
+    try:
+        del seen[:]
+        _toy(op).to(device)(ids)
+    finally:
+        handle.remove()
+    assert seen.count(hz.Block) == 2
+
+
+def test_blocks_are_called():
+    _blocks_are_called(OPSKernelOperator(64, 32), "cpu")
+
+
+@pytest.mark.gpu
+def test_blocks_are_called_on_the_gpu():
+    from rwkv_kernel import RWKVKernelOperator
+
+    _blocks_are_called(RWKVKernelOperator(64, 32), "cuda")
