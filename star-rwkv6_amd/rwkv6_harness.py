@@ -54,11 +54,19 @@ def _bf16_autocast():
     return torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16
 
 
+def _rounds(x, reader):
+    """Whether this module, the only one to read the norm of x, would round it to bf16 first: under bf16 autocast on the GPU, a projection or what begins with the
+    library's input side."""
+    if not (x.is_cuda and _bf16_autocast()):
+        return False
+    return _as_built(reader, nn.Linear) or ((_as_built(reader, TimeMix) or _as_built(reader, ChannelMix)) and reader.rounds_its_input())
+
+
 def add_norm(x, branch, norm, rounded=False):
     """(x + branch, the norm of it), in one kernel where the package has it; branch None: (x, the norm of x).  rounded: under bf16 autocast the norm's readers
     round it to bf16, and it comes out so there."""
     kernels, autocast = _kernels(x), torch.is_autocast_enabled('cuda')
-    if kernels is None or type(norm) is not nn.LayerNorm or (x.dtype != torch.float32 and (autocast or (branch is not None and branch.dtype != x.dtype))):
+    if kernels is None or not _as_built(norm, nn.LayerNorm) or (x.dtype != torch.float32 and (autocast or (branch is not None and branch.dtype != x.dtype))):
         x = x if branch is None else x + branch
         return x, norm(x)
     dtype = torch.bfloat16 if rounded and _bf16_autocast() else x.dtype
@@ -200,8 +208,8 @@ class Block(nn.Module):
 
     def stages(self, x, branch, mask=None):
         """From the stream and the branch that the layer before leaves (or None) to those of this one: each addition goes with the norm that follows it."""
-        x, h = add_norm(x, branch, self.layer_norm_att, self.time_mix.rounds_its_input())
-        x, h = add_norm(x, self.time_mix(h, mask), self.layer_norm_ffn, self.channel_mix.rounds_its_input())
+        x, h = add_norm(x, branch, self.layer_norm_att, _rounds(x, self.time_mix))
+        x, h = add_norm(x, self.time_mix(h, mask), self.layer_norm_ffn, _rounds(x, self.channel_mix))
         return x, self.channel_mix(h)
 
     def forward(self, x, mask=None):
@@ -225,7 +233,7 @@ class RWKV6(nn.Module):
 
     def forward(self, ids, mask=None):
         table = self.embedding
-        plain = type(table) is nn.Embedding and table.padding_idx is None and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq
+        plain = _as_built(table, nn.Embedding) and table.padding_idx is None and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq
         kernels = _kernels(table.weight) if plain else None
         x = table(ids) if kernels is None else kernels.embedding(ids.long(), table.weight)
         x, branch = add_norm(x, None, self.embedding_ln)[1], None
@@ -234,7 +242,7 @@ class RWKV6(nn.Module):
                 x, branch = blk.stages(x, branch, mask)
             else:
                 x, branch = blk(x if branch is None else x + branch, mask), None
-        return self.output_layer(add_norm(x, branch, self.output_ln, rounded=True)[1])
+        return self.output_layer(add_norm(x, branch, self.output_ln, _rounds(x, self.output_layer))[1])
 
 
 def _losses(logits):

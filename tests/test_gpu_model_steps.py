@@ -3,6 +3,7 @@ import copy
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import rwkv6_harness as hz
 import rwkv_kernel
@@ -142,3 +143,64 @@ def test_a_captured_step():
         assert torch.equal(loss, want)
         for (name, p), q in zip(ours.named_parameters(), twin.parameters()):
             assert torch.equal(p, q), name
+
+
+def _reruns(module):
+    """The module in another one, which computes its activations again in the backward pass."""
+    class Wrap(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.inner = module
+
+        def forward(self, *a):
+            return torch.utils.checkpoint.checkpoint(self.inner, *a, use_reentrant=False)
+
+    return Wrap()
+
+
+@pytest.mark.parametrize("dtype", [None, BF16])
+def test_hooks_and_wrappers_in_the_model(dtype):
+    """Hooks on the table, the norms, the mixes and the output layer run, with what torch's modules see there (fp32 in and out of the norms), and wrapped modules are called.  The logits
+    are the model's: to 2^-12 of the largest in fp32, as above; under bf16 autocast to half a step of bf16, 2^-9, in each of some 10 stages that a flipped rounding goes through: 2^-5."""
+    _, ours = _models()
+    ids = _ids().cuda()[:, :-1]
+    off = 2.0 ** (-12 if dtype is None else -5)
+
+    def run(model):
+        with torch.autocast("cuda", dtype=BF16, enabled=dtype is not None):
+            return model(ids).float()
+
+    def close(a, b):
+        return float((a - b).detach().abs().max()) <= off * float(b.detach().abs().max())
+
+    want = run(ours)
+    names = ["embedding", "embedding_ln", "output_ln", "output_layer"] + ["blocks.%d.%s" % (k, n) for k in range(2) for n in ("layer_norm_att", "layer_norm_ffn", "time_mix", "channel_mix")]
+    for kind in ("forward", "pre", "backward"):
+        model, seen = copy.deepcopy(ours), {}
+        for name in names:
+            m = model.get_submodule(name)
+            if kind == "forward":
+                m.register_forward_hook(lambda m, a, out, n=name: seen.update({n: (a[0].dtype, out.dtype)}))
+            elif kind == "pre":
+                m.register_forward_pre_hook(lambda m, a, n=name: seen.update({n: (a[0].dtype,)}))
+            else:
+                m.register_full_backward_hook(lambda m, gi, go, n=name: seen.update({n: ()}))
+        logits = run(model)
+        logits.sum().backward()
+        assert close(logits, want) and sorted(seen) == sorted(names), kind
+        if kind != "backward":
+            assert all(all(t == torch.float32 for t in v) for n, v in seen.items() if "norm" in n or "_ln" in n)
+            assert all(v[0] == torch.float32 for n, v in seen.items() if n != "embedding")
+    # a hook that changes what comes out does so
+    for name in ("embedding", "embedding_ln", "output_ln", "blocks.0.layer_norm_att", "blocks.1.layer_norm_ffn"):
+        model = copy.deepcopy(ours)
+        model.get_submodule(name).register_forward_hook(lambda m, a, out: torch.zeros_like(out))
+        assert not close(run(model), want), name
+    # nothing is asked of a module in another one's place
+    for name in names:
+        model = copy.deepcopy(ours)
+        parent, _, child = name.rpartition(".")
+        setattr(model.get_submodule(parent), child, _reruns(model.get_submodule(name)))
+        logits = run(model)
+        assert close(logits, want), name
+        logits.sum().backward()
