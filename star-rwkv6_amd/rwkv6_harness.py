@@ -54,6 +54,11 @@ def _bf16_autocast():
     return torch.is_autocast_enabled('cuda') and torch.get_autocast_dtype('cuda') == torch.bfloat16
 
 
+def _goes_beside(x, branch):
+    """Whether the sum is in x's type, and the kernel has the two."""
+    return branch.dtype == x.dtype or (x.dtype == torch.float32 and branch.dtype in (torch.bfloat16, torch.float16))
+
+
 def _rounds(x, reader):
     """Whether this module, the only one to read the norm of x, would round it to bf16 first: under bf16 autocast on the GPU, a projection or what begins with the
     library's input side."""
@@ -66,7 +71,8 @@ def add_norm(x, branch, norm, rounded=False):
     """(x + branch, the norm of it), in one kernel where the package has it; branch None: (x, the norm of x).  rounded: under bf16 autocast the norm's readers
     round it to bf16, and it comes out so there."""
     kernels, autocast = _kernels(x), torch.is_autocast_enabled('cuda')
-    if kernels is None or not _as_built(norm, nn.LayerNorm) or (x.dtype != torch.float32 and (autocast or (branch is not None and branch.dtype != x.dtype))):
+    if kernels is None or not _as_built(norm, nn.LayerNorm) or norm.normalized_shape != (x.shape[-1],) or x.shape[-1] > kernels.torch_layers.MOST_CHANNELS \
+            or (x.dtype != torch.float32 and autocast) or (branch is not None and (branch.shape != x.shape or not _goes_beside(x, branch))):
         x = x if branch is None else x + branch
         return x, norm(x)
     dtype = torch.bfloat16 if rounded and _bf16_autocast() else x.dtype

@@ -204,3 +204,23 @@ def test_hooks_and_wrappers_in_the_model(dtype):
         logits = run(model)
         assert close(logits, want), name
         logits.sum().backward()
+
+
+def test_norms_that_are_left_to_torch(monkeypatch):
+    """More channels than the kernel takes, several dimensions, branches of other types and shapes: what they were before there was a kernel."""
+    seen = _calls(monkeypatch)
+    g = torch.Generator().manual_seed(4)
+    wide, two = torch.nn.LayerNorm(40000).cuda(), torch.nn.LayerNorm((6, 64)).cuda()
+    for norm, shape, branch in ((wide, (2, 3, 40000), None), (wide, (2, 3, 40000), torch.float32), (two, (5, 6, 64), None), (two, (5, 6, 64), torch.float32),
+                                (torch.nn.LayerNorm(64).cuda(), (5, 6, 64), "row")):
+        x = torch.randn(shape, generator=g).cuda()
+        b = None if branch is None else torch.randn(shape if branch != "row" else shape[-1:], generator=g).cuda()
+        total, h = hz.add_norm(x, b, norm)
+        assert torch.equal(total, x if b is None else x + b) and torch.equal(h, norm(total))
+    norm = torch.nn.LayerNorm(64).cuda().double()
+    x, b = torch.randn(5, 64, generator=g).cuda(), torch.randn(5, 64, generator=g).double().cuda()
+    total, h = hz.add_norm(x, b, norm)
+    assert total.dtype == h.dtype == torch.float64 and torch.equal(h, norm(x + b))
+    assert seen == {}
+    hz.add_norm(x, x, torch.nn.LayerNorm(64).cuda())
+    assert seen == {"layer_norm": 1}
