@@ -224,6 +224,9 @@ class Block(nn.Module):
 
 
 class RWKV6(nn.Module):
+    """ids (B, T) -> logits (B, T, vocabulary).  Ids outside of the table, negative ones among them, are an error on the CPU.  On the GPU, where the host does not see them, their
+    rows are NaN, and with them the logits of their texts and a loss over these."""
+
     def __init__(self, rwkv_kernel, num_layers, vocabulary_size, hidden_size, decomposer_size, head_size, expand_size):
         super().__init__()
         self.embedding = nn.Embedding(vocabulary_size, hidden_size)
@@ -240,8 +243,9 @@ class RWKV6(nn.Module):
     def forward(self, ids, mask=None):
         table = self.embedding
         plain = _as_built(table, nn.Embedding) and table.padding_idx is None and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq
-        kernels = _kernels(table.weight) if plain else None
-        x = table(ids) if kernels is None else kernels.embedding(ids.long(), table.weight)
+        kernels = _kernels(table.weight) if plain and not (ids.is_floating_point() or ids.is_complex()) else None
+        # (the kernel gives a negative id a row of zeros, which would pass for a token's: it goes behind the table)
+        x = table(ids) if kernels is None else kernels.embedding(torch.where(ids < 0, table.num_embeddings, ids.long()), table.weight)
         x, branch = add_norm(x, None, self.embedding_ln)[1], None
         for blk in self.blocks:
             if _as_built(blk, Block):

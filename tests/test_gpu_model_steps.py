@@ -224,3 +224,24 @@ def test_norms_that_are_left_to_torch(monkeypatch):
     assert seen == {}
     hz.add_norm(x, x, torch.nn.LayerNorm(64).cuda())
     assert seen == {"layer_norm": 1}
+
+
+def test_ids_outside_of_the_table():
+    """An error on the CPU; on the GPU NaN in the logits of their text and no others, and in a step's loss.  What is no id at all is refused on either."""
+    plain, ours = _models()
+    ids = torch.randint(0, V, (4, T), generator=torch.Generator().manual_seed(6))
+    want = ours(ids.cuda())
+    for bad in (-1, -V, V, -2 ** 63, 2 ** 63 - 1):
+        x = ids.clone()
+        x[2, 5] = bad
+        with pytest.raises(IndexError):
+            plain(x)
+        got = ours(x.cuda())
+        assert torch.equal(got[[0, 1, 3]], want[[0, 1, 3]]) and bool(got[2, 5:].isnan().all()), bad
+        if bad in (-1, V):
+            assert bool(ours(x.int().cuda())[2, 5:].isnan().all())
+            assert bool(rwkv_kernel.cross_entropy(got, ids.cuda()).isnan())
+    assert torch.equal(ours(ids.int().cuda()), want)
+    for model, x in ((plain, ids), (ours, ids.cuda())):
+        with pytest.raises((RuntimeError, IndexError)):
+            model(x.float())
