@@ -287,19 +287,68 @@ def train_step(model, optimizer, ids, autocast_dtype=None):
     return _update(optimizer, F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), target.reshape(-1)))
 
 
-class Optimizers:
-    """Several optimizers, of a model's parameters each a part, as one."""
+class Optimizers(torch.optim.Optimizer):
+    """Several optimizers, of a model's parameters each a part, as one: groups and state are theirs, one behind the other, and so they are saved and loaded.  A group is added
+    to one of them."""
 
     def __init__(self, *optimizers):
         self.optimizers = optimizers
+        params = [p for group in self.param_groups for p in group["params"]]
+        assert len({id(p) for p in params}) == len(params), "a parameter belongs to one of the optimizers"
+        super().__init__(self.param_groups, {})
+
+    # (the base class sets both once and adds the groups that are there already)
+    @property
+    def param_groups(self):
+        return [group for optimizer in self.optimizers for group in optimizer.param_groups]
+
+    @param_groups.setter
+    def param_groups(self, groups):
+        pass
+
+    @property
+    def state(self):
+        return {p: state for optimizer in self.optimizers for p, state in optimizer.state.items()}
+
+    @state.setter
+    def state(self, state):
+        pass
+
+    def add_param_group(self, param_group):
+        assert any(param_group is group for group in self.param_groups), "a group is added to one of the optimizers"
+
+    def __getstate__(self):
+        return dict(optimizers=self.optimizers, defaults=self.defaults)
 
     def zero_grad(self, set_to_none=True):
         for optimizer in self.optimizers:
             optimizer.zero_grad(set_to_none=set_to_none)
 
-    def step(self):
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         for optimizer in self.optimizers:
             optimizer.step()
+        return loss
+
+    def state_dict(self):
+        state, groups, first = {}, [], 0
+        for optimizer in self.optimizers:
+            d = optimizer.state_dict()
+            state.update({first + i: s for i, s in d["state"].items()})
+            groups += [dict(group, params=[first + i for i in group["params"]]) for group in d["param_groups"]]
+            first += sum(len(group["params"]) for group in d["param_groups"])
+        return {"state": state, "param_groups": groups}
+
+    def load_state_dict(self, state_dict):
+        groups = list(state_dict["param_groups"])
+        assert [len(group["params"]) for group in groups] == [len(group["params"]) for group in self.param_groups], "saved from other groups of parameters"
+        for optimizer in self.optimizers:
+            mine, groups = groups[:len(optimizer.param_groups)], groups[len(optimizer.param_groups):]
+            ids = {i for group in mine for i in group["params"]}
+            optimizer.load_state_dict({"state": {i: s for i, s in state_dict["state"].items() if i in ids}, "param_groups": mine})
 
 
 def muon_and_adamw(model, lr=0.02, weight_decay=0.0, adamw_lr=1e-4, **options):

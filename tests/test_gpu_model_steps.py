@@ -245,3 +245,22 @@ def test_ids_outside_of_the_table():
     for model, x in ((plain, ids), (ours, ids.cuda())):
         with pytest.raises((RuntimeError, IndexError)):
             model(x.float())
+
+
+def test_training_goes_on_from_what_was_saved():
+    """Muon and AdamW as one optimizer, with a schedule, saved after two steps and loaded."""
+    _, ours = _models()
+    _, twin = _models(seed=9)
+    opt, other = hz.muon_and_adamw(ours, lr=0.01), hz.muon_and_adamw(twin, lr=0.5, adamw_lr=0.3)
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda step: 0.5 ** step)
+    for step in range(2):
+        hz.train_step(ours, opt, _ids(10 + step).cuda())
+        schedule.step()
+    assert [g["lr"] for g in opt.param_groups] == [0.0025, 0.25e-4]
+    twin.load_state_dict(ours.state_dict())
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for step in range(2):
+        for model, o in ((ours, opt), (twin, other)):
+            hz.train_step(model, o, _ids(20 + step).cuda())
+    assert all(torch.equal(p, q) for p, q in zip(ours.parameters(), twin.parameters()))
+    assert all(torch.equal(opt.state[p][n], other.state[q][n]) for p, q in zip(ours.parameters(), twin.parameters()) for n in opt.state[p])

@@ -1,6 +1,7 @@
 """The RWKV-6 model harness around the operator (configuration 4 of the baseline, at toy sizes here):
 its layers against independent restatements, a few training steps on the CPU with the python-loop
 operator, and -- on the GPU -- the same model with the HIP operator against the python-loop one."""
+import copy
 import os
 import sys
 
@@ -438,3 +439,63 @@ def test_blocks_are_called_on_the_gpu():
     from rwkv_kernel import RWKVKernelOperator
 
     _blocks_are_called(RWKVKernelOperator(64, 32), "cuda")
+
+
+def _two_optimizers(model):
+    matrices = [p for p in model.parameters() if p.dim() == 2]
+    vectors = [p for p in model.parameters() if p.dim() != 2]
+    return hz.Optimizers(torch.optim.SGD(matrices, lr=0.1, momentum=0.9), torch.optim.AdamW([{"params": vectors[:3]}, {"params": vectors[3:], "lr": 1e-4}], lr=1e-3))
+
+
+def test_optimizers_are_one_optimizer():
+    """Groups, schedules, hooks, closures, copies, and a training that goes on from what was saved."""
+    model = _toy(OPSKernelOperator(64, 32))
+    opt = _two_optimizers(model)
+    ids = [torch.randint(0, TOY["vocabulary_size"], (2, 9), generator=torch.Generator().manual_seed(k)) for k in range(4)]
+    assert [g["lr"] for g in opt.param_groups] == [0.1, 1e-3, 1e-4]
+    assert {id(p) for g in opt.param_groups for p in g["params"]} == {id(p) for p in model.parameters()}
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda step: 0.5 ** step)
+    calls = []
+    opt.register_step_post_hook(lambda *a: calls.append(1))
+    for k in range(2):
+        hz.train_step(model, opt, ids[k])
+        schedule.step()
+    assert [g["lr"] for o in opt.optimizers for g in o.param_groups] == [0.025, 0.25e-3, 0.25e-4] and len(calls) == 2
+    assert set(opt.state) == set(model.parameters())
+    saved, weights = copy.deepcopy(opt.state_dict()), {k: v.clone() for k, v in model.state_dict().items()}
+    assert sorted(saved["state"]) == list(range(len(list(model.parameters())))) == [i for g in saved["param_groups"] for i in g["params"]]
+    twin = _toy(OPSKernelOperator(64, 32), seed=5)
+    twin.load_state_dict(weights)
+    other = _two_optimizers(twin)
+    other.load_state_dict(saved)
+    model2, opt2 = copy.deepcopy((model, opt))
+    for m, o in ((model, opt), (twin, other), (model2, opt2)):
+        for k in (2, 3):
+            hz.train_step(m, o, ids[k])
+    for p, q, r in zip(model.parameters(), twin.parameters(), model2.parameters()):
+        assert torch.equal(p, q) and torch.equal(p, r)
+    assert opt2.param_groups[0]["params"][0] is not opt.param_groups[0]["params"][0]
+
+    def closure():
+        opt.zero_grad()
+        loss = F.cross_entropy(model(ids[0][:, :-1]).reshape(-1, TOY["vocabulary_size"]), ids[0][:, 1:].reshape(-1))
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure).detach()) > 0
+    opt.zero_grad()
+    assert all(p.grad is None for p in model.parameters())
+
+
+def test_what_optimizers_refuse():
+    model = _toy(OPSKernelOperator(64, 32))
+    opt = _two_optimizers(model)
+    extra = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(AssertionError, match="one of the optimizers"):
+        opt.add_param_group({"params": [extra]})
+    with pytest.raises(AssertionError, match="one of the optimizers"):
+        hz.Optimizers(torch.optim.SGD([extra], lr=0.1), torch.optim.SGD([extra], lr=0.1))
+    opt.optimizers[0].add_param_group({"params": [extra], "lr": 0.3})
+    assert [g["lr"] for g in opt.param_groups] == [0.1, 0.3, 1e-3, 1e-4]
+    with pytest.raises(AssertionError, match="other groups"):
+        opt.load_state_dict(_two_optimizers(model).state_dict())
