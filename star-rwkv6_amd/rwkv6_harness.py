@@ -351,15 +351,18 @@ class Optimizers(torch.optim.Optimizer):
             optimizer.load_state_dict({"state": {i: s for i, s in state_dict["state"].items() if i in ids}, "param_groups": mine})
 
 
-def muon_and_adamw(model, lr=0.02, weight_decay=0.0, adamw_lr=1e-4, **options):
+def muon_and_adamw(model, lr=0.02, weight_decay=0.0, adamw_lr=1e-4, adamw=None, **options):
     """The package's Muon for the weight matrices of the model's layers and its AdamW for the rest (embedding, norms, biases, mixes, output layer), as one
-    optimizer for the steps here.  options as of rwkv_kernel.Muon."""
+    optimizer for the steps here.  options as of rwkv_kernel.Muon, adamw: a dict of what AdamW takes beside them (moment_bits, betas, max_grad_norm: of AdamW's
+    gradients alone, which Muon's steps do not depend on the size of).  skip_nonfinite is refused: Muon takes every step, and the model's would be half a step."""
     from rwkv_kernel import AdamW, Muon
 
+    adamw = dict(dict(lr=adamw_lr, weight_decay=weight_decay), **(adamw or {}))
+    assert not adamw.get("skip_nonfinite"), "Muon leaves no step out: skip_nonfinite would leave out AdamW's half of one"
     matrices = [m.weight for m in model.blocks.modules() if isinstance(m, nn.Linear)]
     others = {id(p) for p in matrices}
     others = [p for p in model.parameters() if id(p) not in others]
-    return Optimizers(Muon(matrices, lr=lr, weight_decay=weight_decay, **options), AdamW(others, lr=adamw_lr, weight_decay=weight_decay))
+    return Optimizers(Muon(matrices, lr=lr, weight_decay=weight_decay, **options), AdamW(others, **adamw))
 
 
 # Fine-tuning steps on the operator package's losses (its torch flavour, on the GPU).  Texts are ids (B, T+1); mask (B, T) says which of

@@ -264,3 +264,21 @@ def test_training_goes_on_from_what_was_saved():
             hz.train_step(model, o, _ids(20 + step).cuda())
     assert all(torch.equal(p, q) for p, q in zip(ours.parameters(), twin.parameters()))
     assert all(torch.equal(opt.state[p][n], other.state[q][n]) for p, q in zip(ours.parameters(), twin.parameters()) for n in opt.state[p])
+
+
+def test_options_of_both_optimizers():
+    _, ours = _models()
+    ours = ours.to(BF16)
+    opt = hz.muon_and_adamw(ours, lr=0.01, weight_decay=0.1, adamw_lr=1e-3, adamw=dict(moment_bits=8, master_weights=True, max_grad_norm=1e-3, weight_decay=0.0, betas=(0.8, 0.9)), momentum=0.9,
+                            master_weights=True)
+    muon, adamw = opt.optimizers
+    assert [(g["lr"], g["weight_decay"]) for g in opt.param_groups] == [(0.01, 0.1), (1e-3, 0.0)] and opt.param_groups[0]["momentum"] == 0.9 and opt.param_groups[1]["betas"] == (0.8, 0.9)
+    ids, w = _ids().cuda(), torch.randn(B, T, V, generator=torch.Generator().manual_seed(3)).cuda()
+    for _ in range(2):
+        opt.zero_grad()
+        with torch.autocast("cuda", dtype=BF16):
+            (ours(ids[:, :-1]).float() * w).sum().backward()
+        opt.step()
+    assert all("master" in s for s in opt.state.values()) and all("scales" in s for s in adamw.state.values()) and float(adamw.last_grad_norm) > 1e-3
+    with pytest.raises(AssertionError, match="skip_nonfinite"):
+        hz.muon_and_adamw(ours, adamw=dict(skip_nonfinite=True))
