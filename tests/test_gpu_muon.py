@@ -377,3 +377,76 @@ def test_gradients_in_what_is_written_are_refused():
     g.copy_(_matrix(40, 60, 3))
     rwkv_kernel.muon_step([w, m], [g, g], [other, torch.zeros_like(w)], 0.1)   # (one gradient may be two parameters')
     rwkv_kernel.muon_step([w], [m.view(60, 40).t()], [m], 0.1)                 # (and one that is not contiguous is copied before)
+
+
+# Products are made in tiles of 64, 128 or 256, by how many tiles a launch has, 64 and 128 in two forms (few tiles, alone on their compute units, have four buffers): each of them
+# with rows and columns left over, as results and as steps on weights, and the square of A (its tiles are counted on and above the diagonal).
+FORMS = {"64 alone": [(300, 500)], "64 twice": [(1000, 1100)], "128 alone": [(1100, 2000)], "128 twice": [(2100, 1000)] * 2 + [(1000, 2100)], "256": [(1300, 2070), (2070, 1300)] * 10,
+         "shared": [(300, 9000), (9000, 300)], "two launches": [(70, 90)] * 30 + [(90, 70)] * 30}
+EACH = {"64 alone": [0], "64 twice": [0], "128 alone": [0], "128 twice": [0, 2], "256": [0, 1, 18, 19], "shared": [0, 1], "two launches": [0, 29, 55, 56, 59]}   # of them, what is compared
+
+
+def _pick(lists, which):
+    return tuple(None if l is None else [l[i] for i in which] for l in lists)
+
+
+@pytest.mark.parametrize("dtype,masters", [(F32, False), (BF16, True), (F16, False)])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_steps_in_every_tile_form(form, dtype, masters):
+    print("muon step, tiles", form, dtype, masters, flush=True)
+    before = _step_inputs(FORMS[form], dtype, 11, masters)
+    kept = tuple(None if l is None else [t.clone() for t in l] for l in _pick(before, EACH[form]))
+    rwkv_kernel.muon_step(before[0], before[1], before[2], lr=0.02, weight_decay=0.1, masters=before[3])
+    _check_step(kept, _pick(before, EACH[form]), 0.02, 0.95, True, 0.1, "shape")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shapes", [[(1500, 1600)], [(1600, 1500)], [(1300, 2070)] * 25 + [(2070, 1300)] * 25, [(1290, 1310)] * 56])
+def test_results_in_large_tiles(shapes, dtype):
+    """One matrix whose A has more than 256 tiles of 64 and fewer than 128 of 128; lists whose A has 1024 tiles of 256."""
+    print("orthogonalize, tiles", len(shapes), shapes[0], dtype, flush=True)
+    some = {s: _matrix(*s, s[0], dtype=dtype) for s in set(shapes)}
+    out = rwkv_kernel.orthogonalize([some[s] for s in shapes])
+    for i in {0, len(shapes) // 2, len(shapes) - 1}:
+        _check(out[i], some[shapes[i]])
+
+
+def test_a_list_over_the_workspace():
+    """42 matrices of 2048 x 2048 do not fit the workspace together: 31 and 11 go through, as results and as steps."""
+    from rwkv_kernel import _native
+
+    print("orthogonalize, over the workspace", flush=True)
+    count, most = 42, 2 ** 31
+    rows = (_native.MuonMatrix * count)()
+    for r in rows:
+        r.rows = r.columns = 2048
+    lib = _native.load()
+    one = lib.wkv6_muon_workspace_bytes(1, rows)
+    assert lib.wkv6_muon_workspace_bytes(count, rows) == most < count * one and most // one == 31
+    xs = [_matrix(2048, 2048, i, "normal", BF16) for i in range(5)]
+    at = [i * 2 % 5 for i in range(count)]
+    out = rwkv_kernel.orthogonalize([xs[i] for i in at])
+    for i in (0, 30, 31, 32, 41):
+        _check(out[i], xs[at[i]])
+    assert all(torch.equal(out[i], out[i % 5]) for i in range(31))
+    del out
+    params, bufs = [xs[at[-1 - i]].clone() for i in range(count)], [torch.zeros(2048, 2048, device="cuda") for _ in range(count)]
+    before = _pick((params, [xs[i] for i in at], bufs, None), (0, 30, 31, 41))
+    before = (*([t.clone() for t in l] for l in before[:3]), None)
+    rwkv_kernel.muon_step(params, [xs[i] for i in at], bufs, lr=0.02, weight_decay=0.1)
+    _check_step(before, _pick((params, None, bufs, None), (0, 30, 31, 41)), 0.02, 0.95, True, 0.1, "shape")
+
+
+@pytest.mark.parametrize("shapes", [[(32, 2048)] * 5 + [(2048, 32)] * 5, [(2048, 2048)], [(777, 1311)], [(300, 9000)]])
+def test_calls_repeat_themselves(shapes):
+    """Whatever the memory held that a call gets as its workspace; and a result in 16 bits is the fp32 result, rounded once."""
+    print("orthogonalize, again", shapes[0], flush=True)
+    for dtype in (BF16, F16):
+        xs = [_matrix(*s, i, dtype=dtype) for i, s in enumerate(shapes)]
+        want = rwkv_kernel.orthogonalize(xs)
+        for k in range(6):
+            for n in (1 << 18, 1 << 20, 1 << 22, 1 << 24, 1 << 25):
+                torch.full((n,), (float("nan"), 3.0, float("inf"))[k % 3], device="cuda")
+            assert all(torch.equal(a, b) for a, b in zip(want, rwkv_kernel.orthogonalize(xs)))
+        single = rwkv_kernel.orthogonalize([x.float() for x in xs])
+        assert all(torch.equal(a, b.to(dtype)) for a, b in zip(want, single))
