@@ -282,3 +282,75 @@ def test_options_of_both_optimizers():
     assert all("master" in s for s in opt.state.values()) and all("scales" in s for s in adamw.state.values()) and float(adamw.last_grad_norm) > 1e-3
     with pytest.raises(AssertionError, match="skip_nonfinite"):
         hz.muon_and_adamw(ours, adamw=dict(skip_nonfinite=True))
+
+
+class _Torchs(torch.nn.LayerNorm):   # (not the class that the package's kernel stands in for)
+    pass
+
+
+def _with_torchs_norms(model):
+    model = copy.deepcopy(model)
+    for m in model.modules():
+        if type(m) is torch.nn.LayerNorm:
+            m.__class__ = _Torchs
+    return model
+
+
+def test_types_of_the_norms_under_autocast(monkeypatch):
+    """bf16 where the only reader would round it, fp32 otherwise."""
+    seen = []
+    kernel = rwkv_kernel.layer_norm
+    monkeypatch.setattr(rwkv_kernel, "layer_norm", lambda *a, **k: (seen.append(k["dtype"]), kernel(*a, **k))[1])
+    _, ours = _models()
+    ids = _ids().cuda()[:, :-1]
+    for dtype, want in ((BF16, [torch.float32] + [BF16] * 5), (torch.float16, [torch.float32] * 6), (None, [torch.float32] * 6)):
+        del seen[:]
+        with torch.autocast("cuda", dtype=dtype, enabled=dtype is not None):
+            ours(ids)
+        assert seen == want, dtype
+
+
+@pytest.mark.parametrize("C", [128, 777, 2048])
+def test_an_addition_and_its_norm_under_autocast(C):
+    """One addition with its norm, kernel and torch, with gradients.  The sum is the same to the bit.  The norm, some 8 roundings of 2^-24 in fp32 (and the channels' sums), goes
+    to the other of two neighbours in bf16 only next to the middle between them: in 2^-8 of the elements at most, by a step of 2^-7.  The same for the branch's gradient.  Gradients in
+    fp32 differ by roundings of terms up to 2^3 times what is left of them: 2^-18 of the largest, sums over the rows by 2^-16."""
+    g = torch.Generator().manual_seed(C)
+    norm = torch.nn.LayerNorm(C).cuda()
+    with torch.no_grad():
+        norm.weight.copy_(torch.randn(C, generator=g))
+        norm.bias.copy_(torch.randn(C, generator=g))
+    x, gy, gt = (torch.randn(6, 50, C, generator=g).cuda() for _ in range(3))
+    branch = torch.randn(6, 50, C, generator=g).to(BF16).cuda()
+    res = []
+    for module in (norm, _with_torchs_norms(torch.nn.ModuleList([norm]))[0]):
+        a, b = x.clone().requires_grad_(True), branch.clone().requires_grad_(True)
+        with torch.autocast("cuda", dtype=BF16):
+            total, h = hz.add_norm(a, b, module, rounded=True)
+        assert h.dtype == (BF16 if module is norm else torch.float32)
+        h = h.to(BF16)
+        res.append([total, h, *torch.autograd.grad([total, h], [a, b, module.weight, module.bias], [gt, gy.to(BF16)])])
+    (total, h, gx, gb, gw, gbias), want = res
+    assert torch.equal(total, want[0])
+    for p, q in ((h, want[1]), (gb, want[3])):
+        assert int((p != q).sum()) <= 2.0 ** -8 * p.numel()
+        assert bool(((p.float() - q.float()).abs() <= 2.0 ** -7 * q.float().abs() + 2.0 ** -20).all())
+    assert float((gx - want[2]).abs().max()) <= 2.0 ** -18 * float(want[2].abs().max())
+    for p, q in ((gw, want[4]), (gbias, want[5])):
+        assert float((p - q).abs().max()) <= 2.0 ** -16 * float(q.abs().max())
+
+
+def test_gradients_under_autocast():
+    """The model's gradients under bf16 autocast with the kernel's norms and with torch's.  Either has the errors of its roundings to bf16; these are as large on both sides but not
+    the same ones, so that a gradient of one is off from that of the other by about 1.4 times what torch's is off from float64: by 3 times at most, in the 2-norm of each parameter."""
+    plain, ours = _models()
+    torchs = _with_torchs_norms(ours)
+    ids, w = _ids(), torch.randn(B, T, V, generator=torch.Generator().manual_seed(3))
+    (plain(ids[:, :-1]) * w.double()).sum().backward()
+    for model in (ours, torchs):
+        with torch.autocast("cuda", dtype=BF16):
+            logits = model(ids[:, :-1].cuda())
+        (logits.float() * w.cuda()).sum().backward()
+    for (name, e), p, q in zip(plain.named_parameters(), ours.parameters(), torchs.parameters()):
+        p, q = p.grad.cpu().double(), q.grad.cpu().double()
+        assert float((p - q).norm()) <= 3 * float((q - e.grad).norm()) + 2.0 ** -16 * float(e.grad.norm()), name
