@@ -158,7 +158,6 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(EmbeddingGrad
             if (r * 64 + lane < count) items[start[digit[r]] + counts[wave][digit[r]] + place[r]] = item[r];
         __syncthreads();
     }
-    if (bits == 0) __syncthreads();
     for (int i = tid; i < N; i += kSmallThreads) {
         keys[i] = items[i] >> kPlace;
         places[i] = items[i] & ((1u << kPlace) - 1);
