@@ -450,7 +450,7 @@ int wkv6_adamw_step(void *stream, int dtype, int moment_bits, int64_t count, con
 
 /* Orthogonalized updates.  `matrices` and coefficients lie in HOST memory and may be freed when the call returns.  grad and out are of
  * `dtype`, row-major and contiguous like the rest; addresses need their element's alignment, the workspace 256 bytes.  A matrix without elements is
- * left out. */
+ * left out.  What is written (momentum, out, master) shares no elements with anything else of a call. */
 typedef struct wkv6_muon_matrix {
     const void *grad;
     float *momentum;   /* wkv6_muon_step: the mean of gradients; otherwise NULL */

@@ -6,7 +6,7 @@
 //
 // Precision.  The polynomial takes a singular value s to about a s while it is small, so five steps multiply what is lost in the small ones by up to a^5 = 485: with the
 // matrices in bf16 throughout the result is off by 1 to 16 % of its size, with fp16 by 0.1 to 2 %.  Here every matrix is a pair of fp16 numbers hi + lo,
-// 22 bits, and a product the three matrix instructions hi hi + hi lo + lo hi, which accumulate in fp32: about 1.6 times the error of fp32 throughout, at
+// 22 bits, and a product the three matrix instructions hi hi + hi lo + lo hi, which accumulate in fp32: 0.7 to 1.2 times the error of fp32 throughout, at
 // 5 times the rate of the fp32 matrix instructions.  Values are held times 1024: those of X, A and B stay below some 4, so the pairs' range of
 // 64 is not left by coefficients of any use, and lo keeps its bits down to 2^-13 of 1 (below, the pair is exact to 2^-35).
 //
@@ -837,7 +837,7 @@ template <typename F> hipError_t by_type(int dtype, F &&f) {
 }
 
 template <typename O> void launch_thin(hipStream_t st, Group &g, Step s, int steps, const double *coefficients) {
-    // (workgroups to a matrix: each of them reads all of their parts; 16 while there are few matrices)
+    // (workgroups to a matrix: each of them reads all of their parts; as many as it may have parts while there are few matrices)
     int total = 0;
     for (int i = 0; i < g.count; ++i) {
         g.first[i] = total;

@@ -279,7 +279,7 @@ template <int T, int V, bool W> struct Shape {
 };
 
 // By the number of channels: threads that a row is spread over, and 16-byte pieces of the stream's type to a thread.  (Few to a thread: the backward's sums and the
-// weights take three registers a channel, and four workgroups or more to a compute unit keep the memory busy.  8192 rows of 2048, a stream in fp32 and branches in bf16,
+// weights take three registers a channel.  8192 rows of 2048, a stream in fp32 and branches in bf16,
 // backward, in us: 64 threads to a row 61 to 74, 128 49, 256 47.)
 template <int kE, bool kWhole, typename F> void by_width(int64_t C, F &&f) {
     if (C <= 64 * 8) f(Shape<64, 8 / kE, kWhole>{});
@@ -306,6 +306,7 @@ template <typename F> hipError_t by_types(int stream, int branch, F &&f) {
     return hipGetLastError();
 }
 
+// Two workgroups to a compute unit at most: each leaves 2 C sums in the workspace, which another launch adds up.
 int backward_blocks(int64_t rows, int64_t C) {
     const int64_t at_once = C <= 64 * 16 ? kThreads / 64 : 1, all = (rows + at_once - 1) / at_once;
     return (int)(all < 512 ? all : 512);
